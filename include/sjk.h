@@ -307,7 +307,8 @@ typedef struct sjk_view {
 int          sjk_last_error(void);          /* sticky status of the void-returning calls; clears it */
 /* Device status word of the kernels (synchronizes the device): 0 = fine, bit 1 (SJK_DEVICE_TIMEOUT) = a bounded
  * in-kernel wait ran out (the kernel skipped its remaining work and released its resources), bit 2
- * (SJK_DEVICE_DESC) = a descriptor-driven call met a descriptor that does not fit its cache. Reading clears it. */
+ * (SJK_DEVICE_DESC) = a descriptor-driven call met a descriptor that does not fit its cache, bit 3 (SJK_DEVICE_PAGE) =
+ * a call of the 16-bit layers or of sjk_pages met a row, position or page outside its arrays. Reading clears it. */
 int          sjk_device_status(void);
 int          sjk_last_cuda_error(void);     /* cudaError_t of the last failed CUDA call */
 const char * sjk_version(void);
@@ -415,7 +416,7 @@ enum {
     SJK_DESC_HKV, SJK_DESC_B_OLD, SJK_DESC_TYPE_K, SJK_DESC_TYPE_V, SJK_DESC_BODY_TYPE, SJK_DESC_SINK_TYPE,
     SJK_DESC_N_ENTRIES = 16
 };
-enum { SJK_DEVICE_TIMEOUT = 1, SJK_DEVICE_DESC = 2 };
+enum { SJK_DEVICE_TIMEOUT = 1, SJK_DEVICE_DESC = 2, SJK_DEVICE_PAGE = 4 };
 /* Fill a host descriptor for view v: seal [B_old, B) this ubatch, positions [0, N) visible, first query row at
  * qpos0. Returns SJKVARN_ERR_ARG for values that the kernels would reject. */
 int sjk_desc_fill(const sjk_view * v, uint32_t B_old, uint32_t B, uint32_t N, uint32_t qpos0, int32_t * desc);
@@ -524,6 +525,152 @@ typedef struct sjk_trunc_req {
     int        release;
 } sjk_trunc_req;
 int    sjk_truncate_batch(const sjk_trunc_req * reqs, int n, void * dev_pool, sjk_stream st);
+
+/* =====================================================================================
+ * Layers kept at 16 bits, and what every layer's projection goes through before its cache.
+ *
+ * Beside sealed layers a model may keep some at 16 bits (a head size the codec refuses, first and last layers, a
+ * draft model). These calls are their cache, what writes it, what reads it, and who owns its pages: sjk_qkv (norm
+ * of every query and key head, rotary positions, cache write, in one pass), sjk_kv16_attend (attention of one new
+ * token per sequence over the pages) and sjk_pages_* (fork, extend with copy on write, free, compact). sjk_qkv also
+ * makes the rows that sjk_store and sjk_attend_model take, and the page calls work on the record pool's slab and
+ * block tables as well. Lengths, positions, tables and row lists are DEVICE memory, read when the kernels run, so a
+ * captured step replays. No counterpart in the reference.
+ *
+ * A table row belongs to one sequence: entry g holds the page of positions [g page_tokens, (g + 1) page_tokens), or
+ * SJKVARN_NO_BLOCK. Entries, rows and positions outside their arrays are never followed: the token, position or page
+ * is left out and SJK_DEVICE_PAGE is set in sjk_device_status().
+ * ===================================================================================== */
+enum { SJK_F32 = 0, SJK_F16 = 1, SJK_BF16 = 2 };
+
+/* ---- rotary positions ----
+ * Pair i of a head's first n_rot channels turns by pos * f_i: (a, b) -> amp (a c - b s, a s + b c), with the pairs
+ * (i, i + n_rot / 2) (SJK_ROPE_HALF) or (2 i, 2 i + 1) (SJK_ROPE_PAIR); channels from n_rot on pass through.
+ * f_i = base^(-2 i / n_rot), scaled for contexts longer than the trained n_ctx by `scaling`:
+ *   LINEAR  f / factor
+ *   NTK     base * factor^(n_rot / (n_rot - 2)) in place of base
+ *   YARN    f / factor r + f (1 - r), r = clamp((i - lo) / max(hi - lo, 0.001), 0, 1), lo and hi the pairs (floor,
+ *           ceil, within [0, n_rot - 1]) that turn beta_fast and beta_slow times over n_ctx;
+ *           amp 0 stands for 0.1 ln(factor) + 1
+ *   BANDS   f / factor (1 - s) + f s, s = clamp((n_ctx f / 2 pi - low) / (high - low), 0, 1)
+ * amp 0 stands for 1 in the other forms. Angles are kept as turns in 64-bit fixed point (step[i] = f_i / 2 pi in
+ * units of 2^-64 turns): pos * step modulo 2^64 is the angle modulo a turn for every 31-bit position, where a
+ * product in 32-bit floats is off by 0.03 rad at a million. */
+enum { SJK_ROPE_HALF = 0, SJK_ROPE_PAIR = 1 };
+enum { SJK_ROPE_NONE = 0, SJK_ROPE_LINEAR, SJK_ROPE_NTK, SJK_ROPE_YARN, SJK_ROPE_BANDS };
+typedef struct sjk_rope_config {
+    int    n_rot;              /* channels that rotate: even, 2 .. 512 */
+    int    layout, scaling;
+    double base, factor, n_ctx, beta_fast, beta_slow, low, high, amp;
+} sjk_rope_config;
+typedef struct sjk_rope {
+    int        n_rot, layout;  /* n_rot 0: no rotation */
+    float      amp;
+    uint64_t * step;           /* DEVICE [n_rot / 2] */
+} sjk_rope;
+/* the table on the host: step[n_rot / 2], *amp */
+int  sjk_rope_steps(const sjk_rope_config * cfg, uint64_t * step, float * amp);
+/* the same in device memory (allocates; sjk_rope_free gives it back) */
+int  sjk_rope_init(sjk_rope * r, const sjk_rope_config * cfg);
+void sjk_rope_free(sjk_rope * r);
+
+/* ---- a layer's paged 16-bit cache ----
+ * The K row of (page, slot, head) is the head_dim elements at k + page*page_stride + slot*slot_stride +
+ * head*head_stride (elements), its V row the same at v. */
+typedef struct sjk_kv16 {
+    void *     k, * v;         /* DEVICE */
+    int64_t    page_stride, slot_stride, head_stride;
+    int        type;           /* SJK_F16 or SJK_BF16 */
+    int        head_dim, n_head_kv, page_tokens;
+    uint32_t   n_pages;
+    uint32_t * tables;         /* DEVICE [n_rows][table_stride] */
+    uint32_t   n_rows, table_stride;
+} sjk_kv16;
+
+/* ---- from a projection's output to cache rows, in one pass ----
+ * Heads of token t: element d of head h at p + (t*row_stride + h*head_stride + d). */
+typedef struct sjk_rows {
+    void *  p;                 /* DEVICE; NULL: absent */
+    int64_t row_stride, head_stride;
+    int     n_head, type;
+} sjk_rows;
+typedef struct sjk_qkv_args {
+    int n_tok, head_dim;       /* head_dim even, 2 .. 512 */
+    sjk_rows q, k, v;          /* inputs of one type; any may be absent */
+    sjk_rows q_out, k_out, v_out;   /* row outputs of any type; absent: no row output. May be the inputs' own rows. */
+    const void * q_norm, * k_norm;  /* DEVICE [head_dim] norm weights of norm_type, NULL: no norm of these heads */
+    int norm_type;
+    float norm_bias, eps;      /* y = x / sqrt(mean x^2 + eps) * (w + norm_bias), then the rotation, then one rounding */
+    sjk_rope rope;
+    const int32_t * pos;       /* DEVICE [n_tok] positions; a negative one marks padding: nothing of the token is written */
+    const int32_t * rows;      /* DEVICE [n_tok] table rows of the tokens, NULL: token t is table row t */
+    sjk_kv16 cache;            /* k, v NULL: no cache write. Else K (normed, rotated) and V go to the token's page too. */
+} sjk_qkv_args;
+/* One launch. pos may be NULL without a rotation and a cache. Arithmetic in 32-bit floats, one rounding at the end. */
+int sjk_qkv(const sjk_qkv_args * a, sjk_stream st);
+
+/* ---- attention of one new token per sequence over the pages ----
+ * Sequence i has the table row rows[i] (DEVICE; NULL: row i), len[i] positions (DEVICE, its newest one included) and
+ * the query heads q[i] (type any); query head h reads KV head h / (n_head / n_head_kv). out[i] = sum over its last
+ * min(len, window) positions (window 0: all) of softmax(scale q . k) v; a sequence without a live position (len <= 0,
+ * or all its pages SJKVARN_NO_BLOCK) gets zeros. Positions on a SJKVARN_NO_BLOCK page are left out (pages that a
+ * window has passed may be given back). A draft's several positions are so many entries with one row. Any page size,
+ * any number of query heads per KV head; head_dim 64, 96, 128 or 256, K and V rows 16-byte aligned
+ * (SJKVARN_ERR_ARG); q of the cache's type 4-byte aligned. 32-bit inside; see csrc/sjk_kv16.cu for the products.
+ * scratch: sjk_kv16_attend_scratch_bytes() bytes, 16-byte aligned, for whatever lengths; not shared by calls that overlap.
+ * Two launches; the same inputs give the same bits. */
+size_t sjk_kv16_attend_scratch_bytes(const sjk_kv16 * c, int n_head);
+int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len, const int32_t * rows, int n_seq, float scale,
+                    int window, const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st);
+
+/* ---- who owns the pages ----
+ * A ledger in device memory over the pages of one or more slabs (the K and the V pages of every layer, or the record
+ * pool's slab): the pool's stack of free ids, as sjk_pool_* keep it (so sjk_pool_dev_load, _store and _reserve_batch
+ * work on the same memory), and for every page the number of table entries that hold it beyond the first (its shares).
+ * Tables: DEVICE [n_rows][table_stride]. Row lists are DEVICE int32. Page p of layer l of a slab is the page_bytes
+ * at base + l*layer_stride + p*page_bytes (all multiples of 16). */
+#define SJK_PAGES_MAX      (1u << 20)
+#define SJK_PAGES_MAX_ROWS 1024
+#define SJK_MAX_SLABS      4
+typedef struct sjk_slab {
+    void * base;               /* DEVICE */
+    size_t page_bytes, layer_stride;
+    int    n_layers;
+} sjk_slab;
+typedef struct sjk_pages {
+    void     * ledger;         /* DEVICE, sjk_pages_bytes(n_pages) bytes, 16-byte aligned */
+    uint32_t * tables;         /* DEVICE */
+    uint32_t   n_pages, n_rows, table_stride;
+    int        page_tokens;
+    int        n_slabs;
+    sjk_slab   slabs[SJK_MAX_SLABS];
+} sjk_pages;
+size_t     sjk_pages_bytes(uint32_t n_pages);
+/* all pages free (page 0 is handed out first), no shares; does not touch the tables */
+int        sjk_pages_init(const sjk_pages * p, sjk_stream st);
+uint32_t * sjk_pages_shares(const sjk_pages * p);      /* DEVICE [n_pages], inside the ledger */
+/* Row dst[i] (empty) gets the pages of row src[i], which it then shares: no data moves (sjk_pages_extend splits a
+ * page when one of its owners writes on). status[i] (DEVICE) = 0; SJKVARN_ERR_ARG for rows out of range, a row that is
+ * not empty, or a dst that is also a src or an earlier dst of the call; SJKVARN_ERR_CORRUPT for an entry that is no
+ * page: nothing is done for that request. One launch. */
+int        sjk_pages_fork(const sjk_pages * p, const int32_t * src, const int32_t * dst, int n, int32_t * status, sjk_stream st);
+/* Pages for the positions [len[i], len[i] + add) of each row (add: DEVICE add[i], or add_all where add is NULL), in
+ * (request, page) order: an entry without a page takes the id on top of the stack; a page with other owners is
+ * replaced by an own one, which gets its contents if the row keeps positions on it (copy on write), except that when
+ * all owners of a page are in the call the last one keeps it. All or nothing: status[0] (DEVICE) = 0,
+ * SJKVARN_ERR_POOL_FULL (too few free pages), SJKVARN_ERR_ARG (rows out of range or named twice, positions beyond the
+ * table) or SJKVARN_ERR_CORRUPT. n <= SJK_PAGES_MAX_ROWS. Two launches. */
+int        sjk_pages_extend(const sjk_pages * p, const int32_t * rows, const int32_t * len, const int32_t * add, int add_all, int n,
+                            int32_t * status, sjk_stream st);
+/* The entries [g0[i], g1[i]) of each row (DEVICE; NULL: from the first, to the last) give their pages up and become
+ * SJKVARN_NO_BLOCK; pages without an owner left go onto the stack, the lowest id on top. One launch. */
+int        sjk_pages_free(const sjk_pages * p, const int32_t * rows, const int32_t * g0, const int32_t * g1, int n, sjk_stream st);
+/* Used pages whose id is not below the number of used pages move, in order, into the free ids below it; tables (all
+ * n_rows), shares and stack follow (afterwards the next id handed out is the number of used pages). info (DEVICE, may
+ * be NULL): [0] used pages, [1] moved ones. Two launches. */
+int        sjk_pages_compact(const sjk_pages * p, int32_t * info, sjk_stream st);
+/* Contents of page src[i] to page dst[i] (DEVICE) in every layer of every slab; no page is both. One launch. */
+int        sjk_pages_copy(const sjk_pages * p, const int32_t * src, const int32_t * dst, int n, sjk_stream st);
 
 /* ---- seeded synthetic inputs of the benchmark configurations (DEVICE outputs) ----
  * Input generation for benchmarks and parity tests; no counterpart in the reference. K = X * s with X ~ N(0, 1)

@@ -55,6 +55,12 @@ int sjk_tc_body_status_take(void);
 int sjk_tc_dense_status_take(void);
 int sjk_tc_trellis_status_take(void);
 int sjk_xchg_status_take(void);
+// the 16-bit layers' and the page ledger's (SJK_DEVICE_PAGE)
+int sjk_qkv_status_take(void);
+int sjk_kv16_status_take(void);
+int sjk_pages_status_take(void);
+// 0 where the fields of a 16-bit cache are possible ones (sjk_qkv.cu)
+int sjk_kv16_check(const sjk_kv16 * c);
 
 // Move the record groups [g0, g0 + n) of one layer (group_bytes = n_head_kv x record bytes) through
 // an optional device block table: op 0 gathers them into buf (group order), op 1 scatters buf into them, op 2

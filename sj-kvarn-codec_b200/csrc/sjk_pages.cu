@@ -1,0 +1,499 @@
+// sjk_pages.cu - who owns the pages of a cache: forks that share pages, copy on write, freeing, compaction, and the
+// copies of page contents these need. Integer bookkeeping with a fixed result: where requests meet on one page, counts
+// go by atomics (their order does not matter) and every choice - who keeps a page, which id a request takes, in which
+// order ids return to the stack - by request and page numbers.
+//
+// Bound: the contents' copies by HBM (every moved page once in and once out), the bookkeeping by latency: one CTA per
+// call, phases in a row, each a few dependent loads.
+#include "sjk_kv16.cuh"
+#include "sjk_internal.h"
+
+namespace {
+
+using namespace sjk16;
+
+constexpr int NT = 256;                     // fork, free, copy
+constexpr int NB = 1024;                    // one-CTA bookkeeping
+constexpr uint32_t NO_BLOCK = SJKVARN_NO_BLOCK;
+__device__ unsigned int g_pages_status;
+
+SJK_DEV void flag() { atomicOr(&g_pages_status, (unsigned) SJK_DEVICE_PAGE); }
+
+// The ledger: the device pool's header and stack (sjk_pool_dev_bytes), then per-page words. Ticket, count, last and
+// marks are zero between calls.
+struct Ledger {
+    uint32_t * head;                        // n_free, n_pages, ticket of sjk_pages_free, copies of the last call
+    uint32_t * ids, * shares, * count, * last, * old, * src, * dst, * map, * marks;
+};
+SJK_HD Ledger ledger_of(void * base, uint32_t n) {
+    Ledger l;
+    uint32_t * w = static_cast<uint32_t *>(base);
+    l.head = w;      w += 4;
+    l.ids = w;       w += n;
+    l.shares = w;    w += n;
+    l.count = w;     w += n;
+    l.last = w;      w += n;
+    l.old = w;       w += n;
+    l.src = w;       w += n;
+    l.dst = w;       w += n;
+    l.map = w;       w += n;
+    l.marks = w;
+    return l;
+}
+
+struct Params {
+    Ledger l;
+    uint32_t * tables;
+    uint32_t n_pages, n_rows, stride;
+    int page_tokens, n_slabs;
+    sjk_slab slabs[SJK_MAX_SLABS];
+    const int32_t * a, * b, * c;            // the call's lists
+    int n, add_all;
+    int32_t * status;
+};
+
+// exclusive prefix sum over a CTA of NTHR threads; *total gets the sum. s: NTHR / 32 words
+template <int NTHR>
+SJK_DEV uint32_t cta_scan(uint32_t v, uint32_t * s, uint32_t * total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint32_t x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) s[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        uint32_t w = lane < NTHR / 32 ? s[lane] : 0u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xFFFFFFFFu, w, o);
+            if (lane >= o) w += y;
+        }
+        if (lane < NTHR / 32) s[lane] = w;
+    }
+    __syncthreads();
+    const uint32_t before = (warp ? s[warp - 1] : 0u) + x - v;
+    *total = s[NTHR / 32 - 1];
+    __syncthreads();
+    return before;
+}
+
+// ---- fork: one CTA per request -------------------------------------------------------------------------------
+__global__ void __launch_bounds__(NT) pages_fork_kernel(const __grid_constant__ Params p) {
+    pdl_wait();
+    pdl_release();
+    const int i = blockIdx.x;
+    const int32_t src = p.a[i], dst = p.b[i];
+    int bad = src < 0 || dst < 0 || (uint32_t) src >= p.n_rows || (uint32_t) dst >= p.n_rows ? 1 : 0;
+    for (int j = threadIdx.x; j < p.n && !bad; j += NT)
+        if (p.a[j] == dst || (j < i && p.b[j] == dst)) bad = 1;
+    if (__syncthreads_or(bad)) {
+        if (threadIdx.x == 0) p.status[i] = SJKVARN_ERR_ARG;
+        return;
+    }
+    const uint32_t * from = p.tables + (size_t) src * p.stride;
+    uint32_t * to = p.tables + (size_t) dst * p.stride;
+    int full = 0, wrong = 0;
+    for (uint32_t g = threadIdx.x; g < p.stride; g += NT) {
+        full |= to[g] != NO_BLOCK ? 1 : 0;
+        wrong |= from[g] != NO_BLOCK && from[g] >= p.n_pages ? 1 : 0;
+    }
+    full = __syncthreads_or(full);
+    wrong = __syncthreads_or(wrong);
+    if (full || wrong) {
+        if (threadIdx.x == 0) p.status[i] = full ? SJKVARN_ERR_ARG : SJKVARN_ERR_CORRUPT;
+        return;
+    }
+    for (uint32_t g = threadIdx.x; g < p.stride; g += NT) {
+        const uint32_t e = from[g];
+        if (e == NO_BLOCK) continue;
+        to[g] = e;
+        atomicAdd(&p.l.shares[e], 1u);
+    }
+    if (threadIdx.x == 0) p.status[i] = 0;
+}
+
+// ---- free: grid.x requests, grid.y runs of a row; the last CTA pushes what lost its last owner ------------------
+__global__ void __launch_bounds__(NT) pages_free_kernel(const __grid_constant__ Params p) {
+    __shared__ uint32_t s_scan[NT / 32];
+    __shared__ int s_last;
+    pdl_wait();
+    pdl_release();
+    const int i = blockIdx.x;
+    const int32_t row = p.a[i];
+    if (row < 0 || (uint32_t) row >= p.n_rows) {
+        if (threadIdx.x == 0) flag();
+    } else {
+        const int64_t g0 = p.b && p.b[i] > 0 ? p.b[i] : 0;
+        const int64_t g1 = p.c && (uint32_t) p.c[i] < p.stride ? p.c[i] : p.c && p.c[i] < 0 ? 0 : (int64_t) p.stride;
+        for (int64_t g = g0 + (int64_t) blockIdx.y * NT + threadIdx.x; g < g1; g += (int64_t) gridDim.y * NT) {
+            uint32_t * at = p.tables + (size_t) row * p.stride + g;
+            if (*at == NO_BLOCK) continue;
+            const uint32_t e = atomicExch(at, NO_BLOCK);    // a row that is named twice gives each entry up once
+            if (e == NO_BLOCK) continue;
+            if (e >= p.n_pages) { flag(); continue; }
+            if (atomicSub(&p.l.shares[e], 1u) == 0u) atomicOr(&p.l.marks[e >> 5], 1u << (e & 31u));
+        }
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(&p.l.head[2], 1u) == gridDim.x * gridDim.y - 1u;
+    __syncthreads();
+    if (!s_last) return;
+    __threadfence();
+    // marked pages in descending order, from the last word of the bitmap to the first
+    const uint32_t words = (p.n_pages + 31u) / 32u;
+    uint32_t n_free = p.l.head[0];
+    for (uint32_t w0 = 0; w0 < words; w0 += NT) {
+        const uint32_t k = w0 + threadIdx.x;
+        const bool on = k < words;
+        const uint32_t w = on ? words - 1u - k : 0u;
+        uint32_t m = on ? __ldcg(&p.l.marks[w]) : 0u;
+        if (m) p.l.marks[w] = 0u;
+        uint32_t total;
+        uint32_t at = n_free + cta_scan<NT>((uint32_t) __popc(m), s_scan, &total);
+        while (m) {
+            const uint32_t bit = 31u - (uint32_t) __clz(m), id = w * 32u + bit;
+            m &= ~(1u << bit);
+            if (at < p.n_pages) p.l.ids[at] = id;
+            ++at;
+            p.l.shares[id] = 0u;
+        }
+        n_free = n_free + total < p.n_pages ? n_free + total : p.n_pages;
+    }
+    if (threadIdx.x == 0) { p.l.head[0] = n_free; p.l.head[2] = 0u; }
+}
+
+// ---- extend: one CTA; an item is an entry (request, page) -----------------------------------------------------------
+__global__ void __launch_bounds__(NB) pages_extend_kernel(const __grid_constant__ Params p) {
+    __shared__ uint32_t s_scan[NB / 32];
+    __shared__ int32_t s_row[NB], s_len[NB];
+    __shared__ uint32_t s_g0[NB], s_off[NB];
+    pdl_wait();
+    pdl_release();
+    const int tid = threadIdx.x;
+    const uint32_t P = (uint32_t) p.page_tokens;
+    // the requests: rows, first pages, and where their items begin
+    int bad = 0, much = 0;                                  // much: more entries than there are pages
+    uint32_t items = 0;
+    if (tid < p.n) {
+        const int32_t row = p.a[tid], len = p.b[tid], add = p.c ? p.c[tid] : p.add_all;
+        s_row[tid] = row;
+        s_len[tid] = len;
+        if (row < 0 || (uint32_t) row >= p.n_rows || len < 0 || add < 0 || (add > 0 && ((uint32_t) len + (uint32_t) add - 1u) / P >= p.stride)) bad = 1;
+        else if (add > 0) {
+            s_g0[tid] = (uint32_t) len / P;
+            items = ((uint32_t) len + (uint32_t) add - 1u) / P - s_g0[tid] + 1u;
+            much = items > p.n_pages;
+        }
+    }
+    __syncthreads();
+    if (tid < p.n && !bad)
+        for (int j = 0; j < tid; ++j) bad |= s_row[j] == s_row[tid] ? 1 : 0;
+    bad = __syncthreads_or(bad);
+    much = __syncthreads_or(much);
+    if (bad || much) {
+        if (tid == 0) { p.status[0] = bad ? SJKVARN_ERR_ARG : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
+        return;
+    }
+    uint32_t n_items;
+    const uint32_t off = cta_scan<NB>(items, s_scan, &n_items);
+    s_off[tid] = off;
+    __syncthreads();
+    auto find = [&](uint32_t it) {                          // request of an item: the last whose items begin at or before it
+        int lo = 0, hi = p.n - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_off[mid] <= it) lo = mid; else hi = mid - 1;
+        }
+        return lo;
+    };
+    auto entry = [&](int r, uint32_t it) { return p.tables + (size_t) s_row[r] * p.stride + s_g0[r] + (it - s_off[r]); };
+    // who holds the shared pages: how many of the call, and the last of them
+    int wrong = 0;
+    for (uint32_t it = tid; it < n_items; it += NB) {
+        const int r = find(it);
+        const uint32_t e = *entry(r, it);
+        if (e == NO_BLOCK) continue;
+        if (e >= p.n_pages) { wrong = 1; continue; }
+        if (p.l.shares[e]) { atomicAdd(&p.l.count[e], 1u); atomicMax(&p.l.last[e], (uint32_t) r); }
+    }
+    wrong = __syncthreads_or(wrong);
+    // a hole, or a shared page that is not kept
+    auto takes = [&](int r, uint32_t e) {
+        if (e == NO_BLOCK) return true;
+        if (e >= p.n_pages || !p.l.shares[e]) return false;
+        return !(__ldcg(&p.l.count[e]) == p.l.shares[e] + 1u && __ldcg(&p.l.last[e]) == (uint32_t) r);
+    };
+    const uint32_t n_free = p.l.head[0];
+    uint32_t need = 0;
+    for (uint32_t it = tid; it < n_items; it += NB) {
+        const int r = find(it);
+        need += takes(r, *entry(r, it)) ? 1u : 0u;
+    }
+    uint32_t total;
+    cta_scan<NB>(need, s_scan, &total);
+    if (wrong || total > n_free) {                          // nothing is done: only the counts go back
+        for (uint32_t it = tid; it < n_items; it += NB) {
+            const uint32_t e = *entry(find(it), it);
+            if (e < p.n_pages) { p.l.count[e] = 0u; p.l.last[e] = 0u; }
+        }
+        if (tid == 0) { p.status[0] = wrong ? SJKVARN_ERR_CORRUPT : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
+        return;
+    }
+    uint32_t taken = 0, copies = 0;
+    for (uint32_t it0 = 0; it0 < n_items; it0 += NB) {
+        const uint32_t it = it0 + tid;
+        uint32_t e = NO_BLOCK, * at = nullptr;
+        bool take = false, keep = false;
+        if (it < n_items) {
+            const int r = find(it);
+            at = entry(r, it);
+            e = *at;
+            take = takes(r, e);
+            keep = take && e != NO_BLOCK && (uint64_t) (s_g0[r] + (it - s_off[r])) * P < (uint64_t) (uint32_t) s_len[r];
+        }
+        uint32_t both;
+        const uint32_t before = cta_scan<NB>((take ? 1u : 0u) | (keep ? 0x10000u : 0u), s_scan, &both);
+        if (take) {
+            const uint32_t k = taken + (before & 0xFFFFu), id = p.l.ids[n_free - 1u - k];
+            *at = id;
+            p.l.old[k] = e;
+            if (keep) {
+                const uint32_t q = copies + (before >> 16);
+                p.l.src[q] = e;
+                p.l.dst[q] = id;
+            }
+        }
+        taken += both & 0xFFFFu;
+        copies += both >> 16;
+    }
+    __syncthreads();
+    for (uint32_t k = tid; k < total; k += NB) {
+        const uint32_t e = p.l.old[k];
+        if (e == NO_BLOCK) continue;
+        atomicSub(&p.l.shares[e], 1u);
+        p.l.count[e] = 0u;
+        p.l.last[e] = 0u;
+    }
+    if (tid == 0) {
+        p.l.head[0] = n_free - total;
+        p.l.head[3] = copies;
+        p.status[0] = 0;
+    }
+}
+
+// ---- compact: the moves (one CTA, a bitmap of the used pages in shared memory), then tables and contents ---------------
+__global__ void __launch_bounds__(NB) pages_plan_kernel(const __grid_constant__ Params p) {
+    extern __shared__ uint32_t s_used[];
+    __shared__ uint32_t s_scan[NB / 32];
+    pdl_wait();
+    pdl_release();
+    const uint32_t tid = threadIdx.x, n = p.n_pages, words = (n + 31u) / 32u;
+    const uint32_t n_free = p.l.head[0] < n ? p.l.head[0] : n, top = n - n_free;
+    for (uint32_t w = tid; w < words; w += NB) s_used[w] = w * 32u + 32u <= n ? 0xFFFFFFFFu : (1u << (n & 31u)) - 1u;
+    __syncthreads();
+    for (uint32_t i = tid; i < n_free; i += NB) {
+        const uint32_t id = p.l.ids[i];
+        if (id < n) atomicAnd(&s_used[id >> 5], ~(1u << (id & 31u)));
+        else flag();
+    }
+    __syncthreads();
+    uint32_t holes = 0, movers = 0;
+    for (uint32_t w0 = 0; w0 < words; w0 += NB) {
+        const uint32_t w = w0 + tid;
+        uint32_t h = 0, m = 0;
+        if (w < words) {
+            const uint32_t below = top <= w * 32u ? 0u : top - w * 32u >= 32u ? 0xFFFFFFFFu : (1u << (top - w * 32u)) - 1u;
+            h = ~s_used[w] & below;
+            m = s_used[w] & ~below;
+        }
+        uint32_t nh, nm;
+        uint32_t ah = holes + cta_scan<NB>((uint32_t) __popc(h), s_scan, &nh);
+        uint32_t am = movers + cta_scan<NB>((uint32_t) __popc(m), s_scan, &nm);
+        for (; h; h &= h - 1u) p.l.dst[ah++] = w * 32u + (uint32_t) __ffs(h) - 1u;
+        for (; m; m &= m - 1u) p.l.src[am++] = w * 32u + (uint32_t) __ffs(m) - 1u;
+        holes += nh;
+        movers += nm;
+    }
+    __syncthreads();
+    // equal where the stack holds every free id once; a damaged one moves nothing
+    const uint32_t moves = holes == movers ? movers : 0u;
+    if (holes != movers && tid == 0) flag();
+    for (uint32_t k = tid; k < moves; k += NB) {
+        const uint32_t s = p.l.src[k], d = p.l.dst[k];
+        p.l.map[s] = k;
+        p.l.shares[d] = p.l.shares[s];
+        p.l.shares[s] = 0u;
+    }
+    if (holes == movers)
+        for (uint32_t i = tid; i < n_free; i += NB) p.l.ids[i] = n - 1u - i;
+    if (tid == 0) {
+        p.l.head[3] = moves;
+        if (p.status) { p.status[0] = (int32_t) top; p.status[1] = (int32_t) moves; }
+    }
+}
+
+// Contents of the listed pages in every layer of every slab, in segments of SEG bytes over a grid that fills the GPU;
+// remap: the tables' entries of moved pages as well. n < 0: as many as the ledger says.
+constexpr uint32_t SEG = 16384;
+__global__ void __launch_bounds__(NT) pages_copy_kernel(const __grid_constant__ Params p, const uint32_t * src, const uint32_t * dst, int n_fixed,
+                                                        int remap) {
+    pdl_wait();
+    pdl_release();
+    const uint32_t n = n_fixed >= 0 ? (uint32_t) n_fixed : p.l.head[3];
+    if (n == 0) return;
+    if (remap) {
+        const uint32_t top = p.n_pages - p.l.head[0];
+        const uint64_t all = (uint64_t) p.n_rows * p.stride;
+        for (uint64_t i = (uint64_t) blockIdx.x * NT + threadIdx.x; i < all; i += (uint64_t) gridDim.x * NT) {
+            const uint32_t e = p.tables[i];
+            if (e < top || e == NO_BLOCK) continue;
+            const uint32_t k = e < p.n_pages ? p.l.map[e] : n;
+            if (k < n && src[k] == e) p.tables[i] = dst[k];
+            else flag();                                    // an entry whose page is not in use
+        }
+    }
+    for (int s = 0; s < p.n_slabs; ++s) {
+        const sjk_slab & sl = p.slabs[s];
+        const uint32_t segs = (uint32_t) ((sl.page_bytes + SEG - 1) / SEG);
+        const uint64_t units = (uint64_t) n * sl.n_layers * segs;
+        for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
+            const uint32_t seg = (uint32_t) (u % segs);
+            const uint64_t q = u / segs;
+            const uint32_t k = (uint32_t) (q / sl.n_layers), layer = (uint32_t) (q - (uint64_t) k * sl.n_layers);
+            const uint32_t a = src[k], b = dst[k];
+            if (a >= p.n_pages || b >= p.n_pages) { if (threadIdx.x == 0) flag(); continue; }
+            uint8_t * base = static_cast<uint8_t *>(sl.base) + (size_t) layer * sl.layer_stride + (size_t) seg * SEG;
+            const uint4 * from = reinterpret_cast<const uint4 *>(base + (size_t) a * sl.page_bytes);
+            uint4 * to = reinterpret_cast<uint4 *>(base + (size_t) b * sl.page_bytes);
+            const size_t left = sl.page_bytes - (size_t) seg * SEG;
+            const uint32_t words = (uint32_t) ((left < SEG ? left : SEG) / 16);
+            uint4 x[SEG / 16 / NT];
+#pragma unroll
+            for (int i = 0; i < (int) (SEG / 16 / NT); ++i)
+                if (i * NT + threadIdx.x < words) x[i] = from[i * NT + threadIdx.x];
+#pragma unroll
+            for (int i = 0; i < (int) (SEG / 16 / NT); ++i)
+                if (i * NT + threadIdx.x < words) to[i * NT + threadIdx.x] = x[i];
+        }
+    }
+}
+
+int params_of(const sjk_pages * g, Params * p, bool tables) {
+    if (!g || !g->ledger || !aligned(g->ledger, 16) || g->n_pages < 1 || g->n_pages > SJK_PAGES_MAX) return SJKVARN_ERR_ARG;
+    if (tables && (!g->tables || g->n_rows < 1 || g->n_rows > 0x7FFFFFFFu || g->table_stride < 1 || g->page_tokens < 1)) return SJKVARN_ERR_ARG;
+    if (g->n_slabs < 0 || g->n_slabs > SJK_MAX_SLABS) return SJKVARN_ERR_ARG;
+    for (int i = 0; i < g->n_slabs; ++i) {
+        const sjk_slab & s = g->slabs[i];
+        if (!s.base || !aligned(s.base, 16) || s.page_bytes < 16 || s.page_bytes % 16 || s.layer_stride % 16 || s.n_layers < 1) return SJKVARN_ERR_ARG;
+    }
+    *p = Params();
+    p->l = ledger_of(g->ledger, g->n_pages);
+    p->tables = g->tables;
+    p->n_pages = g->n_pages; p->n_rows = g->n_rows; p->stride = g->table_stride;
+    p->page_tokens = g->page_tokens; p->n_slabs = g->n_slabs;
+    for (int i = 0; i < g->n_slabs; ++i) p->slabs[i] = g->slabs[i];
+    return 0;
+}
+
+__global__ void __launch_bounds__(NT) pages_init_kernel(Ledger l, uint32_t n) {
+    pdl_wait();
+    pdl_release();
+    for (uint32_t i = blockIdx.x * NT + threadIdx.x; i < n; i += gridDim.x * NT) {
+        l.ids[i] = n - 1u - i;
+        l.shares[i] = l.count[i] = l.last[i] = 0u;
+        if (i < (n + 31u) / 32u) l.marks[i] = 0u;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) { l.head[0] = l.head[1] = n; l.head[2] = l.head[3] = 0u; }
+}
+
+int copy_launch(const Params & p, const uint32_t * src, const uint32_t * dst, int n, int remap, sjk_stream st) {
+    if (p.n_slabs == 0 && !remap) return 0;
+    return launch(pages_copy_kernel, dim3(148 * 4), dim3(NT), 0, st, p, src, dst, n, remap);
+}
+
+}  // namespace
+
+extern "C" size_t sjk_pages_bytes(uint32_t n) { return 16u + ((size_t) n * 8u + (n + 31u) / 32u) * sizeof(uint32_t); }
+
+extern "C" int sjk_pages_init(const sjk_pages * g, sjk_stream st) {
+    Params p;
+    const int rc = params_of(g, &p, false);
+    if (rc) return rc;
+    const uint32_t ctas = (p.n_pages + NT - 1) / NT;
+    return launch(pages_init_kernel, dim3(ctas < 148u ? ctas : 148u), dim3(NT), 0, st, p.l, p.n_pages);
+}
+
+extern "C" uint32_t * sjk_pages_shares(const sjk_pages * g) {
+    return g && g->ledger ? ledger_of(g->ledger, g->n_pages).shares : nullptr;
+}
+
+extern "C" int sjk_pages_fork(const sjk_pages * g, const int32_t * src, const int32_t * dst, int n, int32_t * status, sjk_stream st) {
+    Params p;
+    const int rc = params_of(g, &p, true);
+    if (rc) return rc;
+    if (n < 0 || (n && (!src || !dst || !status))) return SJKVARN_ERR_ARG;
+    if (n == 0) return 0;
+    p.a = src; p.b = dst; p.n = n; p.status = status;
+    return launch(pages_fork_kernel, dim3((unsigned) n), dim3(NT), 0, st, p);
+}
+
+extern "C" int sjk_pages_free(const sjk_pages * g, const int32_t * rows, const int32_t * g0, const int32_t * g1, int n, sjk_stream st) {
+    Params p;
+    const int rc = params_of(g, &p, true);
+    if (rc) return rc;
+    if (n < 0 || (n && !rows)) return SJKVARN_ERR_ARG;
+    if (n == 0) return 0;
+    p.a = rows; p.b = g0; p.c = g1; p.n = n;
+    uint32_t runs = (p.stride + 4 * NT - 1) / (4 * NT);     // about four entries a thread, at most a wave over all rows
+    const uint32_t most = 148u * 4u / (uint32_t) n + 1u;
+    if (runs > most) runs = most;
+    return launch(pages_free_kernel, dim3((unsigned) n, runs), dim3(NT), 0, st, p);
+}
+
+extern "C" int sjk_pages_extend(const sjk_pages * g, const int32_t * rows, const int32_t * len, const int32_t * add, int add_all, int n,
+                                int32_t * status, sjk_stream st) {
+    Params p;
+    int rc = params_of(g, &p, true);
+    if (rc) return rc;
+    if (n < 0 || n > SJK_PAGES_MAX_ROWS || (n && (!rows || !len || !status)) || (!add && add_all < 0)) return SJKVARN_ERR_ARG;
+    if (n == 0) return 0;
+    p.a = rows; p.b = len; p.c = add; p.add_all = add_all; p.n = n; p.status = status;
+    rc = launch(pages_extend_kernel, dim3(1), dim3(NB), 0, st, p);
+    if (rc) return rc;
+    return copy_launch(p, p.l.src, p.l.dst, -1, 0, st);
+}
+
+extern "C" int sjk_pages_compact(const sjk_pages * g, int32_t * info, sjk_stream st) {
+    Params p;
+    int rc = params_of(g, &p, true);
+    if (rc) return rc;
+    p.status = info;
+    const size_t smem = (size_t) ((p.n_pages + 31u) / 32u) * sizeof(uint32_t);
+    if (smem > 40 * 1024 && sjk_check(cudaFuncSetAttribute(pages_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem))) return SJK_ERR_DEVICE;
+    rc = launch(pages_plan_kernel, dim3(1), dim3(NB), smem, st, p);
+    if (rc) return rc;
+    return copy_launch(p, p.l.src, p.l.dst, -1, 1, st);
+}
+
+extern "C" int sjk_pages_copy(const sjk_pages * g, const int32_t * src, const int32_t * dst, int n, sjk_stream st) {
+    Params p;
+    const int rc = params_of(g, &p, false);
+    if (rc) return rc;
+    if (n < 0 || (n && (!src || !dst))) return SJKVARN_ERR_ARG;
+    if (n == 0) return 0;
+    return copy_launch(p, reinterpret_cast<const uint32_t *>(src), reinterpret_cast<const uint32_t *>(dst), n, 0, st);
+}
+
+int sjk_pages_status_take(void) {
+    unsigned v = 0;
+    if (sjk_check(cudaMemcpyFromSymbol(&v, g_pages_status, sizeof v))) return -1;
+    if (v) {
+        const unsigned z = 0;
+        if (sjk_check(cudaMemcpyToSymbol(g_pages_status, &z, sizeof z))) return -1;
+    }
+    return (int) v;
+}

@@ -79,6 +79,40 @@ class StateInfo(C.Structure):
                 ("B_prev", u32), ("draining", u32), ("total_bytes", C.c_size_t)]
 
 
+class RopeConfig(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("n_rot", "layout", "scaling")] + \
+               [(n, C.c_double) for n in ("base", "factor", "n_ctx", "beta_fast", "beta_slow", "low", "high", "amp")]
+
+
+class RopeC(C.Structure):
+    _fields_ = [("n_rot", C.c_int), ("layout", C.c_int), ("amp", C.c_float), ("step", vp)]
+
+
+class Kv16(C.Structure):
+    _fields_ = [("k", vp), ("v", vp)] + [(n, C.c_int64) for n in ("page_stride", "slot_stride", "head_stride")] + \
+               [(n, C.c_int) for n in ("type", "head_dim", "n_head_kv", "page_tokens")] + \
+               [("n_pages", u32), ("tables", vp), ("n_rows", u32), ("table_stride", u32)]
+
+
+class Rows(C.Structure):
+    _fields_ = [("p", vp), ("row_stride", C.c_int64), ("head_stride", C.c_int64), ("n_head", C.c_int), ("type", C.c_int)]
+
+
+class QkvArgs(C.Structure):
+    _fields_ = [("n_tok", C.c_int), ("head_dim", C.c_int)] + [(n, Rows) for n in ("q", "k", "v", "q_out", "k_out", "v_out")] + \
+               [("q_norm", vp), ("k_norm", vp), ("norm_type", C.c_int), ("norm_bias", C.c_float), ("eps", C.c_float),
+                ("rope", RopeC), ("pos", vp), ("rows", vp), ("cache", Kv16)]
+
+
+class Slab(C.Structure):
+    _fields_ = [("base", vp), ("page_bytes", C.c_size_t), ("layer_stride", C.c_size_t), ("n_layers", C.c_int)]
+
+
+class PagesC(C.Structure):
+    _fields_ = [("ledger", vp), ("tables", vp), ("n_pages", u32), ("n_rows", u32), ("table_stride", u32),
+                ("page_tokens", C.c_int), ("n_slabs", C.c_int), ("slabs", Slab * 4)]
+
+
 P = C.POINTER
 SIGNATURES = {
     # host helpers
@@ -194,6 +228,21 @@ SIGNATURES = {
     "sjk_xchg_exchange": (C.c_int, [P(XchgPeers), vp, C.c_int, C.c_int, u32, vp, vp]),
     "sjk_attend_partial_xchg": (C.c_int, [P(View), u32, u32, u32, C.c_int, C.c_int, C.c_uint, vp, C.c_float, vp, C.c_size_t,
                                           P(XchgPeers), u32, vp, vp]),
+    # layers kept at 16 bits
+    "sjk_rope_steps": (C.c_int, [P(RopeConfig), P(C.c_uint64), P(C.c_float)]),
+    "sjk_rope_init": (C.c_int, [P(RopeC), P(RopeConfig)]),
+    "sjk_rope_free": (None, [P(RopeC)]),
+    "sjk_qkv": (C.c_int, [P(QkvArgs), vp]),
+    "sjk_kv16_attend_scratch_bytes": (C.c_size_t, [P(Kv16), C.c_int]),
+    "sjk_kv16_attend": (C.c_int, [P(Kv16), P(Rows), vp, vp, C.c_int, C.c_float, C.c_int, P(Rows), vp, C.c_size_t, vp]),
+    "sjk_pages_bytes": (C.c_size_t, [u32]),
+    "sjk_pages_init": (C.c_int, [P(PagesC), vp]),
+    "sjk_pages_shares": (vp, [P(PagesC)]),
+    "sjk_pages_fork": (C.c_int, [P(PagesC), vp, vp, C.c_int, vp, vp]),
+    "sjk_pages_extend": (C.c_int, [P(PagesC), vp, vp, vp, C.c_int, C.c_int, vp, vp]),
+    "sjk_pages_free": (C.c_int, [P(PagesC), vp, vp, vp, C.c_int, vp]),
+    "sjk_pages_compact": (C.c_int, [P(PagesC), vp, vp]),
+    "sjk_pages_copy": (C.c_int, [P(PagesC), vp, vp, C.c_int, vp]),
     # seeded synthetic inputs
     "sjk_synth_scales": (C.c_int, [C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp]),
     "sjk_synth_kv": (C.c_int, [C.c_uint64, C.c_int, C.c_int, C.c_int, C.c_int, vp, u32, u32, vp, vp, vp]),
@@ -257,7 +306,7 @@ def config(head_dim=256, n_head_kv=4, n_ctx=16384, n_ubatch=512, **kw):
 (DESC_S, DESC_CAP, DESC_B, DESC_N, DESC_QPOS0, DESC_G, DESC_D, DESC_RECBYTES, DESC_HKV, DESC_B_OLD, DESC_TYPE_K,
  DESC_TYPE_V, DESC_BODY_TYPE, DESC_SINK_TYPE) = range(14)
 DESC_N_ENTRIES = 16
-DEVICE_TIMEOUT, DEVICE_DESC = 1, 2
+DEVICE_TIMEOUT, DEVICE_DESC, DEVICE_PAGE = 1, 2, 4
 
 
 def desc_fill(view, B_old, B, N, qpos0):
