@@ -5,21 +5,24 @@
 // byte for 16 query heads, far under the tensor cores' ridge). So the work is to keep loads in flight:
 //  - A warp is a worker of its own. The (sequence, KV head, step of TS tokens) triples of a call form one list, cut
 //    into equal runs, one per warp of a grid that fills the GPU; lengths are read from device memory, so every warp
-//    finds its run with a scan over them. Ragged batches balance by construction and no CTA barrier exists.
-//  - A warp streams its steps through a ring in shared memory with cp.async, NST steps ahead and across the ends of
+//    finds its run with a scan over them. A (sequence, KV head) weighs OV units beside its steps, for what its start
+//    and its output cost. Ragged batches balance by construction and no CTA barrier exists.
+//  - A warp streams its steps through a ring in shared memory with cp.async, NE tiles ahead and across the ends of
 //    sequences; positions that are not live are filled with zeros, not read.
-//  - The grp query heads of a KV head are the N = 8 columns of mma.m16n8k16: S^T = K Q^T with 16 tokens as rows, and
+//  - The query heads of a KV head are the N = 8 columns of mma.m16n8k16: S^T = K Q^T with 16 tokens as rows, and
 //    O^T = V^T P with 16 channels as rows, so a group of up to 8 heads wastes no rows of the accumulators, P goes from
 //    the first product's layout to the second's with one 8x8 transpose (movmatrix), and the rescaling of O needs
 //    values of its own lane only. These instructions are bound to registers and issue per warp, which lets every warp
 //    run on its own; the tensor pipe is far from its limit here (16 flops per byte at most).
 //  - A worker that held all of a sequence and head writes the output; otherwise (m, l, o[D]) per query head goes to
 //    the worker's slot in the scratch, and the merge kernel joins the slots in list order (the result does not depend
-//    on which worker came first).
+//    on which worker came first). The worker that begins a split pair leaves word of it, so the merge looks at as many
+//    entries as there can be split pairs and scans nothing.
 // Softmax statistics, sums and outputs are 32-bit. Queries of the cache's type enter as they are and P is rounded
 // once to it (up to 2^-8 of each weight for bf16, the size of the output's own rounding). For 32-bit queries or outputs
-// (or a type other than the cache's) q is the sum of two (f16) or three (bf16) 16-bit terms and P of two, which keeps
-// the products' errors at 2^-16 and below.
+// (or a type other than the cache's) q and P are the sums of two (f16) or three (bf16) 16-bit terms side by side in the
+// columns of the same products (4 or 2 heads in 8 columns), and each step's products are summed apart from what came
+// before them, which keeps the result near 32 bits.
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
@@ -29,9 +32,9 @@ namespace {
 
 using namespace sjk16;
 
-constexpr int W = 4;                        // warps of a CTA
 constexpr unsigned FULL = 0xFFFFFFFFu;
-constexpr int MIN_STEPS = 2;                // steps of a worker's run, at least
+constexpr int OV = 4;                       // what a (sequence, KV head, row tile) costs beside its steps, in steps
+constexpr int MIN_RUN = 2;                  // units of a worker's run, at least
 __device__ unsigned int g_kv16_status;
 
 struct Params {
@@ -39,11 +42,13 @@ struct Params {
     sjk_rows q, out;
     const int32_t * len, * rows;
     int n_seq, grp, tiles;                  // tiles: row tiles of a KV head (8 NT8 query heads each)
-    int window;
+    int window, page_shift;                 // page_shift: log2 of the page's tokens, -1 where it is no power of two
     float scale;
     int n_work;                             // workers
-    float * part;                           // [n_work][2][8 NT8][D]
-    float * ml;                             // [n_work][2][8 NT8][2]
+    float * part;                           // [n_work][2][R][D]
+    float * ml;                             // [n_work][2][R][2]
+    int4 * split;                           // by pair (or, with more pairs than workers, by worker): sequence (-1: not
+    int by_pair;                            // split), (KV head, row tile), first and last worker
 };
 
 // 16 tokens per m tile; steps of 32 tokens for small heads, whose rows are short
@@ -66,43 +71,33 @@ SJK_DEV Span span_of(const Params & p, int seq) {
     return s;
 }
 
-SJK_DEV int64_t warp_sum(int64_t x) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) x += __shfl_xor_sync(FULL, x, m);
-    return x;
-}
-// steps per (KV head, row tile) of all sequences before `seq` (all lanes get the sum)
-template <int TS>
-SJK_DEV int64_t steps_before(const Params & p, int seq, int lane) {
-    int64_t n = 0;
-    for (int s = lane; s < seq; s += 32) n += span_of<TS>(p, s).n;
-    return warp_sum(n);
-}
-// steps of a worker's run: the list has `total` steps
-SJK_DEV int64_t run_steps(int64_t total, int n_work) {
-    const int64_t per = (total + n_work - 1) / n_work;
-    return per < MIN_STEPS ? MIN_STEPS : per;
-}
+// units of a sequence's (KV head, row tile): its steps behind OV that stand for its start and end
+SJK_DEV int units_of(const Span & s) { return s.n ? s.n + OV : 0; }
 
 template <int TS>
 struct Cursor {                             // a place in the list
     int seq, hp, st;                        // sequence, (KV head, row tile), step
+    int64_t rem;                            // units of the run from this step on; <= 0: the run is done
+    int64_t base;                           // unit at which the pair begins
     Span s;
-    SJK_DEV void skip_empty(const Params & p) {
-        while (seq < p.n_seq && (s = span_of<TS>(p, seq)).n == 0) ++seq;
-    }
     SJK_DEV void next(const Params & p, int HP) {
+        --rem;
         if (++st < s.n) return;
         st = 0;
+        rem -= OV;
+        base += s.n + OV;
         if (++hp < HP) return;
         hp = 0;
-        ++seq;
-        skip_empty(p);
+        if (rem <= 0) return;
+        do ++seq; while (seq < p.n_seq && (s = span_of<TS>(p, seq)).n == 0);
     }
 };
 
 SJK_DEV uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
-SJK_DEV void cp16(uint32_t dst, const void * src, bool on) {
+SJK_DEV void cp16(uint32_t dst, const void * src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+SJK_DEV void cp16_or_zero(uint32_t dst, const void * src, bool on) {
     const int n = on ? 16 : 0;
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -137,45 +132,82 @@ SJK_DEV float ex2(float x) {
     return y;
 }
 
-// Kernel shape: TYPE of the cache, head size, NQ 16-bit terms of q and NP of P, NT8 tiles of 8 query heads.
-template <int TYPE_, int D_, int NQ_, int NP_, int NT8_>
+// Kernel shape: TYPE of the cache, head size, T 16-bit terms of q and P, NT8 tiles of 8 columns.
+template <int TYPE_, int D_, int T_, int NT8_>
 struct Shape {
-    static constexpr int TYPE = TYPE_, D = D_, NQ = NQ_, NP = NP_, NT8 = NT8_;
+    static constexpr int TYPE = TYPE_, D = D_, T = T_, NT8 = NT8_;
+    static constexpr int HT = T == 1 ? 8 : T == 2 ? 4 : 2;  // query heads of a tile
+    static constexpr int R = HT * NT8;                      // and of a pass
     static constexpr int TM = tok_tiles(D), TS = step_toks(D), KS = D / 16;
     static constexpr int PITCH = 2 * D + 16;                // an odd number of 16-byte words: ldmatrix without conflicts
     static constexpr int ENTRY = TS * PITCH;
-    static constexpr bool Q_REG = KS * 2 * NT8 * NQ <= 64;  // q in registers, else in shared memory
-    static constexpr int Q_BYTES = Q_REG ? 0 : NQ * NT8 * 8 * PITCH;
-    static constexpr int NST = D >= 256 && NQ > 1 && NT8 > 1 ? 1 : D >= 256 && (NQ > 1 || NT8 > 1) ? 2 : 3;
-    static constexpr int WARP_BYTES = 2 * NST * ENTRY + Q_BYTES + 16;
+    // warps of the one CTA of an SM: as many as registers and the ring leave room for
+    static constexpr int W = D >= 256 || NT8 > 1 || T > 1 ? 8 : 12;
+    static constexpr int FIT = (227 * 1024 / W - 16) / ENTRY;
+    static constexpr int NE = FIT < 6 ? FIT : 6;            // K and V tiles in a warp's ring
+    static constexpr int WARP_BYTES = NE * ENTRY + 16;
     static constexpr int CTA_BYTES = W * WARP_BYTES;
+    static_assert(NE >= 2 && NE <= 7, "a step's tiles, and the four masks, have to fit the ring");
 };
 
+// pairs of channels 8 apart, from element `at` on
+template <int TYPE, int N>
+SJK_DEV void load_pairs(float2 (&x)[N], const void * p, int64_t at, bool on) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        x[k] = make_float2(0.0f, 0.0f);
+        if (on) x[k] = make_float2(load1(p, at + 8 * k, TYPE), load1(p, at + 8 * k + 1, TYPE));
+    }
+}
+template <int TYPE, int KS>
+SJK_DEV void store_channels(void * p, int64_t at, const float (&o)[KS][4], int j, float f) {
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+        store1(p, at + 16 * k, TYPE, o[k][j] * f);
+        store1(p, at + 16 * k + 8, TYPE, o[k][2 + j] * f);
+    }
+}
+
 template <typename S>
-__global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_constant__ Params p) {
-    constexpr int D = S::D, TS = S::TS, TM = S::TM, KS = S::KS, NT8 = S::NT8, NQ = S::NQ, NP = S::NP, NST = S::NST, PITCH = S::PITCH;
-    constexpr int R = 8 * NT8;
+__global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_constant__ Params p) {
+    constexpr int D = S::D, TS = S::TS, TM = S::TM, KS = S::KS, NT8 = S::NT8, T = S::T, HT = S::HT, R = S::R, NE = S::NE, PITCH = S::PITCH, W = S::W;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t * mine = smem + (size_t) warp * S::WARP_BYTES;
     const uint32_t ring = smem_addr(mine);
-    uint32_t * s_mask = reinterpret_cast<uint32_t *>(mine + 2 * NST * S::ENTRY + S::Q_BYTES);
+    uint32_t * s_mask = reinterpret_cast<uint32_t *>(mine + NE * S::ENTRY);
     pdl_wait();
     pdl_release();
 
-    // the worker's run [run0, run1) of the list
+    // the worker's run of the list: 32 sequences at a time, first all units, then the sequence where the run begins
     const int worker = blockIdx.x * W + warp;
     const int HP = p.c.n_head_kv * p.tiles;
-    const int64_t total = steps_before<TS>(p, p.n_seq, lane) * HP;
-    const int64_t per = run_steps(total, p.n_work);
-    const int64_t run0 = worker * per, run1 = run0 + per < total ? run0 + per : total;
-    if (run0 >= run1) return;
+    for (int seq = worker; seq < p.n_seq; seq += p.n_work) {            // sequences without a live position
+        if (span_of<TS>(p, seq).n) continue;
+        for (int h = 0; h < p.out.n_head; ++h)
+            for (int d = lane; d < D; d += 32)
+                store1(p.out.p, (int64_t) seq * p.out.row_stride + (int64_t) h * p.out.head_stride + d, p.out.type, 0.0f);
+        if (p.by_pair)
+            for (int i = lane; i < HP; i += 32) p.split[seq * HP + i] = make_int4(-1, 0, 0, 0);
+    }
+    if (!p.by_pair && lane == 0) p.split[worker] = make_int4(-1, 0, 0, 0);
+    const Span mine0 = lane < p.n_seq ? span_of<TS>(p, lane) : Span{0, 0, 0, 0};
+    int64_t total = (int64_t) units_of(mine0) * HP;
+    for (int i = 32 + lane; i < p.n_seq; i += 32) total += (int64_t) units_of(span_of<TS>(p, i)) * HP;
+#pragma unroll
+    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(FULL, total, x);
+    int64_t per = total < 0x7FFFFFFF ? (int64_t) (((uint32_t) total + (uint32_t) p.n_work - 1u) / (uint32_t) p.n_work) : (total + p.n_work - 1) / p.n_work;
+    if (per < MIN_RUN) per = MIN_RUN;
+    const int64_t run0 = worker * per;
     Cursor<TS> at;                          // where the products are; `ld` below: where the loads are
+    at.rem = 0;
+    bool joint = false;                     // the CTA's warps all work on one pair: their partials are joined here
+    if (run0 < total)
     {
         int64_t before = 0;
-        int s0 = 0;
-        for (;; s0 += 32) {                 // the sequence that holds step run0: 32 sequences at a time
-            const int64_t n = s0 + lane < p.n_seq ? (int64_t) span_of<TS>(p, s0 + lane).n * HP : 0;
+        for (int s0 = 0;; s0 += 32) {
+            const Span s = s0 == 0 ? mine0 : s0 + lane < p.n_seq ? span_of<TS>(p, s0 + lane) : Span{0, 0, 0, 0};
+            const int64_t n = (int64_t) units_of(s) * HP;
             int64_t incl = n;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -185,28 +217,39 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
             const unsigned past = __ballot_sync(FULL, before + incl > run0);
             if (past) {
                 const int f = __ffs(past) - 1;
-                const int64_t start = before + __shfl_sync(FULL, incl - n, f);
+                const int64_t start = before + __shfl_sync(FULL, incl - n, f), rel = run0 - start;
                 at.seq = s0 + f;
-                at.s = span_of<TS>(p, at.seq);
-                at.hp = (int) ((run0 - start) / at.s.n);
-                at.st = (int) ((run0 - start) - (int64_t) at.hp * at.s.n);
+                at.s.lo = __shfl_sync(FULL, s.lo, f);
+                at.s.hi = __shfl_sync(FULL, s.hi, f);
+                at.s.first = __shfl_sync(FULL, s.first, f);
+                at.s.n = __shfl_sync(FULL, s.n, f);
+                const int u = at.s.n + OV;
+                at.hp = rel < 0x7FFFFFFF ? (int) ((uint32_t) rel / (uint32_t) u) : (int) (rel / u);
+                at.base = start + (int64_t) at.hp * u;
+                // step j lies at unit OV + j of its pair; the units before it go with its start
+                const int off = (int) (run0 - at.base);
+                at.st = off > OV ? off - OV : 0;
+                at.rem = (run0 + per < total ? per : total - run0) - (off < OV ? OV - off : 0);
+                const int64_t cta0 = (int64_t) blockIdx.x * W * per;
+                joint = cta0 >= at.base && cta0 + per > at.base + OV && cta0 + W * per <= at.base + u;
                 break;
             }
             before += __shfl_sync(FULL, incl, 31);
         }
     }
-    Cursor<TS> ld = at;
-    const int64_t steps = run1 - run0;
+    Cursor<TS> ld = at;                     // (no steps where the run has only units before a first step)
 
     // ---- loads: the row of token `lane` of the step at ld, as an element offset; < 0 where it is not live ----
-    int64_t ld_row = -1;
-    const uint16_t * ld_k = nullptr, * ld_v = nullptr;      // the KV head's rows
-    int64_t issued = 0;                                      // steps whose K and V went out
+    int64_t ld_row = -1, ld_first = 0;
+    unsigned ld_live = 0;                                    // live tokens of the step
+    int64_t ld_head = 0;                                     // the KV head's offset
+    constexpr unsigned ALL = TS == 32 ? FULL : 0xFFFFu;
+    const bool whole = p.c.page_tokens % TS == 0;            // a step lies in one page: its rows are a stride apart
     auto look_up = [&]() {
         ld_row = -1;
         const int tok = (ld.s.first + ld.st) * TS + (lane & (TS - 1));
         if (tok >= ld.s.lo && tok < ld.s.hi) {
-            const uint32_t g = (uint32_t) tok / (uint32_t) p.c.page_tokens;
+            const uint32_t g = p.page_shift >= 0 ? (uint32_t) tok >> p.page_shift : (uint32_t) tok / (uint32_t) p.c.page_tokens;
             const int64_t row = p.rows ? (int64_t) p.rows[ld.seq] : (int64_t) ld.seq;
             const uint32_t page = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables[row * p.c.table_stride + g] : SJKVARN_NO_BLOCK - 1u;
             if (page < p.c.n_pages)
@@ -214,88 +257,108 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
             else if (page != SJKVARN_NO_BLOCK)
                 atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
         }
-        const int64_t head = (int64_t) (ld.hp / p.tiles) * p.c.head_stride;
-        ld_k = static_cast<const uint16_t *>(p.c.k) + head;
-        ld_v = static_cast<const uint16_t *>(p.c.v) + head;
+        ld_head = (int64_t) (ld.hp / p.tiles) * p.c.head_stride;
     };
-    auto copy = [&](uint32_t dst, const uint16_t * base) {
+    auto copy = [&](uint32_t dst, const void * kv) {
         constexpr int CH = D / 8;                            // 16-byte words of a row
+        const uint16_t * base = static_cast<const uint16_t *>(kv) + ld_head;
+        if (whole && ld_live == ALL) {
+            base += ld_first;
 #pragma unroll
-        for (int i = 0; i < (TS * CH + 31) / 32; ++i) {
-            const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
-            const int64_t row = __shfl_sync(FULL, ld_row, r & (TS - 1));
-            if (TS * CH % 32 == 0 || w < TS * CH) cp16(dst + r * PITCH + c * 16, base + (row < 0 ? 0 : row) + c * 8, row >= 0);
+            for (int i = 0; i < TS * CH / 32; ++i) {
+                const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
+                cp16(dst + r * PITCH + c * 16, base + (int64_t) r * p.c.slot_stride + c * 8);
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < TS * CH / 32; ++i) {
+                const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
+                const int64_t row = __shfl_sync(FULL, ld_row, r);
+                cp16_or_zero(dst + r * PITCH + c * 16, base + (row < 0 ? 0 : row) + c * 8, row >= 0);
+            }
         }
     };
-    auto issue_k = [&]() {
-        if (issued < steps) {
-            const unsigned live = __ballot_sync(FULL, ld_row >= 0);
-            const int slot = (int) (issued % NST);
-            if (lane == 0) s_mask[slot] = TS == 32 ? live : live & 0xFFFFu;
-            copy(ring + slot * 2 * S::ENTRY, ld_k);
+    // tiles go out in the order K, V of the first step, K, V of the second, ..., each into the ring's next entry
+    int ld_entry = 0, ld_mask = 0;
+    auto issue = [&](bool v) {
+        if (ld.rem > 0) {
+            const uint32_t dst = ring + ld_entry * S::ENTRY;
+            if (!v) {
+                ld_live = __ballot_sync(FULL, ld_row >= 0) & ALL;
+                ld_first = __shfl_sync(FULL, ld_row, 0);
+                if (lane == 0) s_mask[ld_mask] = ld_live;
+                ld_mask = (ld_mask + 1) & 3;
+                copy(dst, p.c.k);
+            } else {
+                copy(dst, p.c.v);
+                ld.next(p, HP);
+                if (ld.rem > 0) look_up();
+            }
+            ld_entry = ld_entry + 1 == NE ? 0 : ld_entry + 1;
         }
         cp_commit();
     };
-    auto issue_v = [&]() {
-        if (issued < steps) {
-            copy(ring + (int) (issued % NST) * 2 * S::ENTRY + S::ENTRY, ld_v);
-            if (++issued < steps) { ld.next(p, HP); look_up(); }
-        }
-        cp_commit();
-    };
-    look_up();
-#pragma unroll
-    for (int i = 0; i < NST; ++i) { issue_k(); issue_v(); }
+    if (ld.rem > 0) look_up();
+#pragma unroll 1
+    for (int i = 0; i < NE; ++i) issue(i & 1);
 
     // ---- products ----
-    const int col = (lane & 3) * 2;                          // this lane's query heads of a tile of 8: col, col + 1
-    uint32_t qf[S::Q_REG ? KS * NQ * NT8 * 2 : 1];
+    // Column lane / 4 of a tile, as B operand: head and term. This lane's columns 2 (lane & 3) + j, as results: heads
+    // first + j, of which it has term `mine_t`; with several terms the lanes of a quad sum what they have of a head.
+    const int qcol = lane >> 2, qhead = T == 1 ? qcol : T == 2 ? qcol & 3 : qcol & 1, qterm = T == 1 ? 0 : T == 2 ? qcol >> 2 : qcol >> 1;
+    const int first = T == 1 ? (lane & 3) * 2 : T == 2 ? (lane & 1) * 2 : 0, mine_t = T == 1 ? 0 : T == 2 ? (lane & 3) >> 1 : lane & 3;
+    auto terms = [](float x) {                               // the sum over a head's terms
+        if (T == 2) x += __shfl_xor_sync(FULL, x, 2);
+        if (T == 3) { x += __shfl_xor_sync(FULL, x, 1); x += __shfl_xor_sync(FULL, x, 2); }
+        return x;
+    };
+    uint32_t qf[KS][NT8][2];
     float o[NT8][KS][4], m[NT8][2], l[NT8][2], sc[NT8][2];
-    for (int64_t i = 0; i < steps; ++i) {
-        if (i == 0 || at.st == 0) {                          // a (sequence, KV head, row tile) begins
-            const int kv = at.hp / p.tiles, h0 = kv * p.grp + (at.hp - kv * p.tiles) * R;
-            const int64_t qrow = (int64_t) at.seq * p.q.row_stride;
+    bool fresh = true, begun = false;                        // a pair comes next; its first step is in this run
+    int entry = 0;                                           // the ring's entry that comes next
+    for (int step = 0; at.rem > 0; step = (step + 1) & 3) {
+        if (fresh) {                                         // a (sequence, KV head, row tile) begins
+            fresh = false;
+            begun = at.st == 0;
+            const int kv = at.hp / p.tiles, r0 = (at.hp - kv * p.tiles) * R;
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
-                const int rel = h0 - kv * p.grp + 8 * n + (lane >> 2);
-                const bool on = rel < p.grp;
-                const int64_t src = qrow + (int64_t) (h0 + 8 * n + (lane >> 2)) * p.q.head_stride + (lane & 3) * 2;
-                float mul = 1.0f;
-                if constexpr (NQ > 1) {                      // the row to [1, 2) by an exact power of two
-                    float big = 0.0f;
+                const int rel = r0 + HT * n + qhead;
+                const bool on = rel < p.grp && qterm < T;
+                const int64_t src = (int64_t) at.seq * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
+                if constexpr (T == 1) {
+#pragma unroll
                     for (int k = 0; k < 2 * KS; ++k)
-                        if (on) big = fmaxf(big, fmaxf(fabsf(load1(p.q.p, src + 8 * k, p.q.type)), fabsf(load1(p.q.p, src + 8 * k + 1, p.q.type))));
+                        qf[k >> 1][n][k & 1] = on ? *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p.q.p) + src + 8 * k) : 0u;
+                    sc[n][0] = sc[n][1] = p.scale * 1.4426950408889634f;
+                } else {
+                    float2 x[2 * KS];
+                    if (p.q.type == SJK_F32) load_pairs<SJK_F32>(x, p.q.p, src, on);
+                    else if (p.q.type == SJK_F16) load_pairs<SJK_F16>(x, p.q.p, src, on);
+                    else load_pairs<SJK_BF16>(x, p.q.p, src, on);
+                    float big = 0.0f;                        // the row to [1, 2) by an exact power of two
+#pragma unroll
+                    for (int k = 0; k < 2 * KS; ++k) big = fmaxf(big, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
                     const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 0;
-                    mul = ldexpf(1.0f, e < -120 ? 120 : e > 120 ? -120 : -e);
-                    const float c0 = __shfl_sync(FULL, mul, (col) * 4), c1 = __shfl_sync(FULL, mul, (col + 1) * 4);
-                    sc[n][0] = p.scale * 1.4426950408889634f / c0;
-                    sc[n][1] = p.scale * 1.4426950408889634f / c1;
-                } else {
-                    sc[n][0] = sc[n][1] = p.scale * 1.4426950408889634f;
-                }
+                    const float mul = ldexpf(1.0f, e < -120 ? 120 : e > 120 ? -120 : -e);
 #pragma unroll
-                for (int k = 0; k < 2 * KS; ++k) {
-                    float2 x = make_float2(0.0f, 0.0f);
-                    uint32_t w[NQ];
-                    if constexpr (NQ == 1) {
-                        w[0] = on ? *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p.q.p) + src + 8 * k) : 0u;
-                    } else {
-                        if (on) x = make_float2(load1(p.q.p, src + 8 * k, p.q.type) * mul, load1(p.q.p, src + 8 * k + 1, p.q.type) * mul);
+                    for (int j = 0; j < 2; ++j) sc[n][j] = p.scale * 1.4426950408889634f / __shfl_sync(FULL, mul, (first + j) * 4);
 #pragma unroll
-                        for (int t = 0; t < NQ; ++t) {
-                            w[t] = pack2<S::TYPE>(x.x, x.y);
-                            const float2 y = widen2<S::TYPE>(w[t]);
-                            x.x -= y.x;
-                            x.y -= y.y;
+                    for (int k = 0; k < 2 * KS; ++k) {
+                        float a = x[k].x * mul, b = x[k].y * mul;
+                        uint32_t w = pack2<S::TYPE>(a, b);
+#pragma unroll
+                        for (int t = 1; t < T; ++t) {        // the column's term: what is left after those before it
+                            const float2 z = widen2<S::TYPE>(w);
+                            a -= z.x;
+                            b -= z.y;
+                            const uint32_t v = pack2<S::TYPE>(a, b);
+                            if (qterm >= t) w = v;
+                            else { a += z.x; b += z.y; }
                         }
-                    }
-#pragma unroll
-                    for (int t = 0; t < NQ; ++t) {
-                        if constexpr (S::Q_REG) qf[((k >> 1) * NQ + t) * NT8 * 2 + n * 2 + (k & 1)] = w[t];
-                        else
-                            *reinterpret_cast<uint32_t *>(mine + 2 * NST * S::ENTRY + (t * NT8 * 8 + n * 8 + (lane >> 2)) * PITCH + k * 16 + (lane & 3) * 4) = w[t];
+                        qf[k >> 1][n][k & 1] = w;
                     }
                 }
                 m[n][0] = m[n][1] = -INFINITY;
@@ -303,75 +366,69 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
 #pragma unroll
                 for (int k = 0; k < KS; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.0f;
             }
-            if constexpr (!S::Q_REG) __syncwarp();
         }
-        const int slot = (int) (i % NST);
-        const uint32_t kb = ring + slot * 2 * S::ENTRY, vb = kb + S::ENTRY;
+        const uint32_t kb = ring + entry * S::ENTRY;
+        entry = entry + 1 == NE ? 0 : entry + 1;
+        const uint32_t vb = ring + entry * S::ENTRY;
+        entry = entry + 1 == NE ? 0 : entry + 1;
 
         // S^T = K Q^T
-        cp_wait<2 * NST - 1>();
+        cp_wait<NE - 1>();
         __syncwarp();
         float s[TM][NT8][4];
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm) {
-            float s2[NT8][4];                                // two chains, so that products overlap
+            constexpr int CH = T > 1 && (D < 256 || NT8 == 1) ? 4 : 2;       // several chains: products overlap, sums stay short
+            float c[CH][NT8][4];
 #pragma unroll
-            for (int n = 0; n < NT8; ++n)
+            for (int x = 0; x < CH; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[tm][n][e] = s2[n][e] = 0.0f;
+                for (int n = 0; n < NT8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[x][n][e] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint32_t a[4];
                 ldsm4(a, kb + (tm * 16 + (lane & 15)) * PITCH + k * 32 + (lane >> 4) * 16);
 #pragma unroll
-                for (int t = 0; t < NQ; ++t) {
-#pragma unroll
-                    for (int n = 0; n < NT8; ++n) {
-                        uint32_t b0, b1;
-                        if constexpr (S::Q_REG) {
-                            b0 = qf[(k * NQ + t) * NT8 * 2 + n * 2];
-                            b1 = qf[(k * NQ + t) * NT8 * 2 + n * 2 + 1];
-                        } else {
-                            const uint8_t * qs = mine + 2 * NST * S::ENTRY + (t * NT8 * 8 + n * 8 + (lane >> 2)) * PITCH + k * 32 + (lane & 3) * 4;
-                            b0 = *reinterpret_cast<const uint32_t *>(qs);
-                            b1 = *reinterpret_cast<const uint32_t *>(qs + 16);
-                        }
-                        if ((k + t) & 1) mma<S::TYPE>(s2[n], a, b0, b1);
-                        else mma<S::TYPE>(s[tm][n], a, b0, b1);
-                    }
-                }
+                for (int n = 0; n < NT8; ++n) mma<S::TYPE>(c[k % CH][n], a, qf[k][n][0], qf[k][n][1]);
             }
 #pragma unroll
             for (int n = 0; n < NT8; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[tm][n][e] += s2[n][e];
+                for (int e = 0; e < 4; ++e)
+                    s[tm][n][e] = terms(CH == 2 ? c[0][n][e] + c[1][n][e] : (c[0][n][e] + c[1][n][e]) + (c[CH - 2][n][e] + c[CH - 1][n][e]));
         }
-        const unsigned live = s_mask[slot];
+        const unsigned live = s_mask[step];
         __syncwarp();
-        issue_k();
+        issue(NE & 1);
 
-        // softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16, heads col and col + 1
-        uint32_t pb[TM][NP][NT8][2];
+        // softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16 of its two heads
+        uint32_t pb[TM][NT8][2];
 #pragma unroll
         for (int n = 0; n < NT8; ++n) {
-            float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int tok = tm * 16 + (lane >> 2) + (e >> 1) * 8;
-                    float x = s[tm][n][e] * sc[n][e & 1];
-                    if (!((live >> tok) & 1u)) x = -INFINITY;
-                    s[tm][n][e] = x;
-                    top[e & 1] = fmaxf(top[e & 1], x);
-                }
+                for (int e = 0; e < 4; ++e) s[tm][n][e] *= sc[n][e & 1];
+            if (live != ALL) {
+#pragma unroll
+                for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (!((live >> (tm * 16 + (lane >> 2) + (e >> 1) * 8)) & 1u)) s[tm][n][e] = -INFINITY;
+            }
+            float top[2] = {m[n][0], m[n][1]};
+#pragma unroll
+            for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[tm][n][e]);
             float use[2], fix[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 4));
                 top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 8));
                 top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 16));
-                top[j] = fmaxf(top[j], m[n][j]);
                 use[j] = top[j] == -INFINITY ? 0.0f : top[j];
                 fix[j] = ex2(m[n][j] - use[j]);
             }
@@ -393,18 +450,24 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float x = s[tm][n][2 * h], y = s[tm][n][2 * h + 1];
+                    uint32_t w = pack2<S::TYPE>(x, y);
 #pragma unroll
-                    for (int t = 0; t < NP; ++t) {
-                        const uint32_t w = pack2<S::TYPE>(x, y);
-                        pb[tm][t][n][h] = transpose8(w);
-                        if (t + 1 < NP) { const float2 f = widen2<S::TYPE>(w); x -= f.x; y -= f.y; }
+                    for (int t = 1; t < T; ++t) {
+                        const float2 f = widen2<S::TYPE>(w);
+                        x -= f.x;
+                        y -= f.y;
+                        const uint32_t v = pack2<S::TYPE>(x, y);
+                        if (mine_t >= t) w = v;
+                        else { x += f.x; y += f.y; }
                     }
+                    if (T == 3 && mine_t == 3) w = 0u;
+                    pb[tm][n][h] = transpose8(w);
                 }
             }
         }
 
         // O^T += V^T P
-        cp_wait<2 * NST - 1>();
+        cp_wait<NE - 1>();
         __syncwarp();
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm)
@@ -413,16 +476,29 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
                 uint32_t a[4];
                 ldsm4t(a, vb + (tm * 16 + (lane & 7) + (lane >> 4) * 8) * PITCH + k * 32 + ((lane >> 3) & 1) * 16);
 #pragma unroll
-                for (int t = 0; t < NP; ++t)
+                for (int n = 0; n < NT8; ++n) {
+                    if constexpr (T == 1) {
+                        mma<S::TYPE>(o[n][k], a, pb[tm][n][0], pb[tm][n][1]);
+                    } else {                                 // the step's sum apart, joined by a rounded addition
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma<S::TYPE>(c, a, pb[tm][n][0], pb[tm][n][1]);
 #pragma unroll
-                    for (int n = 0; n < NT8; ++n) mma<S::TYPE>(o[n][k], a, pb[tm][t][n][0], pb[tm][t][n][1]);
+                        for (int e = 0; e < 4; ++e) o[n][k][e] += c[e];
+                    }
+                }
             }
         __syncwarp();
-        issue_v();
+        issue(!(NE & 1));
 
         // the pair's last step of this run: its output, or its partial
-        if (at.st + 1 == at.s.n || i + 1 == steps) {
-            const bool begun = i >= at.st, ended = at.st + 1 == at.s.n;     // begun: its first step is in this run
+        if (at.st + 1 == at.s.n || at.rem == 1) {
+            const bool ended = at.st + 1 == at.s.n;
+            fresh = true;
+            if (begun && lane == 0) {
+                const int last = ended ? worker : (int) ((at.base + at.s.n + OV - 1) / per);
+                if (p.by_pair) p.split[at.seq * HP + at.hp] = make_int4(ended ? -1 : at.seq, at.hp, worker, last);
+                else if (!ended) p.split[worker] = make_int4(at.seq, at.hp, worker, last);
+            }
             const int kv = at.hp / p.tiles, r0 = (at.hp - kv * p.tiles) * R;
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
@@ -434,22 +510,24 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const int r = 8 * n + col + j;
+                    const int r = HT * n + first + j;
+                    if constexpr (T > 1) {
+#pragma unroll
+                        for (int k = 0; k < KS; ++k) { o[n][k][j] = terms(o[n][k][j]); o[n][k][2 + j] = terms(o[n][k][2 + j]); }
+                        if (mine_t) continue;
+                    }
                     if (r0 + r >= p.grp) continue;
+                    if (joint) continue;                     // written below
                     if (begun && ended) {
                         const float inv = l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j];
                         const int64_t dst = (int64_t) at.seq * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride + (lane >> 2);
-#pragma unroll
-                        for (int k = 0; k < KS; ++k) {
-                            store1(p.out.p, dst + 16 * k, p.out.type, o[n][k][j] * inv);
-                            store1(p.out.p, dst + 16 * k + 8, p.out.type, o[n][k][2 + j] * inv);
-                        }
+                        if (p.out.type == SJK_F32) store_channels<SJK_F32>(p.out.p, dst, o[n], j, inv);
+                        else if (p.out.type == SJK_F16) store_channels<SJK_F16>(p.out.p, dst, o[n], j, inv);
+                        else store_channels<SJK_BF16>(p.out.p, dst, o[n], j, inv);
                     } else {
-                        const int64_t slot_row = ((int64_t) worker * 2 + (begun ? 1 : 0)) * R + r;
-                        float * dst = p.part + slot_row * D + (lane >> 2);
-#pragma unroll
-                        for (int k = 0; k < KS; ++k) { dst[16 * k] = o[n][k][j]; dst[16 * k + 8] = o[n][k][2 + j]; }
-                        if (lane < 4) { p.ml[slot_row * 2] = m[n][j]; p.ml[slot_row * 2 + 1] = l[n][j]; }
+                        const int64_t slot = ((int64_t) worker * 2 + (begun ? 1 : 0)) * R + r;
+                        store_channels<SJK_F32>(p.part, slot * D + (lane >> 2), o[n], j, 1.0f);
+                        if (lane < 4) *reinterpret_cast<float2 *>(p.ml + slot * 2) = make_float2(m[n][j], l[n][j]);
                     }
                 }
             }
@@ -457,110 +535,170 @@ __global__ void __launch_bounds__(32 * W) kv16_attend_kernel(const __grid_consta
         at.next(p, HP);
     }
     cp_wait<0>();
+
+    // The CTA's partials of one pair as the first warp's, in the warps' order; the others' slots are left without weight.
+    if (!joint) return;                     // the same for all warps: each looks at the CTA's whole run
+    __syncthreads();                        // nothing reads the rings any more
+    float * s_o = reinterpret_cast<float *>(smem);          // [W][R][D]
+    float2 * s_ml = reinterpret_cast<float2 *>(s_o + W * R * D);
+    static_assert(W * R * (D + 2) * 4 <= S::CTA_BYTES, "partials in the rings' place");
+    if (lane < 4 && mine_t == 0)
+#pragma unroll
+        for (int n = 0; n < NT8; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) s_ml[warp * R + HT * n + first + j] = make_float2(m[n][j], l[n][j]);
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NT8; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = HT * n + first + j;
+            float top = -INFINITY;
+            for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w * R + r].x);
+            if (mine_t == 0) store_channels<SJK_F32>(s_o, (warp * R + r) * D + (lane >> 2), o[n], j, ex2(m[n][j] - (top == -INFINITY ? 0.0f : top)));
+        }
+    __syncthreads();
+    const bool first_begun = __syncthreads_or(warp == 0 && begun);
+    const int64_t slot = ((int64_t) blockIdx.x * W * 2 + (first_begun ? 1 : 0)) * R;
+    for (int i = threadIdx.x; i < R * D; i += 32 * W) {
+        float x = 0.0f;
+        for (int w = 0; w < W; ++w) x += s_o[w * R * D + i];
+        p.part[slot * D + i] = x;
+    }
+    for (int i = threadIdx.x; i < W * R; i += 32 * W) {
+        const int w = i / R, r = i - w * R;
+        if (w) { *reinterpret_cast<float2 *>(p.ml + ((int64_t) (blockIdx.x * W + w) * 2 * R + r) * 2) = make_float2(-INFINITY, 0.0f); continue; }
+        float top = -INFINITY, sum = 0.0f;
+        for (int v = 0; v < W; ++v) top = fmaxf(top, s_ml[v * R + r].x);
+        for (int v = 0; v < W; ++v) sum = fmaf(s_ml[v * R + r].y, ex2(s_ml[v * R + r].x - (top == -INFINITY ? 0.0f : top)), sum);
+        *reinterpret_cast<float2 *>(p.ml + (slot + r) * 2) = make_float2(top, sum);
+    }
 }
 
-// Joins the slots of every (sequence, query head) that was split, in list order; G warps share one.
-template <int TS>
-__global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__ Params p, int D, int R, int G) {
-    extern __shared__ float s_acc[];        // [8 / G][G][D + 2]
+// Joins the slots of a split pair, in list order. grid.x: entries of p.split; G warps of the CTA's 8 share a query head
+// (grid.y CTAs then take the heads of an entry in turn).
+template <int D>
+__global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__ Params p, int R, int G) {
+    constexpr int NV = (D / 4 + 31) / 32;   // 16-byte words of a lane
+    __shared__ float s_acc[8 * (D + 4)];
     pdl_wait();
     pdl_release();
+    const int4 e = p.split[blockIdx.x];
+    if (e.x < 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % G;
-    const int n_head = p.q.n_head;
-    const int64_t item = (int64_t) blockIdx.x * (8 / G) + warp / G;
-    const bool on = item < (int64_t) p.n_seq * n_head;
-    const int seq = on ? (int) (item / n_head) : 0, h = on ? (int) (item - (int64_t) seq * n_head) : 0;
-    const int HP = p.c.n_head_kv * p.tiles;
-    const int64_t total = steps_before<TS>(p, p.n_seq, lane) * HP, per = run_steps(total, p.n_work);
-    const Span s = span_of<TS>(p, seq);
-    const int kv = h / p.grp, rel = h - kv * p.grp, tile = rel / R, r = rel - tile * R;
-    const int64_t a = steps_before<TS>(p, seq, lane) * HP + (int64_t) (kv * p.tiles + tile) * s.n;
-    const int64_t first = s.n ? a / per : 0, last = s.n ? (a + s.n - 1) / per : 0;
-    const bool join = on && s.n && first != last, zero = on && !s.n;
-    const int64_t dst = (int64_t) seq * p.out.row_stride + (int64_t) h * p.out.head_stride;
-    if (zero && sub == 0)
-        for (int d = lane; d < D; d += 32) store1(p.out.p, dst + d, p.out.type, 0.0f);
-    float top = -INFINITY, sum = 0.0f, o[8];
+    const int kv = e.y / p.tiles, r0 = (e.y - kv * p.tiles) * R, nr = p.grp - r0 < R ? p.grp - r0 : R;
+    const int n = e.w - e.z + 1, lo = (int) ((int64_t) n * sub / G), hi = (int) ((int64_t) n * (sub + 1) / G);
+    for (int r = blockIdx.y * (8 / G) + warp / G; r < nr; r += gridDim.y * (8 / G)) {
+        float top = -INFINITY, sum = 0.0f;
+        float4 o[NV];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) o[k] = 0.0f;
-    if (join) {
-        const int64_t n = last - first + 1, lo = first + n * sub / G, hi = first + n * (sub + 1) / G;
-        for (int64_t w = lo + lane; w < hi; w += 32) top = fmaxf(top, p.ml[((w * 2 + (w == first ? 1 : 0)) * R + r) * 2]);
+        for (int v = 0; v < NV; ++v) o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int w0 = lo; w0 < hi; w0 += 32) {
+            // slot 1 of the first worker, slot 0 of the others
+            const int w = w0 + lane;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (w < hi) ml = *reinterpret_cast<const float2 *>(p.ml + (((int64_t) (e.z + w) * 2 + (w == 0 ? 1 : 0)) * R + r) * 2);
+            float t = ml.x;
 #pragma unroll
-        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, x));
-        const float use = top == -INFINITY ? 0.0f : top;
-#pragma unroll 4
-        for (int64_t w = lo; w < hi; ++w) {
-            const int64_t slot = (w * 2 + (w == first ? 1 : 0)) * R + r;
-            const float2 ml = *reinterpret_cast<const float2 *>(p.ml + slot * 2);
-            const float f = ex2(ml.x - use);
-            sum = fmaf(ml.y, f, sum);
+            for (int x = 16; x; x >>= 1) t = fmaxf(t, __shfl_xor_sync(FULL, t, x));
+            t = fmaxf(t, top);
+            const float use = t == -INFINITY ? 0.0f : t, fix = ex2(top - use), f = ex2(ml.x - use);
+            top = t;
+            sum = sum * fix + (w < hi ? ml.y * f : 0.0f);    // a lane's own share; joined below
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (32 * k + lane < D) o[k] = fmaf(p.part[slot * D + 32 * k + lane], f, o[k]);
-        }
-    }
-    if (G > 1) {
-        float * acc = s_acc + (size_t) warp * (D + 2);
-        if (lane == 0) { acc[0] = top; acc[1] = sum; }
+            for (int v = 0; v < NV; ++v) { o[v].x *= fix; o[v].y *= fix; o[v].z *= fix; o[v].w *= fix; }
+            for (unsigned some = __ballot_sync(FULL, f != 0.0f); some;) {   // four parts with a weight at a time
+                float g[4];
+                float4 x[4][NV];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (32 * k + lane < D) acc[2 + 32 * k + lane] = o[k];
-        __syncthreads();
-        if (sub == 0 && join) {
-            const float * all = s_acc + (size_t) warp * (D + 2);
-            for (int g = 1; g < G; ++g) top = fmaxf(top, all[(size_t) g * (D + 2)]);
-            const float use = top == -INFINITY ? 0.0f : top;
-            sum = 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    const int j = some ? __ffs(some) - 1 : 0;
+                    g[i] = __shfl_sync(FULL, f, j);
+                    if (!some) g[i] = 0.0f;
+                    some &= some - 1u;
+                    const float4 * src = reinterpret_cast<const float4 *>(p.part + (((int64_t) (e.z + w0 + j) * 2 + (w0 + j == 0 ? 1 : 0)) * R + r) * D);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] = 0.0f;
-            for (int g = 0; g < G; ++g) {
-                const float * x = all + (size_t) g * (D + 2);
-                const float f = ex2(x[0] - use);
-                sum = fmaf(x[1], f, sum);
+                    for (int v = 0; v < NV; ++v) x[i][v] = g[i] != 0.0f && 32 * v + lane < D / 4 ? src[32 * v + lane] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (32 * k + lane < D) o[k] = fmaf(x[2 + 32 * k + lane], f, o[k]);
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) {
+                        o[v].x = fmaf(x[i][v].x, g[i], o[v].x); o[v].y = fmaf(x[i][v].y, g[i], o[v].y);
+                        o[v].z = fmaf(x[i][v].z, g[i], o[v].z); o[v].w = fmaf(x[i][v].w, g[i], o[v].w);
+                    }
             }
         }
-    }
-    if (join && sub == 0) {
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (32 * k + lane < D) store1(p.out.p, dst + 32 * k + lane, p.out.type, o[k] * inv);
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+        if (G > 1) {
+            float * acc = s_acc + warp * (D + 4);
+            if (lane == 0) { acc[0] = top; acc[1] = sum; }
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (32 * v + lane < D / 4) *reinterpret_cast<float4 *>(acc + 4 + 4 * (32 * v + lane)) = o[v];
+            __syncthreads();
+            if (sub == 0) {
+                for (int g = 1; g < G; ++g) top = fmaxf(top, acc[g * (D + 4)]);
+                const float use = top == -INFINITY ? 0.0f : top;
+                sum = 0.0f;
+#pragma unroll
+                for (int v = 0; v < NV; ++v) o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                for (int g = 0; g < G; ++g) {
+                    const float * y = acc + g * (D + 4);
+                    const float f = ex2(y[0] - use);
+                    sum = fmaf(y[1], f, sum);
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+                        if (32 * v + lane < D / 4) {
+                            const float4 x = *reinterpret_cast<const float4 *>(y + 4 + 4 * (32 * v + lane));
+                            o[v].x = fmaf(x.x, f, o[v].x); o[v].y = fmaf(x.y, f, o[v].y);
+                            o[v].z = fmaf(x.z, f, o[v].z); o[v].w = fmaf(x.w, f, o[v].w);
+                        }
+                }
+            }
+            __syncthreads();
+        }
+        if (sub == 0) {
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t dst = (int64_t) e.x * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+                if (32 * v + lane < D / 4) {
+                    const int d = 4 * (32 * v + lane);
+                    store1(p.out.p, dst + d, p.out.type, o[v].x * inv);
+                    store1(p.out.p, dst + d + 1, p.out.type, o[v].y * inv);
+                    store1(p.out.p, dst + d + 2, p.out.type, o[v].z * inv);
+                    store1(p.out.p, dst + d + 3, p.out.type, o[v].w * inv);
+                }
+        }
     }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------
 
-struct Plan { int ctas, R, tiles; size_t part, ml; };       // part, ml: floats
-
-template <typename S>
-int ctas_per_sm() { return S::CTA_BYTES <= 75 * 1024 ? 3 : S::CTA_BYTES <= 113 * 1024 ? 2 : 1; }
+struct Plan { int work, R, nt8, tiles; size_t part, ml, bytes; };    // part, ml: floats
 
 template <typename S>
 int run(const Params & p0, const Plan & pl, sjk_stream st) {
     static_assert(S::CTA_BYTES <= 227 * 1024, "shared memory of a CTA");
     Params p = p0;
     if (sjk_check(cudaFuncSetAttribute(kv16_attend_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::CTA_BYTES))) return SJK_ERR_DEVICE;
-    const int rc = launch(kv16_attend_kernel<S>, dim3((unsigned) pl.ctas), dim3(32 * W), S::CTA_BYTES, st, p);
+    const int rc = launch(kv16_attend_kernel<S>, dim3(148), dim3(32 * S::W), S::CTA_BYTES, st, p);
     if (rc) return rc;
-    const int64_t items = (int64_t) p.n_seq * p.q.n_head;
-    const int G = items <= 148 * 8 ? 8 : 1;                 // few outputs: a CTA each
-    const int64_t ctas = (items + 8 / G - 1) / (8 / G);
-    return launch(kv16_merge_kernel<S::TS>, dim3((unsigned) ctas), dim3(256), G > 1 ? (size_t) 8 * (S::D + 2) * sizeof(float) : 0, st, p, S::D, pl.R, G);
+    // few pairs: many slots each, so a CTA per query head; many: two or three slots each, a warp per query head
+    const int64_t pairs = (int64_t) p.n_seq * p.c.n_head_kv * p.tiles;
+    const bool few = pairs * 8 <= p.n_work;
+    const int rows = p.grp < pl.R ? p.grp : pl.R;
+    return launch(kv16_merge_kernel<S::D>, dim3((unsigned) (p.by_pair ? pairs : p.n_work), few ? (unsigned) rows : 1u), dim3(256), 0, st, p, pl.R, few ? 8 : 1);
 }
 
-template <typename S>
-int ctas_of() { return 148 * ctas_per_sm<S>(); }
-
-// f(Shape) for the call's types and sizes
+// f(Shape) for the call's types and sizes: nt8 1 or 2 tiles of columns in one pass over K and V
 template <int TYPE, int D, typename F>
 int with_terms(bool split, int nt8, F && f) {
-    constexpr int NQ = TYPE == SJK_F16 ? 2 : 3;
-    if (!split) return nt8 == 1 ? f(Shape<TYPE, D, 1, 1, 1>()) : f(Shape<TYPE, D, 1, 1, 2>());
-    return nt8 == 1 ? f(Shape<TYPE, D, NQ, 2, 1>()) : f(Shape<TYPE, D, NQ, 2, 2>());
+    constexpr int T = TYPE == SJK_F16 ? 2 : 3;
+    if (!split) return nt8 == 1 ? f(Shape<TYPE, D, 1, 1>()) : f(Shape<TYPE, D, 1, 2>());
+    return nt8 == 1 ? f(Shape<TYPE, D, T, 1>()) : f(Shape<TYPE, D, T, 2>());
 }
 template <int TYPE, typename F>
 int with_dim(int D, bool split, int nt8, F && f) {
@@ -578,13 +716,14 @@ int with_shape(int type, int D, bool split, int nt8, F && f) {
 }
 
 int plan_of(const sjk_kv16 * c, int n_head, bool split, Plan * pl) {
-    const int grp = n_head / c->n_head_kv, nt8 = grp <= 8 ? 1 : 2;
-    pl->R = 8 * nt8;
-    pl->tiles = (grp + pl->R - 1) / pl->R;
-    const int rc = with_shape(c->type, c->head_dim, split, nt8, [&](auto s) { pl->ctas = ctas_of<decltype(s)>(); return 0; });
+    const int grp = n_head / c->n_head_kv, ht = !split ? 8 : c->type == SJK_F16 ? 4 : 2;
+    pl->nt8 = grp <= ht ? 1 : 2;
+    const int rc = with_shape(c->type, c->head_dim, split, pl->nt8, [&](auto s) { pl->work = 148 * decltype(s)::W; pl->R = decltype(s)::R; return 0; });
     if (rc) return rc;
-    pl->part = (size_t) pl->ctas * W * 2 * pl->R * c->head_dim;
-    pl->ml = (size_t) pl->ctas * W * 2 * pl->R * 2;
+    pl->tiles = (grp + pl->R - 1) / pl->R;
+    pl->part = (size_t) pl->work * 2 * pl->R * c->head_dim;
+    pl->ml = (size_t) pl->work * 2 * pl->R * 2;
+    pl->bytes = (pl->part + pl->ml) * sizeof(float) + (size_t) pl->work * sizeof(int4);
     return 0;
 }
 
@@ -596,8 +735,7 @@ extern "C" size_t sjk_kv16_attend_scratch_bytes(const sjk_kv16 * c, int n_head) 
     for (int split = 0; split < 2; ++split) {
         Plan pl;
         if (plan_of(c, n_head, split != 0, &pl)) return 0;
-        const size_t n = (pl.part + pl.ml) * sizeof(float);
-        if (n > most) most = n;
+        if (pl.bytes > most) most = pl.bytes;
     }
     return most;
 }
@@ -618,16 +756,21 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     const int rc = plan_of(c, q->n_head, split, &pl);
     if (rc) return rc;
     if (n_seq == 0) return 0;
-    if (!scratch || !aligned(scratch, 16) || scratch_bytes < (pl.part + pl.ml) * sizeof(float)) return SJKVARN_ERR_BUFFER;
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < pl.bytes) return SJKVARN_ERR_BUFFER;
     Params p = {};
     p.c = *c; p.q = *q; p.out = *out;
     p.len = len; p.rows = rows; p.n_seq = n_seq;
     p.grp = q->n_head / c->n_head_kv; p.tiles = pl.tiles;
     p.window = window; p.scale = scale;
-    p.n_work = pl.ctas * W;
+    p.page_shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (c->page_tokens == 1 << b) p.page_shift = b;
+    p.n_work = pl.work;
     p.part = static_cast<float *>(scratch);
     p.ml = p.part + pl.part;
-    return with_shape(c->type, c->head_dim, split, pl.R / 8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
+    p.split = reinterpret_cast<int4 *>(p.ml + pl.ml);
+    p.by_pair = (int64_t) n_seq * c->n_head_kv * pl.tiles <= p.n_work;
+    return with_shape(c->type, c->head_dim, split, pl.nt8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
 }
 
 int sjk_kv16_status_take(void) {
