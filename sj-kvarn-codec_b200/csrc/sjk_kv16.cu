@@ -3,10 +3,11 @@
 //
 // Bound: HBM, every live K and V row once (4 D bytes per position and KV head for 4 D grp flops: at most 16 flops per
 // byte for 16 query heads, far under the tensor cores' ridge). So the work is to keep loads in flight:
-//  - A warp is a worker of its own. The (sequence, KV head, step of TS tokens) triples of a call form one list, cut
+//  - A warp is a worker of its own. Per KV head, the (sequence, step of TS tokens) pairs of a call form one list, cut
 //    into equal runs, one per warp of a grid that fills the GPU; lengths are read from device memory, so every warp
-//    finds its run with a scan over them. A (sequence, KV head) weighs OV units beside its steps, for what its start
-//    and its output cost. Ragged batches balance by construction and no CTA barrier exists.
+//    finds its run with a scan over them. A sequence weighs OV units beside its steps, for what its start and its
+//    output cost. Ragged batches balance by construction, no CTA barrier paces the work, and the workers of all heads
+//    are at the same tokens at the same time, whose rows lie side by side in memory.
 //  - A warp streams its steps through a ring in shared memory with cp.async, NE tiles ahead and across the ends of
 //    sequences; positions that are not live are filled with zeros, not read.
 //  - The query heads of a KV head are the N = 8 columns of mma.m16n8k16: S^T = K Q^T with 16 tokens as rows, and
@@ -43,8 +44,9 @@ struct Params {
     const int32_t * len, * rows;
     int n_seq, grp, tiles;                  // tiles: row tiles of a KV head (8 NT8 query heads each)
     int window, page_shift;                 // page_shift: log2 of the page's tokens, -1 where it is no power of two
+    uint32_t slot_stride;
     float scale;
-    int n_work;                             // workers
+    int n_work, wph;                        // workers; workers of a (KV head, row tile), 0: all share one list
     float * part;                           // [n_work][2][R][D]
     float * ml;                             // [n_work][2][R][2]
     int4 * split;                           // by pair (or, with more pairs than workers, by worker): sequence (-1: not
@@ -71,27 +73,41 @@ SJK_DEV Span span_of(const Params & p, int seq) {
     return s;
 }
 
-// units of a sequence's (KV head, row tile): its steps behind OV that stand for its start and end
-SJK_DEV int units_of(const Span & s) { return s.n ? s.n + OV : 0; }
+// units of a sequence in a (KV head, row tile)'s list: its steps behind OV that stand for its start and end
+SJK_DEV uint32_t units_of(const Span & s) { return s.n ? (uint32_t) (s.n + OV) : 0u; }
 
 template <int TS>
-struct Cursor {                             // a place in the list
+struct Cursor {                             // a place in the lists
     int seq, hp, st;                        // sequence, (KV head, row tile), step
-    int64_t rem;                            // units of the run from this step on; <= 0: the run is done
-    int64_t base;                           // unit at which the pair begins
+    int rem;                                // units of the run from this step on; <= 0: the run is done
+    uint32_t base;                          // unit of its list at which the sequence begins
     Span s;
-    SJK_DEV void next(const Params & p, int HP) {
+    SJK_DEV bool next(const Params & p) {   // true: to another pair
         --rem;
-        if (++st < s.n) return;
+        if (++st < s.n) return false;
         st = 0;
         rem -= OV;
-        base += s.n + OV;
-        if (++hp < HP) return;
-        hp = 0;
-        if (rem <= 0) return;
-        do ++seq; while (seq < p.n_seq && (s = span_of<TS>(p, seq)).n == 0);
+        base += units_of(s);
+        if (rem <= 0) return true;
+        do {
+            if (++seq == p.n_seq) { seq = 0; ++hp; base = 0u; }
+            s = span_of<TS>(p, seq);
+        } while (s.n == 0);
+        return true;
     }
 };
+
+// exclusive prefix sum over the warp's lanes; *total gets the sum
+SJK_DEV uint32_t warp_scan(uint32_t x, int lane, uint32_t * total) {
+    uint32_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl += y;
+    }
+    *total = __shfl_sync(FULL, incl, 31);
+    return incl - x;
+}
 
 SJK_DEV uint32_t smem_addr(const void * p) { return (uint32_t) __cvta_generic_to_shared(p); }
 SJK_DEV void cp16(uint32_t dst, const void * src) {
@@ -179,102 +195,159 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
     pdl_wait();
     pdl_release();
 
-    // the worker's run of the list: 32 sequences at a time, first all units, then the sequence where the run begins
-    const int worker = blockIdx.x * W + warp;
+    // The worker's run: units of all sequences (a lane sums a block of them), then the block and the sequence at which
+    // the run begins.
     const int HP = p.c.n_head_kv * p.tiles;
-    for (int seq = worker; seq < p.n_seq; seq += p.n_work) {            // sequences without a live position
-        if (span_of<TS>(p, seq).n) continue;
-        for (int h = 0; h < p.out.n_head; ++h)
-            for (int d = lane; d < D; d += 32)
-                store1(p.out.p, (int64_t) seq * p.out.row_stride + (int64_t) h * p.out.head_stride + d, p.out.type, 0.0f);
-        if (p.by_pair)
-            for (int i = lane; i < HP; i += 32) p.split[seq * HP + i] = make_int4(-1, 0, 0, 0);
+    const int block = (p.n_seq + 31) / 32;
+    Span s0 = lane < p.n_seq ? span_of<TS>(p, lane) : Span{0, 0, 0, 0};
+    uint32_t mine_u = block == 1 ? units_of(s0) : 0u, list;             // list: units of one (KV head, row tile)
+    if (block > 1) {
+#pragma unroll 8
+        for (int i = 0; i < block; ++i) {
+            const int q = lane * block + i;
+            if (q < p.n_seq) mine_u += units_of(span_of<TS>(p, q));
+        }
     }
-    if (!p.by_pair && lane == 0) p.split[worker] = make_int4(-1, 0, 0, 0);
-    const Span mine0 = lane < p.n_seq ? span_of<TS>(p, lane) : Span{0, 0, 0, 0};
-    int64_t total = (int64_t) units_of(mine0) * HP;
-    for (int i = 32 + lane; i < p.n_seq; i += 32) total += (int64_t) units_of(span_of<TS>(p, i)) * HP;
-#pragma unroll
-    for (int x = 16; x; x >>= 1) total += __shfl_xor_sync(FULL, total, x);
-    int64_t per = total < 0x7FFFFFFF ? (int64_t) (((uint32_t) total + (uint32_t) p.n_work - 1u) / (uint32_t) p.n_work) : (total + p.n_work - 1) / p.n_work;
-    if (per < MIN_RUN) per = MIN_RUN;
-    const int64_t run0 = worker * per;
+    const uint32_t mine_0 = warp_scan(mine_u, lane, &list);
     Cursor<TS> at;                          // where the products are; `ld` below: where the loads are
     at.rem = 0;
-    bool joint = false;                     // the CTA's warps all work on one pair: their partials are joined here
-    if (run0 < total)
-    {
-        int64_t before = 0;
-        for (int s0 = 0;; s0 += 32) {
-            const Span s = s0 == 0 ? mine0 : s0 + lane < p.n_seq ? span_of<TS>(p, s0 + lane) : Span{0, 0, 0, 0};
-            const int64_t n = (int64_t) units_of(s) * HP;
-            int64_t incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t y = __shfl_up_sync(FULL, incl, o);
-                if (lane >= o) incl += y;
-            }
-            const unsigned past = __ballot_sync(FULL, before + incl > run0);
-            if (past) {
-                const int f = __ffs(past) - 1;
-                const int64_t start = before + __shfl_sync(FULL, incl - n, f), rel = run0 - start;
-                at.seq = s0 + f;
-                at.s.lo = __shfl_sync(FULL, s.lo, f);
-                at.s.hi = __shfl_sync(FULL, s.hi, f);
-                at.s.first = __shfl_sync(FULL, s.first, f);
-                at.s.n = __shfl_sync(FULL, s.n, f);
-                const int u = at.s.n + OV;
-                at.hp = rel < 0x7FFFFFFF ? (int) ((uint32_t) rel / (uint32_t) u) : (int) (rel / u);
-                at.base = start + (int64_t) at.hp * u;
-                // step j lies at unit OV + j of its pair; the units before it go with its start
-                const int off = (int) (run0 - at.base);
-                at.st = off > OV ? off - OV : 0;
-                at.rem = (run0 + per < total ? per : total - run0) - (off < OV ? OV - off : 0);
-                const int64_t cta0 = (int64_t) blockIdx.x * W * per;
-                joint = cta0 >= at.base && cta0 + per > at.base + OV && cta0 + W * per <= at.base + u;
-                break;
-            }
-            before += __shfl_sync(FULL, incl, 31);
+    int worker = blockIdx.x * W + warp, wph = p.wph, ahead = warp;      // ahead: warps of the CTA in front of this one
+    uint32_t off = 0;                       // where the run begins in its list
+    int64_t per;
+    if (wph) {
+        per = (list + (uint32_t) wph - 1u) / (uint32_t) wph;
+        if (per < MIN_RUN) {
+            // fewer runs than workers: neighbours in the list go to different SMs
+            per = MIN_RUN;
+            wph = (int) ((list + MIN_RUN - 1u) / MIN_RUN);
+            worker = warp * gridDim.x + blockIdx.x;
+            ahead = -1;
+        }
+        at.hp = wph ? worker / wph : HP;
+        const int64_t o = (int64_t) (worker - at.hp * wph) * per;
+        if (at.hp < HP && o < list) { off = (uint32_t) o; at.rem = (int) (o + per < list ? per : list - o); }
+    } else {
+        const int64_t total = (int64_t) list * HP;
+        per = (total + p.n_work - 1) / p.n_work;
+        if (per < MIN_RUN) per = MIN_RUN;
+        const int64_t run0 = worker * per;
+        if (run0 < total) {
+            at.hp = (int) (run0 / list);
+            off = (uint32_t) (run0 - (int64_t) at.hp * list);
+            at.rem = (int) (run0 + per < total ? per : total - run0);
         }
     }
-    Cursor<TS> ld = at;                     // (no steps where the run has only units before a first step)
-
-    // ---- loads: the row of token `lane` of the step at ld, as an element offset; < 0 where it is not live ----
-    int64_t ld_row = -1, ld_first = 0;
-    unsigned ld_live = 0;                                    // live tokens of the step
-    int64_t ld_head = 0;                                     // the KV head's offset
-    constexpr unsigned ALL = TS == 32 ? FULL : 0xFFFFu;
-    const bool whole = p.c.page_tokens % TS == 0;            // a step lies in one page: its rows are a stride apart
-    auto look_up = [&]() {
-        ld_row = -1;
-        const int tok = (ld.s.first + ld.st) * TS + (lane & (TS - 1));
-        if (tok >= ld.s.lo && tok < ld.s.hi) {
-            const uint32_t g = p.page_shift >= 0 ? (uint32_t) tok >> p.page_shift : (uint32_t) tok / (uint32_t) p.c.page_tokens;
-            const int64_t row = p.rows ? (int64_t) p.rows[ld.seq] : (int64_t) ld.seq;
-            const uint32_t page = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables[row * p.c.table_stride + g] : SJKVARN_NO_BLOCK - 1u;
-            if (page < p.c.n_pages)
-                ld_row = (int64_t) page * p.c.page_stride + (int64_t) ((uint32_t) tok - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride;
-            else if (page != SJKVARN_NO_BLOCK)
-                atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
+    if (!p.by_pair && lane == 0) p.split[worker] = make_int4(-1, 0, 0, 0);
+    bool joint = false;                     // the CTA's warps all work on one pair: their partials are joined here
+    if (at.rem > 0) {
+        int g = 31 - __clz(__ballot_sync(FULL, mine_u > 0u && mine_0 <= off));
+        at.base = __shfl_sync(FULL, mine_0, g);
+        at.seq = g;
+        if (block > 1) {
+            const int end = (g + 1) * block;
+            for (int q0 = g * block;; q0 += 32) {           // (one round for up to 1,024 sequences)
+                s0 = q0 + lane < p.n_seq && q0 + lane < end ? span_of<TS>(p, q0 + lane) : Span{0, 0, 0, 0};
+                uint32_t all;
+                const uint32_t before = at.base + warp_scan(units_of(s0), lane, &all);
+                if (at.base + all <= off) { at.base += all; continue; }
+                g = 31 - __clz(__ballot_sync(FULL, s0.n > 0 && before <= off));
+                at.seq = q0 + g;
+                at.base = __shfl_sync(FULL, before, g);
+                break;
+            }
         }
-        ld_head = (int64_t) (ld.hp / p.tiles) * p.c.head_stride;
+        at.s.lo = __shfl_sync(FULL, s0.lo, g);
+        at.s.hi = __shfl_sync(FULL, s0.hi, g);
+        at.s.first = __shfl_sync(FULL, s0.first, g);
+        at.s.n = __shfl_sync(FULL, s0.n, g);
+        // step j lies at unit OV + j of its sequence; the units before it go with its start
+        const int in = (int) (off - at.base);
+        const int64_t cta0 = (int64_t) off - ahead * per, j0 = wph ? worker % wph - ahead : 0;
+        joint = ahead >= 0 && (wph == 0 || (j0 >= 0 && j0 + W <= wph)) && cta0 >= at.base && cta0 + per > (int64_t) at.base + OV &&
+                cta0 + W * per <= (int64_t) at.base + at.s.n + OV;
+        at.st = in > OV ? in - OV : 0;
+        if (in < OV) at.rem -= OV - in;     // no steps where the run has only units before a first step
+    }
+    Cursor<TS> ld = at;
+
+    // ---- loads ----
+    constexpr unsigned ALL = TS == 32 ? FULL : 0xFFFFu;
+    const bool whole = p.c.page_tokens % 16 == 0;            // 16 tokens lie in one page: their rows are a stride apart
+    const uint16_t * ld_kp = nullptr, * ld_vp = nullptr;     // the KV head's rows
+    const uint32_t * ld_table = nullptr;                     // the sequence's table row; NULL: out of range
+    unsigned ld_live = 0;                                    // live tokens of the step at ld
+    int64_t ld_off[TM];                                      // whole: element offsets of its 16-token groups
+    int64_t ld_row = -1;                                     // whole: of group ld_win + lane, else of token `lane` of the step;
+    int ld_win = 0;                                          // < 0: no page, or not live
+    auto row_of = [&](int tok) {
+        const uint32_t g = p.page_shift >= 0 ? (uint32_t) tok >> p.page_shift : (uint32_t) tok / (uint32_t) p.c.page_tokens;
+        const uint32_t page = ld_table[g];
+        if (page < p.c.n_pages)
+            return (int64_t) page * p.c.page_stride + (int64_t) (((uint32_t) tok - g * (uint32_t) p.c.page_tokens) * (uint64_t) p.slot_stride);
+        if (page != SJKVARN_NO_BLOCK) atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
+        return (int64_t) -1;
     };
-    auto copy = [&](uint32_t dst, const void * kv) {
-        constexpr int CH = D / 8;                            // 16-byte words of a row
-        const uint16_t * base = static_cast<const uint16_t *>(kv) + ld_head;
-        if (whole && ld_live == ALL) {
-            base += ld_first;
+    auto enter = [&]() {                                     // the pair at ld
+        const int64_t row = p.rows ? (int64_t) p.rows[ld.seq] : (int64_t) ld.seq;
+        const bool on = row >= 0 && row < (int64_t) p.c.n_rows;
+        if (!on) atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
+        ld_table = on ? p.c.tables + row * p.c.table_stride : nullptr;
+        const int64_t head = (int64_t) (ld.hp / p.tiles) * p.c.head_stride;
+        ld_kp = static_cast<const uint16_t *>(p.c.k) + head;
+        ld_vp = static_cast<const uint16_t *>(p.c.v) + head;
+        ld_win = -64;
+    };
+    auto look_up = [&]() {                                   // the step at ld
+        const int step = ld.s.first + ld.st, tok0 = step * TS;
+        const int a = ld.s.lo - tok0, b = ld.s.hi - tok0;    // its tokens [a, b) are in the span
+        if (whole) {
+            const int g = step * TM;
+            if (g - ld_win >= 32) {                          // the pages of the next 32 groups
+                ld_win = g;
+                const int tok = (g + lane) * 16;
+                ld_row = tok < ld.s.hi && tok + 16 > ld.s.lo && ld_table ? row_of(tok) : -1;
+            }
+            ld_live = ALL;
+            if (a > 0) ld_live &= FULL << a;
+            if (b < TS) ld_live &= ~(FULL << b);
 #pragma unroll
-            for (int i = 0; i < TS * CH / 32; ++i) {
-                const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
-                cp16(dst + r * PITCH + c * 16, base + (int64_t) r * p.c.slot_stride + c * 8);
+            for (int h = 0; h < TM; ++h) {
+                ld_off[h] = __shfl_sync(FULL, ld_row, g + h - ld_win);
+                if (ld_off[h] < 0) ld_live &= ~(0xFFFFu << (16 * h));
+            }
+        } else {
+            const int t = lane & (TS - 1);
+            ld_row = t >= a && t < b && ld_table ? row_of(tok0 + t) : -1;
+            ld_live = __ballot_sync(FULL, ld_row >= 0) & ALL;
+        }
+    };
+    auto copy = [&](uint32_t dst, const uint16_t * base) {
+        constexpr int CH = D / 8;                            // 16-byte words of a row
+        if (whole && ld_live == ALL) {
+#pragma unroll
+            for (int h = 0; h < TM; ++h) {                   // 16 rows: 32 words at a time, D / 16 times
+                const uint16_t * src = base + ld_off[h];
+                if constexpr (32 % CH == 0) {
+                    src += (uint64_t) (lane / CH) * p.slot_stride + (lane % CH) * 8;
+                    const uint64_t step = (uint64_t) (32 / CH) * p.slot_stride;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i, src += step) cp16(dst + (16 * h + i * (32 / CH) + lane / CH) * PITCH + (lane % CH) * 16, src);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
+                        cp16(dst + (16 * h + r) * PITCH + c * 16, src + (uint64_t) r * p.slot_stride + c * 8);
+                    }
+                }
             }
         } else {
 #pragma unroll 1
             for (int i = 0; i < TS * CH / 32; ++i) {
                 const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
-                const int64_t row = __shfl_sync(FULL, ld_row, r);
-                cp16_or_zero(dst + r * PITCH + c * 16, base + (row < 0 ? 0 : row) + c * 8, row >= 0);
+                const int64_t one = __shfl_sync(FULL, ld_row, r);
+                const int64_t row = whole ? (TM == 2 && r >= 16 ? ld_off[TM - 1] : ld_off[0]) + (int64_t) ((uint64_t) (r & 15) * p.slot_stride) : one;
+                const bool on = (ld_live >> r) & 1u;
+                cp16_or_zero(dst + r * PITCH + c * 16, base + (on ? row : 0) + c * 8, on);
             }
         }
     };
@@ -284,23 +357,21 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         if (ld.rem > 0) {
             const uint32_t dst = ring + ld_entry * S::ENTRY;
             if (!v) {
-                ld_live = __ballot_sync(FULL, ld_row >= 0) & ALL;
-                ld_first = __shfl_sync(FULL, ld_row, 0);
                 if (lane == 0) s_mask[ld_mask] = ld_live;
                 ld_mask = (ld_mask + 1) & 3;
-                copy(dst, p.c.k);
+                copy(dst, ld_kp);
             } else {
-                copy(dst, p.c.v);
-                ld.next(p, HP);
-                if (ld.rem > 0) look_up();
+                copy(dst, ld_vp);
+                const bool crossed = ld.next(p);
+                if (ld.rem > 0) {
+                    if (crossed) enter();
+                    look_up();
+                }
             }
             ld_entry = ld_entry + 1 == NE ? 0 : ld_entry + 1;
         }
         cp_commit();
     };
-    if (ld.rem > 0) look_up();
-#pragma unroll 1
-    for (int i = 0; i < NE; ++i) issue(i & 1);
 
     // ---- products ----
     // Column lane / 4 of a tile, as B operand: head and term. This lane's columns 2 (lane & 3) + j, as results: heads
@@ -314,31 +385,53 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
     };
     uint32_t qf[KS][NT8][2];
     float o[NT8][KS][4], m[NT8][2], l[NT8][2], sc[NT8][2];
-    bool fresh = true, begun = false;                        // a pair comes next; its first step is in this run
+    bool fresh = true, begun = false, started = false;       // a pair comes next; its first step is in this run; loads are out
+    // the first loads: behind those of the queries, which would wait for them
+    auto start = [&]() {
+        if (started) return;
+        started = true;
+        enter();
+        look_up();
+#pragma unroll 1
+        for (int i = 0; i < NE; ++i) issue(i & 1);
+    };
     int entry = 0;                                           // the ring's entry that comes next
     for (int step = 0; at.rem > 0; step = (step + 1) & 3) {
         if (fresh) {                                         // a (sequence, KV head, row tile) begins
             fresh = false;
             begun = at.st == 0;
             const int kv = at.hp / p.tiles, r0 = (at.hp - kv * p.tiles) * R;
+            int64_t src[NT8];
+            bool on[NT8];
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
                 const int rel = r0 + HT * n + qhead;
-                const bool on = rel < p.grp && qterm < T;
-                const int64_t src = (int64_t) at.seq * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
-                if constexpr (T == 1) {
+                on[n] = rel < p.grp && qterm < T;
+                src[n] = (int64_t) at.seq * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
+            }
+            if constexpr (T == 1) {
+#pragma unroll
+                for (int n = 0; n < NT8; ++n) {
 #pragma unroll
                     for (int k = 0; k < 2 * KS; ++k)
-                        qf[k >> 1][n][k & 1] = on ? *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p.q.p) + src + 8 * k) : 0u;
+                        qf[k >> 1][n][k & 1] = on[n] ? *reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(p.q.p) + src[n] + 8 * k) : 0u;
                     sc[n][0] = sc[n][1] = p.scale * 1.4426950408889634f;
-                } else {
-                    float2 x[2 * KS];
-                    if (p.q.type == SJK_F32) load_pairs<SJK_F32>(x, p.q.p, src, on);
-                    else if (p.q.type == SJK_F16) load_pairs<SJK_F16>(x, p.q.p, src, on);
-                    else load_pairs<SJK_BF16>(x, p.q.p, src, on);
+                }
+                start();
+            } else {
+                float2 x[NT8][2 * KS];
+#pragma unroll
+                for (int n = 0; n < NT8; ++n) {
+                    if (p.q.type == SJK_F32) load_pairs<SJK_F32>(x[n], p.q.p, src[n], on[n]);
+                    else if (p.q.type == SJK_F16) load_pairs<SJK_F16>(x[n], p.q.p, src[n], on[n]);
+                    else load_pairs<SJK_BF16>(x[n], p.q.p, src[n], on[n]);
+                }
+                start();
+#pragma unroll
+                for (int n = 0; n < NT8; ++n) {
                     float big = 0.0f;                        // the row to [1, 2) by an exact power of two
 #pragma unroll
-                    for (int k = 0; k < 2 * KS; ++k) big = fmaxf(big, fmaxf(fabsf(x[k].x), fabsf(x[k].y)));
+                    for (int k = 0; k < 2 * KS; ++k) big = fmaxf(big, fmaxf(fabsf(x[n][k].x), fabsf(x[n][k].y)));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
                     const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 0;
@@ -347,7 +440,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                     for (int j = 0; j < 2; ++j) sc[n][j] = p.scale * 1.4426950408889634f / __shfl_sync(FULL, mul, (first + j) * 4);
 #pragma unroll
                     for (int k = 0; k < 2 * KS; ++k) {
-                        float a = x[k].x * mul, b = x[k].y * mul;
+                        float a = x[n][k].x * mul, b = x[n][k].y * mul;
                         uint32_t w = pack2<S::TYPE>(a, b);
 #pragma unroll
                         for (int t = 1; t < T; ++t) {        // the column's term: what is left after those before it
@@ -361,6 +454,9 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                         qf[k >> 1][n][k & 1] = w;
                     }
                 }
+            }
+#pragma unroll
+            for (int n = 0; n < NT8; ++n) {
                 m[n][0] = m[n][1] = -INFINITY;
                 l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
@@ -403,43 +499,57 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         __syncwarp();
         issue(NE & 1);
 
-        // softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16 of its two heads
+        // Softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16 of its two heads. The maximum is
+        // looked for only when some score is above the one so far: seldom after a sequence's first steps.
         uint32_t pb[TM][NT8][2];
+        bool above = false;
 #pragma unroll
-        for (int n = 0; n < NT8; ++n) {
+        for (int n = 0; n < NT8; ++n)
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s[tm][n][e] *= sc[n][e & 1];
-            if (live != ALL) {
+        if (live != ALL) {
+#pragma unroll
+            for (int n = 0; n < NT8; ++n)
 #pragma unroll
                 for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         if (!((live >> (tm * 16 + (lane >> 2) + (e >> 1) * 8)) & 1u)) s[tm][n][e] = -INFINITY;
-            }
-            float top[2] = {m[n][0], m[n][1]};
+        }
+#pragma unroll
+        for (int n = 0; n < NT8; ++n)
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top[e & 1] = fmaxf(top[e & 1], s[tm][n][e]);
-            float use[2], fix[2];
+                for (int e = 0; e < 4; ++e) above |= s[tm][n][e] > m[n][e & 1];
+        if (__any_sync(FULL, above)) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 4));
-                top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 8));
-                top[j] = fmaxf(top[j], __shfl_xor_sync(FULL, top[j], 16));
-                use[j] = top[j] == -INFINITY ? 0.0f : top[j];
-                fix[j] = ex2(m[n][j] - use[j]);
-            }
-            if (__any_sync(FULL, top[0] != m[n][0] || top[1] != m[n][1])) {
+            for (int n = 0; n < NT8; ++n) {
+                float up[2] = {m[n][0], m[n][1]}, fix[2];
+#pragma unroll
+                for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) up[e & 1] = fmaxf(up[e & 1], s[tm][n][e]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    up[j] = fmaxf(up[j], __shfl_xor_sync(FULL, up[j], 4));
+                    up[j] = fmaxf(up[j], __shfl_xor_sync(FULL, up[j], 8));
+                    up[j] = fmaxf(up[j], __shfl_xor_sync(FULL, up[j], 16));
+                    fix[j] = up[j] == m[n][j] ? 1.0f : ex2(m[n][j] - up[j]);
+                    l[n][j] *= fix[j];
+                    m[n][j] = up[j];
+                }
 #pragma unroll
                 for (int k = 0; k < KS; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[n][k][e] *= fix[e & 1];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) { l[n][j] *= fix[j]; m[n][j] = top[j]; }
             }
+        }
+#pragma unroll
+        for (int n = 0; n < NT8; ++n) {
+            const float use[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
 #pragma unroll
             for (int tm = 0; tm < TM; ++tm) {
 #pragma unroll
@@ -495,7 +605,8 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
             const bool ended = at.st + 1 == at.s.n;
             fresh = true;
             if (begun && lane == 0) {
-                const int last = ended ? worker : (int) ((at.base + at.s.n + OV - 1) / per);
+                const uint32_t end = at.base + (uint32_t) (at.s.n + OV - 1);
+                const int last = ended ? worker : wph ? at.hp * wph + (int) (end / (uint32_t) per) : (int) (((int64_t) at.hp * list + end) / per);
                 if (p.by_pair) p.split[at.seq * HP + at.hp] = make_int4(ended ? -1 : at.seq, at.hp, worker, last);
                 else if (!ended) p.split[worker] = make_int4(at.seq, at.hp, worker, last);
             }
@@ -532,7 +643,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 }
             }
         }
-        at.next(p, HP);
+        at.next(p);
     }
     cp_wait<0>();
 
@@ -575,14 +686,26 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
     }
 }
 
-// Joins the slots of a split pair, in list order. grid.x: entries of p.split; G warps of the CTA's 8 share a query head
+// Joins the slots of a split pair, in list order, and writes the zeros of sequences without a live position. grid.x:
+// entries of p.split, then 8 sequences each (before the wait: the lengths are older than the kernel waited for); G warps of the CTA's 8 share a query head
 // (grid.y CTAs then take the heads of an entry in turn).
 template <int D>
-__global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__ Params p, int R, int G) {
+__global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__ Params p, int R, int G, int entries) {
     constexpr int NV = (D / 4 + 31) / 32;   // 16-byte words of a lane
     __shared__ float s_acc[8 * (D + 4)];
+    if (blockIdx.x >= entries) {
+        const int seq = (blockIdx.x - entries) * 8 + (threadIdx.x >> 5);
+        if (blockIdx.y == 0 && seq < p.n_seq && p.len[seq] <= 0)
+            for (int i = threadIdx.x & 31; i < p.out.n_head * D; i += 32)
+                store1(p.out.p, (int64_t) seq * p.out.row_stride + (int64_t) (i / D) * p.out.head_stride + i % D, p.out.type, 0.0f);
+        pdl_wait();
+        pdl_release();
+        return;
+    }
     pdl_wait();
     pdl_release();
+    // (in the order of pairs, the entry of a sequence without a live position was not written)
+    if (p.by_pair && p.len[blockIdx.x / (p.c.n_head_kv * p.tiles)] <= 0) return;
     const int4 e = p.split[blockIdx.x];
     if (e.x < 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % G;
@@ -689,8 +812,8 @@ int run(const Params & p0, const Plan & pl, sjk_stream st) {
     // few pairs: many slots each, so a CTA per query head; many: two or three slots each, a warp per query head
     const int64_t pairs = (int64_t) p.n_seq * p.c.n_head_kv * p.tiles;
     const bool few = pairs * 8 <= p.n_work;
-    const int rows = p.grp < pl.R ? p.grp : pl.R;
-    return launch(kv16_merge_kernel<S::D>, dim3((unsigned) (p.by_pair ? pairs : p.n_work), few ? (unsigned) rows : 1u), dim3(256), 0, st, p, pl.R, few ? 8 : 1);
+    const int rows = p.grp < pl.R ? p.grp : pl.R, entries = p.by_pair ? (int) pairs : p.n_work;
+    return launch(kv16_merge_kernel<S::D>, dim3((unsigned) (entries + (p.n_seq + 7) / 8), few ? (unsigned) rows : 1u), dim3(256), 0, st, p, pl.R, few ? 8 : 1, entries);
 }
 
 // f(Shape) for the call's types and sizes: nt8 1 or 2 tiles of columns in one pass over K and V
@@ -752,16 +875,22 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     // q of the cache's type is read two elements at a time
     const bool split = q->type != c->type || out->type == SJK_F32;
     if (!split && (!aligned(q->p, 4) || (q->row_stride & 1) || (q->head_stride & 1))) return SJKVARN_ERR_ARG;
+    if (c->slot_stride > 0x7FFFFFFF) return SJK_ERR_UNSUPPORTED;
     Plan pl;
     const int rc = plan_of(c, q->n_head, split, &pl);
     if (rc) return rc;
     if (n_seq == 0) return 0;
+    // a list counts its units in 32 bits, and a worker its run, whatever the lengths
+    const double most = (fmin((double) c->table_stride * c->page_tokens, 2147483647.0) / 16 + OV + 1) * n_seq;
+    const int HP = c->n_head_kv * pl.tiles;
+    if (most > 2e9 || most * HP / pl.work > 2e9) return SJK_ERR_UNSUPPORTED;
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < pl.bytes) return SJKVARN_ERR_BUFFER;
     Params p = {};
     p.c = *c; p.q = *q; p.out = *out;
     p.len = len; p.rows = rows; p.n_seq = n_seq;
     p.grp = q->n_head / c->n_head_kv; p.tiles = pl.tiles;
     p.window = window; p.scale = scale;
+    p.slot_stride = (uint32_t) c->slot_stride;
     p.page_shift = -1;
     for (int b = 0; b < 31; ++b)
         if (c->page_tokens == 1 << b) p.page_shift = b;
@@ -769,7 +898,9 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     p.part = static_cast<float *>(scratch);
     p.ml = p.part + pl.part;
     p.split = reinterpret_cast<int4 *>(p.ml + pl.ml);
-    p.by_pair = (int64_t) n_seq * c->n_head_kv * pl.tiles <= p.n_work;
+    p.by_pair = (int64_t) n_seq * HP <= p.n_work;
+    // a list per head where that leaves under a sixteenth of the workers without one
+    p.wph = HP * 16 <= p.n_work ? p.n_work / HP : 0;
     return with_shape(c->type, c->head_dim, split, pl.nt8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
 }
 
