@@ -24,7 +24,7 @@ namespace {
 using namespace sjk16;
 
 constexpr int NT = 256;
-constexpr int MAX_T = 8;                    // tokens of a CTA
+constexpr int MAX_T = 32;                   // tokens of a CTA, at most
 __device__ unsigned int g_qkv_status;
 
 struct Params {
@@ -99,13 +99,21 @@ template <int TYPE>
 SJK_DEV uint4 pack8(const float (&x)[8]) {
     return make_uint4(pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3]), pack2<TYPE>(x[4], x[5]), pack2<TYPE>(x[6], x[7]));
 }
-SJK_DEV void store8(void * base, int64_t off, int type, const float (&x)[8]) {
+SJK_DEV void store16(void * base, int64_t off, int d0, int d1, int type, const float (&a)[8], const float (&b)[8]) {
     if (type == SJK_F32) {
-        float4 * d = reinterpret_cast<float4 *>(static_cast<float *>(base) + off);
-        d[0] = make_float4(x[0], x[1], x[2], x[3]);
-        d[1] = make_float4(x[4], x[5], x[6], x[7]);
+        float * x = static_cast<float *>(base) + off;
+        float4 * u = reinterpret_cast<float4 *>(x + d0), * v = reinterpret_cast<float4 *>(x + d1);
+        u[0] = make_float4(a[0], a[1], a[2], a[3]);
+        u[1] = make_float4(a[4], a[5], a[6], a[7]);
+        v[0] = make_float4(b[0], b[1], b[2], b[3]);
+        v[1] = make_float4(b[4], b[5], b[6], b[7]);
     } else {
-        *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(base) + off) = type == SJK_F16 ? pack8<SJK_F16>(x) : pack8<SJK_BF16>(x);
+        uint16_t * x = static_cast<uint16_t *>(base) + off;
+        uint4 u, v;
+        if (type == SJK_F16) { u = pack8<SJK_F16>(a); v = pack8<SJK_F16>(b); }
+        else { u = pack8<SJK_BF16>(a); v = pack8<SJK_BF16>(b); }
+        *reinterpret_cast<uint4 *>(x + d0) = u;
+        *reinterpret_cast<uint4 *>(x + d1) = v;
     }
 }
 
@@ -118,20 +126,103 @@ SJK_DEV bool lane_chunks(const Params & p, int c, int * d0, int * d1) {
     return rot;
 }
 
-// grid.x: tiles of T tokens; grid.y: the heads in runs of NT / L. L = lanes of a head (a power of two, >= D / 16).
-template <int TYPE>
-__global__ void __launch_bounds__(NT) qkv_vec_kernel(const __grid_constant__ Params p, int L) {
-    extern __shared__ float4 s_tab[];       // [T][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7 of a lane's 8 angles
-    __shared__ int32_t s_pos[MAX_T];
+// The tokens of blocks [ka, kb) of a tile in one head of q, k or v: norm (NORM) and rotation (ROT). A block is a token
+// for each of the warp's groups of L lanes; the loads of the next block are out while one is worked on.
+template <int TYPE, int L, bool NORM, bool ROT>
+SJK_DEV void head_tokens(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const float4 * s_tab, const float * s_w,
+                         const int32_t * s_pos, const int64_t * s_slot) {
+    const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
+    const sjk_rows & out = part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2];
+    void * cache = part == 0 ? nullptr : part == 1 ? p.c.k : p.c.v;
+    const int c = threadIdx.x & (L - 1), nr = p.n_rot / 16;
+    int d0, d1;
+    const bool rot = lane_chunks(p, c, &d0, &d1) && ROT;
+    const bool on = 16 * L == p.D || 16 * c < p.D;
+    constexpr int G = 32 / L;
+    int t = ka * G + (threadIdx.x & 31) / L;
+    const int end = min(nt, kb * G);
+    int64_t src = (int64_t) (t0 + t) * in.row_stride + (int64_t) hh * in.head_stride;
+    int64_t dst = (int64_t) (t0 + t) * out.row_stride + (int64_t) hh * out.head_stride;
+    const int64_t head = (int64_t) hh * p.c.head_stride;
+    float w0[8], w1[8];
+    if constexpr (NORM) {
+        const float4 * w = reinterpret_cast<const float4 *>(s_w + (part ? p.D : 0));
+        const float4 x[4] = {w[d0 / 4 * on], w[(d0 / 4 + 1) * on], w[d1 / 4 * on], w[(d1 / 4 + 1) * on]};
+        w0[0] = x[0].x; w0[1] = x[0].y; w0[2] = x[0].z; w0[3] = x[0].w; w0[4] = x[1].x; w0[5] = x[1].y; w0[6] = x[1].z; w0[7] = x[1].w;
+        w1[0] = x[2].x; w1[1] = x[2].y; w1[2] = x[2].z; w1[3] = x[2].w; w1[4] = x[3].x; w1[5] = x[3].y; w1[6] = x[3].z; w1[7] = x[3].w;
+    }
+    Raw<TYPE> ra = {}, rb = {};
+    if (on && t < end) { ra = load8<TYPE>(in.p, src + d0); rb = load8<TYPE>(in.p, src + d1); }
+    for (int k = ka; k < kb; ++k, t += G) {
+        float a[8], b[8];
+        widen8<TYPE>(ra, a);
+        widen8<TYPE>(rb, b);
+        src += G * in.row_stride;
+        if (on && t + G < end) { ra = load8<TYPE>(in.p, src + d0); rb = load8<TYPE>(in.p, src + d1); }
+        if constexpr (NORM) {
+            float s0 = 0.0f, s1 = 0.0f;     // idle lanes hold zeros
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { s0 = fmaf(a[i], a[i], s0); s1 = fmaf(b[i], b[i], s1); }
+            float ss = s0 + s1;
+#pragma unroll
+            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
+            const float r = rsqrtf(ss * p.inv_d + p.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { a[i] *= r * w0[i]; b[i] *= r * w1[i]; }
+        }
+        if (t >= end) break;                // (its groups' last tokens; the sums above needed all lanes)
+        if (rot) {
+            const float4 * tab = s_tab + (size_t) t * 4 * nr + c;
+            const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
+            const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            if (p.layout == SJK_ROPE_HALF) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = a[i], y = b[i];
+                    a[i] = x * cs[i] - y * sn[i];
+                    b[i] = x * sn[i] + y * cs[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float x = a[2 * i], y = a[2 * i + 1];
+                    a[2 * i] = x * cs[i] - y * sn[i];
+                    a[2 * i + 1] = x * sn[i] + y * cs[i];
+                    x = b[2 * i]; y = b[2 * i + 1];
+                    b[2 * i] = x * cs[4 + i] - y * sn[4 + i];
+                    b[2 * i + 1] = x * sn[4 + i] + y * cs[4 + i];
+                }
+            }
+        }
+        const bool live = on && s_pos[t] >= 0;
+        if (live && out.p) store16(out.p, dst, d0, d1, out.type, a, b);
+        if (live && cache && s_slot[t] >= 0) store16(cache, s_slot[t] + head, d0, d1, p.c.type, a, b);
+        dst += G * out.row_stride;
+    }
+}
+
+// grid.x: tiles of T tokens; grid.y CTAs share a tile's heads. L: lanes of a head, the power of two from D / 16 on.
+// The (head, block of tokens) items of a tile, in the order of heads, are cut into equal runs, one per warp: its groups of L
+// lanes work on as many tokens of the same head.
+template <int TYPE, int L>
+__global__ void __launch_bounds__(NT, 3) qkv_vec_kernel(const __grid_constant__ Params p) {
+    extern __shared__ float4 s_tab[];       // [T][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7 of a lane's 8 angles,
+    __shared__ int32_t s_pos[MAX_T];        // then the norm weights of q and k
     __shared__ int64_t s_slot[MAX_T];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, t0 = blockIdx.x * p.T, nt = min(p.T, p.n_tok - t0);
     const int half = p.n_rot / 2, nr = p.n_rot / 16;
+    float * s_w = reinterpret_cast<float *>(s_tab + p.T * 4 * nr);
     if (tid < nt) {
         const int32_t pos = p.pos ? p.pos[t0 + tid] : 0;
         s_pos[tid] = pos;
         s_slot[tid] = p.c.k && pos >= 0 ? cache_slot(p, t0 + tid, pos) : -1;
+    }
+    for (int i = tid; i < 2 * p.D; i += NT) {
+        const void * w = i < p.D ? p.w[0] : p.w[1];
+        if (w) s_w[i] = load1(w, i < p.D ? i : i - p.D, p.w_type) + p.w_bias;
     }
     for (int i = tid; i < nt * half; i += NT) {
         const int t = i / half, j = i - t * half, c = j >> 3, e = j & 7;
@@ -141,87 +232,19 @@ __global__ void __launch_bounds__(NT) qkv_vec_kernel(const __grid_constant__ Par
         d[((2 + (e >> 2)) * nr + c) * 4 + (e & 3)] = cs.y;
     }
     __syncthreads();
-    const int c = tid & (L - 1), per = NT / L;
-    int d0, d1;
-    const bool rot_lane = lane_chunks(p, c, &d0, &d1);
-    const bool on = 16 * c < p.D;
-    for (int h = blockIdx.y * per + tid / L; h < (p.n_all + per - 1) / per * per; h += gridDim.y * per) {
-        // every lane of the warp goes through the loop: the norm's butterfly needs them
-        const bool live = on && h < p.n_all;
-        int hh = 0;
-        const int part = h < p.n_all ? part_of(p, h, &hh) : 2;
-        const sjk_rows & in = p.in[part];
-        const sjk_rows & out = p.out[part];
-        const void * w = part < 2 ? p.w[part] : nullptr;
-        const bool rot = rot_lane && part < 2;
-        float w0[8], w1[8];
-        if (w && live) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                w0[i] = load1(w, d0 + i, p.w_type) + p.w_bias;
-                w1[i] = load1(w, d1 + i, p.w_type) + p.w_bias;
-            }
-        }
-        const int64_t hoff = (int64_t) hh * in.head_stride;
-        for (int t = 0; t < nt; ++t) {
-            const int64_t src = (int64_t) (t0 + t) * in.row_stride + hoff;
-            float a[8], b[8];
-            if (live) {
-                const Raw<TYPE> ra = load8<TYPE>(in.p, src + d0), rb = load8<TYPE>(in.p, src + d1);
-                widen8<TYPE>(ra, a);
-                widen8<TYPE>(rb, b);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) a[i] = b[i] = 0.0f;
-            }
-            if (p.w[0] || p.w[1]) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-                for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
-                if (w && live) {
-                    const float r = rsqrtf(ss * p.inv_d + p.eps);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) { a[i] *= r * w0[i]; b[i] *= r * w1[i]; }
-                }
-            }
-            if (!live || s_pos[t] < 0) continue;
-            if (rot) {
-                const float4 * tab = s_tab + (size_t) t * 4 * nr + c;
-                const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
-                const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-                const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-                if (p.layout == SJK_ROPE_HALF) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float x = a[i], y = b[i];
-                        a[i] = x * cs[i] - y * sn[i];
-                        b[i] = x * sn[i] + y * cs[i];
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float x = a[2 * i], y = a[2 * i + 1];
-                        a[2 * i] = x * cs[i] - y * sn[i];
-                        a[2 * i + 1] = x * sn[i] + y * cs[i];
-                        x = b[2 * i]; y = b[2 * i + 1];
-                        b[2 * i] = x * cs[4 + i] - y * sn[4 + i];
-                        b[2 * i + 1] = x * sn[4 + i] + y * cs[4 + i];
-                    }
-                }
-            }
-            if (out.p) {
-                const int64_t dst = (int64_t) (t0 + t) * out.row_stride + (int64_t) hh * out.head_stride;
-                store8(out.p, dst + d0, out.type, a);
-                store8(out.p, dst + d1, out.type, b);
-            }
-            if (part && s_slot[t] >= 0) {
-                void * base = part == 1 ? p.c.k : p.c.v;
-                const int64_t dst = s_slot[t] + (int64_t) hh * p.c.head_stride;
-                store8(base, dst + d0, p.c.type, a);
-                store8(base, dst + d1, p.c.type, b);
-            }
-        }
+    constexpr int G = 32 / L, WARPS = NT / 32;
+    const int blocks = (nt + G - 1) / G, items = blocks * p.n_all;
+    const int each = (items + WARPS * (int) gridDim.y - 1) / (WARPS * (int) gridDim.y);
+    int item = ((int) blockIdx.y * WARPS + tid / 32) * each;
+    const int end = min(item + each, items);
+    while (item < end) {
+        const int h = item / blocks, ka = item - h * blocks, kb = min(blocks, ka + end - item);
+        int hh;
+        const int part = part_of(p, h, &hh);
+        if (part == 2) head_tokens<TYPE, L, false, false>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
+        else if (part == 0 ? p.w[0] : p.w[1]) head_tokens<TYPE, L, true, true>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
+        else head_tokens<TYPE, L, false, true>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
+        item += kb - ka;
     }
 }
 
@@ -279,6 +302,18 @@ __global__ void __launch_bounds__(NT) qkv_scalar_kernel(const __grid_constant__ 
             }
         }
         __syncwarp();
+    }
+}
+
+template <int TYPE>
+int launch_vec(int L, dim3 grid, size_t smem, sjk_stream st, const Params & p) {
+    switch (L) {
+        case 1: return launch(qkv_vec_kernel<TYPE, 1>, grid, dim3(NT), smem, st, p);
+        case 2: return launch(qkv_vec_kernel<TYPE, 2>, grid, dim3(NT), smem, st, p);
+        case 4: return launch(qkv_vec_kernel<TYPE, 4>, grid, dim3(NT), smem, st, p);
+        case 8: return launch(qkv_vec_kernel<TYPE, 8>, grid, dim3(NT), smem, st, p);
+        case 16: return launch(qkv_vec_kernel<TYPE, 16>, grid, dim3(NT), smem, st, p);
+        default: return launch(qkv_vec_kernel<TYPE, 32>, grid, dim3(NT), smem, st, p);
     }
 }
 
@@ -432,21 +467,21 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
     }
     int L = 1;
     while (16 * L < p.D) L <<= 1;
-    // Few tokens: one token per CTA and the heads over grid.y. Many: all heads in one CTA and up to MAX_T tokens, so
-    // that the table and the norm weights serve several rows, as long as every SM still gets several CTAs.
-    const int per = NT / L, runs = (p.n_all + per - 1) / per;
-    int T = 1, ny = runs;
-    if ((int64_t) p.n_tok >= 148 * 8) {
+    // Few tokens: one token per CTA and the heads over grid.y. Many: all heads in one CTA and several tokens (a block
+    // of 32 / L at least), so that the table and the norm weights serve several rows.
+    int T = 1, ny = (p.n_all + NT / 32 - 1) / (NT / 32);
+    if (p.n_tok >= 148 * 8) {
         ny = 1;
-        T = p.n_tok / (148 * 8) < MAX_T ? p.n_tok / (148 * 8) : MAX_T;
+        T = 32 / L > 8 ? 32 / L : 8;
+        while (T > 32 / L && p.n_tok / T < 148 * 4) T /= 2;
     }
     p.T = T;
     const dim3 grid((unsigned) ((p.n_tok + T - 1) / T), (unsigned) ny);
-    const size_t smem = (size_t) T * p.n_rot * sizeof(float);
+    const size_t smem = ((size_t) T * p.n_rot + 2 * (size_t) p.D) * sizeof(float);
     switch (type) {
-        case SJK_F32: return launch(qkv_vec_kernel<SJK_F32>, grid, dim3(NT), smem, st, p, L);
-        case SJK_F16: return launch(qkv_vec_kernel<SJK_F16>, grid, dim3(NT), smem, st, p, L);
-        default: return launch(qkv_vec_kernel<SJK_BF16>, grid, dim3(NT), smem, st, p, L);
+        case SJK_F32: return launch_vec<SJK_F32>(L, grid, smem, st, p);
+        case SJK_F16: return launch_vec<SJK_F16>(L, grid, smem, st, p);
+        default: return launch_vec<SJK_BF16>(L, grid, smem, st, p);
     }
 }
 
