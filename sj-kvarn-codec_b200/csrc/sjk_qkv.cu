@@ -7,24 +7,31 @@
 // The angle is an integer: pos * step_i modulo 2^64, in units of 2^-64 turns, of which the top 32 bits, read as a
 // signed fraction of a turn, go to sincospif. That keeps 2^-32 of a turn at every position, for one wide multiply.
 //
-// Bound: HBM, every element once in and once out. The vector kernel gives a lane 16 channels of a head: for the half
+// Bound: HBM, every element once in and once out. The vector kernels give a lane 16 channels of a head: for the half
 // layout the two 8-channel chunks that rotate into one another, so the rotation needs no exchange between lanes, and
-// the norm's sum is a butterfly over the head's D / 16 lanes (a fixed order). A CTA works on T tokens: their cosines
-// and sines are computed once into shared memory for all heads (n_rot / 2 sincos per token instead of per head), and
-// every lane keeps its channels and its head over the tokens, so that norm weights are loaded once per head.
+// the norm's sum is a butterfly over the head's D / 16 lanes (a fixed order). Products of channel pairs are packed
+// (f32x2). The cosines and sines of a token are computed once into shared memory for all its heads (n_rot / 2 sincos
+// per token instead of per head), and a warp stays with a head over the tokens of its tile, for its norm weights.
+//  - Many tokens: a few waves of CTAs, each with a run of tokens that it takes in tiles of up to MAX_T.
+//  - Few tokens: a token per CTA and the heads over grid.y: a launch's latency.
 // Shapes whose chunks would straddle (n_rot or head_dim not a multiple of 16, rows off 16 bytes) take the scalar
 // kernel, one warp per (token, head) through shared memory.
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
 #include <math.h>
+#include <type_traits>
 
 namespace {
 
 using namespace sjk16;
 
 constexpr int NT = 256;
-constexpr int MAX_T = 32;                   // tokens of a CTA, at most
+constexpr int MAX_T = 16;                   // tokens of a tile, at most (32 where a warp takes so many at once)
+// CTAs of the many-token kernel per SM: 64 registers do for the 16-bit types (prefill of 32,768 tokens 160 us with four,
+// 166 with three), floats need 80 (8,320 rows 68 us with three, 74 with four)
+constexpr int ctas_of(int type) { return type == SJK_F32 ? 3 : 4; }
+constexpr int WAVES = 4;                    // runs per CTA slot, at most: SMs are not equally fast (f32: 82 us with one, 74 with four)
 __device__ unsigned int g_qkv_status;
 
 struct Params {
@@ -69,182 +76,278 @@ SJK_DEV int part_of(const Params & p, int h, int * hh) {
     return 2;
 }
 
+// two floats in one 64-bit register, and their packed products
+SJK_DEV uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+SJK_DEV float2 both(uint64_t x) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(x));
+    return f;
+}
+SJK_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+SJK_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+SJK_DEV uint64_t neg2(uint64_t a) { return a ^ 0x8000000080000000ull; }
+
+// A lane's 16 channels: 16-byte words that lie side by side over the head's lanes, so that every load and store is of
+// whole sectors. Region: the rotating channels, or those behind them; the lane's words are a half (16-bit types: two
+// words) or a quarter (floats: four) of the region apart. In the half layout the last 8 are the partners of the first 8.
 template <int TYPE>
-struct Raw { uint4 a, b; };                 // 8 channels: 16 bytes, or 32 for floats
+struct Lane {
+    static constexpr int N = TYPE == SJK_F32 ? 4 : 2, WORD = 16 / N;    // words, and channels of one
+    int first, apart;                       // first channel of word 0, and from word to word
+    bool rot, on;                           // rotates; has channels at all
+    SJK_DEV Lane(const Params & p, int c) {
+        const int nr = p.n_rot / 16, all = p.D / 16;
+        rot = c < nr;
+        on = c < all;
+        first = rot ? WORD * c : on ? p.n_rot + WORD * (c - nr) : 0;
+        apart = rot ? p.n_rot / N : on ? (p.D - p.n_rot) / N : 0;
+    }
+};
 
 template <int TYPE>
-SJK_DEV Raw<TYPE> load8(const void * base, int64_t off) {
+struct Raw { uint4 w[TYPE == SJK_F32 ? 4 : 2]; };
+
+template <int TYPE>
+SJK_DEV Raw<TYPE> load16(const void * base, int64_t off, const Lane<TYPE> & l) {
+    using E = typename std::conditional<TYPE == SJK_F32, float, uint16_t>::type;
     Raw<TYPE> r;
-    if constexpr (TYPE == SJK_F32) {
-        const uint4 * s = reinterpret_cast<const uint4 *>(static_cast<const float *>(base) + off);
-        r.a = s[0]; r.b = s[1];
-    } else {
-        r.a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + off);
-    }
+#pragma unroll
+    for (int i = 0; i < Lane<TYPE>::N; ++i) r.w[i] = *reinterpret_cast<const uint4 *>(static_cast<const E *>(base) + off + l.first + i * l.apart);
     return r;
 }
 template <int TYPE>
-SJK_DEV void widen8(const Raw<TYPE> & r, float (&x)[8]) {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-    if constexpr (TYPE == SJK_F32) {
-        const uint32_t u[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+SJK_DEV void widen16(const Raw<TYPE> & r, uint64_t (&x)[8]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { x[i] = __uint_as_float(w[i]); x[4 + i] = __uint_as_float(u[i]); }
-    } else {
+    for (int i = 0; i < Lane<TYPE>::N; ++i) {
+        const uint32_t w[4] = {r.w[i].x, r.w[i].y, r.w[i].z, r.w[i].w};
+        if constexpr (TYPE == SJK_F32) {
+            x[2 * i] = two(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            x[2 * i + 1] = two(__uint_as_float(w[2]), __uint_as_float(w[3]));
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { const float2 f = widen2<TYPE>(w[i]); x[2 * i] = f.x; x[2 * i + 1] = f.y; }
+            for (int k = 0; k < 4; ++k) { const float2 f = widen2<TYPE>(w[k]); x[4 * i + k] = two(f.x, f.y); }
+        }
     }
 }
+// the lane's channels to a row of any type (TYPE is the input's, which chose the channels)
 template <int TYPE>
-SJK_DEV uint4 pack8(const float (&x)[8]) {
-    return make_uint4(pack2<TYPE>(x[0], x[1]), pack2<TYPE>(x[2], x[3]), pack2<TYPE>(x[4], x[5]), pack2<TYPE>(x[6], x[7]));
-}
-SJK_DEV void store16(void * base, int64_t off, int d0, int d1, int type, const float (&a)[8], const float (&b)[8]) {
+SJK_DEV void store16(void * base, int64_t off, const Lane<TYPE> & l, int type, const uint64_t (&x)[8]) {
+    constexpr int N = Lane<TYPE>::N, P = 8 / N;             // words, and channel pairs of one
+    off += l.first;
     if (type == SJK_F32) {
-        float * x = static_cast<float *>(base) + off;
-        float4 * u = reinterpret_cast<float4 *>(x + d0), * v = reinterpret_cast<float4 *>(x + d1);
-        u[0] = make_float4(a[0], a[1], a[2], a[3]);
-        u[1] = make_float4(a[4], a[5], a[6], a[7]);
-        v[0] = make_float4(b[0], b[1], b[2], b[3]);
-        v[1] = make_float4(b[4], b[5], b[6], b[7]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            ulonglong2 * d = reinterpret_cast<ulonglong2 *>(static_cast<float *>(base) + off + i * l.apart);
+#pragma unroll
+            for (int k = 0; k < P / 2; ++k) d[k] = make_ulonglong2(x[P * i + 2 * k], x[P * i + 2 * k + 1]);
+        }
+        return;
+    }
+    uint32_t w[8];
+    if (type == SJK_F16) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const float2 f = both(x[i]); w[i] = pack2<SJK_F16>(f.x, f.y); }
     } else {
-        uint16_t * x = static_cast<uint16_t *>(base) + off;
-        uint4 u, v;
-        if (type == SJK_F16) { u = pack8<SJK_F16>(a); v = pack8<SJK_F16>(b); }
-        else { u = pack8<SJK_BF16>(a); v = pack8<SJK_BF16>(b); }
-        *reinterpret_cast<uint4 *>(x + d0) = u;
-        *reinterpret_cast<uint4 *>(x + d1) = v;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const float2 f = both(x[i]); w[i] = pack2<SJK_BF16>(f.x, f.y); }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        uint16_t * d = static_cast<uint16_t *>(base) + off + i * l.apart;
+        if constexpr (P == 4) *reinterpret_cast<uint4 *>(d) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        else *reinterpret_cast<uint2 *>(d) = make_uint2(w[2 * i], w[2 * i + 1]);
     }
 }
 
-// Lane c of a head: its two chunks' first channels, and whether they rotate.
-SJK_DEV bool lane_chunks(const Params & p, int c, int * d0, int * d1) {
-    const int nr = p.n_rot / 16;
-    const bool rot = c < nr;
-    if (p.layout == SJK_ROPE_HALF && rot) { *d0 = 8 * c; *d1 = p.n_rot / 2 + 8 * c; }
-    else { *d0 = 16 * c; *d1 = 16 * c + 8; }
-    return rot;
-}
-
-// The tokens of blocks [ka, kb) of a tile in one head of q, k or v: norm (NORM) and rotation (ROT). A block is a token
-// for each of the warp's groups of L lanes; the loads of the next block are out while one is worked on.
-template <int TYPE, int L, bool NORM, bool ROT>
-SJK_DEV void head_tokens(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const float4 * s_tab, const float * s_w,
-                         const int32_t * s_pos, const int64_t * s_slot) {
-    const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
-    const sjk_rows & out = part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2];
-    void * cache = part == 0 ? nullptr : part == 1 ? p.c.k : p.c.v;
-    const int c = threadIdx.x & (L - 1), nr = p.n_rot / 16;
-    int d0, d1;
-    const bool rot = lane_chunks(p, c, &d0, &d1) && ROT;
-    const bool on = 16 * L == p.D || 16 * c < p.D;
-    constexpr int G = 32 / L;
-    int t = ka * G + (threadIdx.x & 31) / L;
-    const int end = min(nt, kb * G);
-    int64_t src = (int64_t) (t0 + t) * in.row_stride + (int64_t) hh * in.head_stride;
-    int64_t dst = (int64_t) (t0 + t) * out.row_stride + (int64_t) hh * out.head_stride;
-    const int64_t head = (int64_t) hh * p.c.head_stride;
-    float w0[8], w1[8];
-    if constexpr (NORM) {
-        const float4 * w = reinterpret_cast<const float4 *>(s_w + (part ? p.D : 0));
-        const float4 x[4] = {w[d0 / 4 * on], w[(d0 / 4 + 1) * on], w[d1 / 4 * on], w[(d1 / 4 + 1) * on]};
-        w0[0] = x[0].x; w0[1] = x[0].y; w0[2] = x[0].z; w0[3] = x[0].w; w0[4] = x[1].x; w0[5] = x[1].y; w0[6] = x[1].z; w0[7] = x[1].w;
-        w1[0] = x[2].x; w1[1] = x[2].y; w1[2] = x[2].z; w1[3] = x[2].w; w1[4] = x[3].x; w1[5] = x[3].y; w1[6] = x[3].z; w1[7] = x[3].w;
-    }
-    Raw<TYPE> ra = {}, rb = {};
-    if (on && t < end) { ra = load8<TYPE>(in.p, src + d0); rb = load8<TYPE>(in.p, src + d1); }
-    for (int k = ka; k < kb; ++k, t += G) {
-        float a[8], b[8];
-        widen8<TYPE>(ra, a);
-        widen8<TYPE>(rb, b);
-        src += G * in.row_stride;
-        if (on && t + G < end) { ra = load8<TYPE>(in.p, src + d0); rb = load8<TYPE>(in.p, src + d1); }
-        if constexpr (NORM) {
-            float s0 = 0.0f, s1 = 0.0f;     // idle lanes hold zeros
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { s0 = fmaf(a[i], a[i], s0); s1 = fmaf(b[i], b[i], s1); }
-            float ss = s0 + s1;
-#pragma unroll
-            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
-            const float r = rsqrtf(ss * p.inv_d + p.eps);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { a[i] *= r * w0[i]; b[i] *= r * w1[i]; }
-        }
-        if (t >= end) break;                // (its groups' last tokens; the sums above needed all lanes)
-        if (rot) {
-            const float4 * tab = s_tab + (size_t) t * 4 * nr + c;
-            const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
-            const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-            const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-            if (p.layout == SJK_ROPE_HALF) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = a[i], y = b[i];
-                    a[i] = x * cs[i] - y * sn[i];
-                    b[i] = x * sn[i] + y * cs[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = a[2 * i], y = a[2 * i + 1];
-                    a[2 * i] = x * cs[i] - y * sn[i];
-                    a[2 * i + 1] = x * sn[i] + y * cs[i];
-                    x = b[2 * i]; y = b[2 * i + 1];
-                    b[2 * i] = x * cs[4 + i] - y * sn[4 + i];
-                    b[2 * i + 1] = x * sn[4 + i] + y * cs[4 + i];
-                }
-            }
-        }
-        const bool live = on && s_pos[t] >= 0;
-        if (live && out.p) store16(out.p, dst, d0, d1, out.type, a, b);
-        if (live && cache && s_slot[t] >= 0) store16(cache, s_slot[t] + head, d0, d1, p.c.type, a, b);
-        dst += G * out.row_stride;
-    }
-}
-
-// grid.x: tiles of T tokens; grid.y CTAs share a tile's heads. L: lanes of a head, the power of two from D / 16 on.
-// The (head, block of tokens) items of a tile, in the order of heads, are cut into equal runs, one per warp: its groups of L
-// lanes work on as many tokens of the same head.
-template <int TYPE, int L>
-__global__ void __launch_bounds__(NT, 3) qkv_vec_kernel(const __grid_constant__ Params p) {
-    extern __shared__ float4 s_tab[];       // [T][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7 of a lane's 8 angles,
-    __shared__ int32_t s_pos[MAX_T];        // then the norm weights of q and k
-    __shared__ int64_t s_slot[MAX_T];
-    pdl_wait();
-    pdl_release();
-    const int tid = threadIdx.x, t0 = blockIdx.x * p.T, nt = min(p.T, p.n_tok - t0);
-    const int half = p.n_rot / 2, nr = p.n_rot / 16;
-    float * s_w = reinterpret_cast<float *>(s_tab + p.T * 4 * nr);
+// What the tokens of a tile share: positions, cache slots, and the cosines and sines of every lane's 8 angles, as
+// tab[t][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7.
+template <int TYPE>
+SJK_DEV void tile_table(const Params & p, int t0, int nt, float4 * tab, int32_t * s_pos, int64_t * s_slot) {
+    const int tid = threadIdx.x, half = p.n_rot / 2, nr = p.n_rot / 16;
     if (tid < nt) {
         const int32_t pos = p.pos ? p.pos[t0 + tid] : 0;
         s_pos[tid] = pos;
         s_slot[tid] = p.c.k && pos >= 0 ? cache_slot(p, t0 + tid, pos) : -1;
     }
-    for (int i = tid; i < 2 * p.D; i += NT) {
+    if (half == 0) return;
+    // angles of a word (side by side in the head), as a power of two: a channel each, or in pairs
+    const int lw = (TYPE == SJK_F32 ? 2 : 3) - (p.layout == SJK_ROPE_PAIR ? 1 : 0);
+    const int dt = NT / half, dj = NT - dt * half;
+    for (int t = tid / half, j = tid - t * half; t < nt;) {
+        const float2 cs = angle(p.step[j], p.pos[t0 + t], p.amp);
+        int q = 0, k = j;                   // word, and angle within the words q of all lanes
+        while (k >= nr << lw) { k -= nr << lw; ++q; }
+        const int c = k >> lw, e = (q << lw) + (k & ((1 << lw) - 1));
+        float * d = reinterpret_cast<float *>(tab + (size_t) t * 4 * nr) + (e >> 2) * nr * 4 + c * 4 + (e & 3);
+        d[0] = cs.x;
+        d[2 * nr * 4] = cs.y;
+        t += dt;
+        j += dj;
+        if (j >= half) { j -= half; ++t; }
+    }
+}
+SJK_DEV void norm_weights(const Params & p, float * s_w) {
+    for (int i = threadIdx.x; i < 2 * p.D; i += NT) {
         const void * w = i < p.D ? p.w[0] : p.w[1];
         if (w) s_w[i] = load1(w, i < p.D ? i : i - p.D, p.w_type) + p.w_bias;
     }
-    for (int i = tid; i < nt * half; i += NT) {
-        const int t = i / half, j = i - t * half, c = j >> 3, e = j & 7;
-        const float2 cs = angle(p.step[j], p.pos[t0 + t], p.amp);
-        float * d = reinterpret_cast<float *>(s_tab + (size_t) t * 4 * nr);
-        d[((e >> 2) * nr + c) * 4 + (e & 3)] = cs.x;
-        d[((2 + (e >> 2)) * nr + c) * 4 + (e & 3)] = cs.y;
+}
+
+// The tokens of blocks [ka, kb) of a tile in one head of q, k or v: norm (NORM) and rotation (ROT). A block is a token
+// for each of the warp's groups of L lanes; the loads of the next block are out while one is worked on. The head's row
+// of the tile's token 0 begins at element `src` of x.
+template <int TYPE, int L, bool NORM, bool ROT>
+SJK_DEV void head_tokens(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const void * x, int64_t src, int64_t step,
+                         const float4 * tab0, const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
+    const sjk_rows & out = part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2];
+    void * cache = part == 0 ? nullptr : part == 1 ? p.c.k : p.c.v;
+    const int c = threadIdx.x & (L - 1), nr = p.n_rot / 16;
+    const Lane<TYPE> l(p, c);
+    constexpr int G = 32 / L, N = Lane<TYPE>::N, WORD = Lane<TYPE>::WORD;
+    int t = ka * G + (threadIdx.x & 31) / L;
+    const int end = min(nt, kb * G);
+    src += t * step;
+    int64_t dst = (int64_t) (t0 + t) * out.row_stride + (int64_t) hh * out.head_stride;
+    const int64_t head = (int64_t) hh * p.c.head_stride;
+    const float * w = s_w + (part ? p.D : 0) + l.first;
+    Raw<TYPE> raw = {};
+    if (l.on && t < end) raw = load16<TYPE>(x, src, l);
+    for (int k = ka; k < kb; ++k, t += G) {
+        uint64_t a[8];
+        widen16<TYPE>(raw, a);
+        src += G * step;
+        if (l.on && t + G < end) raw = load16<TYPE>(x, src, l);
+        if constexpr (NORM) {
+            uint64_t s0 = mul2(a[0], a[0]), s1 = mul2(a[1], a[1]);      // idle lanes hold zeros
+#pragma unroll
+            for (int i = 2; i < 8; i += 2) { s0 = fma2(a[i], a[i], s0); s1 = fma2(a[i + 1], a[i + 1], s1); }
+            const float2 f0 = both(s0), f1 = both(s1);
+            float ss = (f0.x + f0.y) + (f1.x + f1.y);
+#pragma unroll
+            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
+            const float r = rsqrtf(ss * p.inv_d + p.eps);
+            const uint64_t r2 = two(r, r);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+#pragma unroll
+                for (int j = 0; j < WORD / 4; ++j) {
+                    const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(w + i * l.apart + 4 * j);
+                    uint64_t & u = a[i * WORD / 2 + 2 * j], & v = a[i * WORD / 2 + 2 * j + 1];
+                    u = mul2(u, mul2(r2, y.x));
+                    v = mul2(v, mul2(r2, y.y));
+                }
+        }
+        if (t >= end) break;                // (its groups' last tokens; the sums above needed all lanes)
+        if (ROT && l.rot) {
+            const float4 * tab = tab0 + (size_t) t * 4 * nr + c;
+            if (p.layout == SJK_ROPE_HALF) {
+                const ulonglong2 c0 = *reinterpret_cast<const ulonglong2 *>(tab), c1 = *reinterpret_cast<const ulonglong2 *>(tab + nr);
+                const ulonglong2 s0 = *reinterpret_cast<const ulonglong2 *>(tab + 2 * nr), s1 = *reinterpret_cast<const ulonglong2 *>(tab + 3 * nr);
+                const uint64_t cs[4] = {c0.x, c0.y, c1.x, c1.y}, sn[4] = {s0.x, s0.y, s1.x, s1.y};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint64_t u = a[i], v = a[4 + i];
+                    a[i] = fma2(u, cs[i], mul2(neg2(v), sn[i]));
+                    a[4 + i] = fma2(v, cs[i], mul2(u, sn[i]));
+                }
+            } else {
+                const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
+                const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+                const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 u = both(a[i]);
+                    a[i] = two(fmaf(u.x, cs[i], -u.y * sn[i]), fmaf(u.y, cs[i], u.x * sn[i]));
+                }
+            }
+        }
+        const bool live = l.on && s_pos[t] >= 0;
+        if (live && out.p) store16<TYPE>(out.p, dst, l, out.type, a);
+        if (live && cache && s_slot[t] >= 0) store16<TYPE>(cache, s_slot[t] + head, l, p.c.type, a);
+        dst += G * out.row_stride;
     }
+}
+template <int TYPE, int L>
+SJK_DEV void head_blocks(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const void * x, int64_t src, int64_t step,
+                         const float4 * tab, const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
+    if (part == 2) head_tokens<TYPE, L, false, false>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
+    else if (part == 0 ? p.w[0] : p.w[1]) head_tokens<TYPE, L, true, true>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
+    else head_tokens<TYPE, L, false, true>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
+}
+
+// Few tokens. grid.x: tokens; grid.y CTAs share the heads, a warp each. L: lanes of a head, the power of two from
+// D / 16 on.
+template <int TYPE, int L>
+__global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ Params p) {
+    extern __shared__ float4 s_tab[];       // [4][n_rot / 16], then the norm weights of q and k
+    __shared__ int32_t s_pos[1];
+    __shared__ int64_t s_slot[1];
+    pdl_wait();
+    pdl_release();
+    float * s_w = reinterpret_cast<float *>(s_tab + p.n_rot / 4);
+    const int t0 = blockIdx.x, h = blockIdx.y * (NT / 32) + threadIdx.x / 32;
+    tile_table<TYPE>(p, t0, 1, s_tab, s_pos, s_slot);
+    if (p.w[0] || p.w[1]) norm_weights(p, s_w);
     __syncthreads();
+    if (h >= p.n_all) return;
+    int hh;
+    const int part = part_of(p, h, &hh);
+    const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
+    head_blocks<TYPE, L>(p, part, hh, t0, 1, 0, 1, in.p, (int64_t) t0 * in.row_stride + (int64_t) hh * in.head_stride, 0, s_tab, s_w, s_pos, s_slot);
+}
+
+// Many tokens. A CTA has the tokens [n i / ctas, n (i + 1) / ctas), in tiles of T. Its warps take neighbouring heads of
+// a tile's tokens at a time; the heads that do not go round are cut by blocks of tokens.
+template <int TYPE, int L>
+__global__ void __launch_bounds__(NT, ctas_of(TYPE)) qkv_tile_kernel(const __grid_constant__ Params p) {
+    extern __shared__ float4 s_tab[];       // [2][T][4][n_rot / 16], then the norm weights of q and k
+    __shared__ int32_t s_pos[2][32];
+    __shared__ int64_t s_slot[2][32];
+    pdl_wait();
+    pdl_release();
     constexpr int G = 32 / L, WARPS = NT / 32;
-    const int blocks = (nt + G - 1) / G, items = blocks * p.n_all;
-    const int each = (items + WARPS * (int) gridDim.y - 1) / (WARPS * (int) gridDim.y);
-    int item = ((int) blockIdx.y * WARPS + tid / 32) * each;
-    const int end = min(item + each, items);
-    while (item < end) {
-        const int h = item / blocks, ka = item - h * blocks, kb = min(blocks, ka + end - item);
-        int hh;
-        const int part = part_of(p, h, &hh);
-        if (part == 2) head_tokens<TYPE, L, false, false>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
-        else if (part == 0 ? p.w[0] : p.w[1]) head_tokens<TYPE, L, true, true>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
-        else head_tokens<TYPE, L, false, true>(p, part, hh, t0, nt, ka, kb, s_tab, s_w, s_pos, s_slot);
-        item += kb - ka;
+    const int one = p.T * (p.n_rot / 4);
+    float * s_w = reinterpret_cast<float *>(s_tab + 2 * one);
+    if (p.w[0] || p.w[1]) norm_weights(p, s_w);
+    const int last = (int) ((int64_t) p.n_tok * (blockIdx.x + 1) / gridDim.x), warp = threadIdx.x / 32;
+    int t0 = (int) ((int64_t) p.n_tok * blockIdx.x / gridDim.x);
+    if (t0 < last) tile_table<TYPE>(p, t0, min(p.T, last - t0), s_tab, s_pos[0], s_slot[0]);
+    for (int s = 0; t0 < last; t0 += p.T, s ^= 1) {
+        const int nt = min(p.T, last - t0), next = t0 + p.T;
+        __syncthreads();                    // this tile's table is complete, the other one is free
+        if (next < last) tile_table<TYPE>(p, next, min(p.T, last - next), s_tab + (s ? 0 : one), s_pos[s ^ 1], s_slot[s ^ 1]);
+        const int blocks = (nt + G - 1) / G, full = p.n_all / WARPS * WARPS;
+        const int items = blocks * (p.n_all - full), each = (items + WARPS - 1) / WARPS;
+        int h = warp, ka = 0, kb = blocks, item = warp * each;
+        const int end = min(item + each, items);
+        for (;;) {
+            if (h >= full) {                // the heads that are left
+                if (item >= end) break;
+                h = item / blocks;
+                ka = item - h * blocks;
+                kb = min(blocks, ka + end - item);
+                h += full;
+                item += kb - ka;
+            }
+            int hh;
+            const int part = part_of(p, h, &hh);
+            const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
+            head_blocks<TYPE, L>(p, part, hh, t0, nt, ka, kb, in.p, (int64_t) t0 * in.row_stride + (int64_t) hh * in.head_stride, in.row_stride, s_tab + (s ? one : 0), s_w, s_pos[s],
+                                 s_slot[s]);
+            h += WARPS;
+        }
     }
 }
 
@@ -305,16 +408,28 @@ __global__ void __launch_bounds__(NT) qkv_scalar_kernel(const __grid_constant__ 
     }
 }
 
-template <int TYPE>
-int launch_vec(int L, dim3 grid, size_t smem, sjk_stream st, const Params & p) {
-    switch (L) {
-        case 1: return launch(qkv_vec_kernel<TYPE, 1>, grid, dim3(NT), smem, st, p);
-        case 2: return launch(qkv_vec_kernel<TYPE, 2>, grid, dim3(NT), smem, st, p);
-        case 4: return launch(qkv_vec_kernel<TYPE, 4>, grid, dim3(NT), smem, st, p);
-        case 8: return launch(qkv_vec_kernel<TYPE, 8>, grid, dim3(NT), smem, st, p);
-        case 16: return launch(qkv_vec_kernel<TYPE, 16>, grid, dim3(NT), smem, st, p);
-        default: return launch(qkv_vec_kernel<TYPE, 32>, grid, dim3(NT), smem, st, p);
+template <int TYPE, int L>
+int launch_vec(sjk_stream st, Params & p) {
+    const size_t weights = 2 * (size_t) p.D * sizeof(float);
+    constexpr int slots = 148 * ctas_of(TYPE), least = 32 / L > 4 ? 32 / L : 4;      // tokens of a run, at least
+    if (p.n_tok >= slots) {
+        int waves = p.n_tok / (slots * least);
+        waves = waves < 1 ? 1 : waves > WAVES ? WAVES : waves;
+        const int ctas = slots * waves, run = (p.n_tok + ctas - 1) / ctas, most = 32 / L > MAX_T ? 32 / L : MAX_T;
+        const int tiles = (run + most - 1) / most;
+        p.T = (run + tiles - 1) / tiles;
+        const size_t smem = 2 * (size_t) p.T * p.n_rot * sizeof(float) + weights;
+        if (smem > 47 * 1024 && sjk_check(cudaFuncSetAttribute(qkv_tile_kernel<TYPE, L>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem))) return SJK_ERR_DEVICE;
+        return launch(qkv_tile_kernel<TYPE, L>, dim3((unsigned) ctas), dim3(NT), smem, st, p);
     }
+    p.T = 1;
+    const dim3 grid((unsigned) p.n_tok, (unsigned) ((p.n_all + NT / 32 - 1) / (NT / 32)));
+    return launch(qkv_token_kernel<TYPE, L>, grid, dim3(NT), (size_t) p.n_rot * sizeof(float) + weights, st, p);
+}
+template <int TYPE>
+int launch_lanes(sjk_stream st, Params & p) {
+    return p.D <= 16 ? launch_vec<TYPE, 1>(st, p) : p.D <= 32 ? launch_vec<TYPE, 2>(st, p) : p.D <= 64 ? launch_vec<TYPE, 4>(st, p) :
+           p.D <= 128 ? launch_vec<TYPE, 8>(st, p) : p.D <= 256 ? launch_vec<TYPE, 16>(st, p) : launch_vec<TYPE, 32>(st, p);
 }
 
 bool rows_vec(const sjk_rows & r) {
@@ -465,23 +580,10 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
         const int64_t warps = (int64_t) p.n_tok * p.n_all, ctas = (warps + NT / 32 - 1) / (NT / 32);
         return launch(qkv_scalar_kernel, dim3((unsigned) (ctas < 148 * 8 ? ctas : 148 * 8)), dim3(NT), (size_t) (NT / 32) * p.D * sizeof(float), st, p);
     }
-    int L = 1;
-    while (16 * L < p.D) L <<= 1;
-    // Few tokens: one token per CTA and the heads over grid.y. Many: all heads in one CTA and several tokens (a block
-    // of 32 / L at least), so that the table and the norm weights serve several rows.
-    int T = 1, ny = (p.n_all + NT / 32 - 1) / (NT / 32);
-    if (p.n_tok >= 148 * 8) {
-        ny = 1;
-        T = 32 / L > 8 ? 32 / L : 8;
-        while (T > 32 / L && p.n_tok / T < 148 * 4) T /= 2;
-    }
-    p.T = T;
-    const dim3 grid((unsigned) ((p.n_tok + T - 1) / T), (unsigned) ny);
-    const size_t smem = ((size_t) T * p.n_rot + 2 * (size_t) p.D) * sizeof(float);
     switch (type) {
-        case SJK_F32: return launch_vec<SJK_F32>(L, grid, smem, st, p);
-        case SJK_F16: return launch_vec<SJK_F16>(L, grid, smem, st, p);
-        default: return launch_vec<SJK_BF16>(L, grid, smem, st, p);
+        case SJK_F32: return launch_lanes<SJK_F32>(st, p);
+        case SJK_F16: return launch_lanes<SJK_F16>(st, p);
+        default: return launch_lanes<SJK_BF16>(st, p);
     }
 }
 
