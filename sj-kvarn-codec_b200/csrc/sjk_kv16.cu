@@ -806,8 +806,9 @@ template <typename S>
 int run(const Params & p0, const Plan & pl, sjk_stream st) {
     static_assert(S::CTA_BYTES <= 227 * 1024, "shared memory of a CTA");
     Params p = p0;
-    if (sjk_check(cudaFuncSetAttribute(kv16_attend_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::CTA_BYTES))) return SJK_ERR_DEVICE;
-    const int rc = launch(kv16_attend_kernel<S>, dim3(148), dim3(32 * S::W), S::CTA_BYTES, st, p);
+    int rc = smem_limit<kv16_attend_kernel<S>>(S::CTA_BYTES);
+    if (rc) return rc;
+    rc = launch(kv16_attend_kernel<S>, dim3(148), dim3(32 * S::W), S::CTA_BYTES, st, p);
     if (rc) return rc;
     // few pairs: many slots each, so a CTA per query head; many: two or three slots each, a warp per query head
     const int64_t pairs = (int64_t) p.n_seq * p.c.n_head_kv * p.tiles;

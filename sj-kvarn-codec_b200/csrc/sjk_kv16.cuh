@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "sjk_common.cuh"
 
 namespace sjk16 {
@@ -54,6 +56,19 @@ static inline int launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return sjk_check(cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...));
+}
+
+// A kernel's dynamic shared memory limit, raised to `bytes` on the current device at the first call there.
+template <auto KERNEL>
+static inline int smem_limit(size_t bytes) {
+    static std::atomic<uint64_t> done{0};
+    int dev = 0;
+    if (sjk_check(cudaGetDevice(&dev))) return SJK_ERR_DEVICE;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0ull;
+    if (done.load(std::memory_order_relaxed) & bit) return 0;
+    if (sjk_check(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) bytes))) return SJK_ERR_DEVICE;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return 0;
 }
 
 }  // namespace sjk16

@@ -19,11 +19,11 @@ __device__ unsigned int g_pages_status;
 
 SJK_DEV void flag() { atomicOr(&g_pages_status, (unsigned) SJK_DEVICE_PAGE); }
 
-// The ledger: the device pool's header and stack (sjk_pool_dev_bytes), then per-page words. Ticket, count, last and
-// marks are zero between calls.
+// The ledger: the device pool's header and stack (sjk_pool_dev_bytes), then per-page words. Ticket, claims, count, last
+// and marks are zero between calls.
 struct Ledger {
     uint32_t * head;                        // n_free, n_pages, ticket of sjk_pages_free, copies of the last call
-    uint32_t * ids, * shares, * count, * last, * old, * src, * dst, * map, * marks;
+    uint32_t * ids, * shares, * count, * last, * old, * src, * dst, * map, * marks, * claims;
 };
 SJK_HD Ledger ledger_of(void * base, uint32_t n) {
     Ledger l;
@@ -37,7 +37,8 @@ SJK_HD Ledger ledger_of(void * base, uint32_t n) {
     l.src = w;       w += n;
     l.dst = w;       w += n;
     l.map = w;       w += n;
-    l.marks = w;
+    l.marks = w;     w += (n + 31u) / 32u;
+    l.claims = w;
     return l;
 }
 
@@ -167,14 +168,17 @@ __global__ void __launch_bounds__(NT) pages_free_kernel(const __grid_constant__ 
 }
 
 // ---- extend: one CTA; an item is an entry (request, page) -----------------------------------------------------------
-__global__ void __launch_bounds__(NB) pages_extend_kernel(const __grid_constant__ Params p) {
-    __shared__ uint32_t s_scan[NB / 32];
-    __shared__ int32_t s_row[NB], s_len[NB];
-    __shared__ uint32_t s_g0[NB], s_off[NB];
+// NTHR threads, at least a thread per request. Up to NTHR items (a decode step) stay in registers from phase to phase;
+// more go round by NTHR.
+template <int NTHR>
+__global__ void __launch_bounds__(NTHR) pages_extend_kernel(const __grid_constant__ Params p) {
+    __shared__ uint32_t s_scan[NTHR / 32];
+    __shared__ int32_t s_row[NTHR], s_len[NTHR];
+    __shared__ uint32_t s_g0[NTHR], s_off[NTHR];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x;
-    const uint32_t P = (uint32_t) p.page_tokens;
+    const uint32_t P = (uint32_t) p.page_tokens, n_free = p.l.head[0];
     // the requests: rows, first pages, and where their items begin
     int bad = 0, much = 0;                                  // much: more entries than there are pages
     uint32_t items = 0;
@@ -189,8 +193,10 @@ __global__ void __launch_bounds__(NB) pages_extend_kernel(const __grid_constant_
             much = items > p.n_pages;
         }
     }
-    __syncthreads();
-    if (tid < p.n && !bad)
+    uint32_t n_items;
+    const uint32_t off = cta_scan<NTHR>(much || bad ? 0u : items, s_scan, &n_items);
+    s_off[tid] = off;
+    if (tid < p.n)
         for (int j = 0; j < tid; ++j) bad |= s_row[j] == s_row[tid] ? 1 : 0;
     bad = __syncthreads_or(bad);
     much = __syncthreads_or(much);
@@ -198,80 +204,73 @@ __global__ void __launch_bounds__(NB) pages_extend_kernel(const __grid_constant_
         if (tid == 0) { p.status[0] = bad ? SJKVARN_ERR_ARG : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
         return;
     }
-    uint32_t n_items;
-    const uint32_t off = cta_scan<NB>(items, s_scan, &n_items);
-    s_off[tid] = off;
-    __syncthreads();
-    auto find = [&](uint32_t it) {                          // request of an item: the last whose items begin at or before it
+    // an item: its request (the last whose items begin at or before it), table entry, page and how many share that
+    struct Item { int r; uint32_t * at; uint32_t e, shares; };
+    auto item_of = [&](uint32_t it) {
+        Item x = {0, nullptr, NO_BLOCK, 0u};
+        if (it >= n_items) return x;
         int lo = 0, hi = p.n - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (s_off[mid] <= it) lo = mid; else hi = mid - 1;
         }
-        return lo;
+        x.r = lo;
+        x.at = p.tables + (size_t) s_row[lo] * p.stride + s_g0[lo] + (it - s_off[lo]);
+        x.e = *x.at;
+        if (x.e < p.n_pages) x.shares = p.l.shares[x.e];
+        return x;
     };
-    auto entry = [&](int r, uint32_t it) { return p.tables + (size_t) s_row[r] * p.stride + s_g0[r] + (it - s_off[r]); };
+    // a hole, or a shared page that is not kept: the last of a page's owners keeps it when all are in the call
+    auto takes = [&](const Item & x) {
+        if (!x.at) return false;
+        if (x.e == NO_BLOCK) return true;
+        return x.shares && !(__ldcg(&p.l.count[x.e]) == x.shares + 1u && __ldcg(&p.l.last[x.e]) == (uint32_t) x.r);
+    };
+    const bool one = n_items <= (uint32_t) NTHR;
+    const Item mine = item_of(tid);
     // who holds the shared pages: how many of the call, and the last of them
     int wrong = 0;
-    for (uint32_t it = tid; it < n_items; it += NB) {
-        const int r = find(it);
-        const uint32_t e = *entry(r, it);
-        if (e == NO_BLOCK) continue;
-        if (e >= p.n_pages) { wrong = 1; continue; }
-        if (p.l.shares[e]) { atomicAdd(&p.l.count[e], 1u); atomicMax(&p.l.last[e], (uint32_t) r); }
+    for (uint32_t it = tid; it < n_items; it += NTHR) {
+        const Item x = one ? mine : item_of(it);
+        if (x.e != NO_BLOCK && x.e >= p.n_pages) wrong = 1;
+        else if (x.shares) { atomicAdd(&p.l.count[x.e], 1u); atomicMax(&p.l.last[x.e], (uint32_t) x.r); }
     }
     wrong = __syncthreads_or(wrong);
-    // a hole, or a shared page that is not kept
-    auto takes = [&](int r, uint32_t e) {
-        if (e == NO_BLOCK) return true;
-        if (e >= p.n_pages || !p.l.shares[e]) return false;
-        return !(__ldcg(&p.l.count[e]) == p.l.shares[e] + 1u && __ldcg(&p.l.last[e]) == (uint32_t) r);
-    };
-    const uint32_t n_free = p.l.head[0];
     uint32_t need = 0;
-    for (uint32_t it = tid; it < n_items; it += NB) {
-        const int r = find(it);
-        need += takes(r, *entry(r, it)) ? 1u : 0u;
-    }
+    for (uint32_t it = tid; it < n_items; it += NTHR) need += takes(one ? mine : item_of(it)) ? 1u : 0u;
     uint32_t total;
-    cta_scan<NB>(need, s_scan, &total);
+    const uint32_t before_mine = cta_scan<NTHR>(need, s_scan, &total);
     if (wrong || total > n_free) {                          // nothing is done: only the counts go back
-        for (uint32_t it = tid; it < n_items; it += NB) {
-            const uint32_t e = *entry(find(it), it);
+        for (uint32_t it = tid; it < n_items; it += NTHR) {
+            const uint32_t e = (one ? mine : item_of(it)).e;
             if (e < p.n_pages) { p.l.count[e] = 0u; p.l.last[e] = 0u; }
         }
         if (tid == 0) { p.status[0] = wrong ? SJKVARN_ERR_CORRUPT : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
         return;
     }
     uint32_t taken = 0, copies = 0;
-    for (uint32_t it0 = 0; it0 < n_items; it0 += NB) {
+    for (uint32_t it0 = 0; it0 < n_items; it0 += NTHR) {
         const uint32_t it = it0 + tid;
-        uint32_t e = NO_BLOCK, * at = nullptr;
-        bool take = false, keep = false;
-        if (it < n_items) {
-            const int r = find(it);
-            at = entry(r, it);
-            e = *at;
-            take = takes(r, e);
-            keep = take && e != NO_BLOCK && (uint64_t) (s_g0[r] + (it - s_off[r])) * P < (uint64_t) (uint32_t) s_len[r];
-        }
-        uint32_t both;
-        const uint32_t before = cta_scan<NB>((take ? 1u : 0u) | (keep ? 0x10000u : 0u), s_scan, &both);
+        const Item x = one ? mine : item_of(it);
+        const bool take = one ? need != 0u : takes(x);
+        const bool keep = take && x.e != NO_BLOCK && (uint64_t) (s_g0[x.r] + (it - s_off[x.r])) * P < (uint64_t) (uint32_t) s_len[x.r];
+        uint32_t takes_all = total, keeps_all, before = before_mine;
+        if (!one) before = cta_scan<NTHR>(take ? 1u : 0u, s_scan, &takes_all);
+        const uint32_t q = cta_scan<NTHR>(keep ? 1u : 0u, s_scan, &keeps_all);
         if (take) {
-            const uint32_t k = taken + (before & 0xFFFFu), id = p.l.ids[n_free - 1u - k];
-            *at = id;
-            p.l.old[k] = e;
+            const uint32_t k = taken + before, id = p.l.ids[n_free - 1u - k];
+            *x.at = id;
+            p.l.old[k] = x.e;
             if (keep) {
-                const uint32_t q = copies + (before >> 16);
-                p.l.src[q] = e;
-                p.l.dst[q] = id;
+                p.l.src[copies + q] = x.e;
+                p.l.dst[copies + q] = id;
             }
         }
-        taken += both & 0xFFFFu;
-        copies += both >> 16;
+        taken += takes_all;
+        copies += keeps_all;
     }
     __syncthreads();
-    for (uint32_t k = tid; k < total; k += NB) {
+    for (uint32_t k = tid; k < total; k += NTHR) {
         const uint32_t e = p.l.old[k];
         if (e == NO_BLOCK) continue;
         atomicSub(&p.l.shares[e], 1u);
@@ -336,11 +335,13 @@ __global__ void __launch_bounds__(NB) pages_plan_kernel(const __grid_constant__ 
     }
 }
 
-// Contents of the listed pages in every layer of every slab, in segments of SEG bytes over a grid that fills the GPU;
-// remap: the tables' entries of moved pages as well. n < 0: as many as the ledger says.
+// Contents of the listed pages in every layer of every slab, in segments of SEG bytes, which the CTAs of a grid that
+// fills the GPU claim one by one (SMs are not equally fast: with equal shares the slow ones would end last); remap: the
+// tables' entries of moved pages as well. n_fixed < 0: as many as the ledger says.
 constexpr uint32_t SEG = 16384;
 __global__ void __launch_bounds__(NT) pages_copy_kernel(const __grid_constant__ Params p, const uint32_t * src, const uint32_t * dst, int n_fixed,
                                                         int remap) {
+    __shared__ uint32_t s_next[2];
     pdl_wait();
     pdl_release();
     const uint32_t n = n_fixed >= 0 ? (uint32_t) n_fixed : p.l.head[3];
@@ -356,16 +357,28 @@ __global__ void __launch_bounds__(NT) pages_copy_kernel(const __grid_constant__ 
             else flag();                                    // an entry whose page is not in use
         }
     }
-    for (int s = 0; s < p.n_slabs; ++s) {
+    if (p.n_slabs == 0) return;
+    uint64_t u = blockIdx.x;
+    for (uint32_t i = 0;; i ^= 1u) {
+        uint64_t at = u;
+        int s = 0;
+        uint32_t segs = 1, layers = 1;
+        for (; s < p.n_slabs; ++s) {
+            segs = (uint32_t) ((p.slabs[s].page_bytes + SEG - 1) / SEG);
+            layers = (uint32_t) p.slabs[s].n_layers;
+            const uint64_t units = (uint64_t) n * layers * segs;
+            if (at < units) break;
+            at -= units;
+        }
+        if (s == p.n_slabs) break;
+        uint32_t claim = 0;
+        if (threadIdx.x == 0) claim = atomicAdd(p.l.claims, 1u);            // the next one, while this one is copied
         const sjk_slab & sl = p.slabs[s];
-        const uint32_t segs = (uint32_t) ((sl.page_bytes + SEG - 1) / SEG);
-        const uint64_t units = (uint64_t) n * sl.n_layers * segs;
-        for (uint64_t u = blockIdx.x; u < units; u += gridDim.x) {
-            const uint32_t seg = (uint32_t) (u % segs);
-            const uint64_t q = u / segs;
-            const uint32_t k = (uint32_t) (q / sl.n_layers), layer = (uint32_t) (q - (uint64_t) k * sl.n_layers);
-            const uint32_t a = src[k], b = dst[k];
-            if (a >= p.n_pages || b >= p.n_pages) { if (threadIdx.x == 0) flag(); continue; }
+        const uint32_t seg = (uint32_t) (at % segs);
+        const uint64_t q = at / segs;
+        const uint32_t k = (uint32_t) (q / layers), layer = (uint32_t) (q - (uint64_t) k * layers);
+        const uint32_t a = src[k], b = dst[k];
+        if (a < p.n_pages && b < p.n_pages) {
             uint8_t * base = static_cast<uint8_t *>(sl.base) + (size_t) layer * sl.layer_stride + (size_t) seg * SEG;
             const uint4 * from = reinterpret_cast<const uint4 *>(base + (size_t) a * sl.page_bytes);
             uint4 * to = reinterpret_cast<uint4 *>(base + (size_t) b * sl.page_bytes);
@@ -373,12 +386,20 @@ __global__ void __launch_bounds__(NT) pages_copy_kernel(const __grid_constant__ 
             const uint32_t words = (uint32_t) ((left < SEG ? left : SEG) / 16);
             uint4 x[SEG / 16 / NT];
 #pragma unroll
-            for (int i = 0; i < (int) (SEG / 16 / NT); ++i)
-                if (i * NT + threadIdx.x < words) x[i] = from[i * NT + threadIdx.x];
+            for (int j = 0; j < (int) (SEG / 16 / NT); ++j)
+                if (j * NT + threadIdx.x < words) x[j] = from[j * NT + threadIdx.x];
 #pragma unroll
-            for (int i = 0; i < (int) (SEG / 16 / NT); ++i)
-                if (i * NT + threadIdx.x < words) to[i * NT + threadIdx.x] = x[i];
-        }
+            for (int j = 0; j < (int) (SEG / 16 / NT); ++j)
+                if (j * NT + threadIdx.x < words) to[j * NT + threadIdx.x] = x[j];
+        } else if (threadIdx.x == 0) flag();
+        if (threadIdx.x == 0) s_next[i] = claim;
+        __syncthreads();
+        u = (uint64_t) gridDim.x + s_next[i];
+    }
+    // the last CTA leaves the counters as they were
+    if (threadIdx.x == 0 && atomicAdd(&p.l.head[2], 1u) == gridDim.x - 1u) {
+        p.l.claims[0] = 0u;
+        p.l.head[2] = 0u;
     }
 }
 
@@ -407,17 +428,17 @@ __global__ void __launch_bounds__(NT) pages_init_kernel(Ledger l, uint32_t n) {
         l.shares[i] = l.count[i] = l.last[i] = 0u;
         if (i < (n + 31u) / 32u) l.marks[i] = 0u;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) { l.head[0] = l.head[1] = n; l.head[2] = l.head[3] = 0u; }
+    if (blockIdx.x == 0 && threadIdx.x == 0) { l.head[0] = l.head[1] = n; l.head[2] = l.head[3] = l.claims[0] = 0u; }
 }
 
 int copy_launch(const Params & p, const uint32_t * src, const uint32_t * dst, int n, int remap, sjk_stream st) {
     if (p.n_slabs == 0 && !remap) return 0;
-    return launch(pages_copy_kernel, dim3(148 * 4), dim3(NT), 0, st, p, src, dst, n, remap);
+    return launch(pages_copy_kernel, dim3(148 * 6), dim3(NT), 0, st, p, src, dst, n, remap);
 }
 
 }  // namespace
 
-extern "C" size_t sjk_pages_bytes(uint32_t n) { return 16u + ((size_t) n * 8u + (n + 31u) / 32u) * sizeof(uint32_t); }
+extern "C" size_t sjk_pages_bytes(uint32_t n) { return 16u + ((size_t) n * 8u + (n + 31u) / 32u + 1u) * sizeof(uint32_t); }
 
 extern "C" int sjk_pages_init(const sjk_pages * g, sjk_stream st) {
     Params p;
@@ -462,7 +483,7 @@ extern "C" int sjk_pages_extend(const sjk_pages * g, const int32_t * rows, const
     if (n < 0 || n > SJK_PAGES_MAX_ROWS || (n && (!rows || !len || !status)) || (!add && add_all < 0)) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
     p.a = rows; p.b = len; p.c = add; p.add_all = add_all; p.n = n; p.status = status;
-    rc = launch(pages_extend_kernel, dim3(1), dim3(NB), 0, st, p);
+    rc = n <= 256 ? launch(pages_extend_kernel<256>, dim3(1), dim3(256), 0, st, p) : launch(pages_extend_kernel<NB>, dim3(1), dim3(NB), 0, st, p);
     if (rc) return rc;
     return copy_launch(p, p.l.src, p.l.dst, -1, 0, st);
 }
@@ -473,7 +494,7 @@ extern "C" int sjk_pages_compact(const sjk_pages * g, int32_t * info, sjk_stream
     if (rc) return rc;
     p.status = info;
     const size_t smem = (size_t) ((p.n_pages + 31u) / 32u) * sizeof(uint32_t);
-    if (smem > 40 * 1024 && sjk_check(cudaFuncSetAttribute(pages_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem))) return SJK_ERR_DEVICE;
+    if (smem > 40 * 1024 && smem_limit<pages_plan_kernel>(SJK_PAGES_MAX / 8)) return SJK_ERR_DEVICE;
     rc = launch(pages_plan_kernel, dim3(1), dim3(NB), smem, st, p);
     if (rc) return rc;
     return copy_launch(p, p.l.src, p.l.dst, -1, 1, st);

@@ -419,7 +419,7 @@ int launch_vec(sjk_stream st, Params & p) {
         const int tiles = (run + most - 1) / most;
         p.T = (run + tiles - 1) / tiles;
         const size_t smem = 2 * (size_t) p.T * p.n_rot * sizeof(float) + weights;
-        if (smem > 47 * 1024 && sjk_check(cudaFuncSetAttribute(qkv_tile_kernel<TYPE, L>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int) smem))) return SJK_ERR_DEVICE;
+        if (smem > 47 * 1024 && smem_limit<qkv_tile_kernel<TYPE, L>>(2 * (size_t) MAX_T * 512 * sizeof(float) + 4096)) return SJK_ERR_DEVICE;
         return launch(qkv_tile_kernel<TYPE, L>, dim3((unsigned) ctas), dim3(NT), smem, st, p);
     }
     p.T = 1;

@@ -36,29 +36,50 @@ def _lib():
     return _L
 
 
-def _stream():
-    return torch.cuda.current_stream().cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(device):
+    """torch's current stream of a device index, as a number."""
+    return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
+def _index(t):
+    return t.device.index if t.device.index is not None else torch.cuda.current_device()
 
 
 def _list(t, what, n=None):
     """Device pointer of an int32 CUDA vector (None passes)."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or not t.is_cuda or t.dim() != 1 or (t.shape[0] > 1 and t.stride(0) != 1) or (n is not None and t.shape[0] != n):
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.shape[0] != n):
         raise ValueError(f"{what}: an int32 CUDA vector" + (f" of {n} values" if n is not None else ""))
     return t.data_ptr()
 
 
-def _rows(r, t, what, n, D):
-    """Fill a sjk_rows from a [n][heads][D] tensor."""
-    if t is None:
-        r.p = None
-        return
-    shape, stride = t.shape, t.stride()
-    if len(shape) != 3 or shape[0] != n or shape[2] != D or stride[2] != 1 or not t.is_cuda or t.dtype not in _TYPE:
-        raise ValueError(f"{what}: a CUDA tensor [{n}][heads][{D}] of 16- or 32-bit floats, channels adjacent")
-    r.p = t.data_ptr()
-    r.row_stride, r.head_stride, r.n_head, r.type = stride[0], stride[1], shape[1], _TYPE[t.dtype]
+class _Rows:
+    """A sjk_rows filled from [n][heads][D] tensors; a tensor of the last one's shape, strides and type changes the
+    pointer only."""
+
+    def __init__(self, c, what, D):
+        self.c, self.what, self.D, self.like = c, what, D, None
+
+    def set(self, t, n):
+        c = self.c
+        if t is None:
+            if self.like is not None:
+                c.p, self.like = None, None
+            return
+        shape = t.shape
+        like = (shape, t.stride(), t.dtype)
+        if like != self.like or shape[0] != n:
+            if len(shape) != 3 or shape[0] != n or shape[2] != self.D or like[1][2] != 1 or t.dtype not in _TYPE:
+                raise ValueError(f"{self.what}: a CUDA tensor [{n}][heads][{self.D}] of 16- or 32-bit floats, channels adjacent")
+            c.row_stride, c.head_stride, c.n_head, c.type = like[1][0], like[1][1], shape[1], _TYPE[t.dtype]
+            self.like = like
+        if not t.is_cuda:
+            raise ValueError(f"{self.what}: a CUDA tensor")
+        c.p = t.data_ptr()
 
 
 class Rope:
@@ -105,14 +126,14 @@ class Pages:
                 raise ValueError("slabs: CUDA tensors [layers][pages][...], pages of a layer contiguous")
             size = s.element_size()
             c.slabs[i] = sjk.Slab(s.data_ptr(), s.stride(1) * size, s.stride(0) * size, s.shape[0])
-        sjk.check(_lib().sjk_pages_init(C.byref(c), _stream()), "pages_init")
-        self._c = C.byref(c)
+        self._c, self._dev, self._L = C.byref(c), _index(tables), _lib()
+        sjk.check(self._L.sjk_pages_init(self._c, _stream(self._dev)), "pages_init")
         # what the last fork, extend and compact call reported (each overwritten by the next of its kind)
         self._forked = torch.zeros(1024, dtype=torch.int32, device=tables.device)
         self._extended = torch.zeros(1, dtype=torch.int32, device=tables.device)
         self._compacted = torch.zeros(2, dtype=torch.int32, device=tables.device)
         self.n_free, self.ids = self._buf[0:1], self._buf[4:4 + n]
-        at = (_lib().sjk_pages_shares(self._c) - self._buf.data_ptr()) // 4
+        at = (self._L.sjk_pages_shares(self._c) - self._buf.data_ptr()) // 4
         self.shares = self._buf[at:at + n]
         if ids is not None:
             self.ids.copy_(ids)
@@ -122,7 +143,7 @@ class Pages:
         """Rows dst get the pages of rows src, shared. Returns the device status vector (0, or a status code each)."""
         n = src.shape[0]
         st = self._forked if n <= 1024 else torch.empty(n, dtype=torch.int32, device=src.device)
-        rc = _lib().sjk_pages_fork(self._c, _list(src, "src"), _list(dst, "dst", n), n, st.data_ptr(), _stream())
+        rc = self._L.sjk_pages_fork(self._c, _list(src, "src"), _list(dst, "dst", n), n, st.data_ptr(), _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_fork")
         return st[:n]
@@ -132,8 +153,8 @@ class Pages:
         Returns the device status (one value: 0, or why nothing was done)."""
         n = rows.shape[0]
         vec = isinstance(add, torch.Tensor)
-        rc = _lib().sjk_pages_extend(self._c, _list(rows, "rows"), _list(lens, "lens", n), _list(add, "add", n) if vec else None,
-                                     0 if vec else add, n, self._extended.data_ptr(), _stream())
+        rc = self._L.sjk_pages_extend(self._c, _list(rows, "rows"), _list(lens, "lens", n), _list(add, "add", n) if vec else None,
+                                     0 if vec else add, n, self._extended.data_ptr(), _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_extend")
         return self._extended
@@ -141,13 +162,13 @@ class Pages:
     def free(self, rows, first=None, end=None):
         """Entries [first, end) of the rows give their pages up (vectors; None: all)."""
         n = rows.shape[0]
-        rc = _lib().sjk_pages_free(self._c, _list(rows, "rows"), _list(first, "first", n), _list(end, "end", n), n, _stream())
+        rc = self._L.sjk_pages_free(self._c, _list(rows, "rows"), _list(first, "first", n), _list(end, "end", n), n, _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_free")
 
     def compact(self):
         """Used pages to the lowest ids. Returns a device vector: used pages, moved ones."""
-        rc = _lib().sjk_pages_compact(self._c, self._compacted.data_ptr(), _stream())
+        rc = self._L.sjk_pages_compact(self._c, self._compacted.data_ptr(), _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_compact")
         return self._compacted
@@ -155,7 +176,7 @@ class Pages:
     def copy(self, src, dst):
         """Contents of pages src to pages dst, every layer of every slab."""
         n = src.shape[0]
-        rc = _lib().sjk_pages_copy(self._c, _list(src, "src"), _list(dst, "dst", n), n, _stream())
+        rc = self._L.sjk_pages_copy(self._c, _list(src, "src"), _list(dst, "dst", n), n, _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_copy")
 
@@ -177,7 +198,9 @@ class Cache:
         self.layers = [sjk.Kv16(k[i].data_ptr(), v[i].data_ptr(), st[1], st[2], st[3], _TYPE[k.dtype], D, H, page, n_pages,
                                 tables.data_ptr(), tables.shape[0], tables.shape[1]) for i in range(n_layers)]
         self._refs = [C.byref(x) for x in self.layers]
-        self._q, self._o = sjk.Rows(), sjk.Rows()
+        self._q, self._o = _Rows(sjk.Rows(), "q", D), _Rows(sjk.Rows(), "out", D)
+        self._qo = C.byref(self._q.c), C.byref(self._o.c)
+        self._dev, self._L = _index(k), _lib()
         self._scratch = {}                       # by stream and number of query heads: calls of one stream follow one another
 
     @classmethod
@@ -196,18 +219,19 @@ class Cache:
         n = q.shape[0]
         if out is None:
             out = torch.empty_like(q)
-        _rows(self._q, q, "q", n, self.head_dim)
-        _rows(self._o, out, "out", n, self.head_dim)
+        self._q.set(q, n)
+        self._o.set(out, n)
         if n == 0:
             return out
-        st = _stream()
+        st = _stream(self._dev)
         key = (st, q.shape[1])
         scratch = self._scratch.get(key)
         if scratch is None:
-            size = _lib().sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
-            scratch = self._scratch[key] = torch.empty(size, dtype=torch.uint8, device=q.device)
-        rc = _lib().sjk_kv16_attend(self._refs[layer], C.byref(self._q), _list(lens, "lens", n), _list(rows, "rows", n), n, scale,
-                                    window, C.byref(self._o), scratch.data_ptr(), scratch.numel(), st)
+            size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
+            buf = torch.empty(size, dtype=torch.uint8, device=q.device)
+            scratch = self._scratch[key] = (buf, buf.data_ptr(), size)
+        rc = self._L.sjk_kv16_attend(self._refs[layer], self._qo[0], _list(lens, "lens", n), _list(rows, "rows", n), n, scale,
+                                     window, self._qo[1], scratch[1], scratch[2], st)
         if rc:
             raise sjk.SjkError(rc, "kv16_attend")
         return out
@@ -232,22 +256,20 @@ class Qkv:
         a.norm_type = _TYPE[kinds.pop()] if kinds else F32
         if rope is not None:
             a.rope = rope.c
-        self._ref = C.byref(a)
+        self._ref, self._L = C.byref(a), _lib()
         self._layer = None
+        # (the struct's own fields: setting them sets the struct's)
+        self._rows = [_Rows(getattr(a, f), f, head_dim) for f in ("q", "k", "v", "q_out", "k_out", "v_out")]
 
     def __call__(self, q=None, k=None, v=None, pos=None, q_out=None, k_out=None, v_out=None, layer=0, rows=None, to_cache=True):
         """q, k, v: [n][heads][D] (views of one projection's rows are fine); pos int32 [n], a negative one is padding;
         rows int32 [n]: table row of every token (None: token i is row i). K and V go to the cache's layer unless
         to_cache is false; row outputs go where given (an input's own rows too)."""
         a = self._a
-        n = (q if q is not None else k if k is not None else v).shape[0]
-        D = self.head_dim
-        _rows(a.q, q, "q", n, D)
-        _rows(a.k, k, "k", n, D)
-        _rows(a.v, v, "v", n, D)
-        _rows(a.q_out, q_out, "q_out", n, D)
-        _rows(a.k_out, k_out, "k_out", n, D)
-        _rows(a.v_out, v_out, "v_out", n, D)
+        some = q if q is not None else k if k is not None else v
+        n = some.shape[0]
+        for r, t in zip(self._rows, (q, k, v, q_out, k_out, v_out)):
+            r.set(t, n)
         a.n_tok = n
         a.pos = _list(pos, "pos", n)
         a.rows = _list(rows, "rows", n)
@@ -257,6 +279,6 @@ class Qkv:
         if at != self._layer:
             a.cache = self.cache.layers[at] if at is not None else sjk.Kv16()
             self._layer = at
-        rc = _lib().sjk_qkv(self._ref, _stream())
+        rc = self._L.sjk_qkv(self._ref, _stream(_index(some)))
         if rc:
             raise sjk.SjkError(rc, "qkv")
