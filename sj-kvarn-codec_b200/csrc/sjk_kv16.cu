@@ -687,14 +687,15 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 }
 
 // Joins the slots of a split pair, in list order, and writes the zeros of sequences without a live position. grid.x:
-// entries of p.split, then 8 sequences each (before the wait: the lengths are older than the kernel waited for); G warps of the CTA's 8 share a query head
-// (grid.y CTAs then take the heads of an entry in turn).
+// entries of p.split, then a sequence per warp (before the wait: the lengths are older than the kernel waited for). G of
+// the CTA's warps share a query head; grid.y CTAs and their other warps take the heads of an entry in turn.
 template <int D>
-__global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__ Params p, int R, int G, int entries) {
+__global__ void __launch_bounds__(512) kv16_merge_kernel(const __grid_constant__ Params p, int R, int G, int entries) {
     constexpr int NV = (D / 4 + 31) / 32;   // 16-byte words of a lane
-    __shared__ float s_acc[8 * (D + 4)];
+    extern __shared__ __align__(16) float s_acc[];          // [warps][D + 4] where they share a head
+    const int warps = blockDim.x >> 5;
     if (blockIdx.x >= entries) {
-        const int seq = (blockIdx.x - entries) * 8 + (threadIdx.x >> 5);
+        const int seq = (blockIdx.x - entries) * warps + (threadIdx.x >> 5);
         if (blockIdx.y == 0 && seq < p.n_seq && p.len[seq] <= 0)
             for (int i = threadIdx.x & 31; i < p.out.n_head * D; i += 32)
                 store1(p.out.p, (int64_t) seq * p.out.row_stride + (int64_t) (i / D) * p.out.head_stride + i % D, p.out.type, 0.0f);
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(256) kv16_merge_kernel(const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % G;
     const int kv = e.y / p.tiles, r0 = (e.y - kv * p.tiles) * R, nr = p.grp - r0 < R ? p.grp - r0 : R;
     const int n = e.w - e.z + 1, lo = (int) ((int64_t) n * sub / G), hi = (int) ((int64_t) n * (sub + 1) / G);
-    for (int r = blockIdx.y * (8 / G) + warp / G; r < nr; r += gridDim.y * (8 / G)) {
+    for (int r = blockIdx.y * (warps / G) + warp / G; r < nr; r += gridDim.y * (warps / G)) {
         float top = -INFINITY, sum = 0.0f;
         float4 o[NV];
 #pragma unroll
@@ -814,7 +815,11 @@ int run(const Params & p0, const Plan & pl, sjk_stream st) {
     const int64_t pairs = (int64_t) p.n_seq * p.c.n_head_kv * p.tiles;
     const bool few = pairs * 8 <= p.n_work;
     const int rows = p.grp < pl.R ? p.grp : pl.R, entries = p.by_pair ? (int) pairs : p.n_work;
-    return launch(kv16_merge_kernel<S::D>, dim3((unsigned) (entries + (p.n_seq + 7) / 8), few ? (unsigned) rows : 1u), dim3(256), 0, st, p, pl.R, few ? 8 : 1, entries);
+    // (16 warps for a head with hundreds of slots: 78.1 against 79.6 us at 100,000 tokens; 8 do for a few dozen)
+    const double steps = fmin((double) p.c.table_stride * p.c.page_tokens, 2147483647.0) / S::TS;
+    const int warps = few ? (fmin(steps / MIN_RUN, (double) p.n_work / pairs) > 64.0 ? 16 : 8) : rows < 8 ? rows : 8;
+    return launch(kv16_merge_kernel<S::D>, dim3((unsigned) (entries + (p.n_seq + warps - 1) / warps), few ? (unsigned) rows : 1u), dim3(32 * warps),
+                  few ? (size_t) warps * (S::D + 4) * sizeof(float) : 0, st, p, pl.R, few ? warps : 1, entries);
 }
 
 // f(Shape) for the call's types and sizes: nt8 1 or 2 tiles of columns in one pass over K and V
