@@ -8,7 +8,7 @@
 //    finds its run with a scan over them. A sequence weighs OV units beside its steps, for what its start and its
 //    output cost. Ragged batches balance by construction, no CTA barrier paces the work, and the workers of all heads
 //    are at the same tokens at the same time, whose rows lie side by side in memory.
-//  - A warp streams its steps through a ring in shared memory with cp.async, NE tiles ahead and across the ends of
+//  - A warp streams its steps through a ring in shared memory with cp.async, a step ahead and across the ends of
 //    sequences; positions that are not live are filled with zeros, not read.
 //  - The query heads of a KV head are the N = 8 columns of mma.m16n8k16: S^T = K Q^T with 16 tokens as rows, and
 //    O^T = V^T P with 16 channels as rows, so a group of up to 8 heads wastes no rows of the accumulators, P goes from
@@ -157,13 +157,14 @@ struct Shape {
     static constexpr int TM = tok_tiles(D), TS = step_toks(D), KS = D / 16;
     static constexpr int PITCH = 2 * D + 16;                // an odd number of 16-byte words: ldmatrix without conflicts
     static constexpr int ENTRY = TS * PITCH;
-    // warps of the one CTA of an SM: as many as registers and the ring leave room for
-    static constexpr int W = D >= 256 || NT8 > 1 || T > 1 ? 8 : 12;
-    static constexpr int FIT = (227 * 1024 / W - 16) / ENTRY;
-    static constexpr int NE = FIT < 6 ? FIT : 6;            // K and V tiles in a warp's ring
+    // Eight warps in the one CTA of an SM, and a ring of one step (its K and its V tile, each asked for again as soon as
+    // its products are done). More in flight was slower: the SMs' shares of the memory drift apart, and the slowest SM
+    // ends last (48 windowed sequences of 64 channels: 90 us, 96 with three tiles, 100 with four; 32 sequences of
+    // 8K-64K at 256 channels: 775, 778 with three). Six warps: 256 short chats 76 us against 67; ten and more: 11.2 us
+    // against 9.3 for one sequence of 611 tokens, no gain elsewhere.
+    static constexpr int W = 8, NE = 2;
     static constexpr int WARP_BYTES = NE * ENTRY + 16;
     static constexpr int CTA_BYTES = W * WARP_BYTES;
-    static_assert(NE >= 2 && NE <= 7, "a step's tiles, and the four masks, have to fit the ring");
 };
 
 // pairs of channels 8 apart, from element `at` on
