@@ -27,7 +27,7 @@ namespace {
 using namespace sjk16;
 
 constexpr int NT = 256;
-constexpr int MAX_T = 16;                   // tokens of a tile, at most (32 where a warp takes so many at once)
+constexpr int MAX_T = 16;                   // tokens of a tile, at most
 // CTAs of the many-token kernel per SM: 64 registers do for the 16-bit types (prefill of 32,768 tokens 160 us with four,
 // 166 with three), floats need 80 (8,320 rows 68 us with three, 74 with four)
 constexpr int ctas_of(int type) { return type == SJK_F32 ? 3 : 4; }
@@ -205,90 +205,100 @@ SJK_DEV void norm_weights(const Params & p, float * s_w) {
     }
 }
 
-// The tokens of blocks [ka, kb) of a tile in one head of q, k or v: norm (NORM) and rotation (ROT). A block is a token
-// for each of the warp's groups of L lanes; the loads of the next block are out while one is worked on. The head's row
-// of the tile's token 0 begins at element `src` of x.
+// Groups of G neighbouring heads of q, of k and of v, one head per L lanes of a warp: what a warp takes at a time.
+template <int L>
+struct Groups {
+    static constexpr int G = 32 / L;
+    int q, k, all;                          // groups of q; of q and k; of all three
+    SJK_DEV explicit Groups(const Params & p) {
+        q = (p.n_q + G - 1) / G;
+        k = q + (p.n_k + G - 1) / G;
+        all = k + (p.n_v + G - 1) / G;
+    }
+};
+// A lane's head of group g, and its channels' row for token `tok`.
+template <int TYPE, int L>
+struct Place {
+    int part, hh;
+    bool on;
+    Raw<TYPE> raw;
+    SJK_DEV void load(const Params & p, const Groups<L> & gr, const Lane<TYPE> & l, int g, int tok, bool live) {
+        part = g < gr.q ? 0 : g < gr.k ? 1 : 2;
+        hh = (g - (part == 0 ? 0 : part == 1 ? gr.q : gr.k)) * Groups<L>::G + (threadIdx.x & 31) / L;
+        const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
+        on = live && l.on && hh < (part == 0 ? p.n_q : part == 1 ? p.n_k : p.n_v);
+        raw = Raw<TYPE>();
+        if (on) raw = load16<TYPE>(in.p, (int64_t) tok * in.row_stride + (int64_t) hh * in.head_stride, l);
+    }
+};
+
+// Norm (NORM) and rotation (ROT) of the lanes' heads for token t of a tile (token `tok` of the call), and their stores.
 template <int TYPE, int L, bool NORM, bool ROT>
-SJK_DEV void head_tokens(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const void * x, int64_t src, int64_t step,
-                         const float4 * tab0, const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
-    const sjk_rows & out = part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2];
-    void * cache = part == 0 ? nullptr : part == 1 ? p.c.k : p.c.v;
-    const int c = threadIdx.x & (L - 1), nr = p.n_rot / 16;
-    const Lane<TYPE> l(p, c);
-    constexpr int G = 32 / L, N = Lane<TYPE>::N, WORD = Lane<TYPE>::WORD;
-    int t = ka * G + (threadIdx.x & 31) / L;
-    const int end = min(nt, kb * G);
-    src += t * step;
-    int64_t dst = (int64_t) (t0 + t) * out.row_stride + (int64_t) hh * out.head_stride;
-    const int64_t head = (int64_t) hh * p.c.head_stride;
-    const float * w = s_w + (part ? p.D : 0) + l.first;
-    Raw<TYPE> raw = {};
-    if (l.on && t < end) raw = load16<TYPE>(x, src, l);
-    for (int k = ka; k < kb; ++k, t += G) {
-        uint64_t a[8];
-        widen16<TYPE>(raw, a);
-        src += G * step;
-        if (l.on && t + G < end) raw = load16<TYPE>(x, src, l);
-        if constexpr (NORM) {
-            uint64_t s0 = mul2(a[0], a[0]), s1 = mul2(a[1], a[1]);      // idle lanes hold zeros
+SJK_DEV void head_row(const Params & p, const Lane<TYPE> & l, int part, int hh, bool on, const Raw<TYPE> & raw, int t, int tok, const float4 * tab0,
+                      const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
+    constexpr int N = Lane<TYPE>::N, WORD = Lane<TYPE>::WORD;
+    uint64_t a[8];
+    widen16<TYPE>(raw, a);
+    if constexpr (NORM) {
+        uint64_t s0 = mul2(a[0], a[0]), s1 = mul2(a[1], a[1]);          // idle lanes hold zeros
 #pragma unroll
-            for (int i = 2; i < 8; i += 2) { s0 = fma2(a[i], a[i], s0); s1 = fma2(a[i + 1], a[i + 1], s1); }
-            const float2 f0 = both(s0), f1 = both(s1);
-            float ss = (f0.x + f0.y) + (f1.x + f1.y);
+        for (int i = 2; i < 8; i += 2) { s0 = fma2(a[i], a[i], s0); s1 = fma2(a[i + 1], a[i + 1], s1); }
+        const float2 f0 = both(s0), f1 = both(s1);
+        float ss = (f0.x + f0.y) + (f1.x + f1.y);
 #pragma unroll
-            for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
-            const float r = rsqrtf(ss * p.inv_d + p.eps);
-            const uint64_t r2 = two(r, r);
+        for (int m = 1; m < L; m <<= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, m);
+        const float r = rsqrtf(ss * p.inv_d + p.eps);
+        const uint64_t r2 = two(r, r);
+        const float * w = s_w + (part ? p.D : 0) + l.first;
 #pragma unroll
-            for (int i = 0; i < N; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
-                for (int j = 0; j < WORD / 4; ++j) {
-                    const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(w + i * l.apart + 4 * j);
-                    uint64_t & u = a[i * WORD / 2 + 2 * j], & v = a[i * WORD / 2 + 2 * j + 1];
-                    u = mul2(u, mul2(r2, y.x));
-                    v = mul2(v, mul2(r2, y.y));
-                }
-        }
-        if (t >= end) break;                // (its groups' last tokens; the sums above needed all lanes)
-        if (ROT && l.rot) {
-            const float4 * tab = tab0 + (size_t) t * 4 * nr + c;
-            if (p.layout == SJK_ROPE_HALF) {
-                const ulonglong2 c0 = *reinterpret_cast<const ulonglong2 *>(tab), c1 = *reinterpret_cast<const ulonglong2 *>(tab + nr);
-                const ulonglong2 s0 = *reinterpret_cast<const ulonglong2 *>(tab + 2 * nr), s1 = *reinterpret_cast<const ulonglong2 *>(tab + 3 * nr);
-                const uint64_t cs[4] = {c0.x, c0.y, c1.x, c1.y}, sn[4] = {s0.x, s0.y, s1.x, s1.y};
+            for (int j = 0; j < WORD / 4; ++j) {
+                const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(w + i * l.apart + 4 * j);
+                uint64_t & u = a[i * WORD / 2 + 2 * j], & v = a[i * WORD / 2 + 2 * j + 1];
+                u = mul2(u, mul2(r2, y.x));
+                v = mul2(v, mul2(r2, y.y));
+            }
+    }
+    if (ROT && l.rot) {
+        const int nr = p.n_rot / 16;
+        const float4 * tab = tab0 + (size_t) t * 4 * nr + (threadIdx.x & (L - 1));
+        if (p.layout == SJK_ROPE_HALF) {
+            const ulonglong2 c0 = *reinterpret_cast<const ulonglong2 *>(tab), c1 = *reinterpret_cast<const ulonglong2 *>(tab + nr);
+            const ulonglong2 s0 = *reinterpret_cast<const ulonglong2 *>(tab + 2 * nr), s1 = *reinterpret_cast<const ulonglong2 *>(tab + 3 * nr);
+            const uint64_t cs[4] = {c0.x, c0.y, c1.x, c1.y}, sn[4] = {s0.x, s0.y, s1.x, s1.y};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint64_t u = a[i], v = a[4 + i];
-                    a[i] = fma2(u, cs[i], mul2(neg2(v), sn[i]));
-                    a[4 + i] = fma2(v, cs[i], mul2(u, sn[i]));
-                }
-            } else {
-                const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
-                const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-                const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t u = a[i], v = a[4 + i];
+                a[i] = fma2(u, cs[i], mul2(neg2(v), sn[i]));
+                a[4 + i] = fma2(v, cs[i], mul2(u, sn[i]));
+            }
+        } else {
+            const float4 c0 = tab[0], c1 = tab[nr], s0 = tab[2 * nr], s1 = tab[3 * nr];
+            const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+            const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 u = both(a[i]);
-                    a[i] = two(fmaf(u.x, cs[i], -u.y * sn[i]), fmaf(u.y, cs[i], u.x * sn[i]));
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float2 u = both(a[i]);
+                a[i] = two(fmaf(u.x, cs[i], -u.y * sn[i]), fmaf(u.y, cs[i], u.x * sn[i]));
             }
         }
-        const bool live = l.on && s_pos[t] >= 0;
-        if (live && out.p) store16<TYPE>(out.p, dst, l, out.type, a);
-        if (live && cache && s_slot[t] >= 0) store16<TYPE>(cache, s_slot[t] + head, l, p.c.type, a);
-        dst += G * out.row_stride;
     }
+    if (!on || s_pos[t] < 0) return;
+    const sjk_rows & out = part == 0 ? p.out[0] : part == 1 ? p.out[1] : p.out[2];
+    if (out.p) store16<TYPE>(out.p, (int64_t) tok * out.row_stride + (int64_t) hh * out.head_stride, l, out.type, a);
+    if (part && s_slot[t] >= 0) store16<TYPE>(part == 1 ? p.c.k : p.c.v, s_slot[t] + (int64_t) hh * p.c.head_stride, l, p.c.type, a);
 }
 template <int TYPE, int L>
-SJK_DEV void head_blocks(const Params & p, int part, int hh, int t0, int nt, int ka, int kb, const void * x, int64_t src, int64_t step,
-                         const float4 * tab, const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
-    if (part == 2) head_tokens<TYPE, L, false, false>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
-    else if (part == 0 ? p.w[0] : p.w[1]) head_tokens<TYPE, L, true, true>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
-    else head_tokens<TYPE, L, false, true>(p, part, hh, t0, nt, ka, kb, x, src, step, tab, s_w, s_pos, s_slot);
+SJK_DEV void head_group(const Params & p, const Lane<TYPE> & l, const Place<TYPE, L> & x, int t, int tok, const float4 * tab, const float * s_w,
+                        const int32_t * s_pos, const int64_t * s_slot) {
+    if (x.part == 2) head_row<TYPE, L, false, false>(p, l, 2, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
+    else if (x.part == 0 ? p.w[0] : p.w[1]) head_row<TYPE, L, true, true>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
+    else head_row<TYPE, L, false, true>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
 }
 
-// Few tokens. grid.x: tokens; grid.y CTAs share the heads, a warp each. L: lanes of a head, the power of two from
-// D / 16 on.
+// Few tokens. grid.x: tokens; grid.y CTAs share the groups of heads, a warp each. L: lanes of a head, the power of two
+// from D / 16 on.
 template <int TYPE, int L>
 __global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ Params p) {
     extern __shared__ float4 s_tab[];       // [4][n_rot / 16], then the norm weights of q and k
@@ -297,56 +307,53 @@ __global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ P
     pdl_wait();
     pdl_release();
     float * s_w = reinterpret_cast<float *>(s_tab + p.n_rot / 4);
-    const int t0 = blockIdx.x, h = blockIdx.y * (NT / 32) + threadIdx.x / 32;
-    tile_table<TYPE>(p, t0, 1, s_tab, s_pos, s_slot);
+    const int tok = blockIdx.x, g = blockIdx.y * (NT / 32) + threadIdx.x / 32;
+    const Groups<L> gr(p);
+    const Lane<TYPE> l(p, threadIdx.x & (L - 1));
+    Place<TYPE, L> x;
+    x.load(p, gr, l, g, tok, g < gr.all);
+    tile_table<TYPE>(p, tok, 1, s_tab, s_pos, s_slot);
     if (p.w[0] || p.w[1]) norm_weights(p, s_w);
     __syncthreads();
-    if (h >= p.n_all) return;
-    int hh;
-    const int part = part_of(p, h, &hh);
-    const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
-    head_blocks<TYPE, L>(p, part, hh, t0, 1, 0, 1, in.p, (int64_t) t0 * in.row_stride + (int64_t) hh * in.head_stride, 0, s_tab, s_w, s_pos, s_slot);
+    if (g < gr.all) head_group<TYPE, L>(p, l, x, 0, tok, s_tab, s_w, s_pos, s_slot);
 }
 
-// Many tokens. A CTA has the tokens [n i / ctas, n (i + 1) / ctas), in tiles of T. Its warps take neighbouring heads of
-// a tile's tokens at a time; the heads that do not go round are cut by blocks of tokens.
+// Many tokens. A CTA has the tokens [n i / ctas, n (i + 1) / ctas), in tiles of T; the table of the next tile is made
+// while one is worked on. Its warps take the groups of a token's heads in turn, so that the CTA goes through its rows in
+// the order of memory (a warp that stayed with a head over the tokens went by strides of a row: more of them in flight
+// slowed the memory down, 240 us against 160 for 32,768 tokens).
 template <int TYPE, int L>
 __global__ void __launch_bounds__(NT, ctas_of(TYPE)) qkv_tile_kernel(const __grid_constant__ Params p) {
     extern __shared__ float4 s_tab[];       // [2][T][4][n_rot / 16], then the norm weights of q and k
-    __shared__ int32_t s_pos[2][32];
-    __shared__ int64_t s_slot[2][32];
+    __shared__ int32_t s_pos[2][MAX_T];
+    __shared__ int64_t s_slot[2][MAX_T];
     pdl_wait();
     pdl_release();
-    constexpr int G = 32 / L, WARPS = NT / 32;
+    constexpr int WARPS = NT / 32;
     const int one = p.T * (p.n_rot / 4);
     float * s_w = reinterpret_cast<float *>(s_tab + 2 * one);
+    const Groups<L> gr(p);
+    const Lane<TYPE> l(p, threadIdx.x & (L - 1));
     if (p.w[0] || p.w[1]) norm_weights(p, s_w);
     const int last = (int) ((int64_t) p.n_tok * (blockIdx.x + 1) / gridDim.x), warp = threadIdx.x / 32;
     int t0 = (int) ((int64_t) p.n_tok * blockIdx.x / gridDim.x);
     if (t0 < last) tile_table<TYPE>(p, t0, min(p.T, last - t0), s_tab, s_pos[0], s_slot[0]);
+    // the warp's next item: token (of the CTA's) and group, and its rows
+    int tok = t0, g = warp;
+    while (g >= gr.all) { g -= gr.all; ++tok; }
+    Place<TYPE, L> x;
+    x.load(p, gr, l, g, tok, tok < last);
     for (int s = 0; t0 < last; t0 += p.T, s ^= 1) {
-        const int nt = min(p.T, last - t0), next = t0 + p.T;
+        const int end = min(t0 + p.T, last), next = t0 + p.T;
         __syncthreads();                    // this tile's table is complete, the other one is free
         if (next < last) tile_table<TYPE>(p, next, min(p.T, last - next), s_tab + (s ? 0 : one), s_pos[s ^ 1], s_slot[s ^ 1]);
-        const int blocks = (nt + G - 1) / G, full = p.n_all / WARPS * WARPS;
-        const int items = blocks * (p.n_all - full), each = (items + WARPS - 1) / WARPS;
-        int h = warp, ka = 0, kb = blocks, item = warp * each;
-        const int end = min(item + each, items);
-        for (;;) {
-            if (h >= full) {                // the heads that are left
-                if (item >= end) break;
-                h = item / blocks;
-                ka = item - h * blocks;
-                kb = min(blocks, ka + end - item);
-                h += full;
-                item += kb - ka;
-            }
-            int hh;
-            const int part = part_of(p, h, &hh);
-            const sjk_rows & in = part == 0 ? p.in[0] : part == 1 ? p.in[1] : p.in[2];
-            head_blocks<TYPE, L>(p, part, hh, t0, nt, ka, kb, in.p, (int64_t) t0 * in.row_stride + (int64_t) hh * in.head_stride, in.row_stride, s_tab + (s ? one : 0), s_w, s_pos[s],
-                                 s_slot[s]);
-            h += WARPS;
+        while (tok < end) {
+            const Place<TYPE, L> y = x;
+            const int now = tok;
+            g += WARPS;
+            while (g >= gr.all) { g -= gr.all; ++tok; }
+            x.load(p, gr, l, g, tok, tok < last);
+            head_group<TYPE, L>(p, l, y, now - t0, now, s_tab + (s ? one : 0), s_w, s_pos[s], s_slot[s]);
         }
     }
 }
@@ -411,19 +418,20 @@ __global__ void __launch_bounds__(NT) qkv_scalar_kernel(const __grid_constant__ 
 template <int TYPE, int L>
 int launch_vec(sjk_stream st, Params & p) {
     const size_t weights = 2 * (size_t) p.D * sizeof(float);
-    constexpr int slots = 148 * ctas_of(TYPE), least = 32 / L > 4 ? 32 / L : 4;      // tokens of a run, at least
+    constexpr int slots = 148 * ctas_of(TYPE);
     if (p.n_tok >= slots) {
-        int waves = p.n_tok / (slots * least);
+        int waves = p.n_tok / (slots * 4);  // four tokens of a run, at least
         waves = waves < 1 ? 1 : waves > WAVES ? WAVES : waves;
-        const int ctas = slots * waves, run = (p.n_tok + ctas - 1) / ctas, most = 32 / L > MAX_T ? 32 / L : MAX_T;
-        const int tiles = (run + most - 1) / most;
+        const int ctas = slots * waves, run = (p.n_tok + ctas - 1) / ctas, tiles = (run + MAX_T - 1) / MAX_T;
         p.T = (run + tiles - 1) / tiles;
         const size_t smem = 2 * (size_t) p.T * p.n_rot * sizeof(float) + weights;
         if (smem > 47 * 1024 && smem_limit<qkv_tile_kernel<TYPE, L>>(2 * (size_t) MAX_T * 512 * sizeof(float) + 4096)) return SJK_ERR_DEVICE;
         return launch(qkv_tile_kernel<TYPE, L>, dim3((unsigned) ctas), dim3(NT), smem, st, p);
     }
     p.T = 1;
-    const dim3 grid((unsigned) p.n_tok, (unsigned) ((p.n_all + NT / 32 - 1) / (NT / 32)));
+    constexpr int G = 32 / L;
+    const int groups = (p.n_q + G - 1) / G + (p.n_k + G - 1) / G + (p.n_v + G - 1) / G;
+    const dim3 grid((unsigned) p.n_tok, (unsigned) ((groups + NT / 32 - 1) / (NT / 32)));
     return launch(qkv_token_kernel<TYPE, L>, grid, dim3(NT), (size_t) p.n_rot * sizeof(float) + weights, st, p);
 }
 template <int TYPE>
