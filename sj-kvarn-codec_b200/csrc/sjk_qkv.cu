@@ -7,15 +7,16 @@
 // The angle is an integer: pos * step_i modulo 2^64, in units of 2^-64 turns, of which the top 32 bits, read as a
 // signed fraction of a turn, go to sincospif. That keeps 2^-32 of a turn at every position, for one wide multiply.
 //
-// Bound: HBM, every element once in and once out. The vector kernels give a lane 16 channels of a head: for the half
-// layout the two 8-channel chunks that rotate into one another, so the rotation needs no exchange between lanes, and
-// the norm's sum is a butterfly over the head's D / 16 lanes (a fixed order). Products of channel pairs are packed
-// (f32x2). The cosines and sines of a token are computed once into shared memory for all its heads (n_rot / 2 sincos
-// per token instead of per head), and a warp stays with a head over the tokens of its tile, for its norm weights.
+// Bound: HBM, every element once in and once out; a launch's latency for a decode step's few tokens. The vector kernels
+// give a lane 16 channels of a head, as 16-byte words that lie side by side over the head's lanes; in the half layout
+// its last 8 channels are the partners of its first 8, in the pair layout pairs stay together, so the rotation needs no
+// exchange between lanes. The norm's sum is a butterfly over the head's D / 16 lanes (a fixed order). Products of channel
+// pairs are packed (f32x2). The cosines and sines of a token are computed once into shared memory for all its heads
+// (n_rot / 2 of each per token instead of per head).
 //  - Many tokens: a few waves of CTAs, each with a run of tokens that it takes in tiles of up to MAX_T.
-//  - Few tokens: a token per CTA and the heads over grid.y: a launch's latency.
-// Shapes whose chunks would straddle (n_rot or head_dim not a multiple of 16, rows off 16 bytes) take the scalar
-// kernel, one warp per (token, head) through shared memory.
+//  - Few tokens: a token per CTA and the heads over grid.y (one token of 48 heads of 128 channels: 3.2 us a launch).
+// Shapes whose words would straddle (n_rot or head_dim not a multiple of 16, rows off 16 bytes) take the scalar kernel,
+// one warp per (token, head) through shared memory.
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
@@ -28,10 +29,10 @@ using namespace sjk16;
 
 constexpr int NT = 256;
 constexpr int MAX_T = 16;                   // tokens of a tile, at most
-// CTAs of the many-token kernel per SM: 64 registers do for the 16-bit types (prefill of 32,768 tokens 160 us with four,
-// 166 with three), floats need 80 (8,320 rows 68 us with three, 74 with four)
+// CTAs of the many-token kernel per SM: 64 registers do for the 16-bit types (prefill of 32,768 tokens 145 us with four,
+// 162 with three), floats need 80 (8,320 rows 67 us with three, 76 with four)
 constexpr int ctas_of(int type) { return type == SJK_F32 ? 3 : 4; }
-constexpr int WAVES = 4;                    // runs per CTA slot, at most: SMs are not equally fast (f32: 82 us with one, 74 with four)
+constexpr int WAVES = 4;                    // runs per CTA slot, at most: SMs are not equally fast (f32: 74 us with one, 67 with four)
 __device__ unsigned int g_qkv_status;
 
 struct Params {
@@ -320,8 +321,10 @@ __global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ P
 
 // Many tokens. A CTA has the tokens [n i / ctas, n (i + 1) / ctas), in tiles of T; the table of the next tile is made
 // while one is worked on. Its warps take the groups of a token's heads in turn, so that the CTA goes through its rows in
-// the order of memory (a warp that stayed with a head over the tokens went by strides of a row: more of them in flight
-// slowed the memory down, 240 us against 160 for 32,768 tokens).
+// the order of memory, with the next item's loads out while one is worked on (32,768 tokens of 24 heads of 256 bf16
+// channels: 145 us = 5.5 TB/s of rows read and written, 85 % of a plain copy's rate, bound by instruction issue; 8,320
+// rows of floats 67 us = 6.1 TB/s, 93 %). Staying with a head over the tile's tokens took 160 us, several tokens per item
+// 217 and more: both need registers that four CTAs an SM do not have.
 template <int TYPE, int L>
 __global__ void __launch_bounds__(NT, ctas_of(TYPE)) qkv_tile_kernel(const __grid_constant__ Params p) {
     extern __shared__ float4 s_tab[];       // [2][T][4][n_rot / 16], then the norm weights of q and k
