@@ -627,8 +627,10 @@ int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len,
  * A ledger in device memory over the pages of one or more slabs (the K and the V pages of every layer, or the record
  * pool's slab): the pool's stack of free ids, as sjk_pool_* keep it (so sjk_pool_dev_load, _store and _reserve_batch
  * work on the same memory), and for every page the number of table entries that hold it beyond the first (its shares).
+ * sjk_pool_release_batch and the release of sjk_truncate_batch know no shares: give back through sjk_pages_free.
  * Tables: DEVICE [n_rows][table_stride]. Row lists are DEVICE int32. Page p of layer l of a slab is the page_bytes
- * at base + l*layer_stride + p*page_bytes (all multiples of 16). */
+ * at base + l*layer_stride + p*page_bytes (all multiples of 16). Calls on one ledger follow one another (one stream, or
+ * streams ordered by events). */
 #define SJK_PAGES_MAX      (1u << 20)
 #define SJK_PAGES_MAX_ROWS 1024
 #define SJK_MAX_SLABS      4
