@@ -3,7 +3,7 @@
 //
 // Bound: HBM, every live K and V row once (4 D bytes per position and KV head for 4 D grp flops: at most 16 flops per
 // byte for 16 query heads, far under the tensor cores' ridge). Measured (us a call, GB/s of live rows): 32 sequences of
-// 8K-64K, 4 KV heads of 256 bf16 channels 775-790 (6,360-6,470: a plain copy's rate is 6,539); one of 100,000 tokens with
+// 8K-64K, 4 KV heads of 256 bf16 channels 775-797 by machine (6,290-6,470: a plain copy's rate is 6,539); one of 100,000 tokens with
 // 32-bit queries and outputs 78 (5,230); 48 windows of 4,096, 24 heads of 64 channels 91 (5,540); 256 short chats of 0 to
 // 2,048 tokens 68 (4,810); one of 611 tokens 9.4. What is left above the bytes: 4-5 us until the first products (launch,
 // lengths, table, queries, first rows, each behind the other), 3 us for the merge, and SMs whose share of the memory is
