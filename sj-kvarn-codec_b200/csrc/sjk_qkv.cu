@@ -15,8 +15,10 @@
 // (n_rot / 2 of each per token instead of per head).
 //  - Many tokens: a few waves of CTAs, each with a run of tokens that it takes in tiles of up to MAX_T.
 //  - Few tokens: a token per CTA and the heads over grid.y (one token of 48 heads of 128 channels: 3.2 us a launch).
-// Shapes whose words would straddle (n_rot or head_dim not a multiple of 16, rows off 16 bytes) take the scalar kernel,
-// one warp per (token, head) through shared memory.
+// Where n_rot is no multiple of 16 partners are in other lanes: lanes take words of the whole head, and the rotating
+// channels go once through shared memory (8,046 tokens of 12 heads of 256 bf16 channels, 20 of them rotating: 26 us; the
+// scalar kernel took 93, at five tokens 4.5 against 3.4). Shapes without whole words (head_dim not a multiple of 16,
+// rows off 16 bytes) take the scalar kernel, one warp per (token, head) through shared memory.
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
@@ -108,12 +110,12 @@ struct Lane {
     static constexpr int N = TYPE == SJK_F32 ? 4 : 2, WORD = 16 / N;    // words, and channels of one
     int first, apart;                       // first channel of word 0, and from word to word
     bool rot, on;                           // rotates; has channels at all
-    SJK_DEV Lane(const Params & p, int c) {
-        const int nr = p.n_rot / 16, all = p.D / 16;
+    SJK_DEV Lane(const Params & p, int n_rot, int c) {
+        const int nr = n_rot / 16, all = p.D / 16;
         rot = c < nr;
         on = c < all;
-        first = rot ? WORD * c : on ? p.n_rot + WORD * (c - nr) : 0;
-        apart = rot ? p.n_rot / N : on ? (p.D - p.n_rot) / N : 0;
+        first = rot ? WORD * c : on ? n_rot + WORD * (c - nr) : 0;
+        apart = rot ? n_rot / N : on ? (p.D - n_rot) / N : 0;
     }
 };
 
@@ -173,8 +175,9 @@ SJK_DEV void store16(void * base, int64_t off, const Lane<TYPE> & l, int type, c
 }
 
 // What the tokens of a tile share: positions, cache slots, and the cosines and sines of every lane's 8 angles, as
-// tab[t][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7.
-template <int TYPE>
+// tab[t][4][n_rot / 16]: cosines 0-3, 4-7, sines 0-3, 4-7. ODD (n_rot no multiple of 16): (cosine, sine) by angle.
+SJK_DEV int table_words(const Params & p) { return (p.n_rot + 3) / 4; }         // of a token, in 16 bytes
+template <int TYPE, bool ODD>
 SJK_DEV void tile_table(const Params & p, int t0, int nt, float4 * tab, int32_t * s_pos, int64_t * s_slot) {
     const int tid = threadIdx.x, half = p.n_rot / 2, nr = p.n_rot / 16;
     if (tid < nt) {
@@ -188,12 +191,16 @@ SJK_DEV void tile_table(const Params & p, int t0, int nt, float4 * tab, int32_t 
     const int dt = NT / half, dj = NT - dt * half;
     for (int t = tid / half, j = tid - t * half; t < nt;) {
         const float2 cs = angle(p.step[j], p.pos[t0 + t], p.amp);
-        int q = 0, k = j;                   // word, and angle within the words q of all lanes
-        while (k >= nr << lw) { k -= nr << lw; ++q; }
-        const int c = k >> lw, e = (q << lw) + (k & ((1 << lw) - 1));
-        float * d = reinterpret_cast<float *>(tab + (size_t) t * 4 * nr) + (e >> 2) * nr * 4 + c * 4 + (e & 3);
-        d[0] = cs.x;
-        d[2 * nr * 4] = cs.y;
+        if constexpr (ODD) {
+            reinterpret_cast<float2 *>(tab + (size_t) t * table_words(p))[j] = cs;
+        } else {
+            int q = 0, k = j;               // word, and angle within the words q of all lanes
+            while (k >= nr << lw) { k -= nr << lw; ++q; }
+            const int c = k >> lw, e = (q << lw) + (k & ((1 << lw) - 1));
+            float * d = reinterpret_cast<float *>(tab + (size_t) t * 4 * nr) + (e >> 2) * nr * 4 + c * 4 + (e & 3);
+            d[0] = cs.x;
+            d[2 * nr * 4] = cs.y;
+        }
         t += dt;
         j += dj;
         if (j >= half) { j -= half; ++t; }
@@ -234,9 +241,11 @@ struct Place {
 };
 
 // Norm (NORM) and rotation (ROT) of the lanes' heads for token t of a tile (token `tok` of the call), and their stores.
-template <int TYPE, int L, bool NORM, bool ROT>
+// ODD: partners are in other lanes, so the rotating channels go through the head's row s_x, where the lanes take a pair
+// each. A lane writes and reads its own words there, and others' only between the two barriers.
+template <int TYPE, int L, bool NORM, bool ROT, bool ODD>
 SJK_DEV void head_row(const Params & p, const Lane<TYPE> & l, int part, int hh, bool on, const Raw<TYPE> & raw, int t, int tok, const float4 * tab0,
-                      const float * s_w, const int32_t * s_pos, const int64_t * s_slot) {
+                      const float * s_w, float * s_x, const int32_t * s_pos, const int64_t * s_slot) {
     constexpr int N = Lane<TYPE>::N, WORD = Lane<TYPE>::WORD;
     uint64_t a[8];
     widen16<TYPE>(raw, a);
@@ -261,7 +270,39 @@ SJK_DEV void head_row(const Params & p, const Lane<TYPE> & l, int part, int hh, 
                 v = mul2(v, mul2(r2, y.y));
             }
     }
-    if (ROT && l.rot) {
+    if constexpr (ROT && ODD) {
+        const int half = p.n_rot / 2;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = l.first + i * l.apart;
+            if (!l.on || at >= p.n_rot) continue;
+#pragma unroll
+            for (int j = 0; j < WORD / 4; ++j)
+                *reinterpret_cast<ulonglong2 *>(s_x + at + 4 * j) = make_ulonglong2(a[i * WORD / 2 + 2 * j], a[i * WORD / 2 + 2 * j + 1]);
+        }
+        __syncwarp();
+        const float2 * tab = reinterpret_cast<const float2 *>(tab0 + (size_t) t * table_words(p));
+        const bool pair = p.layout == SJK_ROPE_PAIR;
+        for (int j = threadIdx.x & (L - 1); j < half; j += L) {
+            const float2 cs = tab[j];
+            const int iu = pair ? 2 * j : j, iv = pair ? 2 * j + 1 : j + half;
+            const float u = s_x[iu], v = s_x[iv];
+            s_x[iu] = fmaf(u, cs.x, -v * cs.y);
+            s_x[iv] = fmaf(v, cs.x, u * cs.y);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int at = l.first + i * l.apart;
+            if (!l.on || at >= p.n_rot) continue;
+#pragma unroll
+            for (int j = 0; j < WORD / 4; ++j) {
+                const ulonglong2 y = *reinterpret_cast<const ulonglong2 *>(s_x + at + 4 * j);
+                a[i * WORD / 2 + 2 * j] = y.x;
+                a[i * WORD / 2 + 2 * j + 1] = y.y;
+            }
+        }
+    } else if (ROT && l.rot) {
         const int nr = p.n_rot / 16;
         const float4 * tab = tab0 + (size_t) t * 4 * nr + (threadIdx.x & (L - 1));
         if (p.layout == SJK_ROPE_HALF) {
@@ -290,33 +331,37 @@ SJK_DEV void head_row(const Params & p, const Lane<TYPE> & l, int part, int hh, 
     if (out.p) store16<TYPE>(out.p, (int64_t) tok * out.row_stride + (int64_t) hh * out.head_stride, l, out.type, a);
     if (part && s_slot[t] >= 0) store16<TYPE>(part == 1 ? p.c.k : p.c.v, s_slot[t] + (int64_t) hh * p.c.head_stride, l, p.c.type, a);
 }
-template <int TYPE, int L>
+template <int TYPE, int L, bool ODD>
 SJK_DEV void head_group(const Params & p, const Lane<TYPE> & l, const Place<TYPE, L> & x, int t, int tok, const float4 * tab, const float * s_w,
-                        const int32_t * s_pos, const int64_t * s_slot) {
-    if (x.part == 2) head_row<TYPE, L, false, false>(p, l, 2, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
-    else if (x.part == 0 ? p.w[0] : p.w[1]) head_row<TYPE, L, true, true>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
-    else head_row<TYPE, L, false, true>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_pos, s_slot);
+                        float * s_x, const int32_t * s_pos, const int64_t * s_slot) {
+    if (x.part == 2) head_row<TYPE, L, false, false, ODD>(p, l, 2, x.hh, x.on, x.raw, t, tok, tab, s_w, s_x, s_pos, s_slot);
+    else if (x.part == 0 ? p.w[0] : p.w[1]) head_row<TYPE, L, true, true, ODD>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_x, s_pos, s_slot);
+    else head_row<TYPE, L, false, true, ODD>(p, l, x.part, x.hh, x.on, x.raw, t, tok, tab, s_w, s_x, s_pos, s_slot);
+}
+// ODD: floats of a head's row, and the row of the lane's head behind the norm weights
+SJK_DEV float * head_buffer(const Params & p, float * s_w, int L) {
+    return s_w + 2 * p.D + (threadIdx.x / L) * ((p.n_rot + 15) & ~15);
 }
 
 // Few tokens. grid.x: tokens; grid.y CTAs share the groups of heads, a warp each. L: lanes of a head, the power of two
 // from D / 16 on.
-template <int TYPE, int L>
+template <int TYPE, int L, bool ODD>
 __global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ Params p) {
-    extern __shared__ float4 s_tab[];       // [4][n_rot / 16], then the norm weights of q and k
+    extern __shared__ float4 s_tab[];       // the table, the norm weights of q and k, and (ODD) a row per head of the warps
     __shared__ int32_t s_pos[1];
     __shared__ int64_t s_slot[1];
     pdl_wait();
     pdl_release();
-    float * s_w = reinterpret_cast<float *>(s_tab + p.n_rot / 4);
+    float * s_w = reinterpret_cast<float *>(s_tab + table_words(p));
     const int tok = blockIdx.x, g = blockIdx.y * (NT / 32) + threadIdx.x / 32;
     const Groups<L> gr(p);
-    const Lane<TYPE> l(p, threadIdx.x & (L - 1));
+    const Lane<TYPE> l(p, ODD ? 0 : p.n_rot, threadIdx.x & (L - 1));
     Place<TYPE, L> x;
     x.load(p, gr, l, g, tok, g < gr.all);
-    tile_table<TYPE>(p, tok, 1, s_tab, s_pos, s_slot);
+    tile_table<TYPE, ODD>(p, tok, 1, s_tab, s_pos, s_slot);
     if (p.w[0] || p.w[1]) norm_weights(p, s_w);
     __syncthreads();
-    if (g < gr.all) head_group<TYPE, L>(p, l, x, 0, tok, s_tab, s_w, s_pos, s_slot);
+    if (g < gr.all) head_group<TYPE, L, ODD>(p, l, x, 0, tok, s_tab, s_w, head_buffer(p, s_w, L), s_pos, s_slot);
 }
 
 // Many tokens. A CTA has the tokens [n i / ctas, n (i + 1) / ctas), in tiles of T; the table of the next tile is made
@@ -325,22 +370,22 @@ __global__ void __launch_bounds__(NT) qkv_token_kernel(const __grid_constant__ P
 // channels: 145 us = 5.5 TB/s of rows read and written, 85 % of a plain copy's rate, bound by instruction issue; 8,320
 // rows of floats 67 us = 6.1 TB/s, 93 %). Staying with a head over the tile's tokens took 160 us, several tokens per item
 // 217 and more: both need registers that four CTAs an SM do not have.
-template <int TYPE, int L>
+template <int TYPE, int L, bool ODD>
 __global__ void __launch_bounds__(NT, ctas_of(TYPE)) qkv_tile_kernel(const __grid_constant__ Params p) {
-    extern __shared__ float4 s_tab[];       // [2][T][4][n_rot / 16], then the norm weights of q and k
+    extern __shared__ float4 s_tab[];       // two tables, the norm weights of q and k, and (ODD) a row per head of the warps
     __shared__ int32_t s_pos[2][MAX_T];
     __shared__ int64_t s_slot[2][MAX_T];
     pdl_wait();
     pdl_release();
     constexpr int WARPS = NT / 32;
-    const int one = p.T * (p.n_rot / 4);
+    const int one = p.T * table_words(p);
     float * s_w = reinterpret_cast<float *>(s_tab + 2 * one);
     const Groups<L> gr(p);
-    const Lane<TYPE> l(p, threadIdx.x & (L - 1));
+    const Lane<TYPE> l(p, ODD ? 0 : p.n_rot, threadIdx.x & (L - 1));
     if (p.w[0] || p.w[1]) norm_weights(p, s_w);
     const int last = (int) ((int64_t) p.n_tok * (blockIdx.x + 1) / gridDim.x), warp = threadIdx.x / 32;
     int t0 = (int) ((int64_t) p.n_tok * blockIdx.x / gridDim.x);
-    if (t0 < last) tile_table<TYPE>(p, t0, min(p.T, last - t0), s_tab, s_pos[0], s_slot[0]);
+    if (t0 < last) tile_table<TYPE, ODD>(p, t0, min(p.T, last - t0), s_tab, s_pos[0], s_slot[0]);
     // the warp's next item: token (of the CTA's) and group, and its rows
     int tok = t0, g = warp;
     while (g >= gr.all) { g -= gr.all; ++tok; }
@@ -349,14 +394,14 @@ __global__ void __launch_bounds__(NT, ctas_of(TYPE)) qkv_tile_kernel(const __gri
     for (int s = 0; t0 < last; t0 += p.T, s ^= 1) {
         const int end = min(t0 + p.T, last), next = t0 + p.T;
         __syncthreads();                    // this tile's table is complete, the other one is free
-        if (next < last) tile_table<TYPE>(p, next, min(p.T, last - next), s_tab + (s ? 0 : one), s_pos[s ^ 1], s_slot[s ^ 1]);
+        if (next < last) tile_table<TYPE, ODD>(p, next, min(p.T, last - next), s_tab + (s ? 0 : one), s_pos[s ^ 1], s_slot[s ^ 1]);
         while (tok < end) {
             const Place<TYPE, L> y = x;
             const int now = tok;
             g += WARPS;
             while (g >= gr.all) { g -= gr.all; ++tok; }
             x.load(p, gr, l, g, tok, tok < last);
-            head_group<TYPE, L>(p, l, y, now - t0, now, s_tab + (s ? one : 0), s_w, s_pos[s], s_slot[s]);
+            head_group<TYPE, L, ODD>(p, l, y, now - t0, now, s_tab + (s ? one : 0), s_w, head_buffer(p, s_w, L), s_pos[s], s_slot[s]);
         }
     }
 }
@@ -418,29 +463,37 @@ __global__ void __launch_bounds__(NT) qkv_scalar_kernel(const __grid_constant__ 
     }
 }
 
-template <int TYPE, int L>
+template <int TYPE, int L, bool ODD>
 int launch_vec(sjk_stream st, Params & p) {
-    const size_t weights = 2 * (size_t) p.D * sizeof(float);
+    const size_t table = (size_t) ((p.n_rot + 3) / 4) * 16;             // of a token
+    const size_t rest = 2 * (size_t) p.D * sizeof(float) + (ODD ? (size_t) (NT / L) * ((p.n_rot + 15) & ~15) * sizeof(float) : 0);
     constexpr int slots = 148 * ctas_of(TYPE);
     if (p.n_tok >= slots) {
         int waves = p.n_tok / (slots * 4);  // four tokens of a run, at least
         waves = waves < 1 ? 1 : waves > WAVES ? WAVES : waves;
         const int ctas = slots * waves, run = (p.n_tok + ctas - 1) / ctas, tiles = (run + MAX_T - 1) / MAX_T;
         p.T = (run + tiles - 1) / tiles;
-        const size_t smem = 2 * (size_t) p.T * p.n_rot * sizeof(float) + weights;
-        if (smem > 47 * 1024 && smem_limit<qkv_tile_kernel<TYPE, L>>(2 * (size_t) MAX_T * 512 * sizeof(float) + 4096)) return SJK_ERR_DEVICE;
-        return launch(qkv_tile_kernel<TYPE, L>, dim3((unsigned) ctas), dim3(NT), smem, st, p);
+        const size_t smem = 2 * (size_t) p.T * table + rest;
+        // (the rows of a CTA's heads hold at most the 16 channels of every thread)
+        if (smem > 47 * 1024 && smem_limit<qkv_tile_kernel<TYPE, L, ODD>>(2 * (size_t) MAX_T * 512 * sizeof(float) + 4096 + (ODD ? NT * 64 : 0)))
+            return SJK_ERR_DEVICE;
+        return launch(qkv_tile_kernel<TYPE, L, ODD>, dim3((unsigned) ctas), dim3(NT), smem, st, p);
     }
     p.T = 1;
     constexpr int G = 32 / L;
     const int groups = (p.n_q + G - 1) / G + (p.n_k + G - 1) / G + (p.n_v + G - 1) / G;
     const dim3 grid((unsigned) p.n_tok, (unsigned) ((groups + NT / 32 - 1) / (NT / 32)));
-    return launch(qkv_token_kernel<TYPE, L>, grid, dim3(NT), (size_t) p.n_rot * sizeof(float) + weights, st, p);
+    return launch(qkv_token_kernel<TYPE, L, ODD>, grid, dim3(NT), table + rest, st, p);
+}
+template <int TYPE, bool ODD>
+int launch_lanes(sjk_stream st, Params & p) {
+    return p.D <= 16 ? launch_vec<TYPE, 1, ODD>(st, p) : p.D <= 32 ? launch_vec<TYPE, 2, ODD>(st, p) :
+           p.D <= 64 ? launch_vec<TYPE, 4, ODD>(st, p) : p.D <= 128 ? launch_vec<TYPE, 8, ODD>(st, p) :
+           p.D <= 256 ? launch_vec<TYPE, 16, ODD>(st, p) : launch_vec<TYPE, 32, ODD>(st, p);
 }
 template <int TYPE>
-int launch_lanes(sjk_stream st, Params & p) {
-    return p.D <= 16 ? launch_vec<TYPE, 1>(st, p) : p.D <= 32 ? launch_vec<TYPE, 2>(st, p) : p.D <= 64 ? launch_vec<TYPE, 4>(st, p) :
-           p.D <= 128 ? launch_vec<TYPE, 8>(st, p) : p.D <= 256 ? launch_vec<TYPE, 16>(st, p) : launch_vec<TYPE, 32>(st, p);
+int launch_type(sjk_stream st, Params & p) {
+    return p.n_rot % 16 ? launch_lanes<TYPE, true>(st, p) : launch_lanes<TYPE, false>(st, p);
 }
 
 bool rows_vec(const sjk_rows & r) {
@@ -581,7 +634,7 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
     p.n_rot = a->rope.n_rot; p.layout = a->rope.layout; p.amp = a->rope.amp; p.step = a->rope.step;
     p.pos = a->pos; p.rows = a->rows;
     if (cached) p.c = a->cache;
-    bool vec = p.D % 16 == 0 && p.n_rot % 16 == 0;
+    bool vec = p.D % 16 == 0;
     for (int i = 0; i < 3; ++i) vec = vec && rows_vec(p.in[i]) && rows_vec(p.out[i]);
     if (cached) {
         const int64_t s = p.c.page_stride | p.c.slot_stride | p.c.head_stride;
@@ -592,9 +645,9 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
         return launch(qkv_scalar_kernel, dim3((unsigned) (ctas < 148 * 8 ? ctas : 148 * 8)), dim3(NT), (size_t) (NT / 32) * p.D * sizeof(float), st, p);
     }
     switch (type) {
-        case SJK_F32: return launch_lanes<SJK_F32>(st, p);
-        case SJK_F16: return launch_lanes<SJK_F16>(st, p);
-        default: return launch_lanes<SJK_BF16>(st, p);
+        case SJK_F32: return launch_type<SJK_F32>(st, p);
+        case SJK_F16: return launch_type<SJK_F16>(st, p);
+        default: return launch_type<SJK_BF16>(st, p);
     }
 }
 

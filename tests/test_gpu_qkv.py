@@ -269,3 +269,45 @@ def test_rows_feed_the_sealed_cache(T):
     assert (gu.d2h_ptr(layer[0].sink, size) == gu.d2h_ptr(layer[1].sink, size)).all()
     for x in layer:
         L.sj_kvarn_layer_free(C.byref(x))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("layout", ["half", "pair"])
+@pytest.mark.parametrize("n,D,n_rot", [(1, 128, 20), (700, 96, 24), (2500, 64, 22), (700, 256, 130), (600, 512, 510), (700, 16, 6), (650, 48, 2)])
+def test_odd_rotations(T, dtype, layout, n, D, n_rot):
+    """Rotating parts that are no multiple of 16 channels, in calls of one token and of many, some of them skipped."""
+    dt = _dt(T, dtype)
+    HQ, H = 5, 2
+    q, k, v, pos, w = _inputs(T, n, HQ, H, D, dt, n + n_rot, far=100000)
+    pos[3::7] = -1
+    live = pos >= 0
+    rope = kv16.Rope(n_rot, layout=layout, base=1e4)
+    step = kv16.Qkv(D, rope=rope, q_norm=w[0], norm_bias=0.25, eps=EPS)
+    q_out, k_out, v_out = T.full_like(q, 7.0), T.full_like(k, 7.0), T.full_like(v, 7.0)
+    step(q, k, v, pos, q_out=q_out, k_out=k_out, v_out=v_out)
+    steps = _freq(n_rot, 1e4, "none", 1.0)
+    some = [t for t in sorted({0, 1, n // 3, n // 2, n - 2, n - 1}) if 0 <= t < n and int(pos[t]) >= 0]
+    _close(T, q_out[some], _want(T, q[some], w[0], 0.25, pos[some], n_rot, layout, steps))
+    _close(T, k_out[some], _want(T, k[some], None, 0.0, pos[some], n_rot, layout, steps))
+    assert T.equal(v_out[live], v[live])
+    for x in (q_out, k_out, v_out):
+        assert bool((x[~live] == 7.0).all())
+    parts = T.full_like(q, 7.0)                 # every token: the same values whatever the batch it came in
+    for t in range(0, n, 100):
+        step(q=q[t:t + 100], pos=pos[t:t + 100], q_out=parts[t:t + 100])
+    assert T.equal(parts, q_out)
+
+
+@pytest.mark.parametrize("layout", ["half", "pair"])
+def test_odd_rotations_leave_the_rest(T, layout):
+    """Infinities, NaN and zeros' signs behind the rotating channels stay as they are and reach no rotating one. (A NaN
+    stays a NaN; its payload is the conversion's.)"""
+    n, D, n_rot = 700, 64, 20
+    q, _, _, pos, _ = _inputs(T, n, 4, 1, D, T.bfloat16, 3)
+    q[..., n_rot], q[..., n_rot + 1], q[..., n_rot + 3] = math.inf, math.nan, -0.0
+    out = T.empty_like(q)
+    kv16.Qkv(D, rope=kv16.Rope(n_rot, layout=layout))(q=q, pos=pos, q_out=out)
+    rest, want = out[..., n_rot:].contiguous(), q[..., n_rot:].contiguous()
+    assert T.equal(rest.isnan(), want.isnan())
+    assert T.equal(rest.view(T.int16)[~want.isnan()], want.view(T.int16)[~want.isnan()])
+    assert bool(out[..., :n_rot].isfinite().all())
