@@ -34,7 +34,11 @@ constexpr int MAX_T = 16;                   // tokens of a tile, at most
 // CTAs of the many-token kernel per SM: 64 registers do for the 16-bit types (prefill of 32,768 tokens 145 us with four,
 // 162 with three), floats need 80 (8,320 rows 67 us with three, 76 with four)
 constexpr int ctas_of(int type) { return type == SJK_F32 ? 3 : 4; }
-constexpr int WAVES = 4;                    // runs per CTA slot, at most: SMs are not equally fast (f32: 74 us with one, 67 with four)
+// Runs per CTA slot: a run costs about 2.5 us to begin, and SMs are not equally fast. Where a slot moves WAVE_BYTES or more,
+// several (us with one / four: floats, 0.9 MB a slot 77 / 70, 1.8 MB 149 / 135; bf16, 1.4 MB 147 / 145); below that one
+// (floats, 0.46 MB 39.0 / 38.3, 0.55 MB 45.7 / 48.7; bf16, 0.69 MB 81 / 83, 0.1 MB 19 / 24).
+constexpr int WAVES = 4;
+constexpr int64_t WAVE_BYTES = 768 * 1024;
 __device__ unsigned int g_qkv_status;
 
 struct Params {
@@ -469,8 +473,9 @@ int launch_vec(sjk_stream st, Params & p) {
     const size_t rest = 2 * (size_t) p.D * sizeof(float) + (ODD ? (size_t) (NT / L) * ((p.n_rot + 15) & ~15) * sizeof(float) : 0);
     constexpr int slots = 148 * ctas_of(TYPE);
     if (p.n_tok >= slots) {
-        int waves = p.n_tok / (slots * 4);  // four tokens of a run, at least
-        waves = waves < 1 ? 1 : waves > WAVES ? WAVES : waves;
+        // rows read and written: their types are near enough the input's
+        const int64_t bytes = (int64_t) p.n_tok * p.n_all * p.D * (2 * (int) type_bytes(TYPE));
+        const int waves = bytes / slots < WAVE_BYTES || p.n_tok < 4 * WAVES * slots ? 1 : WAVES;    // (four tokens of a run, at least)
         const int ctas = slots * waves, run = (p.n_tok + ctas - 1) / ctas, tiles = (run + MAX_T - 1) / MAX_T;
         p.T = (run + tiles - 1) / tiles;
         const size_t smem = 2 * (size_t) p.T * table + rest;
