@@ -153,10 +153,12 @@ SJK_DEV float ex2(float x) {
     return y;
 }
 
-// Kernel shape: TYPE of the cache, head size, T 16-bit terms of q and P, NT8 tiles of 8 columns.
-template <int TYPE_, int D_, int T_, int NT8_>
+// Kernel shape: TYPE of the cache, head size, T 16-bit terms of q and P, NT8 tiles of 8 columns; WHOLE: pages are of a
+// multiple of 16 tokens, so that 16 tokens lie in one page, their rows a stride apart.
+template <int TYPE_, int D_, int T_, int NT8_, bool WHOLE_>
 struct Shape {
     static constexpr int TYPE = TYPE_, D = D_, T = T_, NT8 = NT8_;
+    static constexpr bool WHOLE = WHOLE_;
     static constexpr int HT = T == 1 ? 8 : T == 2 ? 4 : 2;  // query heads of a tile
     static constexpr int R = HT * NT8;                      // and of a pass
     static constexpr int TM = tok_tiles(D), TS = step_toks(D), KS = D / 16;
@@ -278,16 +280,16 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 
     // ---- loads ----
     constexpr unsigned ALL = TS == 32 ? FULL : 0xFFFFu;
-    const bool whole = p.c.page_tokens % 16 == 0;            // 16 tokens lie in one page: their rows are a stride apart
     const uint16_t * ld_kp = nullptr, * ld_vp = nullptr;     // the KV head's rows
     const uint32_t * ld_table = nullptr;                     // the sequence's table row; NULL: out of range
     unsigned ld_live = 0;                                    // live tokens of the step at ld
-    int64_t ld_off[TM];                                      // whole: element offsets of its 16-token groups
-    int64_t ld_row = -1;                                     // whole: of group ld_win + lane, else of token `lane` of the step;
-    int ld_win = 0;                                          // < 0: no page, or not live
-    auto row_of = [&](int tok) {
-        const uint32_t g = p.page_shift >= 0 ? (uint32_t) tok >> p.page_shift : (uint32_t) tok / (uint32_t) p.c.page_tokens;
-        const uint32_t page = ld_table[g];
+    int64_t ld_off[TM];                                      // WHOLE: element offsets of its 16-token groups
+    int64_t ld_row = -1;                                     // of group (WHOLE) or token ld_win + lane; < 0: no page, or
+    int ld_win = 0;                                          // not in the span
+    uint32_t ld_next = SJKVARN_NO_BLOCK;                     // page of token ld_win + 32 + lane, asked for a window ahead:
+    bool ld_has = false;                                     // read when needed, every step would wait for its pages
+    auto group_of = [&](int tok) { return p.page_shift >= 0 ? (uint32_t) tok >> p.page_shift : (uint32_t) tok / (uint32_t) p.c.page_tokens; };
+    auto row_of = [&](int tok, uint32_t g, uint32_t page) {
         if (page < p.c.n_pages)
             return (int64_t) page * p.c.page_stride + (int64_t) (((uint32_t) tok - g * (uint32_t) p.c.page_tokens) * (uint64_t) p.slot_stride);
         if (page != SJKVARN_NO_BLOCK) atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
@@ -302,16 +304,18 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         ld_kp = static_cast<const uint16_t *>(p.c.k) + head;
         ld_vp = static_cast<const uint16_t *>(p.c.v) + head;
         ld_win = -64;
+        ld_has = false;
     };
     auto look_up = [&]() {                                   // the step at ld
         const int step = ld.s.first + ld.st, tok0 = step * TS;
         const int a = ld.s.lo - tok0, b = ld.s.hi - tok0;    // its tokens [a, b) are in the span
-        if (whole) {
+        if constexpr (S::WHOLE) {
             const int g = step * TM;
             if (g - ld_win >= 32) {                          // the pages of the next 32 groups
                 ld_win = g;
                 const int tok = (g + lane) * 16;
-                ld_row = tok < ld.s.hi && tok + 16 > ld.s.lo && ld_table ? row_of(tok) : -1;
+                ld_row = -1;
+                if (tok < ld.s.hi && tok + 16 > ld.s.lo && ld_table) { const uint32_t q = group_of(tok); ld_row = row_of(tok, q, ld_table[q]); }
             }
             ld_live = ALL;
             if (a > 0) ld_live &= FULL << a;
@@ -322,14 +326,33 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 if (ld_off[h] < 0) ld_live &= ~(0xFFFFu << (16 * h));
             }
         } else {
-            const int t = lane & (TS - 1);
-            ld_row = t >= a && t < b && ld_table ? row_of(tok0 + t) : -1;
-            ld_live = __ballot_sync(FULL, ld_row >= 0) & ALL;
+            if (tok0 - ld_win >= 32) {                       // the next 32 tokens
+                ld_has = ld_has && tok0 == ld_win + 32;
+                ld_win = tok0;
+                const int left = ld.s.hi - tok0 - lane;      // tokens from this lane's on (positions reach 2^31 - 2)
+                ld_row = -1;
+                if (left > 0 && tok0 + lane >= ld.s.lo && ld_table) {
+                    const uint32_t q = group_of(tok0 + lane);
+                    ld_row = row_of(tok0 + lane, q, ld_has ? ld_next : ld_table[q]);
+                }
+                ld_has = true;
+                if (left > 32 && ld_table) ld_next = ld_table[group_of(tok0 + lane + 32)];
+            }
+            ld_live = __ballot_sync(FULL, ld_row >= 0) >> (tok0 - ld_win) & ALL;
         }
     };
     auto copy = [&](uint32_t dst, const uint16_t * base) {
         constexpr int CH = D / 8;                            // 16-byte words of a row
-        if (whole && ld_live == ALL) {
+        if constexpr (!S::WHOLE) {
+            const int t0 = (ld.s.first + ld.st) * TS - ld_win;
+#pragma unroll 4
+            for (int i = 0; i < TS * CH / 32; ++i) {
+                const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
+                const int64_t row = __shfl_sync(FULL, ld_row, t0 + r);
+                const bool on = row >= 0;
+                cp16_or_zero(dst + r * PITCH + c * 16, base + (on ? row : 0) + c * 8, on);
+            }
+        } else if (ld_live == ALL) {
 #pragma unroll
             for (int h = 0; h < TM; ++h) {                   // 16 rows: 32 words at a time, D / 16 times
                 const uint16_t * src = base + ld_off[h];
@@ -350,8 +373,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 #pragma unroll 1
             for (int i = 0; i < TS * CH / 32; ++i) {
                 const int w = i * 32 + lane, r = w / CH, c = w - r * CH;
-                const int64_t one = __shfl_sync(FULL, ld_row, r);
-                const int64_t row = whole ? (TM == 2 && r >= 16 ? ld_off[TM - 1] : ld_off[0]) + (int64_t) ((uint64_t) (r & 15) * p.slot_stride) : one;
+                const int64_t row = (TM == 2 && r >= 16 ? ld_off[TM - 1] : ld_off[0]) + (int64_t) ((uint64_t) (r & 15) * p.slot_stride);
                 const bool on = (ld_live >> r) & 1u;
                 cp16_or_zero(dst + r * PITCH + c * 16, base + (on ? row : 0) + c * 8, on);
             }
@@ -829,31 +851,33 @@ int run(const Params & p0, const Plan & pl, sjk_stream st) {
 }
 
 // f(Shape) for the call's types and sizes: nt8 1 or 2 tiles of columns in one pass over K and V
-template <int TYPE, int D, typename F>
+template <int TYPE, int D, bool WHOLE, typename F>
 int with_terms(bool split, int nt8, F && f) {
     constexpr int T = TYPE == SJK_F16 ? 2 : 3;
-    if (!split) return nt8 == 1 ? f(Shape<TYPE, D, 1, 1>()) : f(Shape<TYPE, D, 1, 2>());
-    return nt8 == 1 ? f(Shape<TYPE, D, T, 1>()) : f(Shape<TYPE, D, T, 2>());
+    if (!split) return nt8 == 1 ? f(Shape<TYPE, D, 1, 1, WHOLE>()) : f(Shape<TYPE, D, 1, 2, WHOLE>());
+    return nt8 == 1 ? f(Shape<TYPE, D, T, 1, WHOLE>()) : f(Shape<TYPE, D, T, 2, WHOLE>());
 }
-template <int TYPE, typename F>
+template <int TYPE, bool WHOLE, typename F>
 int with_dim(int D, bool split, int nt8, F && f) {
     switch (D) {
-        case 64: return with_terms<TYPE, 64>(split, nt8, f);
-        case 96: return with_terms<TYPE, 96>(split, nt8, f);
-        case 128: return with_terms<TYPE, 128>(split, nt8, f);
-        case 256: return with_terms<TYPE, 256>(split, nt8, f);
+        case 64: return with_terms<TYPE, 64, WHOLE>(split, nt8, f);
+        case 96: return with_terms<TYPE, 96, WHOLE>(split, nt8, f);
+        case 128: return with_terms<TYPE, 128, WHOLE>(split, nt8, f);
+        case 256: return with_terms<TYPE, 256, WHOLE>(split, nt8, f);
         default: return SJK_ERR_UNSUPPORTED;
     }
 }
 template <typename F>
-int with_shape(int type, int D, bool split, int nt8, F && f) {
-    return type == SJK_F16 ? with_dim<SJK_F16>(D, split, nt8, f) : with_dim<SJK_BF16>(D, split, nt8, f);
+int with_shape(const sjk_kv16 * c, bool split, int nt8, F && f) {
+    if (c->page_tokens % 16 == 0)
+        return c->type == SJK_F16 ? with_dim<SJK_F16, true>(c->head_dim, split, nt8, f) : with_dim<SJK_BF16, true>(c->head_dim, split, nt8, f);
+    return c->type == SJK_F16 ? with_dim<SJK_F16, false>(c->head_dim, split, nt8, f) : with_dim<SJK_BF16, false>(c->head_dim, split, nt8, f);
 }
 
 int plan_of(const sjk_kv16 * c, int n_head, bool split, Plan * pl) {
     const int grp = n_head / c->n_head_kv, ht = !split ? 8 : c->type == SJK_F16 ? 4 : 2;
     pl->nt8 = grp <= ht ? 1 : 2;
-    const int rc = with_shape(c->type, c->head_dim, split, pl->nt8, [&](auto s) { pl->work = 148 * decltype(s)::W; pl->R = decltype(s)::R; return 0; });
+    const int rc = with_shape(c, split, pl->nt8, [&](auto s) { pl->work = 148 * decltype(s)::W; pl->R = decltype(s)::R; return 0; });
     if (rc) return rc;
     pl->tiles = (grp + pl->R - 1) / pl->R;
     pl->part = (size_t) pl->work * 2 * pl->R * c->head_dim;
@@ -913,7 +937,7 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     p.by_pair = (int64_t) n_seq * HP <= p.n_work;
     // a list per head where that leaves under a sixteenth of the workers without one
     p.wph = HP * 16 <= p.n_work ? p.n_work / HP : 0;
-    return with_shape(c->type, c->head_dim, split, pl.nt8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
+    return with_shape(c, split, pl.nt8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
 }
 
 int sjk_kv16_status_take(void) {
