@@ -184,12 +184,9 @@ SJK_DEV void load_pairs(float2 (&x)[N], const void * p, int64_t at, bool on) {
     }
 }
 template <int TYPE, int KS>
-SJK_DEV void store_channels(void * p, int64_t at, const float (&o)[KS][4], int j, float f) {
+SJK_DEV void store_channels(void * p, int64_t at, const float (&o)[KS][4], int i, float f) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-        store1(p, at + 16 * k, TYPE, o[k][j] * f);
-        store1(p, at + 16 * k + 8, TYPE, o[k][2 + j] * f);
-    }
+    for (int k = 0; k < KS; ++k) store1(p, at + 16 * k, TYPE, o[k][i] * f);
 }
 
 template <typename S>
@@ -411,6 +408,11 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         if (T == 3) { x += __shfl_xor_sync(FULL, x, 1); x += __shfl_xor_sync(FULL, x, 2); }
         return x;
     };
+    // A pair's results at its end: with several terms the lanes of a quad divide the sums over them among themselves. Each
+    // has NJ heads (from own_j on) of its NT8 tiles, and NH of the two 8-channel halves (from own_h on) of every 16.
+    constexpr int NJ = T == 3 ? 1 : 2, NH = T == 1 ? 2 : 1;
+    const int own_j = T == 3 ? lane & 1 : 0, own_h = T == 1 ? 0 : (lane >> 1) & 1;
+    auto at_of = [&](int j, int h) { return T == 1 ? 2 * h + j : T == 2 ? j : 0; };      // where in o[n][k]
     uint32_t qf[KS][NT8][2];
     float o[NT8][KS][4], m[NT8][2], l[NT8][2], sc[NT8][2];
     bool fresh = true, begun = false, started = false;       // a pair comes next; its first step is in this run; loads are out
@@ -647,26 +649,40 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                     l[n][j] += __shfl_xor_sync(FULL, l[n][j], 8);
                     l[n][j] += __shfl_xor_sync(FULL, l[n][j], 16);
                 }
+                if constexpr (T > 1) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int r = HT * n + first + j;
-                    if constexpr (T > 1) {
+                    for (int k = 0; k < KS; ++k) {
 #pragma unroll
-                        for (int k = 0; k < KS; ++k) { o[n][k][j] = terms(o[n][k][j]); o[n][k][2 + j] = terms(o[n][k][2 + j]); }
-                        if (mine_t) continue;
+                        for (int j = 0; j < 2; ++j) {
+                            const float lo = o[n][k][j], hi = o[n][k][2 + j];
+                            o[n][k][j] = (own_h ? hi : lo) + __shfl_xor_sync(FULL, own_h ? lo : hi, 2);
+                        }
+                        if constexpr (T == 3) {
+                            const float x = o[n][k][0], y = o[n][k][1];
+                            o[n][k][0] = (own_j ? y : x) + __shfl_xor_sync(FULL, own_j ? x : y, 1);
+                        }
                     }
+                }
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    const int r = HT * n + first + own_j + j;
                     if (r0 + r >= p.grp) continue;
                     if (joint) continue;                     // written below
+                    const float mj = own_j ? m[n][1] : m[n][j], lj = own_j ? l[n][1] : l[n][j];
                     if (begun && ended) {
-                        const float inv = l[n][j] == 0.0f ? 0.0f : 1.0f / l[n][j];
-                        const int64_t dst = (int64_t) at.seq * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride + (lane >> 2);
-                        if (p.out.type == SJK_F32) store_channels<SJK_F32>(p.out.p, dst, o[n], j, inv);
-                        else if (p.out.type == SJK_F16) store_channels<SJK_F16>(p.out.p, dst, o[n], j, inv);
-                        else store_channels<SJK_BF16>(p.out.p, dst, o[n], j, inv);
+                        const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
+                        const int64_t dst = (int64_t) at.seq * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride + (lane >> 2) + 8 * own_h;
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) {
+                            if (p.out.type == SJK_F32) store_channels<SJK_F32>(p.out.p, dst + 8 * h, o[n], at_of(j, h), inv);
+                            else if (p.out.type == SJK_F16) store_channels<SJK_F16>(p.out.p, dst + 8 * h, o[n], at_of(j, h), inv);
+                            else store_channels<SJK_BF16>(p.out.p, dst + 8 * h, o[n], at_of(j, h), inv);
+                        }
                     } else {
                         const int64_t slot = ((int64_t) worker * 2 + (begun ? 1 : 0)) * R + r;
-                        store_channels<SJK_F32>(p.part, slot * D + (lane >> 2), o[n], j, 1.0f);
-                        if (lane < 4) *reinterpret_cast<float2 *>(p.ml + slot * 2) = make_float2(m[n][j], l[n][j]);
+#pragma unroll
+                        for (int h = 0; h < NH; ++h) store_channels<SJK_F32>(p.part, slot * D + (lane >> 2) + 8 * (own_h + h), o[n], at_of(j, h), 1.0f);
+                        if (lane < 4 && own_h == 0) *reinterpret_cast<float2 *>(p.ml + slot * 2) = make_float2(mj, lj);
                     }
                 }
             }
@@ -690,11 +706,13 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 #pragma unroll
     for (int n = 0; n < NT8; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r = HT * n + first + j;
+        for (int j = 0; j < NJ; ++j) {
+            const int r = HT * n + first + own_j + j;
             float top = -INFINITY;
             for (int w = 0; w < W; ++w) top = fmaxf(top, s_ml[w * R + r].x);
-            if (mine_t == 0) store_channels<SJK_F32>(s_o, (warp * R + r) * D + (lane >> 2), o[n], j, ex2(m[n][j] - (top == -INFINITY ? 0.0f : top)));
+            const float f = ex2((own_j ? m[n][1] : m[n][j]) - (top == -INFINITY ? 0.0f : top));
+#pragma unroll
+            for (int h = 0; h < NH; ++h) store_channels<SJK_F32>(s_o, (warp * R + r) * D + (lane >> 2) + 8 * (own_h + h), o[n], at_of(j, h), f);
         }
     __syncthreads();
     const bool first_begun = __syncthreads_or(warp == 0 && begun);
