@@ -174,14 +174,27 @@ struct Shape {
     static constexpr int CTA_BYTES = W * WARP_BYTES;
 };
 
-// pairs of channels 8 apart, from element `at` on
-template <int TYPE, int N>
+// pairs of channels 8 STEP apart, from element `at` on
+template <int TYPE, int STEP, int N>
 SJK_DEV void load_pairs(float2 (&x)[N], const void * p, int64_t at, bool on) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         x[k] = make_float2(0.0f, 0.0f);
-        if (on) x[k] = make_float2(load1(p, at + 8 * k, TYPE), load1(p, at + 8 * k + 1, TYPE));
+        if (on) x[k] = make_float2(load1(p, at + 8 * STEP * k, TYPE), load1(p, at + 8 * STEP * k + 1, TYPE));
     }
+}
+// w[i] to place i ^ u
+template <int N>
+SJK_DEV void swap_by(uint32_t (&w)[N], int u) {
+#pragma unroll
+    for (int b = 1; b < N; b <<= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (!(i & b)) {
+                const uint32_t x = w[i], y = w[i | b];
+                w[i] = u & b ? y : x;
+                w[i | b] = u & b ? x : y;
+            }
 }
 template <int TYPE, int KS>
 SJK_DEV void store_channels(void * p, int64_t at, const float (&o)[KS][4], int i, float f) {
@@ -436,7 +449,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
                 const int rel = r0 + HT * n + qhead;
-                on[n] = rel < p.grp && qterm < T;
+                on[n] = rel < p.grp;
                 src[n] = (int64_t) at.seq * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
             }
             if constexpr (T == 1) {
@@ -449,39 +462,49 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 }
                 start();
             } else {
-                float2 x[NT8][2 * KS];
+                // The GT lanes with a head's terms split every GT-th pair of channels each and exchange the words.
+                constexpr int GT = T == 3 ? 4 : 2, SH = T == 3 ? 8 : 16, NX = 2 * KS / GT;
+                float2 x[NT8][NX];
 #pragma unroll
                 for (int n = 0; n < NT8; ++n) {
-                    if (p.q.type == SJK_F32) load_pairs<SJK_F32>(x[n], p.q.p, src[n], on[n]);
-                    else if (p.q.type == SJK_F16) load_pairs<SJK_F16>(x[n], p.q.p, src[n], on[n]);
-                    else load_pairs<SJK_BF16>(x[n], p.q.p, src[n], on[n]);
+                    const int64_t from = src[n] + 8 * qterm;
+                    if (p.q.type == SJK_F32) load_pairs<SJK_F32, GT>(x[n], p.q.p, from, on[n]);
+                    else if (p.q.type == SJK_F16) load_pairs<SJK_F16, GT>(x[n], p.q.p, from, on[n]);
+                    else load_pairs<SJK_BF16, GT>(x[n], p.q.p, from, on[n]);
                 }
                 start();
 #pragma unroll
                 for (int n = 0; n < NT8; ++n) {
                     float big = 0.0f;                        // the row to [1, 2) by an exact power of two
 #pragma unroll
-                    for (int k = 0; k < 2 * KS; ++k) big = fmaxf(big, fmaxf(fabsf(x[n][k].x), fabsf(x[n][k].y)));
+                    for (int k = 0; k < NX; ++k) big = fmaxf(big, fmaxf(fabsf(x[n][k].x), fabsf(x[n][k].y)));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 2));
+                    big = fmaxf(big, __shfl_xor_sync(FULL, big, SH));
+                    if (T == 3) big = fmaxf(big, __shfl_xor_sync(FULL, big, 2 * SH));
                     const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 0;
                     const float mul = ldexpf(1.0f, e < -120 ? 120 : e > 120 ? -120 : -e);
 #pragma unroll
                     for (int j = 0; j < 2; ++j) sc[n][j] = p.scale * 1.4426950408889634f / __shfl_sync(FULL, mul, (first + j) * 4);
 #pragma unroll
-                    for (int k = 0; k < 2 * KS; ++k) {
+                    for (int k = 0; k < NX; ++k) {
                         float a = x[n][k].x * mul, b = x[n][k].y * mul;
-                        uint32_t w = pack2<S::TYPE>(a, b);
+                        uint32_t w[GT];                      // the terms: what is left after those before them
 #pragma unroll
-                        for (int t = 1; t < T; ++t) {        // the column's term: what is left after those before it
-                            const float2 z = widen2<S::TYPE>(w);
+                        for (int t = 0; t < T; ++t) {
+                            w[t] = pack2<S::TYPE>(a, b);
+                            const float2 z = widen2<S::TYPE>(w[t]);
                             a -= z.x;
                             b -= z.y;
-                            const uint32_t v = pack2<S::TYPE>(a, b);
-                            if (qterm >= t) w = v;
-                            else { a += z.x; b += z.y; }
                         }
-                        qf[k >> 1][n][k & 1] = w;
+                        if constexpr (T == 3) w[3] = 0u;     // the column without a term
+                        // word t to the lane with term t, which puts it at this lane's place
+                        swap_by<GT>(w, qterm);
+#pragma unroll
+                        for (int d = 1; d < GT; ++d) w[d] = __shfl_xor_sync(FULL, w[d], d * SH);
+                        swap_by<GT>(w, qterm);
+#pragma unroll
+                        for (int v = 0; v < GT; ++v) qf[(GT * k + v) >> 1][n][(GT * k + v) & 1] = w[v];
                     }
                 }
             }
