@@ -3,11 +3,12 @@
 //
 // Bound: HBM, every live K and V row once (4 D bytes per position and KV head for 4 D grp flops: at most 16 flops per
 // byte for 16 query heads, far under the tensor cores' ridge). Measured (us a call, GB/s of live rows): 32 sequences of
-// 8K-64K, 4 KV heads of 256 bf16 channels 775-797 by machine (6,290-6,470: a plain copy's rate is 6,539); one of 100,000 tokens with
-// 32-bit queries and outputs 78 (5,230); 48 windows of 4,096, 24 heads of 64 channels 91 (5,540); 256 short chats of 0 to
-// 2,048 tokens 68 (4,810); one of 611 tokens 9.4. What is left above the bytes: 4-5 us until the first products (launch,
-// lengths, table, queries, first rows, each behind the other), 3 us for the merge, and SMs whose share of the memory is
-// smaller than others' (the slowest end 15 % after the mean).
+// 8K-64K, 4 KV heads of 256 bf16 channels 755-797 by machine (6,290-6,640: a plain copy's rate is 6,539); one of 100,000
+// tokens with 32-bit queries and outputs 77 (5,320); 48 windows of 4,096, 24 heads of 64 channels 92 (5,500); 256 short
+// chats of 0 to 2,048 tokens 68 (4,800); one of 611 tokens 9.1. Pages of one token cost a tenth more than those of 16 (88
+// sequences of up to 19,024 tokens, 2 heads of 128: 60 against 55). What is left above the bytes: 4-5 us until the first
+// products (launch, lengths, table, queries, first rows, each behind the other), 3 us for the merge, and SMs whose share
+// of the memory is smaller than others' (the slowest end 15 % after the mean).
 //  - A warp is a worker of its own. Per KV head, the (sequence, step of TS tokens) pairs of a call form one list, cut
 //    into equal runs, one per warp of a grid that fills the GPU; lengths are read from device memory, so every warp
 //    finds its run with a scan over them. A sequence weighs OV units beside its steps, for what its start and its
