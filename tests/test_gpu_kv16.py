@@ -281,3 +281,50 @@ def test_two_streams(T):
     T.cuda.synchronize()
     for j in range(2):
         assert all(T.equal(o, want[j]) for o in outs[j])
+
+
+@pytest.mark.parametrize("dtype,io", [("bf16", "bf16"), ("f16", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("page", [1, 3, 24, 40])
+def test_small_pages(T, dtype, io, D, page):
+    """Pages that are no multiple of 16 tokens: ragged sequences in any order of rows, a long one, missing pages, windows
+    and ids out of range."""
+    import random
+    r = random.Random(page + D)
+    lens = [r.choice([0, 1, 31, 32, 33, 63, 64, 65, r.randint(1, 700)]) for _ in range(40)] + [9001]
+    cache, g = _build(T, lens, page, 2, D, _dt(T, dtype), seed=page)
+    for i, x in enumerate(lens):
+        for _ in range(2 if x > 200 else 0):
+            cache.tables[i, r.randrange((x - 1) // page)] = -1                      # (the last page stays)
+    order = list(range(len(lens)))
+    r.shuffle(order)
+    q = T.randn((len(lens), 10, D), device="cuda", generator=g).to(_dt(T, io))
+    rows, mine = T.tensor(order, dtype=T.int32, device="cuda"), [lens[i] for i in order]
+    dl = T.tensor(mine, dtype=T.int32, device="cuda")
+    for window in (0, 50):
+        got = cache.attend(0, q, dl, 0.1, window=window, rows=rows)
+        _check(T, cache, got, q, mine, 0.1, window, rows=order)
+    assert sjk.lib().sjk_device_status() == 0
+    at = order.index(len(lens) - 1)
+    cache.tables[len(lens) - 1, 4000 // page] = cache.k.shape[1]
+    got = cache.attend(0, q, dl, 0.1, rows=rows)
+    assert sjk.lib().sjk_device_status() == sjk.DEVICE_PAGE
+    cache.tables[len(lens) - 1, 4000 // page] = -1
+    _check(T, cache, got[at:at + 1], q[at:at + 1], [9001], 0.1, rows=[len(lens) - 1])
+
+
+@pytest.mark.parametrize("page,window", [(2 ** 20 + 8, 1000000), (2 ** 20 + 8, 1040000), (2 ** 20, 1000000), (2 ** 20, 1050000)])
+def test_longest_sequence(T, page, window):
+    """The last positions below 2^31 - 1, in one page and over two, whose tokens are and are no multiple of 16."""
+    D, length = 64, 2 ** 31 - 1
+    cache = kv16.Cache.alloc(1, 2, page, 1, D, T.bfloat16, 1, 2048)
+    g = T.Generator(device="cuda")
+    g.manual_seed(page)
+    cache.k.normal_(generator=g)
+    cache.v.normal_(generator=g)
+    cache.tables.fill_(-1)
+    cache.tables[0, 2046:] = T.tensor([1, 0], dtype=T.int32, device="cuda")
+    q = T.randn((1, 2, D), device="cuda", generator=g).bfloat16()
+    got = cache.attend(0, q, T.tensor([length], dtype=T.int32, device="cuda"), 0.5, window=window)
+    _check(T, cache, got, q, [length], 0.5, window)
+    assert sjk.lib().sjk_device_status() == 0
