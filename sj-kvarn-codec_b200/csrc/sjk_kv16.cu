@@ -324,9 +324,12 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
             const int g = step * TM;
             if (g - ld_win >= 32) {                          // the pages of the next 32 groups
                 ld_win = g;
-                const int tok = (g + lane) * 16;
+                const uint32_t tok = (uint32_t) (g + lane) * 16u;            // (past 2^31 - 1 behind the longest sequence)
                 ld_row = -1;
-                if (tok < ld.s.hi && tok + 16 > ld.s.lo && ld_table) { const uint32_t q = group_of(tok); ld_row = row_of(tok, q, ld_table[q]); }
+                if (tok < (uint32_t) ld.s.hi && tok + 16u > (uint32_t) ld.s.lo && ld_table) {
+                    const uint32_t q = group_of((int) tok);
+                    ld_row = row_of((int) tok, q, ld_table[q]);
+                }
             }
             ld_live = ALL;
             if (a > 0) ld_live &= FULL << a;
