@@ -25,11 +25,13 @@
 //    the worker's slot in the scratch, and the merge kernel joins the slots in list order (the result does not depend
 //    on which worker came first). The worker that begins a split pair leaves word of it, so the merge looks at as many
 //    entries as there can be split pairs and scans nothing.
-// Softmax statistics, sums and outputs are 32-bit. Queries of the cache's type enter as they are and P is rounded
-// once to it (up to 2^-8 of each weight for bf16, the size of the output's own rounding). For 32-bit queries or outputs
-// (or a type other than the cache's) q and P are the sums of two (f16) or three (bf16) 16-bit terms side by side in the
-// columns of the same products (4 or 2 heads in 8 columns), and each step's products are summed apart from what came
-// before them, which keeps the result near 32 bits.
+// Softmax statistics, sums and outputs are 32-bit. Queries of the cache's type enter as they are, and P as the sum of
+// two 16-bit terms, one product each: to 2^-16 (bf16) or 2^-22 (f16) of a weight, so that a 16-bit output is off by its
+// own rounding (one term: 2^-8 of a weight, and outputs twice as far off where they nearly cancel; the second term's
+// products cost 1 %: 256 short chats 69 us a pass against 68, 48 windows 95.7 against 94.6). For 32-bit queries or
+// outputs (or a type other than the cache's) q and P are the sums of two (f16) or three (bf16) 16-bit terms side by side
+// in the columns of the same products (4 or 2 heads in 8 columns), and each step's products are summed apart from what
+// came before them, which keeps the result near 32 bits.
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
@@ -428,6 +430,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
     // A pair's results at its end: with several terms the lanes of a quad divide the sums over them among themselves. Each
     // has NJ heads (from own_j on) of its NT8 tiles, and NH of the two 8-channel halves (from own_h on) of every 16.
     constexpr int NJ = T == 3 ? 1 : 2, NH = T == 1 ? 2 : 1;
+    constexpr int PT = T == 1 ? 2 : 1;      // words of a weight in this lane: both terms, or the one of the lane's column
     const int own_j = T == 3 ? lane & 1 : 0, own_h = T == 1 ? 0 : (lane >> 1) & 1;
     auto at_of = [&](int j, int h) { return T == 1 ? 2 * h + j : T == 2 ? j : 0; };      // where in o[n][k]
     uint32_t qf[KS][NT8][2];
@@ -558,7 +561,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 
         // Softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16 of its two heads. The maximum is
         // looked for only when some score is above the one so far: seldom after a sequence's first steps.
-        uint32_t pb[TM][NT8][2];
+        uint32_t pb[PT][TM][NT8][2];
         bool above = false;
 #pragma unroll
         for (int n = 0; n < NT8; ++n)
@@ -618,6 +621,10 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 for (int h = 0; h < 2; ++h) {
                     float x = s[tm][n][2 * h], y = s[tm][n][2 * h + 1];
                     uint32_t w = pack2<S::TYPE>(x, y);
+                    if constexpr (T == 1) {
+                        const float2 f = widen2<S::TYPE>(w);
+                        pb[PT - 1][tm][n][h] = transpose8(pack2<S::TYPE>(x - f.x, y - f.y));
+                    }
 #pragma unroll
                     for (int t = 1; t < T; ++t) {
                         const float2 f = widen2<S::TYPE>(w);
@@ -628,7 +635,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                         else { x += f.x; y += f.y; }
                     }
                     if (T == 3 && mine_t == 3) w = 0u;
-                    pb[tm][n][h] = transpose8(w);
+                    pb[0][tm][n][h] = transpose8(w);
                 }
             }
         }
@@ -645,10 +652,11 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 #pragma unroll
                 for (int n = 0; n < NT8; ++n) {
                     if constexpr (T == 1) {
-                        mma<S::TYPE>(o[n][k], a, pb[tm][n][0], pb[tm][n][1]);
+                        mma<S::TYPE>(o[n][k], a, pb[1][tm][n][0], pb[1][tm][n][1]);
+                        mma<S::TYPE>(o[n][k], a, pb[0][tm][n][0], pb[0][tm][n][1]);
                     } else {                                 // the step's sum apart, joined by a rounded addition
                         float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma<S::TYPE>(c, a, pb[tm][n][0], pb[tm][n][1]);
+                        mma<S::TYPE>(c, a, pb[0][tm][n][0], pb[0][tm][n][1]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) o[n][k][e] += c[e];
                     }
