@@ -32,6 +32,9 @@
 // outputs (or a type other than the cache's) q and P are the sums of two (f16) or three (bf16) 16-bit terms side by side
 // in the columns of the same products (4 or 2 heads in 8 columns), and each step's products are summed apart from what
 // came before them, which keeps the result near 32 bits.
+// Weights lie in (0, 1], and f16 has its last bit at 2^-24 there: weights of f16 caches are held 2^15 times larger, in l as
+// well as in O, so that what is lost of a weight is at most 2^-40 of the largest in the worker's run (without it 2^-25:
+// with one token 17 nats above all others, the others were gone from O while l still had them).
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 
@@ -44,6 +47,7 @@ using namespace sjk16;
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int OV = 4;                       // what a (sequence, KV head, row tile) costs beside its steps, in steps
 constexpr int MIN_RUN = 2;                  // units of a worker's run, at least
+constexpr float F16_UP = 32768.0f;          // weights of f16 caches, and so their sums and partials, are this much larger
 __device__ unsigned int g_kv16_status;
 
 struct Params {
@@ -615,6 +619,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     s[tm][n][e] = ex2(s[tm][n][e] - use[e & 1]);
+                    if constexpr (S::TYPE == SJK_F16) s[tm][n][e] *= F16_UP;
                     l[n][e & 1] += s[tm][n][e];
                 }
 #pragma unroll

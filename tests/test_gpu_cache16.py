@@ -51,3 +51,60 @@ def test_weights_of_16_bit_rows(T, dtype, D, grp, page):
     got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), 1 / math.sqrt(D))
     _check(T, cache, got, q, lens, 1 / math.sqrt(D))
     assert sjk.lib().sjk_device_status() == 0
+
+
+def _peaked(T, dtype, io, out, D, gap, n, spread, many, seed=0):
+    """Sequences whose first token stands `gap` nats above the others, with V = 0 there (an attention sink); the others'
+    scores spread by `spread` nats. many: entries of that one table row, so that one worker holds a whole sequence."""
+    grp, H = 4, 2
+    cache, g = _build(T, [n], 16, H, D, _dt(T, dtype), seed=seed)
+    q0 = T.randn((H, 1, D), device="cuda", generator=g)
+    q = (q0 + 0.05 * T.randn((H, grp, D), device="cuda", generator=g)).reshape(1, H * grp, D).to(_dt(T, io))
+    scale = 1 / math.sqrt(D)
+    unit = q0[:, 0] / q0[:, 0].norm(dim=-1, keepdim=True)
+    first = cache.tables[0, 0].item()
+    others = T.arange(n, device="cuda")[1:]
+    ids = cache.tables[0, others // 16].long()
+    cache.k[0, ids, others % 16] = (spread / q0[:, 0].norm(dim=-1)[None, :, None] * math.sqrt(D) *
+                                    T.randn((n - 1, H, 1), device="cuda", generator=g) * unit).to(cache.k.dtype)
+    cache.k[0, first, 0] = (unit * gap * math.sqrt(D) / q0[:, 0].norm(dim=-1, keepdim=True)).to(cache.k.dtype)
+    cache.v[0, first, 0] = 0
+    qs = q.expand(many, -1, -1).contiguous()
+    rows = T.zeros(many, dtype=T.int32, device="cuda")
+    got = T.full(qs.shape, 9.0, dtype=_dt(T, out), device="cuda")
+    cache.attend(0, qs, T.full((many,), n, dtype=T.int32, device="cuda"), scale, rows=rows, out=got)
+    return cache, qs, got, scale
+
+
+@pytest.mark.parametrize("dtype,io,out", [("f16", "f16", "f16"), ("f16", "f32", "f32"), ("f16", "f16", "f32"), ("f16", "bf16", "bf16"),
+                                          ("bf16", "bf16", "bf16"), ("bf16", "f32", "f32")])
+@pytest.mark.parametrize("gap", [10, 14, 17, 20, 25])
+@pytest.mark.parametrize("many", [1, 1300])
+@pytest.mark.parametrize("spread", [0.1, 1.0])
+def test_tokens_far_below_the_largest(T, dtype, io, out, gap, many, spread):
+    """What stands 10 to 25 nats below one token keeps its share: what a weight of an f16 cache loses beside its rounding is
+    2^-40 of the largest in its worker's run, so n 2^-40 max |V| at most (l is at least the largest weight); bf16 has the
+    range of 32 bits."""
+    n, D = 2048, 128
+    cache, q, got, scale = _peaked(T, dtype, io, out, D, gap, n, spread, many)
+    floor = n * 2.0 ** -40 * float(cache.v[0, cache.tables[0, : n // 16].long()].abs().max()) if dtype == "f16" else 0.0
+    some = [0] if many == 1 else [0, many // 2, many - 1]
+    _check(T, cache, got[some], q[some], [n] * len(some), scale, rows=[0] * len(some), floor=floor)
+    assert sjk.lib().sjk_device_status() == 0
+
+
+@pytest.mark.parametrize("io,out", [("f16", "f16"), ("f16", "f32"), ("f32", "f32")])
+def test_extreme_scores_of_f16_caches(T, io, out):
+    """Large scores of both signs over an f16 cache, one token that takes all, scale 0 and a negative scale."""
+    lens, D = [70, 700], 128
+    cache, g = _build(T, lens, 16, 1, D, T.float16)
+    q = (30 * T.randn((2, 4, D), device="cuda", generator=g)).to(_dt(T, io))
+    dl = T.tensor(lens, dtype=T.int32, device="cuda")
+    floor = 700 * 2.0 ** -40 * 6
+    for scale in (1.0, -1.0, 0.0, 1e-3, 1e4, 1e8):
+        got = T.full(q.shape, 9.0, dtype=_dt(T, out), device="cuda")
+        cache.attend(0, q, dl, scale, out=got)
+        if abs(scale) < 100:
+            _check(T, cache, got, q, lens, scale, floor=floor)
+        else:
+            assert bool(T.isfinite(got).all())
