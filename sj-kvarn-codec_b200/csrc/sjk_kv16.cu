@@ -486,7 +486,8 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 start();
 #pragma unroll
                 for (int n = 0; n < NT8; ++n) {
-                    float big = 0.0f;                        // the row to [1, 2) by an exact power of two
+                    float big = 0.0f;                        // the row's largest to [1, 2) by an exact power of two; f16
+                                                             // terms, whose last bit is 2^-24, to [2^14, 2^15)
 #pragma unroll
                     for (int k = 0; k < NX; ++k) big = fmaxf(big, fmaxf(fabsf(x[n][k].x), fabsf(x[n][k].y)));
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, 1));
@@ -494,7 +495,8 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                     big = fmaxf(big, __shfl_xor_sync(FULL, big, SH));
                     if (T == 3) big = fmaxf(big, __shfl_xor_sync(FULL, big, 2 * SH));
                     const int e = big > 0.0f && big < INFINITY ? ilogbf(big) : 0;
-                    const float mul = ldexpf(1.0f, e < -120 ? 120 : e > 120 ? -120 : -e);
+                    constexpr int UP = S::TYPE == SJK_F16 ? 14 : 0;
+                    const float mul = ldexpf(1.0f, UP - (e < UP - 127 ? UP - 127 : e > UP + 113 ? UP + 113 : e));
 #pragma unroll
                     for (int j = 0; j < 2; ++j) sc[n][j] = p.scale * 1.4426950408889634f / __shfl_sync(FULL, mul, (first + j) * 4);
 #pragma unroll

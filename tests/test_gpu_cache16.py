@@ -108,3 +108,34 @@ def test_extreme_scores_of_f16_caches(T, io, out):
             _check(T, cache, got, q, lens, scale, floor=floor)
         else:
             assert bool(T.isfinite(got).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("grp", [1, 3, 9])
+@pytest.mark.parametrize("small", [8, 12, 16, 20])
+def test_queries_with_one_large_channel(T, dtype, D, grp, small):
+    """32-bit queries whose first channel, where K is 0, stands 2^small above the others. Two f16 terms keep 2^-39 of the
+    largest channel: the scores of an f16 cache may be off by that beside the bound, bf16 has the range of 32 bits."""
+    lens = [40, 300]
+    cache, g = _build(T, lens, 16, 2, D, _dt(T, dtype), seed=D + small)
+    cache.k[..., 0] = 0
+    q = 2.0 ** -small * T.randn((2, 2 * grp, D), device="cuda", generator=g)
+    q[..., 0] = 1.0
+    scale = 2.0 ** small / math.sqrt(D)
+    got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), scale)
+    floor = 0.0
+    if dtype == "f16":
+        live = cache.k[0].nan_to_num(0.0).abs().sum(-1).max()
+        floor = float(2 * 2.0 ** -39 * scale * live * cache.v[0].nan_to_num(0.0).abs().max())
+    _check(T, cache, got, q, lens, scale, floor=floor)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("big", [1e36, 1e12, 1e-12, 1e-36])
+def test_queries_at_the_ends_of_the_range(T, dtype, big):
+    lens, D = [70, 700], 128
+    cache, g = _build(T, lens, 16, 1, D, _dt(T, dtype))
+    q = big * 30 * T.randn((2, 4, D), device="cuda", generator=g)
+    got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), 0.1 / big)
+    _check(T, cache, got, q, lens, 0.1 / big, floor=700 * 2.0 ** -40 * 6 + 2.0 ** -39 * 60)
