@@ -25,15 +25,17 @@ def T():
     return torch
 
 
-def _check(T, cache, got, q, lens, scale, window=0, rows=None, floor=0.0):
-    """floor: what every element may be off beside the bound."""
+def _check(T, cache, got, q, lens, scale, window=0, rows=None, floor=0.0, few=False):
+    """floor: what every element may be off beside the bound. few: one worker holds all of a sequence's few positions: e is
+    2^-22 for ex2 and 2^-20 of the products, a one sum that may drop 2^-23 and at most 7 rounded additions and products."""
     split = q.dtype != cache.k.dtype or got.dtype == T.float32
     p = 2.0 ** -22 if cache.k.dtype == T.float16 else 2.0 ** -24 if split else 2.0 ** -16
     u = {T.float32: 2.0 ** -23, T.float16: 2.0 ** -11, T.bfloat16: 2.0 ** -8}[got.dtype]
     tiny = 2.0 ** -25 if got.dtype == T.float16 else 1e-37
     for i, x in enumerate(lens):
         want, mag_v, mag = _expect(T, cache, 0, i if rows is None else rows[i], x, q[i], scale, window)
-        bound = u * want.abs() * (1 + 2.0 ** -7) + (p + 2.0 ** -19 * (1 + mag) + 2.0 ** -23 * (x / 16 + 8)) * mag_v + tiny + floor
+        e, a = (2.0 ** -22 + 2.0 ** -20 * mag, 2.0 ** -23 + 7 * 2.0 ** -24) if few else (2.0 ** -20 * (1 + mag), 2.0 ** -23 * (x / 16 + 8))
+        bound = u * want.abs() * (1 + 2.0 ** -7) + (p + 2 * e + a) * mag_v + tiny + floor
         err = (got[i].double().cpu() - want).abs()
         assert bool((err <= bound).all()), f"sequence {i} of length {x}: worst {float((err / bound).max()):.3g} of the bound"
 
@@ -139,3 +141,16 @@ def test_queries_at_the_ends_of_the_range(T, dtype, big):
     q = big * 30 * T.randn((2, 4, D), device="cuda", generator=g)
     got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), 0.1 / big)
     _check(T, cache, got, q, lens, 0.1 / big, floor=700 * 2.0 ** -40 * 6 + 2.0 ** -39 * 60)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("grp", [1, 2, 5, 16])
+def test_weights_of_32_bit_rows(T, dtype, D, grp):
+    """Scores of a size of 0.1 or less, whose own error is small: the rounding of the weights shows (with two bf16 terms of
+    a weight in place of three, the worst element would be about twice the bound off)."""
+    lens = [1, 2, 3, 5, 9]
+    cache, g = _build(T, lens, 16, 2, D, _dt(T, dtype), seed=D + grp)
+    q = T.randn((len(lens), 2 * grp, D), device="cuda", generator=g)
+    got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), 0.1 / D)
+    _check(T, cache, got, q, lens, 0.1 / D, few=True)
