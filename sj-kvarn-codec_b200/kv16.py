@@ -122,7 +122,7 @@ class Pages:
             raise ValueError("slabs: at most 4")
         c.n_slabs = len(self.slabs)
         for i, s in enumerate(self.slabs):
-            if s.dim() < 3 or s.shape[1] != n or not s[0].is_contiguous():
+            if not s.is_cuda or s.dim() < 3 or s.shape[1] != n or not s[0].is_contiguous():
                 raise ValueError("slabs: CUDA tensors [layers][pages][...], pages of a layer contiguous")
             size = s.element_size()
             c.slabs[i] = sjk.Slab(s.data_ptr(), s.stride(1) * size, s.stride(0) * size, s.shape[0])

@@ -1,0 +1,133 @@
+"""What kv16 does on the host around a call: tensors and devices it refuses, the device it launches on, threads that share
+an object, scratch memory. On the CPU: tensors that say they are a GPU's, and a library that notes the calls."""
+import ctypes as C
+import math
+import threading
+import time
+import types
+
+import pytest
+import torch
+
+import kv16
+import sjk
+
+
+class Gpu:
+    """A CPU tensor that says it is GPU `index`'s."""
+    is_cuda = True
+
+    def __init__(self, t, index=0):
+        self.t, self.index = t, index
+
+    device = property(lambda self: types.SimpleNamespace(index=self.index))
+
+    def get_device(self):
+        return self.index
+
+    def __getitem__(self, i):
+        return Gpu(self.t[i], self.index)
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+class Host:
+    """Stands for the library and for the current device."""
+
+    def __init__(self, lib):
+        self.lib, self.device, self.calls, self.capturing, self.during = lib, 0, [], False, lambda: None
+
+    def __getattr__(self, name):
+        return getattr(self.lib, name)
+
+    def _note(self, name, **kw):
+        self.calls.append(dict(name=name, device=self.device, **kw))
+        return 0
+
+    def sjk_pages_init(self, p, st):
+        return self._note("init", stream=st)
+
+    def sjk_pages_fork(self, p, src, dst, n, status, st):
+        return self._note("fork", stream=st)
+
+    def sjk_pages_extend(self, p, rows, lens, add, add_all, n, status, st):
+        return self._note("extend", stream=st)
+
+    def sjk_pages_free(self, p, rows, g0, g1, n, st):
+        return self._note("free", stream=st)
+
+    def sjk_pages_compact(self, p, info, st):
+        return self._note("compact", stream=st)
+
+    def sjk_pages_copy(self, p, src, dst, n, st):
+        return self._note("copy", stream=st)
+
+    def sjk_rope_init(self, r, cfg):
+        r._obj.n_rot, r._obj.amp, r._obj.step = cfg._obj.n_rot, 1.0, 0x10000
+        return self._note("rope")
+
+    def sjk_rope_free(self, r):
+        pass
+
+    def sjk_kv16_attend(self, c, q, lens, rows, n, scale, window, out, scratch, size, st):
+        self.during()
+        return self._note("attend", stream=st, scratch=scratch, size=size, q=(q._obj.p, q._obj.row_stride, q._obj.n_head), out=out._obj.p,
+                          lens=lens, n=n)
+
+    def sjk_qkv(self, a, st):
+        self.during()
+        a = a._obj
+        return self._note("qkv", stream=st, q=(a.q.p, a.q.row_stride, a.q.n_head), q_out=a.q_out.p, n=a.n_tok, pos=a.pos, rows=a.rows)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    import build
+    build.build()
+    h = Host(sjk.lib())
+
+    class device:                                # torch.cuda.device
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            self.before, h.device = h.device, self.i
+
+        def __exit__(self, *a):
+            h.device = self.before
+
+    def on_host(make):
+        return lambda *a, device=None, **kw: make(*a, **kw)
+
+    monkeypatch.setattr(kv16, "_L", h)
+    monkeypatch.setattr(kv16, "_stream", lambda d: 1000 + d)
+    monkeypatch.setattr(kv16, "_current_device", lambda: h.device, raising=False)
+    monkeypatch.setattr(kv16, "_capturing", lambda: h.capturing, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: h.device)
+    for name in ("empty", "zeros"):
+        monkeypatch.setattr(torch, name, on_host(getattr(torch, name)))
+    return h
+
+
+def _i32(n, index=0):
+    return Gpu(torch.zeros(n, dtype=torch.int32), index)
+
+
+def _heads(n, heads, D=64, dtype=torch.bfloat16, index=0):
+    return Gpu(torch.zeros((n, heads, D), dtype=dtype), index)
+
+
+def _cache(index=0, tables=None):
+    kv = [Gpu(torch.zeros((1, 8, 16, 2, 64), dtype=torch.bfloat16), index) for _ in range(2)]
+    return kv16.Cache(*kv, Gpu(torch.full((4, 4), -1, dtype=torch.int32), index if tables is None else tables))
+
+
+def test_slabs_in_host_memory_are_refused(host):
+    tables = Gpu(torch.full((4, 4), -1, dtype=torch.int32))
+    on, off = Gpu(torch.zeros((1, 8, 64))), torch.zeros((1, 8, 64))
+    kv16.Pages(tables, 16, slabs=[on])
+    for slabs in ([off], [on, off]):
+        with pytest.raises(ValueError, match="slabs"):
+            kv16.Pages(tables, 16, slabs=slabs)
