@@ -535,7 +535,9 @@ int    sjk_truncate_batch(const sjk_trunc_req * reqs, int n, void * dev_pool, sj
  * token per sequence over the pages) and sjk_pages_* (fork, extend with copy on write, free, compact). sjk_qkv also
  * makes the rows that sjk_store and sjk_attend_model take, and the page calls work on the record pool's slab and
  * block tables as well. Lengths, positions, tables and row lists are DEVICE memory, read when the kernels run, so a
- * captured step replays. No counterpart in the reference.
+ * captured step replays. Like the other calls these launch on the current device: make the one current that the
+ * pointers and the stream belong to (its status word is the one that sjk_device_status() reads). No counterpart in the
+ * reference.
  *
  * A table row belongs to one sequence: entry g holds the page of positions [g page_tokens, (g + 1) page_tokens), or
  * SJKVARN_NO_BLOCK. Entries, rows and positions outside their arrays are never followed: the token, position or page

@@ -11,8 +11,9 @@ that reads it (Cache), and who owns the pages (Pages: fork, extend with copy on 
     step(q, k, v, lens, q_out=q2, rows=rows, layer=il)  # position lens[i] of table row rows[i]
     out = cache.attend(il, q2, lens + 1, scale, rows=rows)
 
-Calls run on torch's current stream and do not synchronise. Lengths, positions and row lists are int32 CUDA tensors,
-read when the kernels run; sjk.lib().sjk_device_status() reports entries that pointed outside their arrays.
+Calls run on the tensors' device, on torch's current stream there, and do not synchronise; tensors of another device raise
+ValueError. Lengths, positions and row lists are int32 CUDA tensors, read when the kernels run;
+sjk.lib().sjk_device_status() reports entries that pointed outside their arrays.
 """
 import ctypes as C
 
@@ -44,16 +45,23 @@ def _stream(device):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
-def _index(t):
-    return t.device.index if t.device.index is not None else torch.cuda.current_device()
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _list(t, what, n=None):
-    """Device pointer of an int32 CUDA vector (None passes)."""
+def _launch(device, call, *args):
+    """call(*args) with `device` current: kernels, and limits set for them, go to the device that is."""
+    if _current_device() == device:
+        return call(*args)
+    with torch.cuda.device(device):
+        return call(*args)
+
+
+def _list(t, what, device, n=None):
+    """Address of an int32 vector on device `device` (None passes)."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_cuda or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-        raise ValueError(f"{what}: an int32 CUDA vector" + (f" of {n} values" if n is not None else ""))
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != device or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+        raise ValueError(f"{what}: an int32 vector" + (f" of {n} values" if n is not None else "") + f" on cuda:{device}")
     return t.data_ptr()
 
 
@@ -64,7 +72,7 @@ class _Rows:
     def __init__(self, c, what, D):
         self.c, self.what, self.D, self.like = c, what, D, None
 
-    def set(self, t, n):
+    def set(self, t, n, device):
         c = self.c
         if t is None:
             if self.like is not None:
@@ -77,20 +85,23 @@ class _Rows:
                 raise ValueError(f"{self.what}: a CUDA tensor [{n}][heads][{self.D}] of 16- or 32-bit floats, channels adjacent")
             c.row_stride, c.head_stride, c.n_head, c.type = like[1][0], like[1][1], shape[1], _TYPE[t.dtype]
             self.like = like
-        if not t.is_cuda:
-            raise ValueError(f"{self.what}: a CUDA tensor")
+        if t.get_device() != device:
+            raise ValueError(f"{self.what}: a tensor on cuda:{device}")
         c.p = t.data_ptr()
 
 
 class Rope:
-    """Rotary positions of the first n_rot channels of a head (include/sjk.h, sjk_rope_config)."""
+    """Rotary positions of the first n_rot channels of a head (include/sjk.h, sjk_rope_config), for tensors of `device`
+    (None: the current one)."""
 
     def __init__(self, n_rot, layout="half", base=10000.0, scaling="none", factor=1.0, n_ctx=0, beta_fast=32.0,
-                 beta_slow=1.0, low=1.0, high=4.0, amp=0.0):
+                 beta_slow=1.0, low=1.0, high=4.0, amp=0.0, device=None):
         self.cfg = sjk.RopeConfig(n_rot, LAYOUTS[layout], SCALINGS[scaling], base, factor, n_ctx, beta_fast, beta_slow,
                                   low, high, amp)
         self.c = sjk.RopeC()
-        sjk.check(_lib().sjk_rope_init(C.byref(self.c), C.byref(self.cfg)), "rope_init")
+        at = torch.device(device).index if isinstance(device, (str, torch.device)) else device
+        self.device = _current_device() if at is None else at
+        sjk.check(_launch(self.device, _lib().sjk_rope_init, C.byref(self.c), C.byref(self.cfg)), "rope_init")
 
     def __del__(self):
         if getattr(self, "c", None) is not None and _L is not None:
@@ -120,14 +131,15 @@ class Pages:
         self.c = c = sjk.PagesC(self._buf.data_ptr(), tables.data_ptr(), n, tables.shape[0], tables.shape[1], page_tokens)
         if len(self.slabs) > 4:
             raise ValueError("slabs: at most 4")
+        self._dev = tables.get_device()
         c.n_slabs = len(self.slabs)
         for i, s in enumerate(self.slabs):
-            if not s.is_cuda or s.dim() < 3 or s.shape[1] != n or not s[0].is_contiguous():
-                raise ValueError("slabs: CUDA tensors [layers][pages][...], pages of a layer contiguous")
+            if s.get_device() != self._dev or s.dim() < 3 or s.shape[1] != n or not s[0].is_contiguous():
+                raise ValueError("slabs: CUDA tensors [layers][pages][...] on the tables' device, pages of a layer contiguous")
             size = s.element_size()
             c.slabs[i] = sjk.Slab(s.data_ptr(), s.stride(1) * size, s.stride(0) * size, s.shape[0])
-        self._c, self._dev, self._L = C.byref(c), _index(tables), _lib()
-        sjk.check(self._L.sjk_pages_init(self._c, _stream(self._dev)), "pages_init")
+        self._c, self._L = C.byref(c), _lib()
+        sjk.check(_launch(self._dev, self._L.sjk_pages_init, self._c, _stream(self._dev)), "pages_init")
         # what the last fork, extend and compact call reported (each overwritten by the next of its kind)
         self._forked = torch.zeros(1024, dtype=torch.int32, device=tables.device)
         self._extended = torch.zeros(1, dtype=torch.int32, device=tables.device)
@@ -143,7 +155,8 @@ class Pages:
         """Rows dst get the pages of rows src, shared. Returns the device status vector (0, or a status code each)."""
         n = src.shape[0]
         st = self._forked if n <= 1024 else torch.empty(n, dtype=torch.int32, device=src.device)
-        rc = self._L.sjk_pages_fork(self._c, _list(src, "src"), _list(dst, "dst", n), n, st.data_ptr(), _stream(self._dev))
+        dev = self._dev
+        rc = _launch(dev, self._L.sjk_pages_fork, self._c, _list(src, "src", dev), _list(dst, "dst", dev, n), n, st.data_ptr(), _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "pages_fork")
         return st[:n]
@@ -153,8 +166,9 @@ class Pages:
         Returns the device status (one value: 0, or why nothing was done)."""
         n = rows.shape[0]
         vec = isinstance(add, torch.Tensor)
-        rc = self._L.sjk_pages_extend(self._c, _list(rows, "rows"), _list(lens, "lens", n), _list(add, "add", n) if vec else None,
-                                     0 if vec else add, n, self._extended.data_ptr(), _stream(self._dev))
+        dev = self._dev
+        rc = _launch(dev, self._L.sjk_pages_extend, self._c, _list(rows, "rows", dev), _list(lens, "lens", dev, n),
+                     _list(add, "add", dev, n) if vec else None, 0 if vec else add, n, self._extended.data_ptr(), _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "pages_extend")
         return self._extended
@@ -162,13 +176,15 @@ class Pages:
     def free(self, rows, first=None, end=None):
         """Entries [first, end) of the rows give their pages up (vectors; None: all)."""
         n = rows.shape[0]
-        rc = self._L.sjk_pages_free(self._c, _list(rows, "rows"), _list(first, "first", n), _list(end, "end", n), n, _stream(self._dev))
+        dev = self._dev
+        rc = _launch(dev, self._L.sjk_pages_free, self._c, _list(rows, "rows", dev), _list(first, "first", dev, n), _list(end, "end", dev, n), n,
+                     _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "pages_free")
 
     def compact(self):
         """Used pages to the lowest ids. Returns a device vector: used pages, moved ones."""
-        rc = self._L.sjk_pages_compact(self._c, self._compacted.data_ptr(), _stream(self._dev))
+        rc = _launch(self._dev, self._L.sjk_pages_compact, self._c, self._compacted.data_ptr(), _stream(self._dev))
         if rc:
             raise sjk.SjkError(rc, "pages_compact")
         return self._compacted
@@ -176,7 +192,8 @@ class Pages:
     def copy(self, src, dst):
         """Contents of pages src to pages dst, every layer of every slab."""
         n = src.shape[0]
-        rc = self._L.sjk_pages_copy(self._c, _list(src, "src"), _list(dst, "dst", n), n, _stream(self._dev))
+        dev = self._dev
+        rc = _launch(dev, self._L.sjk_pages_copy, self._c, _list(src, "src", dev), _list(dst, "dst", dev, n), n, _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "pages_copy")
 
@@ -187,10 +204,10 @@ class Cache:
 
     def __init__(self, k, v, tables):
         if k.dim() != 5 or k.shape != v.shape or k.stride() != v.stride() or k.dtype != v.dtype or k.stride(4) != 1 or \
-                k.dtype not in (torch.float16, torch.bfloat16) or not k.is_cuda or not v.is_cuda:
-            raise ValueError("k, v: 16-bit CUDA tensors [layers][pages][tokens][heads][D] with the same strides, channels adjacent")
-        if tables.dtype != torch.int32 or not tables.is_cuda or tables.dim() != 2 or not tables.is_contiguous():
-            raise ValueError("tables: a contiguous int32 CUDA tensor [rows][stride]")
+                k.dtype not in (torch.float16, torch.bfloat16) or not k.is_cuda or v.get_device() != k.get_device():
+            raise ValueError("k, v: 16-bit tensors [layers][pages][tokens][heads][D] of one GPU with the same strides, channels adjacent")
+        if tables.dtype != torch.int32 or tables.get_device() != k.get_device() or tables.dim() != 2 or not tables.is_contiguous():
+            raise ValueError("tables: a contiguous int32 tensor [rows][stride] on the GPU of k and v")
         self.k, self.v, self.tables = k, v, tables
         n_layers, n_pages, page, H, D = k.shape
         st = k.stride()
@@ -200,7 +217,7 @@ class Cache:
         self._refs = [C.byref(x) for x in self.layers]
         self._q, self._o = _Rows(sjk.Rows(), "q", D), _Rows(sjk.Rows(), "out", D)
         self._qo = C.byref(self._q.c), C.byref(self._o.c)
-        self._dev, self._L = _index(k), _lib()
+        self._dev, self._L = k.get_device(), _lib()
         self._scratch = {}                       # by stream and number of query heads: calls of one stream follow one another
 
     @classmethod
@@ -216,22 +233,22 @@ class Cache:
     def attend(self, layer, q, lens, scale, window=0, rows=None, out=None):
         """Attention of one new token per sequence: q [n][heads][D], lens int32 [n] (the newest position included), rows
         int32 [n] (None: sequence i is table row i). Returns out (q's type unless given)."""
-        n = q.shape[0]
+        n, dev = q.shape[0], self._dev
         if out is None:
             out = torch.empty_like(q)
-        self._q.set(q, n)
-        self._o.set(out, n)
+        self._q.set(q, n, dev)
+        self._o.set(out, n, dev)
         if n == 0:
             return out
-        st = _stream(self._dev)
+        st = _stream(dev)
         key = (st, q.shape[1])
         scratch = self._scratch.get(key)
         if scratch is None:
             size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
             buf = torch.empty(size, dtype=torch.uint8, device=q.device)
             scratch = self._scratch[key] = (buf, buf.data_ptr(), size)
-        rc = self._L.sjk_kv16_attend(self._refs[layer], self._qo[0], _list(lens, "lens", n), _list(rows, "rows", n), n, scale,
-                                     window, self._qo[1], scratch[1], scratch[2], st)
+        rc = _launch(dev, self._L.sjk_kv16_attend, self._refs[layer], self._qo[0], _list(lens, "lens", dev, n), _list(rows, "rows", dev, n), n,
+                     scale, window, self._qo[1], scratch[1], scratch[2], st)
         if rc:
             raise sjk.SjkError(rc, "kv16_attend")
         return out
@@ -256,6 +273,11 @@ class Qkv:
         a.norm_type = _TYPE[kinds.pop()] if kinds else F32
         if rope is not None:
             a.rope = rope.c
+        at = {w.get_device() for w in self._keep if w is not None} | ({rope.device} if rope is not None else set()) | \
+            ({cache._dev} if cache is not None else set())
+        if len(at) > 1:
+            raise ValueError("rope, norm weights and cache: of one GPU")
+        self._dev = at.pop() if at else None
         self._ref, self._L = C.byref(a), _lib()
         self._layer = None
         # (the struct's own fields: setting them sets the struct's)
@@ -267,18 +289,20 @@ class Qkv:
         to_cache is false; row outputs go where given (an input's own rows too)."""
         a = self._a
         some = q if q is not None else k if k is not None else v
-        n = some.shape[0]
+        n, dev = some.shape[0], some.get_device()
+        if dev < 0 or (self._dev is not None and dev != self._dev):
+            raise ValueError("q, k, v: CUDA tensors" + (f" on cuda:{self._dev}" if self._dev is not None else ""))
         for r, t in zip(self._rows, (q, k, v, q_out, k_out, v_out)):
-            r.set(t, n)
+            r.set(t, n, dev)
         a.n_tok = n
-        a.pos = _list(pos, "pos", n)
-        a.rows = _list(rows, "rows", n)
+        a.pos = _list(pos, "pos", dev, n)
+        a.rows = _list(rows, "rows", dev, n)
         if n == 0:                               # empty tensors have no address
             return
         at = layer if self.cache is not None and to_cache else None
         if at != self._layer:
             a.cache = self.cache.layers[at] if at is not None else sjk.Kv16()
             self._layer = at
-        rc = self._L.sjk_qkv(self._ref, _stream(_index(some)))
+        rc = _launch(dev, self._L.sjk_qkv, self._ref, _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "qkv")

@@ -131,3 +131,76 @@ def test_slabs_in_host_memory_are_refused(host):
     for slabs in ([off], [on, off]):
         with pytest.raises(ValueError, match="slabs"):
             kv16.Pages(tables, 16, slabs=slabs)
+
+
+@pytest.mark.parametrize("there", [0, 1])
+@pytest.mark.parametrize("current", [0, 1])
+def test_calls_run_on_their_tensors_device(host, there, current):
+    """Whatever device is current, a call launches on its tensors' device, on that device's stream, and leaves the current
+    device as it was."""
+    host.device = there
+    rope = kv16.Rope(64)
+    host.device = current
+    cache = _cache(there)
+    pages = cache.pages()
+    q, n = _heads(3, 4, index=there), _i32(3, there)
+    cache.attend(0, q, n, 1.0, out=_heads(3, 4, index=there))
+    step = kv16.Qkv(64, rope=rope, cache=cache)
+    step(k=_heads(3, 2, index=there), v=_heads(3, 2, index=there), pos=n)
+    kv16.Qkv(64)(q=q, q_out=q)
+    pages.fork(n, n)
+    pages.extend(n, n, 1)
+    pages.free(n)
+    pages.compact()
+    pages.copy(n, n)
+    assert [c["name"] for c in host.calls] == ["rope", "init", "attend", "qkv", "qkv", "fork", "extend", "free", "compact", "copy"]
+    assert all(c["device"] == there for c in host.calls) and all(c["stream"] == 1000 + there for c in host.calls[1:])
+    assert host.device == current
+
+
+def test_rope_on_a_named_device(host):
+    assert kv16.Rope(64, device=1).device == 1 and kv16.Rope(64, device="cuda:1").device == 1 and kv16.Rope(64).device == 0
+    assert [c["device"] for c in host.calls] == [1, 1, 0] and host.device == 0
+
+
+def test_tensors_of_another_device_are_refused(host):
+    cache, q, n = _cache(0), _heads(3, 4), _i32(3)
+    pages = cache.pages()
+    far_q, far_n, host_q, host_n = _heads(3, 4, index=1), _i32(3, 1), q.t, n.t
+    host.calls.clear()
+
+    def refused(call, *a, **kw):
+        with pytest.raises(ValueError):
+            call(*a, **kw)
+        assert host.calls == []
+
+    for fq, fn in ((far_q, far_n), (host_q, host_n)):
+        refused(cache.attend, 0, fq, n, 1.0, out=q)
+        refused(cache.attend, 0, q, fn, 1.0, out=q)
+        refused(cache.attend, 0, q, n, 1.0, out=fq)
+        refused(cache.attend, 0, q, n, 1.0, out=q, rows=fn)
+        step = kv16.Qkv(64, cache=cache)
+        kv = _heads(3, 2)
+        refused(step, fq, kv, kv, n, q_out=q)
+        refused(step, q, kv, kv, n, q_out=fq)
+        refused(step, q, kv, kv, fn, q_out=q)
+        refused(step, q, kv, kv, n, q_out=q, rows=fn)
+        refused(kv16.Qkv(64), q=q, q_out=fq)
+        refused(kv16.Qkv(64), q=host_q, q_out=host_q)
+        refused(pages.fork, fn, n)
+        refused(pages.fork, n, fn)
+        refused(pages.extend, n, fn, 1)
+        refused(pages.free, n, first=fn)
+        refused(pages.copy, fn, fn)
+    refused(kv16.Cache, cache.k, Gpu(cache.v.t, 1), cache.tables)
+    refused(_cache, 0, tables=1)
+    refused(kv16.Pages, Gpu(cache.tables.t, 1), 16, slabs=[cache.k])
+    # what a Qkv is made of
+    rope = kv16.Rope(64, device=1)
+    host.calls.clear()
+    w = Gpu(torch.ones(64), 1)
+    refused(kv16.Qkv, 64, rope=rope, cache=cache)
+    refused(kv16.Qkv, 64, q_norm=w, cache=cache)
+    refused(kv16.Qkv, 64, q_norm=w, k_norm=Gpu(torch.ones(64), 0))
+    refused(kv16.Qkv(64, rope=rope), q=q, q_out=q, pos=n)
+    refused(kv16.Qkv(64, q_norm=w), q=q, q_out=q)
