@@ -12,10 +12,12 @@ that reads it (Cache), and who owns the pages (Pages: fork, extend with copy on 
     out = cache.attend(il, q2, lens + 1, scale, rows=rows)
 
 Calls run on the tensors' device, on torch's current stream there, and do not synchronise; tensors of another device raise
-ValueError. Lengths, positions and row lists are int32 CUDA tensors, read when the kernels run;
+ValueError. Threads may share an object (a call of one waits for that of another until it is launched); what they launch on
+several streams is theirs to order. Lengths, positions and row lists are int32 CUDA tensors, read when the kernels run;
 sjk.lib().sjk_device_status() reports entries that pointed outside their arrays.
 """
 import ctypes as C
+import threading
 
 import torch
 
@@ -218,6 +220,7 @@ class Cache:
         self._q, self._o = _Rows(sjk.Rows(), "q", D), _Rows(sjk.Rows(), "out", D)
         self._qo = C.byref(self._q.c), C.byref(self._o.c)
         self._dev, self._L = k.get_device(), _lib()
+        self._lock = threading.Lock()
         self._scratch = {}                       # by stream and number of query heads: calls of one stream follow one another
 
     @classmethod
@@ -236,19 +239,20 @@ class Cache:
         n, dev = q.shape[0], self._dev
         if out is None:
             out = torch.empty_like(q)
-        self._q.set(q, n, dev)
-        self._o.set(out, n, dev)
-        if n == 0:
-            return out
-        st = _stream(dev)
-        key = (st, q.shape[1])
-        scratch = self._scratch.get(key)
-        if scratch is None:
-            size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
-            buf = torch.empty(size, dtype=torch.uint8, device=q.device)
-            scratch = self._scratch[key] = (buf, buf.data_ptr(), size)
-        rc = _launch(dev, self._L.sjk_kv16_attend, self._refs[layer], self._qo[0], _list(lens, "lens", dev, n), _list(rows, "rows", dev, n), n,
-                     scale, window, self._qo[1], scratch[1], scratch[2], st)
+        with self._lock:                         # the structs are the object's, and the call reads them without the interpreter's lock
+            self._q.set(q, n, dev)
+            self._o.set(out, n, dev)
+            if n == 0:
+                return out
+            st = _stream(dev)
+            key = (st, q.shape[1])
+            scratch = self._scratch.get(key)
+            if scratch is None:
+                size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
+                buf = torch.empty(size, dtype=torch.uint8, device=q.device)
+                scratch = self._scratch[key] = (buf, buf.data_ptr(), size)
+            rc = _launch(dev, self._L.sjk_kv16_attend, self._refs[layer], self._qo[0], _list(lens, "lens", dev, n),
+                         _list(rows, "rows", dev, n), n, scale, window, self._qo[1], scratch[1], scratch[2], st)
         if rc:
             raise sjk.SjkError(rc, "kv16_attend")
         return out
@@ -280,6 +284,7 @@ class Qkv:
         self._dev = at.pop() if at else None
         self._ref, self._L = C.byref(a), _lib()
         self._layer = None
+        self._lock = threading.Lock()
         # (the struct's own fields: setting them sets the struct's)
         self._rows = [_Rows(getattr(a, f), f, head_dim) for f in ("q", "k", "v", "q_out", "k_out", "v_out")]
 
@@ -292,17 +297,18 @@ class Qkv:
         n, dev = some.shape[0], some.get_device()
         if dev < 0 or (self._dev is not None and dev != self._dev):
             raise ValueError("q, k, v: CUDA tensors" + (f" on cuda:{self._dev}" if self._dev is not None else ""))
-        for r, t in zip(self._rows, (q, k, v, q_out, k_out, v_out)):
-            r.set(t, n, dev)
-        a.n_tok = n
-        a.pos = _list(pos, "pos", dev, n)
-        a.rows = _list(rows, "rows", dev, n)
-        if n == 0:                               # empty tensors have no address
-            return
-        at = layer if self.cache is not None and to_cache else None
-        if at != self._layer:
-            a.cache = self.cache.layers[at] if at is not None else sjk.Kv16()
-            self._layer = at
-        rc = _launch(dev, self._L.sjk_qkv, self._ref, _stream(dev))
+        with self._lock:                         # the struct is the object's, and the call reads it without the interpreter's lock
+            for r, t in zip(self._rows, (q, k, v, q_out, k_out, v_out)):
+                r.set(t, n, dev)
+            a.n_tok = n
+            a.pos = _list(pos, "pos", dev, n)
+            a.rows = _list(rows, "rows", dev, n)
+            if n == 0:                           # empty tensors have no address
+                return
+            at = layer if self.cache is not None and to_cache else None
+            if at != self._layer:
+                a.cache = self.cache.layers[at] if at is not None else sjk.Kv16()
+                self._layer = at
+            rc = _launch(dev, self._L.sjk_qkv, self._ref, _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "qkv")

@@ -5,6 +5,7 @@ import math
 import threading
 import time
 import types
+from collections import Counter
 
 import pytest
 import torch
@@ -204,3 +205,65 @@ def test_tensors_of_another_device_are_refused(host):
     refused(kv16.Qkv, 64, q_norm=w, k_norm=Gpu(torch.ones(64), 0))
     refused(kv16.Qkv(64, rope=rope), q=q, q_out=q, pos=n)
     refused(kv16.Qkv(64, q_norm=w), q=q, q_out=q)
+
+
+def _from_threads(*calls):
+    """Each call in its own thread, all started together; what they raised."""
+    gate, errors = threading.Barrier(len(calls)), []
+
+    def one(call):
+        gate.wait()
+        try:
+            call()
+        except Exception as e:                   # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=one, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+        assert not t.is_alive()
+    assert errors == []
+
+
+def test_threads_on_one_cache(host):
+    """Threads that share a cache: every launch has the pointers, strides and heads of one call."""
+    cache = _cache()
+    kinds = [(3, 4), (2, 8), (4, 6), (1, 2)]
+    args = [(_heads(n, h), _heads(n, h), _i32(n)) for n, h in kinds]
+    host.during = lambda: time.sleep(0.002)      # the library runs outside the interpreter's lock
+    for q, out, n in args:                       # scratch is there before
+        cache.attend(0, q, n, 1.0, out=out)
+    host.calls.clear()
+
+    def calls(q, out, n):
+        def run():
+            for _ in range(20):
+                cache.attend(0, q, n, 1.0, out=out)
+        return run
+
+    _from_threads(*(calls(*a) for a in args))
+    want = {(q.data_ptr(), q.stride(0), q.shape[1]): (out.data_ptr(), n.data_ptr(), n.shape[0]) for q, out, n in args}
+    assert Counter(c["q"] for c in host.calls) == {k: 20 for k in want}
+    for c in host.calls:
+        assert want[c["q"]] == (c["out"], c["lens"], c["n"])
+
+
+def test_threads_on_one_qkv(host):
+    step = kv16.Qkv(64)
+    kinds = [(3, 4), (2, 8), (4, 6), (1, 2)]
+    args = [(_heads(n, h), _heads(n, h), _i32(n)) for n, h in kinds]
+    host.during = lambda: time.sleep(0.002)
+
+    def calls(q, out, pos):
+        def run():
+            for _ in range(20):
+                step(q=q, q_out=out, pos=pos)
+        return run
+
+    _from_threads(*(calls(*a) for a in args))
+    want = {(q.data_ptr(), q.stride(0), q.shape[1]): (out.data_ptr(), pos.data_ptr(), q.shape[0]) for q, out, pos in args}
+    assert Counter(c["q"] for c in host.calls) == {k: 20 for k in want}
+    for c in host.calls:
+        assert want[c["q"]] == (c["q_out"], c["pos"], c["n"])
