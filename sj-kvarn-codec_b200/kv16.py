@@ -47,6 +47,7 @@ def _stream(device):
     return _raw_stream(device) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
 
 
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -233,9 +234,32 @@ class Cache:
         """A ledger over this cache's pages."""
         return Pages(self.tables, self.page_tokens, slabs=[self.k, self.v], ids=ids, n_free=n_free)
 
-    def attend(self, layer, q, lens, scale, window=0, rows=None, out=None):
+    def scratch_bytes(self, heads):
+        """Bytes of scratch that attend needs for queries of so many heads."""
+        size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[0], heads)
+        if not size:
+            raise ValueError(f"{heads} query heads over {self.n_head_kv} heads of {self.head_dim} channels")
+        return size
+
+    def _scratch_of(self, st, q):
+        """(tensor, address, bytes) for a call on stream st."""
+        key, captured = (st, q.shape[1]), _launch(self._dev, _capturing)
+        scratch = None if captured else self._scratch.get(key)
+        if scratch is None:
+            size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[0], q.shape[1])
+            buf = torch.empty(size, dtype=torch.uint8, device=q.device)
+            scratch = buf, buf.data_ptr(), size
+            if not captured:
+                self._scratch[key] = scratch
+        return scratch
+
+    def attend(self, layer, q, lens, scale, window=0, rows=None, out=None, scratch=None):
         """Attention of one new token per sequence: q [n][heads][D], lens int32 [n] (the newest position included), rows
-        int32 [n] (None: sequence i is table row i). Returns out (q's type unless given)."""
+        int32 [n] (None: sequence i is table row i). Returns out (q's type unless given).
+
+        scratch: a uint8 tensor of scratch_bytes(heads) bytes that no overlapping call uses. None: the cache's own for the
+        current stream, whose calls follow one another; while torch captures the stream, memory of the capture's pool, since
+        graphs captured on one stream may be replayed on several. (Captured by other means than torch's: give it.)"""
         n, dev = q.shape[0], self._dev
         if out is None:
             out = torch.empty_like(q)
@@ -245,14 +269,14 @@ class Cache:
             if n == 0:
                 return out
             st = _stream(dev)
-            key = (st, q.shape[1])
-            scratch = self._scratch.get(key)
             if scratch is None:
-                size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[layer], q.shape[1])
-                buf = torch.empty(size, dtype=torch.uint8, device=q.device)
-                scratch = self._scratch[key] = (buf, buf.data_ptr(), size)
+                buf, address, size = self._scratch_of(st, q)
+            elif scratch.dtype is torch.uint8 and scratch.is_contiguous() and scratch.get_device() == dev:
+                address, size = scratch.data_ptr(), scratch.numel()
+            else:
+                raise ValueError(f"scratch: a contiguous uint8 tensor on cuda:{dev}")
             rc = _launch(dev, self._L.sjk_kv16_attend, self._refs[layer], self._qo[0], _list(lens, "lens", dev, n),
-                         _list(rows, "rows", dev, n), n, scale, window, self._qo[1], scratch[1], scratch[2], st)
+                         _list(rows, "rows", dev, n), n, scale, window, self._qo[1], address, size, st)
         if rc:
             raise sjk.SjkError(rc, "kv16_attend")
         return out

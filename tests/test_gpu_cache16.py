@@ -154,3 +154,44 @@ def test_weights_of_32_bit_rows(T, dtype, D, grp):
     q = T.randn((len(lens), 2 * grp, D), device="cuda", generator=g)
     got = cache.attend(0, q, T.tensor(lens, dtype=T.int32, device="cuda"), 0.1 / D)
     _check(T, cache, got, q, lens, 0.1 / D, few=True)
+
+
+def test_graphs_captured_on_one_stream(T):
+    """Two graphs of one cache, captured one after the other on the same stream, replayed at once on two streams beside calls
+    that run on a third: each has scratch of its own."""
+    lens, D = [5000, 4000], 128
+    cache, g = _build(T, lens, 16, 4, D, T.bfloat16)
+    dl = T.tensor(lens, dtype=T.int32, device="cuda")
+    qs = [T.randn((2, 16, D), device="cuda", generator=g).bfloat16() for _ in range(3)]
+    want = [cache.attend(0, q, dl, 0.1) for q in qs]
+    outs, graphs, s = [[T.empty_like(want[0]) for _ in range(4)] for _ in range(2)], [T.cuda.CUDAGraph() for _ in range(2)], T.cuda.Stream()
+    T.cuda.synchronize()
+    for j in range(2):
+        with T.cuda.graph(graphs[j], stream=s):
+            for out in outs[j]:
+                cache.attend(0, qs[j], dl, 0.1, out=out)
+    assert set(key[0] for key in cache._scratch) == {T.cuda.current_stream().cuda_stream}
+    streams = [T.cuda.Stream() for _ in range(3)]
+    for _ in range(20):
+        for j in range(2):
+            with T.cuda.stream(streams[j]):
+                graphs[j].replay()
+        with T.cuda.stream(streams[2]):
+            mine = cache.attend(0, qs[2], dl, 0.1)
+        T.cuda.synchronize()
+        assert all(T.equal(o, want[j]) for j in range(2) for o in outs[j]) and T.equal(mine, want[2])
+        for j in range(2):
+            for o in outs[j]:
+                o.zero_()
+        T.cuda.synchronize()
+
+
+def test_scratch_of_the_callers(T):
+    lens, D = [700, 3], 64
+    cache, g = _build(T, lens, 16, 2, D, T.float16)
+    dl = T.tensor(lens, dtype=T.int32, device="cuda")
+    q = T.randn((2, 8, D), device="cuda", generator=g).half()
+    mine = T.empty(cache.scratch_bytes(8), dtype=T.uint8, device="cuda")
+    assert T.equal(cache.attend(0, q, dl, 0.1, scratch=mine), cache.attend(0, q, dl, 0.1))
+    with pytest.raises(sjk.SjkError):
+        cache.attend(0, q, dl, 0.1, scratch=mine[:1024])

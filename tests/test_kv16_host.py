@@ -267,3 +267,49 @@ def test_threads_on_one_qkv(host):
     assert Counter(c["q"] for c in host.calls) == {k: 20 for k in want}
     for c in host.calls:
         assert want[c["q"]] == (c["q_out"], c["pos"], c["n"])
+
+
+def test_scratch_of_captured_calls(host):
+    """Calls that are captured get scratch of their own, which the graph's memory pool holds; two graphs captured on one
+    stream and calls that run there do not share it. Calls that run keep theirs by stream and heads."""
+    cache, q, n = _cache(), _heads(3, 4), _i32(3)
+    made, keep = [], torch.empty
+
+    def call():
+        host.calls.clear()
+        cache.attend(0, q, n, 1.0, out=q)
+        return host.calls[0]["scratch"], host.calls[0]["size"]
+
+    first = call()
+    assert call() == first and first[1] >= sjk.lib().sjk_kv16_attend_scratch_bytes(C.byref(cache.layers[0]), 4)
+    with pytest.MonkeyPatch.context() as m:
+        m.setattr(torch, "empty", lambda *a, **kw: made.append(keep(*a, **kw)) or made[-1])
+        host.capturing = True
+        one = call()                             # (this test holds what was allocated)
+        two = call()
+        host.capturing = False
+    assert len(made) == 2 and [one[0], two[0]] == [x.data_ptr() for x in made]
+    assert len({first[0], one[0], two[0]}) == 3 and one[1] == two[1] == first[1] and call() == first
+    # a graph captured before any call has run leaves nothing behind for those that run
+    other = _cache()
+    host.capturing = True
+    other.attend(0, q, n, 1.0, out=q)
+    assert other._scratch == {}
+
+
+def test_scratch_of_the_callers(host):
+    cache, q, n = _cache(), _heads(3, 4), _i32(3)
+    size = cache.scratch_bytes(4)
+    assert size == sjk.lib().sjk_kv16_attend_scratch_bytes(C.byref(cache.layers[0]), 4)
+    mine = Gpu(torch.empty(size, dtype=torch.uint8))
+    for host.capturing in (False, True):
+        host.calls.clear()
+        cache.attend(0, q, n, 1.0, out=q, scratch=mine)
+        assert (host.calls[0]["scratch"], host.calls[0]["size"]) == (mine.data_ptr(), size) and cache._scratch == {}
+    host.calls.clear()
+    for bad in (mine.t, Gpu(mine.t, 1), Gpu(torch.empty(size, dtype=torch.int32)), Gpu(torch.empty((2, size), dtype=torch.uint8)[:, ::2])):
+        with pytest.raises(ValueError, match="scratch"):
+            cache.attend(0, q, n, 1.0, out=q, scratch=bad)
+    with pytest.raises(ValueError):
+        cache.scratch_bytes(3)
+    assert host.calls == []
