@@ -663,7 +663,8 @@ int        sjk_pages_fork(const sjk_pages * p, const int32_t * src, const int32_
  * replaced by an own one, which gets its contents if the row keeps positions on it (copy on write), except that when
  * all owners of a page are in the call the last one keeps it. All or nothing: status[0] (DEVICE) = 0,
  * SJKVARN_ERR_POOL_FULL (too few free pages), SJKVARN_ERR_ARG (rows out of range or named twice, positions beyond the
- * table) or SJKVARN_ERR_CORRUPT. n <= SJK_PAGES_MAX_ROWS. Two launches. */
+ * table) or SJKVARN_ERR_CORRUPT (an entry, or an id of the stack that would be handed out, that is no page; more free ids
+ * than pages). n <= SJK_PAGES_MAX_ROWS. Two launches. */
 int        sjk_pages_extend(const sjk_pages * p, const int32_t * rows, const int32_t * len, const int32_t * add, int add_all, int n,
                             int32_t * status, sjk_stream st);
 /* The entries [g0[i], g1[i]) of each row (DEVICE; NULL: from the first, to the last) give their pages up and become

@@ -149,6 +149,8 @@ __global__ void __launch_bounds__(NT) pages_free_kernel(const __grid_constant__ 
     // marked pages in descending order, from the last word of the bitmap to the first
     const uint32_t words = (p.n_pages + 31u) / 32u;
     uint32_t n_free = p.l.head[0];
+    bool torn = n_free > p.n_pages;                         // a stack that is no stack of this pool
+    if (torn) n_free = p.n_pages;
     for (uint32_t w0 = 0; w0 < words; w0 += NT) {
         const uint32_t k = w0 + threadIdx.x;
         const bool on = k < words;
@@ -164,8 +166,13 @@ __global__ void __launch_bounds__(NT) pages_free_kernel(const __grid_constant__ 
             ++at;
             p.l.shares[id] = 0u;
         }
-        n_free = n_free + total < p.n_pages ? n_free + total : p.n_pages;
+        n_free += total;
+        if (n_free > p.n_pages) {                           // more free ids than pages: some were free before
+            torn = true;
+            n_free = p.n_pages;
+        }
     }
+    if (torn && threadIdx.x == 0) flag();
     if (threadIdx.x == 0) { p.l.head[0] = n_free; p.l.head[2] = 0u; }
 }
 
@@ -202,10 +209,12 @@ __global__ void __launch_bounds__(NTHR) pages_extend_kernel(const __grid_constan
         for (int j = 0; j < tid; ++j) bad |= s_row[j] == s_row[tid] ? 1 : 0;
     bad = __syncthreads_or(bad);
     much = __syncthreads_or(much);
-    if (bad || much) {
-        if (tid == 0) { p.status[0] = bad ? SJKVARN_ERR_ARG : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
+    const bool torn = n_free > p.n_pages;                   // a stack that is no stack of this pool
+    if (bad || torn || much) {
+        if (tid == 0) { p.status[0] = bad ? SJKVARN_ERR_ARG : torn ? SJKVARN_ERR_CORRUPT : SJKVARN_ERR_POOL_FULL; p.l.head[3] = 0u; }
         return;
     }
+    const uint32_t top_id = (uint32_t) tid < n_free ? p.l.ids[n_free - 1u - tid] : 0u;
     // an item: its request (the last whose items begin at or before it), table entry, page and how many share that
     struct Item { int r; uint32_t * at; uint32_t e, shares; };
     auto item_of = [&](uint32_t it) {
@@ -242,6 +251,12 @@ __global__ void __launch_bounds__(NTHR) pages_extend_kernel(const __grid_constan
     for (uint32_t it = tid; it < n_items; it += NTHR) need += takes(one ? mine : item_of(it)) ? 1u : 0u;
     uint32_t total;
     const uint32_t before_mine = cta_scan<NTHR>(need, s_scan, &total);
+    // the ids that will be handed out are pages (this thread's first was asked for above)
+    if (!wrong && total <= n_free) {
+        int off_pool = (uint32_t) tid < total && top_id >= p.n_pages ? 1 : 0;
+        for (uint32_t k = (uint32_t) tid + NTHR; k < total; k += NTHR) off_pool |= p.l.ids[n_free - 1u - k] >= p.n_pages ? 1 : 0;
+        wrong = __syncthreads_or(off_pool);
+    }
     if (wrong || total > n_free) {                          // nothing is done: only the counts go back
         for (uint32_t it = tid; it < n_items; it += NTHR) {
             const uint32_t e = (one ? mine : item_of(it)).e;
@@ -293,7 +308,8 @@ __global__ void __launch_bounds__(NB) pages_plan_kernel(const __grid_constant__ 
     pdl_wait();
     pdl_release();
     const uint32_t tid = threadIdx.x, n = p.n_pages, words = (n + 31u) / 32u;
-    const uint32_t n_free = p.l.head[0] < n ? p.l.head[0] : n, top = n - n_free;
+    const bool torn = p.l.head[0] > n;                      // a stack that is no stack of this pool: nothing moves
+    const uint32_t n_free = torn ? n : p.l.head[0], top = n - n_free;
     for (uint32_t w = tid; w < words; w += NB) s_used[w] = w * 32u + 32u <= n ? 0xFFFFFFFFu : (1u << (n & 31u)) - 1u;
     __syncthreads();
     for (uint32_t i = tid; i < n_free; i += NB) {
@@ -321,15 +337,16 @@ __global__ void __launch_bounds__(NB) pages_plan_kernel(const __grid_constant__ 
     }
     __syncthreads();
     // equal where the stack holds every free id once; a damaged one moves nothing
-    const uint32_t moves = holes == movers ? movers : 0u;
-    if (holes != movers && tid == 0) flag();
+    const bool sound = holes == movers && !torn;
+    const uint32_t moves = sound ? movers : 0u;
+    if (!sound && tid == 0) flag();
     for (uint32_t k = tid; k < moves; k += NB) {
         const uint32_t s = p.l.src[k], d = p.l.dst[k];
         p.l.map[s] = k;
         p.l.shares[d] = p.l.shares[s];
         p.l.shares[s] = 0u;
     }
-    if (holes == movers)
+    if (sound)
         for (uint32_t i = tid; i < n_free; i += NB) p.l.ids[i] = n - 1u - i;
     if (tid == 0) {
         p.l.head[3] = moves;

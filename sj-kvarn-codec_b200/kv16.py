@@ -122,8 +122,8 @@ def rope_steps(n_rot, layout="half", base=10000.0, scaling="none", factor=1.0, n
 
 class Pages:
     """Owner ledger of the pages behind `tables` (int32 [rows][stride], NO_BLOCK = no page) and `slabs` (CUDA tensors
-    [layers][pages][...], contiguous within a page). ids, n_free: an existing stack of free ids (pages that tables hold
-    are not on it) with its length; without them every page is free."""
+    [layers][pages][...], contiguous within a page). ids, n_free: an existing stack of free ids (a value per page, of which
+    the first n_free are free pages; pages that tables hold are not among them); without them every page is free."""
 
     def __init__(self, tables, page_tokens, slabs=(), n_pages=None, ids=None, n_free=None):
         if tables.dtype != torch.int32 or not tables.is_cuda or tables.dim() != 2 or not tables.is_contiguous():
@@ -134,6 +134,11 @@ class Pages:
         self.c = c = sjk.PagesC(self._buf.data_ptr(), tables.data_ptr(), n, tables.shape[0], tables.shape[1], page_tokens)
         if len(self.slabs) > 4:
             raise ValueError("slabs: at most 4")
+        if ids is not None and tuple(ids.shape) != (n,):
+            raise ValueError(f"ids: {n} values, the first n_free of them free pages")
+        free = n if n_free is None else int(n_free)
+        if not 0 <= free <= n:
+            raise ValueError(f"n_free: 0 to {n}")
         self._dev = tables.get_device()
         c.n_slabs = len(self.slabs)
         for i, s in enumerate(self.slabs):
@@ -152,7 +157,7 @@ class Pages:
         self.shares = self._buf[at:at + n]
         if ids is not None:
             self.ids.copy_(ids)
-            self.n_free.fill_(n if n_free is None else n_free)
+            self.n_free.fill_(free)
 
     def fork(self, src, dst):
         """Rows dst get the pages of rows src, shared. Returns the device status vector (0, or a status code each)."""

@@ -313,3 +313,15 @@ def test_scratch_of_the_callers(host):
     with pytest.raises(ValueError):
         cache.scratch_bytes(3)
     assert host.calls == []
+
+
+def test_stacks_that_do_not_fit_are_refused(host):
+    tables, slab = Gpu(torch.full((4, 4), -1, dtype=torch.int32)), Gpu(torch.zeros((1, 8, 64)))
+    ids = torch.arange(7, -1, -1, dtype=torch.int32)
+    p = kv16.Pages(tables, 16, slabs=[slab], ids=ids, n_free=3)
+    assert p.n_free.item() == 3 and torch.equal(p.ids, ids)
+    for n_free in (None, 0, 8):
+        assert kv16.Pages(tables, 16, slabs=[slab], ids=ids, n_free=n_free).n_free.item() == (8 if n_free is None else n_free)
+    for bad in (dict(ids=ids, n_free=9), dict(ids=ids, n_free=-1), dict(ids=ids[:1]), dict(ids=ids[:7], n_free=3), dict(ids=ids[None])):
+        with pytest.raises(ValueError):
+            kv16.Pages(tables, 16, slabs=[slab], **bad)
