@@ -674,7 +674,8 @@ int        sjk_pages_free(const sjk_pages * p, const int32_t * rows, const int32
  * n_rows), shares and stack follow (afterwards the next id handed out is the number of used pages). info (DEVICE, may
  * be NULL): [0] used pages, [1] moved ones. Two launches. */
 int        sjk_pages_compact(const sjk_pages * p, int32_t * info, sjk_stream st);
-/* Contents of page src[i] to page dst[i] (DEVICE) in every layer of every slab; no page is both. One launch. */
+/* Contents of page src[i] to page dst[i] (DEVICE) in every layer of every slab; no page is both. One launch. (This call,
+ * extend and compact answer SJK_ERR_UNSUPPORTED where they could copy more than 4e9 segments of 16 KB.) */
 int        sjk_pages_copy(const sjk_pages * p, const int32_t * src, const int32_t * dst, int n, sjk_stream st);
 
 /* ---- seeded synthetic inputs of the benchmark configurations (DEVICE outputs) ----

@@ -450,6 +450,13 @@ __global__ void __launch_bounds__(NT) pages_init_kernel(Ledger l, uint32_t n) {
     if (blockIdx.x == 0 && threadIdx.x == 0) { l.head[0] = l.head[1] = n; l.head[2] = l.head[3] = l.claims[0] = 0u; }
 }
 
+// Whether n copies are more segments than the 32-bit claims can count, with those that the CTAs claim in vain.
+bool too_many(const Params & p, uint32_t n) {
+    double units = 0.0;
+    for (int i = 0; i < p.n_slabs; ++i) units += (double) ((p.slabs[i].page_bytes + SEG - 1) / SEG) * p.slabs[i].n_layers * n;
+    return units > 4e9;
+}
+
 int copy_launch(const Params & p, const uint32_t * src, const uint32_t * dst, int n, int remap, sjk_stream st) {
     if (p.n_slabs == 0 && !remap) return 0;
     return launch(pages_copy_kernel, dim3(148 * 6), dim3(NT), 0, st, p, src, dst, n, remap);
@@ -501,6 +508,7 @@ extern "C" int sjk_pages_extend(const sjk_pages * g, const int32_t * rows, const
     if (rc) return rc;
     if (n < 0 || n > SJK_PAGES_MAX_ROWS || (n && (!rows || !len || !status)) || (!add && add_all < 0)) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
+    if (too_many(p, (uint32_t) n)) return SJK_ERR_UNSUPPORTED;      // a request copies its first page at most
     p.a = rows; p.b = len; p.c = add; p.add_all = add_all; p.n = n; p.status = status;
     rc = n <= 256 ? launch(pages_extend_kernel<256>, dim3(1), dim3(256), 0, st, p) : launch(pages_extend_kernel<NB>, dim3(1), dim3(NB), 0, st, p);
     if (rc) return rc;
@@ -511,6 +519,7 @@ extern "C" int sjk_pages_compact(const sjk_pages * g, int32_t * info, sjk_stream
     Params p;
     int rc = params_of(g, &p, true);
     if (rc) return rc;
+    if (too_many(p, p.n_pages / 2)) return SJK_ERR_UNSUPPORTED;     // a move needs a used page and a free one
     p.status = info;
     const size_t smem = (size_t) ((p.n_pages + 31u) / 32u) * sizeof(uint32_t);
     if (smem > 40 * 1024 && smem_limit<pages_plan_kernel>(SJK_PAGES_MAX / 8)) return SJK_ERR_DEVICE;
@@ -525,6 +534,7 @@ extern "C" int sjk_pages_copy(const sjk_pages * g, const int32_t * src, const in
     if (rc) return rc;
     if (n < 0 || (n && (!src || !dst))) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
+    if (too_many(p, (uint32_t) n)) return SJK_ERR_UNSUPPORTED;
     return copy_launch(p, reinterpret_cast<const uint32_t *>(src), reinterpret_cast<const uint32_t *>(dst), n, 0, st);
 }
 

@@ -325,3 +325,16 @@ def test_stacks_that_do_not_fit_are_refused(host):
     for bad in (dict(ids=ids, n_free=9), dict(ids=ids, n_free=-1), dict(ids=ids[:1]), dict(ids=ids[:7], n_free=3), dict(ids=ids[None])):
         with pytest.raises(ValueError):
             kv16.Pages(tables, 16, slabs=[slab], **bad)
+
+
+def test_copies_beyond_the_claim_counter_are_refused():
+    """Segments are claimed by a 32-bit counter: a call with more of them is refused before its launch (it would never end)."""
+    L = sjk.lib()
+    p = sjk.PagesC(0x10000, 0x10000, 64, 4, 8, 16)
+    p.n_slabs = 2
+    p.slabs[0] = p.slabs[1] = sjk.Slab(0x10000, 64 << 10, 0, 1 << 22)        # 4 segments a page and layer
+    for n in (128, 256, 2 ** 31 - 1):
+        assert L.sjk_pages_copy(C.byref(p), 0x10000, 0x10000, n, None) == -201
+    p.n_pages = 1 << 10
+    assert L.sjk_pages_extend(C.byref(p), 0x10000, 0x10000, None, 1, 512, 0x10000, None) == -201
+    assert L.sjk_pages_compact(C.byref(p), None, None) == -201
