@@ -553,9 +553,9 @@ enum { SJK_F32 = 0, SJK_F16 = 1, SJK_BF16 = 2 };
  *   NTK     base * factor^(n_rot / (n_rot - 2)) in place of base
  *   YARN    f / factor r + f (1 - r), r = clamp((i - lo) / max(hi - lo, 0.001), 0, 1), lo and hi the pairs (floor,
  *           ceil, within [0, n_rot - 1]) that turn beta_fast and beta_slow times over n_ctx;
- *           amp 0 stands for 0.1 ln(factor) + 1
+ *           amp 0 stands for 0.1 ln(factor) + 1 where factor > 1
  *   BANDS   f / factor (1 - s) + f s, s = clamp((n_ctx f / 2 pi - low) / (high - low), 0, 1)
- * amp 0 stands for 1 in the other forms. Angles are kept as turns in 64-bit fixed point (step[i] = f_i / 2 pi in
+ * amp 0 stands for 1 otherwise. Angles are kept as turns in 64-bit fixed point (step[i] = f_i / 2 pi in
  * units of 2^-64 turns): pos * step modulo 2^64 is the angle modulo a turn for every 31-bit position, where a
  * product in 32-bit floats is off by 0.03 rad at a million. */
 enum { SJK_ROPE_HALF = 0, SJK_ROPE_PAIR = 1 };

@@ -556,7 +556,7 @@ extern "C" int sjk_rope_steps(const sjk_rope_config * c, uint64_t * step, float 
         const long double u = roundl(turn * 18446744073709551616.0L);
         step[i] = u >= 18446744073709551616.0L ? 0u : (uint64_t) u;
     }
-    *amp = c->amp != 0.0 ? (float) c->amp : c->scaling == SJK_ROPE_YARN ? (float) (0.1 * log(c->factor) + 1.0) : 1.0f;
+    *amp = c->amp != 0.0 ? (float) c->amp : c->scaling == SJK_ROPE_YARN && c->factor > 1.0 ? (float) (0.1 * log(c->factor) + 1.0) : 1.0f;
     return 0;
 }
 

@@ -338,3 +338,10 @@ def test_copies_beyond_the_claim_counter_are_refused():
     p.n_pages = 1 << 10
     assert L.sjk_pages_extend(C.byref(p), 0x10000, 0x10000, None, 1, 512, 0x10000, None) == -201
     assert L.sjk_pages_compact(C.byref(p), None, None) == -201
+
+
+@pytest.mark.parametrize("factor,amp", [(1e-5, 1.0), (0.25, 1.0), (1.0, 1.0), (1.5, 0.1 * math.log(1.5) + 1), (40.0, 0.1 * math.log(40.0) + 1)])
+def test_yarn_amplitude(factor, amp):
+    """The default amplitude is 0.1 ln(factor) + 1 for contexts that grow and 1 for others."""
+    assert kv16.rope_steps(64, scaling="yarn", factor=factor, n_ctx=4096)[1] == pytest.approx(amp, rel=2 ** -23)
+    assert kv16.rope_steps(64, scaling="yarn", factor=factor, n_ctx=4096, amp=0.7)[1] == pytest.approx(0.7, rel=2 ** -23)
