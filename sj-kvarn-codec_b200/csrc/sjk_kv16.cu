@@ -176,8 +176,8 @@ struct Shape {
     // ends last (48 windowed sequences of 64 channels: 90 us, 96 with three tiles, 100 with four; 32 sequences of
     // 8K-64K at 256 channels: 775, 778 with three). Six warps: 256 short chats 76 us against 67; ten and more: 11.2 us
     // against 9.3 for one sequence of 611 tokens, no gain elsewhere.
-    static constexpr int W = 8, NE = 2;
-    static constexpr int WARP_BYTES = NE * ENTRY + 16;
+    static constexpr int W = 8;
+    static constexpr int WARP_BYTES = 2 * ENTRY + 16;
     static constexpr int CTA_BYTES = W * WARP_BYTES;
 };
 
@@ -211,12 +211,12 @@ SJK_DEV void store_channels(void * p, int64_t at, const float (&o)[KS][4], int i
 
 template <typename S>
 __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_constant__ Params p) {
-    constexpr int D = S::D, TS = S::TS, TM = S::TM, KS = S::KS, NT8 = S::NT8, T = S::T, HT = S::HT, R = S::R, NE = S::NE, PITCH = S::PITCH, W = S::W;
+    constexpr int D = S::D, TS = S::TS, TM = S::TM, KS = S::KS, NT8 = S::NT8, T = S::T, HT = S::HT, R = S::R, PITCH = S::PITCH, W = S::W;
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t * mine = smem + (size_t) warp * S::WARP_BYTES;
     const uint32_t ring = smem_addr(mine);
-    uint32_t * s_mask = reinterpret_cast<uint32_t *>(mine + NE * S::ENTRY);
+    uint32_t * s_mask = reinterpret_cast<uint32_t *>(mine + 2 * S::ENTRY);
     pdl_wait();
     pdl_release();
 
@@ -399,14 +399,12 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
             }
         }
     };
-    // tiles go out in the order K, V of the first step, K, V of the second, ..., each into the ring's next entry
-    int ld_entry = 0, ld_mask = 0;
+    // tiles go out in the order K, V of the first step, K, V of the second, ...: K into the ring's first place, V behind it
     auto issue = [&](bool v) {
         if (ld.rem > 0) {
-            const uint32_t dst = ring + ld_entry * S::ENTRY;
+            const uint32_t dst = ring + (v ? S::ENTRY : 0);
             if (!v) {
-                if (lane == 0) s_mask[ld_mask] = ld_live;
-                ld_mask = (ld_mask + 1) & 3;
+                if (lane == 0) *s_mask = ld_live;
                 copy(dst, ld_kp);
             } else {
                 copy(dst, ld_vp);
@@ -416,7 +414,6 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                     look_up();
                 }
             }
-            ld_entry = ld_entry + 1 == NE ? 0 : ld_entry + 1;
         }
         cp_commit();
     };
@@ -447,10 +444,9 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         enter();
         look_up();
 #pragma unroll 1
-        for (int i = 0; i < NE; ++i) issue(i & 1);
+        for (int i = 0; i < 2; ++i) issue(i != 0);
     };
-    int entry = 0;                                           // the ring's entry that comes next
-    for (int step = 0; at.rem > 0; step = (step + 1) & 3) {
+    while (at.rem > 0) {
         if (fresh) {                                         // a (sequence, KV head, row tile) begins
             fresh = false;
             begun = at.st == 0;
@@ -529,13 +525,10 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 for (int k = 0; k < KS; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.0f;
             }
         }
-        const uint32_t kb = ring + entry * S::ENTRY;
-        entry = entry + 1 == NE ? 0 : entry + 1;
-        const uint32_t vb = ring + entry * S::ENTRY;
-        entry = entry + 1 == NE ? 0 : entry + 1;
+        const uint32_t kb = ring, vb = ring + S::ENTRY;
 
         // S^T = K Q^T
-        cp_wait<NE - 1>();
+        cp_wait<1>();
         __syncwarp();
         float s[TM][NT8][4];
 #pragma unroll
@@ -561,9 +554,9 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 for (int e = 0; e < 4; ++e)
                     s[tm][n][e] = terms(CH == 2 ? c[0][n][e] + c[1][n][e] : (c[0][n][e] + c[1][n][e]) + (c[CH - 2][n][e] + c[CH - 1][n][e]));
         }
-        const unsigned live = s_mask[step];
+        const unsigned live = *s_mask;
         __syncwarp();
-        issue(NE & 1);
+        issue(false);
 
         // Softmax over the step's tokens: this lane has tokens lane / 4 (+ 8) of each 16 of its two heads. The maximum is
         // looked for only when some score is above the one so far: seldom after a sequence's first steps.
@@ -648,7 +641,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         }
 
         // O^T += V^T P
-        cp_wait<NE - 1>();
+        cp_wait<1>();
         __syncwarp();
 #pragma unroll
         for (int tm = 0; tm < TM; ++tm)
@@ -670,7 +663,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 }
             }
         __syncwarp();
-        issue(!(NE & 1));
+        issue(true);
 
         // the pair's last step of this run: its output, or its partial
         if (at.st + 1 == at.s.n || at.rem == 1) {
