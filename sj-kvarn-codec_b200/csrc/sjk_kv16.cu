@@ -45,8 +45,13 @@ namespace {
 using namespace sjk16;
 
 constexpr unsigned FULL = 0xFFFFFFFFu;
-constexpr int OV = 4;                       // what a (sequence, KV head, row tile) costs beside its steps, in steps
-constexpr int MIN_RUN = 2;                  // units of a worker's run, at least
+// What a (sequence, KV head, row tile) costs beside its steps, in steps. 256 short chats, us on the GPU in two turns: 69
+// and 71 with 4; 72 and 80 with 1, 71 and 68 with 2, 76 and 74 with 8 (256 sequences of up to 100 tokens 18.5; 19.4, 18.4, 20.7;
+// long ragged batches within 1 %).
+constexpr int OV = 4;
+// Units of a worker's run, at least: fewer make more partials to join, more leave SMs idle. One sequence of 611 tokens 9.3
+// us with 2, 10.6 with 1, 10.5 with 4, 13.1 with 8; seven of up to 300 with 32-bit rows 10.8, 10.0, 12.2, 14.7.
+constexpr int MIN_RUN = 2;
 constexpr float F16_UP = 32768.0f;          // weights of f16 caches, and so their sums and partials, are this much larger
 __device__ unsigned int g_kv16_status;
 

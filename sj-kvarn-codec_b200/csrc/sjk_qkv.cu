@@ -5,7 +5,8 @@
 //   (a, b) -> amp (a cos t - b sin t, a sin t + b cos t),  t = pos * f_i
 //
 // The angle is an integer: pos * step_i modulo 2^64, in units of 2^-64 turns, of which the top 32 bits, read as a
-// signed fraction of a turn, go to sincospif. That keeps 2^-32 of a turn at every position, for one wide multiply.
+// signed fraction of a turn, go to sincospif as a float: off by 2^-26 of a turn at most (24 bits of half a turn; 1e-7 rad,
+// the size of a cosine's own rounding), at every position alike, for one wide multiply.
 //
 // Bound: HBM, every element once in and once out; a launch's latency for a decode step's few tokens. The vector kernels
 // give a lane 16 channels of a head, as 16-byte words that lie side by side over the head's lanes; in the half layout
@@ -35,8 +36,12 @@ constexpr int MAX_T = 16;                   // tokens of a tile, at most
 // 162 with three), floats need 80 (8,320 rows 67 us with three, 76 with four)
 constexpr int ctas_of(int type) { return type == SJK_F32 ? 3 : 4; }
 // Runs per CTA slot: a run costs about 2.5 us to begin, and SMs are not equally fast. Where a slot moves WAVE_BYTES or more,
-// several (us with one / four: floats, 0.9 MB a slot 77 / 70, 1.8 MB 149 / 135; bf16, 1.4 MB 147 / 145); below that one
-// (floats, 0.46 MB 39.0 / 38.3, 0.55 MB 45.7 / 48.7; bf16, 0.69 MB 81 / 83, 0.1 MB 19 / 24).
+// several; below that one. The border is a compromise: head counts and types pull it either way by a few percent (us with
+// one / four; MB that a slot moves):
+//   floats, 12 heads of 256: 0.5 MB 41.1 / 42.1, 0.6 MB 49.3 / 49.3, 0.75 MB 63.9 / 58.9, 0.9 MB 72.6 / 70.1, 1.6 MB 121.4 / 117.9
+//   floats,  6 heads of 256: 0.5 MB 45.0 / 48.2, 0.75 MB 64.6 / 67.2, 0.9 MB 76.8 / 78.7, 1.6 MB 131.4 / 133.3
+//   bf16,   12 heads of 256: 0.5 MB 62.9 / 65.8, 0.75 MB 91.9 / 91.7, 1.0 MB 122.3 / 122.9, 1.6 MB 192.5 / 190.4
+//   bf16,   24 heads of 256: 0.5 MB 58.0 / 62.6, 0.75 MB 83.7 / 86.1, 1.0 MB 110.1 / 112.1, 1.6 MB 173.3 / 174.0
 constexpr int WAVES = 4;
 constexpr int64_t WAVE_BYTES = 768 * 1024;
 __device__ unsigned int g_qkv_status;
