@@ -247,8 +247,8 @@ class Cache:
         return size
 
     def _scratch_of(self, st, q):
-        """(tensor, address, bytes) for a call on stream st."""
-        key, captured = (st, q.shape[1]), _launch(self._dev, _capturing)
+        """(tensor, address, bytes) for a call on stream st of the current device."""
+        key, captured = (st, q.shape[1]), _capturing()
         scratch = None if captured else self._scratch.get(key)
         if scratch is None:
             size = self._L.sjk_kv16_attend_scratch_bytes(self._refs[0], q.shape[1])
@@ -266,6 +266,9 @@ class Cache:
         current stream, whose calls follow one another; while torch captures the stream, memory of the capture's pool, since
         graphs captured on one stream may be replayed on several. (Captured by other means than torch's: give it.)"""
         n, dev = q.shape[0], self._dev
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.attend(layer, q, lens, scale, window, rows, out, scratch)
         if out is None:
             out = torch.empty_like(q)
         with self._lock:                         # the structs are the object's, and the call reads them without the interpreter's lock
@@ -280,8 +283,8 @@ class Cache:
                 address, size = scratch.data_ptr(), scratch.numel()
             else:
                 raise ValueError(f"scratch: a contiguous uint8 tensor on cuda:{dev}")
-            rc = _launch(dev, self._L.sjk_kv16_attend, self._refs[layer], self._qo[0], _list(lens, "lens", dev, n),
-                         _list(rows, "rows", dev, n), n, scale, window, self._qo[1], address, size, st)
+            rc = self._L.sjk_kv16_attend(self._refs[layer], self._qo[0], _list(lens, "lens", dev, n), _list(rows, "rows", dev, n), n, scale,
+                                         window, self._qo[1], address, size, st)
         if rc:
             raise sjk.SjkError(rc, "kv16_attend")
         return out
