@@ -25,6 +25,7 @@ import sjk
 
 F32, F16, BF16 = 0, 1, 2
 _TYPE = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_I32 = torch.int32
 LAYOUTS = {"half": 0, "pair": 1}
 SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
 NO_BLOCK = -1                                    # SJKVARN_NO_BLOCK in an int32 table
@@ -63,7 +64,7 @@ def _list(t, what, device, n=None):
     """Address of an int32 vector on device `device` (None passes)."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.get_device() != device or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+    if t.dtype is not _I32 or t.dim() != 1 or t.get_device() != device or not t.is_contiguous() or (n is not None and t.numel() != n):
         raise ValueError(f"{what}: an int32 vector" + (f" of {n} values" if n is not None else "") + f" on cuda:{device}")
     return t.data_ptr()
 
@@ -73,7 +74,7 @@ class _Rows:
     pointer only."""
 
     def __init__(self, c, what, D):
-        self.c, self.what, self.D, self.like = c, what, D, None
+        self.c, self.what, self.D, self.like, self.n = c, what, D, None, -1
 
     def set(self, t, n, device):
         c = self.c
@@ -83,11 +84,11 @@ class _Rows:
             return
         shape = t.shape
         like = (shape, t.stride(), t.dtype)
-        if like != self.like or shape[0] != n:
+        if like != self.like or self.n != n:
             if len(shape) != 3 or shape[0] != n or shape[2] != self.D or like[1][2] != 1 or t.dtype not in _TYPE:
                 raise ValueError(f"{self.what}: a CUDA tensor [{n}][heads][{self.D}] of 16- or 32-bit floats, channels adjacent")
             c.row_stride, c.head_stride, c.n_head, c.type = like[1][0], like[1][1], shape[1], _TYPE[t.dtype]
-            self.like = like
+            self.like, self.n = like, n
         if t.get_device() != device:
             raise ValueError(f"{self.what}: a tensor on cuda:{device}")
         c.p = t.data_ptr()
