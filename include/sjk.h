@@ -529,7 +529,7 @@ int    sjk_truncate_batch(const sjk_trunc_req * reqs, int n, void * dev_pool, sj
 /* =====================================================================================
  * Layers kept at 16 bits, and what every layer's projection goes through before its cache.
  *
- * Beside sealed layers a model may keep some at 16 bits (a head size the codec refuses, first and last layers, a
+ * Beside sealed layers a model may keep some at 16 bits (heads of 64 or 96 channels, first and last layers, a
  * draft model). These calls are their cache, what writes it, what reads it, and who owns its pages: sjk_qkv (norm
  * of every query and key head, rotary positions, cache write, in one pass), sjk_kv16_attend (attention of one new
  * token per sequence over the pages) and sjk_pages_* (fork, extend with copy on write, free, compact). sjk_qkv also
@@ -616,9 +616,12 @@ int sjk_qkv(const sjk_qkv_args * a, sjk_stream st);
  * the query heads q[i] (type any); query head h reads KV head h / (n_head / n_head_kv). out[i] = sum over its last
  * min(len, window) positions (window 0: all) of softmax(scale q . k) v; a sequence without a live position (len <= 0,
  * or all its pages SJKVARN_NO_BLOCK) gets zeros. Positions on a SJKVARN_NO_BLOCK page are left out (pages that a
- * window has passed may be given back). A draft's several positions are so many entries with one row. Any page size,
- * any number of query heads per KV head; head_dim 64, 96, 128 or 256, K and V rows 16-byte aligned
- * (SJKVARN_ERR_ARG); q of the cache's type 4-byte aligned. 32-bit inside; see csrc/sjk_kv16.cu for the products.
+ * window has passed may be given back). A draft's several positions are so many entries with one row, each of which reads
+ * the row's K and V anew (a prompt's own attention belongs in a kernel for many positions; there is none here). Any page
+ * size, any number of query heads per KV head; head_dim 64, 96, 128 or 256 (SJK_ERR_UNSUPPORTED), K and V rows 16-byte
+ * aligned (SJKVARN_ERR_ARG); q of the cache's type 4-byte aligned. Sums and softmax statistics are 32-bit; weights, and
+ * queries that are not of the cache's type, enter the products as sums of two or three 16-bit terms: 2^-16 (bf16 rows) or
+ * 2^-22 and finer of their value, and for f16 caches no finer than 2^-39 of the largest of the row.
  * scratch: sjk_kv16_attend_scratch_bytes() bytes, 16-byte aligned, for whatever lengths; not shared by calls that overlap.
  * Two launches; the same inputs give the same bits. */
 size_t sjk_kv16_attend_scratch_bytes(const sjk_kv16 * c, int n_head);

@@ -2,13 +2,13 @@
 // joined: out = sum_t softmax_t(scale q . k_t) v_t over the last min(len, window) positions of each sequence.
 //
 // Bound: HBM, every live K and V row once (4 D bytes per position and KV head for 4 D grp flops: at most 16 flops per
-// byte for 16 query heads, far under the tensor cores' ridge). Measured (us a call, GB/s of live rows): 32 sequences of
-// 8K-64K, 4 KV heads of 256 bf16 channels 755-797 by machine (6,290-6,640: a plain copy's rate is 6,539); one of 100,000
-// tokens with 32-bit queries and outputs 77 (5,320); 48 windows of 4,096, 24 heads of 64 channels 92 (5,500); 256 short
-// chats of 0 to 2,048 tokens 68 (4,800); one of 611 tokens 9.1. Pages of one token cost a tenth more than those of 16 (88
-// sequences of up to 19,024 tokens, 2 heads of 128: 60 against 55). What is left above the bytes: 4-5 us until the first
-// products (launch, lengths, table, queries, first rows, each behind the other), 3 us for the merge, and SMs whose share
-// of the memory is smaller than others' (the slowest end 15 % after the mean).
+// byte for 16 query heads, far under the tensor cores' ridge). Measured (us a call on the GPU alone, by CUDA graphs; GB/s
+// of live rows): 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels 790-800 (6,270-6,350: a plain copy's rate is
+// 6,539); one of 100,000 tokens with 32-bit queries and outputs 77 (5,320); 48 windows of 4,096, 24 heads of 64 channels 94
+// (5,390); 256 short chats of 0 to 2,048 tokens 71 (4,600); one of 611 tokens 9.1. Pages of one token cost 3 to 10 % more
+// than those of 16 (88 sequences of up to 19,024 tokens, 2 heads of 128: 59 against 58). What is left above the bytes:
+// 4-5 us until the first products (launch, lengths, table, queries, first rows, each behind the other), 3 us for the merge,
+// and SMs whose share of the memory is smaller than others' (the slowest end 15 % after the mean).
 //  - A warp is a worker of its own. Per KV head, the (sequence, step of TS tokens) pairs of a call form one list, cut
 //    into equal runs, one per warp of a grid that fills the GPU; lengths are read from device memory, so every warp
 //    finds its run with a scan over them. A sequence weighs OV units beside its steps, for what its start and its
@@ -27,8 +27,8 @@
 //    entries as there can be split pairs and scans nothing.
 // Softmax statistics, sums and outputs are 32-bit. Queries of the cache's type enter as they are, and P as the sum of
 // two 16-bit terms, one product each: to 2^-16 (bf16) or 2^-22 (f16) of a weight, so that a 16-bit output is off by its
-// own rounding (one term: 2^-8 of a weight, and outputs twice as far off where they nearly cancel; the second term's
-// products cost 1 %: 256 short chats 69 us a pass against 68, 48 windows 95.7 against 94.6). For 32-bit queries or
+// own rounding (one term would be 2^-8 of a weight off; the second one's products cost 1 % where one pass over K and V
+// does, 256 short chats 69 us a pass against 68, and 4 % where 20 heads take two). For 32-bit queries or
 // outputs (or a type other than the cache's) q and P are the sums of two (f16) or three (bf16) 16-bit terms side by side
 // in the columns of the same products (4 or 2 heads in 8 columns), and each step's products are summed apart from what
 // came before them, which keeps the result near 32 bits.

@@ -5,7 +5,7 @@
 //
 // Bound: the contents' copies by HBM (every moved page once in and once out), the bookkeeping by latency: one CTA per
 // call, phases in a row, each a few dependent loads. Measured: a beam step of 8 (fork, free, extend with 4 split pages of
-// 16 layers) 13.4 us in four launches; 63 copies of an 8.4 MB block, read from L2 after the first, 93 us (5.7 TB/s
+// 16 layers) 14.1 us in four launches; 63 copies of an 8.4 MB block, read from L2 after the first, 93 us (5.7 TB/s
 // written); 230 MB of pages moved by a compaction about 75 us (6.1 TB/s read and written).
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"

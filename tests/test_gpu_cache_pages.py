@@ -1,6 +1,8 @@
-"""sjk_pages_* on ledgers whose stack was damaged from outside: nothing is followed beyond its array, nothing half done."""
+"""sjk_pages_* on ledgers whose stack was damaged from outside (nothing is followed beyond its array, nothing half done), and
+over caches of other layouts."""
 import pytest
 
+import kv16
 import sjk
 from test_gpu_pages import CORRUPT, FULL, Device, Model
 
@@ -81,3 +83,35 @@ def test_bad_ids_deep_in_a_large_request(T):
     d.same(m)
     assert d.p.extend(d.i32([1]), d.i32([0]), 301).item() == FULL == m.extend([1], [0], [301])
     d.same(m)
+
+
+@pytest.mark.parametrize("layout", ["heads first", "interleaved"])
+def test_ledgers_over_other_layouts(T, layout):
+    """Caches whose K and V are views of whole pages: the ledger's slab is the tensor that they came from."""
+    n, page, H, D = 12, 16, 2, 64
+    if layout == "heads first":
+        slabs = [T.zeros((1, n, H, page, D), dtype=T.bfloat16, device="cuda") for _ in range(2)]
+        k, v = (x.transpose(2, 3) for x in slabs)
+    else:
+        slabs = [T.zeros((1, n, page, H, 2, D), dtype=T.bfloat16, device="cuda")]
+        k, v = slabs[0][..., 0, :], slabs[0][..., 1, :]
+    cache = kv16.Cache(k, v, T.full((2, 4), -1, dtype=T.int32, device="cuda"))
+    pages = kv16.Pages(cache.tables, page, slabs=slabs)
+    i32 = lambda x: T.tensor(x, dtype=T.int32, device="cuda")  # noqa: E731
+    pages.extend(i32([0]), i32([0]), 20)
+    T.manual_seed(0)
+    rows = [T.randn((21, H, D), device="cuda").bfloat16() for _ in range(2)]
+    step = kv16.Qkv(D, cache=cache)
+    step(k=rows[0][:20], v=rows[1][:20], pos=T.arange(20, dtype=T.int32, device="cuda"), rows=i32([0] * 20))
+    q = T.randn((1, 4, D), device="cuda").bfloat16()
+    want = cache.attend(0, q, i32([20]), 0.125, rows=i32([0]))
+    assert pages.fork(i32([0]), i32([1])).tolist() == [0]
+    assert pages.extend(i32([1]), i32([20]), 1).item() == 0         # splits the last page, which gets its contents
+    assert cache.tables[:, :2].tolist() == [[0, 1], [0, 2]]
+    step(k=rows[0][20:], v=rows[1][20:], pos=i32([20]), rows=i32([1]))
+    assert T.equal(cache.attend(0, q, i32([20]), 0.125, rows=i32([0])), want)
+    assert T.equal(cache.attend(0, q, i32([20]), 0.125, rows=i32([1])), want)
+    at = cache.tables[1].long()
+    got = T.cat((cache.k[0, at[0]], cache.k[0, at[1], :5]))
+    assert T.equal(got, rows[0])
+    assert sjk.lib().sjk_device_status() == 0
