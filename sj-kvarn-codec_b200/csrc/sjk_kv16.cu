@@ -961,7 +961,7 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
                                float scale, int window, const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st) {
     if (!c || !q || !out || !len || n_seq < 0 || window < 0 || !isfinite(scale)) return SJKVARN_ERR_ARG;
     if (sjk_kv16_check(c)) return SJKVARN_ERR_ARG;
-    if (!q->p || !out->p || !type_ok(q->type) || !type_ok(out->type) || q->n_head < 1 || q->n_head != out->n_head || q->n_head % c->n_head_kv)
+    if (!q->p || !out->p || !type_ok(q->type) || !type_ok(out->type) || !rows_ok(*q) || !rows_ok(*out) || !list_ok(len) || !list_ok(rows) || q->n_head < 1 || q->n_head != out->n_head || q->n_head % c->n_head_kv)
         return SJKVARN_ERR_ARG;
     if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
     const int64_t strides = c->page_stride | c->slot_stride | c->head_stride;

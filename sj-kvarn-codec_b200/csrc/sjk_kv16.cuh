@@ -15,6 +15,10 @@ SJK_HD size_t type_bytes(int type) { return type == SJK_F32 ? 4u : 2u; }
 static inline bool type_ok(int type) { return type == SJK_F32 || type == SJK_F16 || type == SJK_BF16; }
 static inline bool aligned(const void * p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// rows whose address is a multiple of an element's size; a list of int32 (NULL passes)
+static inline bool rows_ok(const sjk_rows & r) { return aligned(r.p, type_bytes(r.type)); }
+static inline bool list_ok(const void * p) { return aligned(p, 4); }
+
 // two 16-bit values of a word, widened; two floats rounded to nearest even and packed
 template <int TYPE>
 SJK_DEV float2 widen2(uint32_t w) {

@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(NT) pages_copy_kernel(const __grid_constant__ 
 
 int params_of(const sjk_pages * g, Params * p, bool tables) {
     if (!g || !g->ledger || !aligned(g->ledger, 16) || g->n_pages < 1 || g->n_pages > SJK_PAGES_MAX) return SJKVARN_ERR_ARG;
-    if (tables && (!g->tables || g->n_rows < 1 || g->n_rows > 0x7FFFFFFFu || g->table_stride < 1 || g->page_tokens < 1)) return SJKVARN_ERR_ARG;
+    if (tables && (!g->tables || !aligned(g->tables, 4) || g->n_rows < 1 || g->n_rows > 0x7FFFFFFFu || g->table_stride < 1 || g->page_tokens < 1)) return SJKVARN_ERR_ARG;
     if (g->n_slabs < 0 || g->n_slabs > SJK_MAX_SLABS) return SJKVARN_ERR_ARG;
     for (int i = 0; i < g->n_slabs; ++i) {
         const sjk_slab & s = g->slabs[i];
@@ -482,7 +482,7 @@ extern "C" int sjk_pages_fork(const sjk_pages * g, const int32_t * src, const in
     Params p;
     const int rc = params_of(g, &p, true);
     if (rc) return rc;
-    if (n < 0 || (n && (!src || !dst || !status))) return SJKVARN_ERR_ARG;
+    if (n < 0 || (n && (!src || !dst || !status)) || !list_ok(src) || !list_ok(dst) || !list_ok(status)) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
     p.a = src; p.b = dst; p.n = n; p.status = status;
     return launch(pages_fork_kernel, dim3((unsigned) n), dim3(NT), 0, st, p);
@@ -492,7 +492,7 @@ extern "C" int sjk_pages_free(const sjk_pages * g, const int32_t * rows, const i
     Params p;
     const int rc = params_of(g, &p, true);
     if (rc) return rc;
-    if (n < 0 || (n && !rows)) return SJKVARN_ERR_ARG;
+    if (n < 0 || (n && !rows) || !list_ok(rows) || !list_ok(g0) || !list_ok(g1)) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
     p.a = rows; p.b = g0; p.c = g1; p.n = n;
     uint32_t runs = (p.stride + 4 * NT - 1) / (4 * NT);     // about four entries a thread, at most a wave over all rows
@@ -506,7 +506,9 @@ extern "C" int sjk_pages_extend(const sjk_pages * g, const int32_t * rows, const
     Params p;
     int rc = params_of(g, &p, true);
     if (rc) return rc;
-    if (n < 0 || n > SJK_PAGES_MAX_ROWS || (n && (!rows || !len || !status)) || (!add && add_all < 0)) return SJKVARN_ERR_ARG;
+    if (n < 0 || n > SJK_PAGES_MAX_ROWS || (n && (!rows || !len || !status)) || (!add && add_all < 0) || !list_ok(rows) || !list_ok(len) ||
+        !list_ok(add) || !list_ok(status))
+        return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
     if (too_many(p, (uint32_t) n)) return SJK_ERR_UNSUPPORTED;      // a request copies its first page at most
     p.a = rows; p.b = len; p.c = add; p.add_all = add_all; p.n = n; p.status = status;
@@ -519,6 +521,7 @@ extern "C" int sjk_pages_compact(const sjk_pages * g, int32_t * info, sjk_stream
     Params p;
     int rc = params_of(g, &p, true);
     if (rc) return rc;
+    if (!list_ok(info)) return SJKVARN_ERR_ARG;
     if (too_many(p, p.n_pages / 2)) return SJK_ERR_UNSUPPORTED;     // a move needs a used page and a free one
     p.status = info;
     const size_t smem = (size_t) ((p.n_pages + 31u) / 32u) * sizeof(uint32_t);
@@ -532,7 +535,7 @@ extern "C" int sjk_pages_copy(const sjk_pages * g, const int32_t * src, const in
     Params p;
     const int rc = params_of(g, &p, false);
     if (rc) return rc;
-    if (n < 0 || (n && (!src || !dst))) return SJKVARN_ERR_ARG;
+    if (n < 0 || (n && (!src || !dst)) || !list_ok(src) || !list_ok(dst)) return SJKVARN_ERR_ARG;
     if (n == 0) return 0;
     if (too_many(p, (uint32_t) n)) return SJK_ERR_UNSUPPORTED;
     return copy_launch(p, reinterpret_cast<const uint32_t *>(src), reinterpret_cast<const uint32_t *>(dst), n, 0, st);

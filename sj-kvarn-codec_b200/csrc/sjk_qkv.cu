@@ -591,7 +591,7 @@ extern "C" void sjk_rope_free(sjk_rope * r) {
 }
 
 int sjk_kv16_check(const sjk_kv16 * c) {
-    if (!c->k || !c->v || !c->tables || c->page_tokens < 1 || c->n_head_kv < 1 || c->head_dim < 1 || c->n_pages < 1 ||
+    if (!c->k || !c->v || !c->tables || !aligned(c->k, 2) || !aligned(c->v, 2) || !aligned(c->tables, 4) || c->page_tokens < 1 || c->n_head_kv < 1 || c->head_dim < 1 || c->n_pages < 1 ||
         c->n_pages >= SJKVARN_NO_BLOCK || c->n_rows < 1 || c->table_stride < 1 || (c->type != SJK_F16 && c->type != SJK_BF16) ||
         c->page_stride < 0 || c->slot_stride < 0 || c->head_stride < 0)
         return SJKVARN_ERR_ARG;
@@ -617,9 +617,9 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
             if (out[i].p) return SJKVARN_ERR_ARG;
             continue;
         }
-        if (in[i].n_head < 1 || in[i].n_head > 65535 || !type_ok(in[i].type) || (type >= 0 && in[i].type != type)) return SJKVARN_ERR_ARG;
+        if (in[i].n_head < 1 || in[i].n_head > 65535 || !type_ok(in[i].type) || !rows_ok(in[i]) || (type >= 0 && in[i].type != type)) return SJKVARN_ERR_ARG;
         type = in[i].type;
-        if (out[i].p && (out[i].n_head != in[i].n_head || !type_ok(out[i].type))) return SJKVARN_ERR_ARG;
+        if (out[i].p && (out[i].n_head != in[i].n_head || !type_ok(out[i].type) || !rows_ok(out[i]))) return SJKVARN_ERR_ARG;
         // rows in place: an element has to stay where it was read
         if (out[i].p == in[i].p && (out[i].type != type || out[i].row_stride != in[i].row_stride || out[i].head_stride != in[i].head_stride))
             return SJKVARN_ERR_ARG;
@@ -629,11 +629,13 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
     }
     if (type < 0) return SJKVARN_ERR_ARG;
     if ((a->q_norm || a->k_norm) && (!type_ok(a->norm_type) || !(a->eps >= 0.0f) || !isfinite(a->eps))) return SJKVARN_ERR_ARG;
+    for (const void * w : {a->q_norm, a->k_norm})
+        if (w && !aligned(w, type_bytes(a->norm_type))) return SJKVARN_ERR_ARG;
     const bool rope = a->rope.n_rot != 0;
-    if (rope && (a->rope.n_rot < 2 || (a->rope.n_rot & 1) || a->rope.n_rot > a->head_dim || !a->rope.step ||
+    if (rope && (a->rope.n_rot < 2 || (a->rope.n_rot & 1) || a->rope.n_rot > a->head_dim || !a->rope.step || !aligned(a->rope.step, 8) ||
                  (a->rope.layout != SJK_ROPE_HALF && a->rope.layout != SJK_ROPE_PAIR)))
         return SJKVARN_ERR_ROTATION;
-    if ((rope || cached) && !a->pos) return SJKVARN_ERR_ARG;
+    if (((rope || cached) && !a->pos) || !list_ok(a->pos) || !list_ok(a->rows)) return SJKVARN_ERR_ARG;
     if (a->n_tok == 0) return 0;
     p.n_tok = a->n_tok; p.D = a->head_dim;
     p.n_q = n[0]; p.n_k = n[1]; p.n_v = n[2];

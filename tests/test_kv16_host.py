@@ -345,3 +345,58 @@ def test_yarn_amplitude(factor, amp):
     """The default amplitude is 0.1 ln(factor) + 1 for contexts that grow and 1 for others."""
     assert kv16.rope_steps(64, scaling="yarn", factor=factor, n_ctx=4096)[1] == pytest.approx(amp, rel=2 ** -23)
     assert kv16.rope_steps(64, scaling="yarn", factor=factor, n_ctx=4096, amp=0.7)[1] == pytest.approx(0.7, rel=2 ** -23)
+
+
+def test_addresses_off_their_types_are_refused():
+    """Pointers that are no multiple of what they point at would fault on the device: every call refuses them. (Calls without
+    work, which nothing launches.)"""
+    L, P = sjk.lib(), 0x10000
+
+    def rows(heads, type, p=P):
+        return sjk.Rows(p, 1024, 64, heads, type)
+
+    def cache(**kw):
+        c = sjk.Kv16(P, P, 16 * 2 * 64, 2 * 64, 64, kv16.BF16, 64, 2, 16, 8, P, 4, 4)
+        for k, v in kw.items():
+            setattr(c, k, v)
+        return c
+
+    def qkv(**kw):
+        a = sjk.QkvArgs()
+        a.n_tok, a.head_dim, a.eps, a.pos = 0, 64, 1e-6, P
+        a.q, a.k, a.v, a.q_out = rows(4, kv16.BF16), rows(2, kv16.BF16), rows(2, kv16.BF16), rows(4, kv16.F32, 2 * P)
+        a.cache = cache()
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return L.sjk_qkv(C.byref(a), None)
+
+    assert qkv() == qkv(rope=sjk.RopeC(64, 0, 1.0, P), rows=P, q_norm=P, k_norm=P, norm_type=kv16.F32) == 0
+    for bad in (dict(q=rows(4, kv16.BF16, P + 1)), dict(q_out=rows(4, kv16.F32, P + 2)), dict(k=rows(2, kv16.BF16, P + 3)), dict(pos=P + 2),
+                dict(rows=P + 1), dict(q_norm=P + 2, norm_type=kv16.F32), dict(k_norm=P + 1, norm_type=kv16.F16), dict(cache=cache(k=P + 1)),
+                dict(cache=cache(v=P + 1)), dict(cache=cache(tables=P + 2))):
+        assert qkv(**bad) == -100, bad
+    assert qkv(rope=sjk.RopeC(64, 0, 1.0, P + 4)) == -129
+
+    def attend(c=None, q=None, out=None, lens=P, rws=None):
+        c, q, out = c or cache(), q or rows(4, kv16.F32), out or rows(4, kv16.F32)
+        return L.sjk_kv16_attend(C.byref(c), C.byref(q), lens, rws, 0, 1.0, 0, C.byref(out), P, 1 << 30, None)
+
+    assert attend() == attend(rws=P) == 0
+    for bad in (dict(q=rows(4, kv16.F32, P + 2)), dict(q=rows(4, kv16.F16, P + 1)), dict(out=rows(4, kv16.F32, P + 2)),
+                dict(out=rows(4, kv16.BF16, P + 1)), dict(lens=P + 2), dict(rws=P + 1), dict(c=cache(tables=P + 1))):
+        assert attend(**bad) == -100, bad
+
+    p = sjk.PagesC(P, P, 64, 4, 8, 16)
+    r = C.byref(p)
+    assert L.sjk_pages_fork(r, P, P, 0, P, None) == L.sjk_pages_extend(r, P, P, P, 1, 0, P, None) == L.sjk_pages_free(r, P, P, P, 0, None) == 0
+    assert L.sjk_pages_copy(r, P, P, 0, None) == 0
+    for x in (P + 1, P + 2):
+        assert L.sjk_pages_fork(r, x, P, 0, P, None) == -100 and L.sjk_pages_fork(r, P, x, 0, P, None) == -100
+        assert L.sjk_pages_fork(r, P, P, 0, x, None) == -100
+        assert L.sjk_pages_extend(r, x, P, None, 1, 0, P, None) == -100 and L.sjk_pages_extend(r, P, x, None, 1, 0, P, None) == -100
+        assert L.sjk_pages_extend(r, P, P, x, 1, 0, P, None) == -100 and L.sjk_pages_extend(r, P, P, None, 1, 0, x, None) == -100
+        assert L.sjk_pages_free(r, x, None, None, 0, None) == -100 and L.sjk_pages_free(r, P, x, None, 0, None) == -100
+        assert L.sjk_pages_free(r, P, None, x, 0, None) == -100 and L.sjk_pages_compact(r, x, None) == -100
+        assert L.sjk_pages_copy(r, x, P, 0, None) == -100 and L.sjk_pages_copy(r, P, x, 0, None) == -100
+    p.tables = P + 2
+    assert L.sjk_pages_fork(r, P, P, 0, P, None) == -100
