@@ -610,6 +610,9 @@ typedef struct sjk_qkv_args {
 } sjk_qkv_args;
 /* One launch. pos may be NULL without a rotation and a cache. Arithmetic in 32-bit floats, one rounding at the end. */
 int sjk_qkv(const sjk_qkv_args * a, sjk_stream st);
+/* sjk_qkv whose K and V go to the cache positions at[t] (DEVICE [n_tok]; a negative one: not into the cache; NULL: pos),
+ * with pos for the rotation: drafted tokens on several branches have one rotary position and a place each. */
+int sjk_qkv_at(const sjk_qkv_args * a, const int32_t * at, sjk_stream st);
 
 /* ---- attention of one new token per sequence over the pages ----
  * Sequence i has the table row rows[i] (DEVICE; NULL: row i), len[i] positions (DEVICE, its newest one included) and
@@ -627,6 +630,65 @@ int sjk_qkv(const sjk_qkv_args * a, sjk_stream st);
 size_t sjk_kv16_attend_scratch_bytes(const sjk_kv16 * c, int n_head);
 int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len, const int32_t * rows, int n_seq, float scale,
                     int window, const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st);
+
+/* ---- steps that bring several tokens of every sequence ----
+ * Sequence i has len[i] positions and brings add[i] tokens (DEVICE), as many as SJK_MAPS_MAX sequences in a call. Token t
+ * of the call, j-th of sequence i, gets (DEVICE outputs, each NULL where it is not wanted; entries behind the last token
+ * are padding):
+ *   first[i]  where the tokens of sequence i begin (n_seq + 1 values; the last: their number)
+ *   row[t]    its table row, rows[i] (rows NULL: i); padding 0
+ *   at[t]     its cache position len[i] + j; padding -1
+ *   pos[t]    its rotary position: at[t], or with masks (DEVICE [n_tok]: bit k says that the token sees the k-th of its
+ *             sequence's) len[i] plus the number of others that it sees; padding -1
+ *   slot[t]   page * page_tokens + place on the page, -1 without a page
+ * Tokens beyond n_tok, negative lengths and counts, rows and pages outside their arrays are left out (SJK_DEVICE_PAGE).
+ * row, pos and at are what sjk_qkv_at takes. One launch. */
+#define SJK_MAPS_MAX 8192
+typedef struct sjk_kv16_step {
+    int32_t * first, * row, * pos, * at;
+    int64_t * slot;
+} sjk_kv16_step;
+int sjk_kv16_maps(const sjk_kv16 * c, const int32_t * len, const int32_t * add, const int32_t * rows, const uint64_t * masks,
+                  int n_seq, int n_tok, const sjk_kv16_step * out, sjk_stream st);
+/* Accepted drafts to their places: of sequence i the K and V rows of the positions len[i] + path[i][j], j < count[i], go to
+ * len[i] + j in all n_layers layers (layer l's rows at c's plus l * layer_stride elements), and new_len[i] (DEVICE, may be
+ * NULL, not over len) = len[i] + count[i]. path: DEVICE [n_seq][width], ascending; width <= SJK_KEEP_MAX. Where a path does
+ * not ascend, a position has no page, or an earlier entry has the same table row, nothing of the sequence moves, new_len
+ * is len, and SJK_DEVICE_PAGE is set. The pages written to are the sequence's own (sjk_pages_extend has split them). One
+ * launch. */
+#define SJK_KEEP_MAX 256
+int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_stride, const int32_t * len, const int32_t * path,
+                  const int32_t * count, const int32_t * rows, int width, int n_seq, int32_t * new_len, sjk_stream st);
+
+/* ---- attention to a part of a long context ----
+ * bounds: DEVICE [n_pages][2][n_head_kv][head_dim] of the cache's type: the smallest and the largest key of every channel
+ * among a page's tokens. sjk_kv16_bounds makes them anew, from the page's first position on, for the pages that hold
+ * positions in [first[i], end[i]) of sequence i (DEVICE), from their positions before end[i], in n_layers layers (keys
+ * layer_stride, bounds bounds_stride elements apart). A channel with a NaN has NaN as its bounds. Pages without a token
+ * keep theirs. One launch.
+ *
+ * sjk_kv16_select chooses for every sequence and KV head up to `budget` pages of its table row, as their numbers there:
+ * the first `sink` and the newest `recent` ones, and of the others those with the largest
+ *   sum over the group's query heads of sum_d max(q_d lo_d, q_d hi_d)
+ * (in 64 bits; ties to the lower number; a sum that is no number counts as the largest), all where there are no more than
+ * `budget`. blocks[i][h] (DEVICE [n_seq][n_head_kv][budget]): ascending, then -1; count (DEVICE [n_seq][n_head_kv], may be
+ * NULL): how many. Pages that are SJKVARN_NO_BLOCK are never chosen. The newest page's bounds may be older than its last
+ * tokens where `recent` covers it. Two launches.
+ *
+ * sjk_kv16_attend_blocks is sjk_kv16_attend over the positions on the listed pages alone: blocks as above, from any
+ * source; a list ends at its first entry that is -1, does not ascend or lies behind the sequence (the last two set
+ * SJK_DEVICE_PAGE). Three launches. Scratch of both: their *_scratch_bytes(), 16-byte aligned, not shared by calls that
+ * overlap. head_dim, alignment and types as for sjk_kv16_attend; bounds 16-byte aligned. */
+int    sjk_kv16_bounds(const sjk_kv16 * c, int n_layers, int64_t layer_stride, void * bounds, int64_t bounds_stride,
+                       const int32_t * first, const int32_t * end, const int32_t * rows, int n_seq, sjk_stream st);
+size_t sjk_kv16_select_scratch_bytes(const sjk_kv16 * c, int n_seq);
+int    sjk_kv16_select(const sjk_kv16 * c, const void * bounds, const sjk_rows * q, const int32_t * len, const int32_t * rows,
+                       int n_seq, int budget, int sink, int recent, int32_t * blocks, int32_t * count, void * scratch,
+                       size_t scratch_bytes, sjk_stream st);
+size_t sjk_kv16_attend_blocks_scratch_bytes(const sjk_kv16 * c, int n_head, int n_seq, int budget);
+int    sjk_kv16_attend_blocks(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len, const int32_t * rows,
+                              const int32_t * blocks, int n_seq, int budget, float scale, const sjk_rows * out, void * scratch,
+                              size_t scratch_bytes, sjk_stream st);
 
 /* ---- who owns the pages ----
  * A ledger in device memory over the pages of one or more slabs (the K and the V pages of every layer, or the record

@@ -59,8 +59,15 @@ int sjk_xchg_status_take(void);
 int sjk_qkv_status_take(void);
 int sjk_kv16_status_take(void);
 int sjk_pages_status_take(void);
+int sjk_step_status_take(void);
+int sjk_blocks_status_take(void);
 // 0 where the fields of a 16-bit cache are possible ones (sjk_qkv.cu)
 int sjk_kv16_check(const sjk_kv16 * c);
+// sjk_kv16_attend over sequences that are one KV head each (sjk_kv16.cu): c has one KV head, n_seq = `fold` heads of
+// every row of q and out, head s % fold of row s / fold; the lengths are written by the kernel before it in the stream.
+// check: the arguments only, nothing is launched.
+int sjk_kv16_attend_folded(const sjk_kv16 * c, int fold, const sjk_rows * q, const int32_t * len, int n_seq, float scale, const sjk_rows * out,
+                           void * scratch, size_t scratch_bytes, sjk_stream st, bool check);
 
 // Move the record groups [g0, g0 + n) of one layer (group_bytes = n_head_kv x record bytes) through
 // an optional device block table: op 0 gathers them into buf (group order), op 1 scatters buf into them, op 2

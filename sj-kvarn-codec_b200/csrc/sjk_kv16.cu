@@ -60,6 +60,8 @@ struct Params {
     sjk_rows q, out;
     const int32_t * len, * rows;
     int n_seq, grp, tiles;                  // tiles: row tiles of a KV head (R query heads each)
+    int fold;                               // sequences with heads of their own: sequence s is KV head s % fold of row
+                                            // s / fold of q and out (1: every sequence has all KV heads)
     int window, page_shift;                 // page_shift: log2 of the page's tokens, -1 where it is no power of two
     uint32_t slot_stride;
     float scale;
@@ -69,6 +71,18 @@ struct Params {
     int4 * split;                           // by pair (or, with more pairs than workers, by worker): sequence (-1: not
     int by_pair;                            // split), (KV head, row tile), first and last worker
 };
+
+// Row of q and out, KV head, and first query head of its group, of a pair.
+struct Place { int row, kv, r0; };
+SJK_DEV Place place_of(const Params & p, int seq, int hp, int R) {
+    const int kv = hp / p.tiles;
+    Place x = {seq, kv, (hp - kv * p.tiles) * R};
+    if (p.fold > 1) {
+        x.row = seq / p.fold;
+        x.kv = seq - x.row * p.fold;
+    }
+    return x;
+}
 
 // 16 tokens per m tile; steps of 32 tokens for small heads, whose rows are short
 __host__ __device__ constexpr int tok_tiles(int D) { return D <= 64 ? 2 : 1; }
@@ -322,7 +336,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         const bool on = row >= 0 && row < (int64_t) p.c.n_rows;
         if (!on) atomicOr(&g_kv16_status, (unsigned) SJK_DEVICE_PAGE);
         ld_table = on ? p.c.tables + row * p.c.table_stride : nullptr;
-        const int64_t head = (int64_t) (ld.hp / p.tiles) * p.c.head_stride;
+        const int64_t head = (int64_t) place_of(p, ld.seq, ld.hp, R).kv * p.c.head_stride;
         ld_kp = static_cast<const uint16_t *>(p.c.k) + head;
         ld_vp = static_cast<const uint16_t *>(p.c.v) + head;
         ld_win = -64;
@@ -455,14 +469,14 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
         if (fresh) {                                         // a (sequence, KV head, row tile) begins
             fresh = false;
             begun = at.st == 0;
-            const int kv = at.hp / p.tiles, r0 = (at.hp - kv * p.tiles) * R;
+            const auto [row, kv, r0] = place_of(p, at.seq, at.hp, R);
             int64_t src[NT8];
             bool on[NT8];
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
                 const int rel = r0 + HT * n + qhead;
                 on[n] = rel < p.grp;
-                src[n] = (int64_t) at.seq * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
+                src[n] = (int64_t) row * p.q.row_stride + (int64_t) (kv * p.grp + rel) * p.q.head_stride + (lane & 3) * 2;
             }
             if constexpr (T == 1) {
 #pragma unroll
@@ -680,7 +694,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                 if (p.by_pair) p.split[at.seq * HP + at.hp] = make_int4(ended ? -1 : at.seq, at.hp, worker, last);
                 else if (!ended) p.split[worker] = make_int4(at.seq, at.hp, worker, last);
             }
-            const int kv = at.hp / p.tiles, r0 = (at.hp - kv * p.tiles) * R;
+            const auto [row, kv, r0] = place_of(p, at.seq, at.hp, R);
 #pragma unroll
             for (int n = 0; n < NT8; ++n) {
 #pragma unroll
@@ -711,7 +725,7 @@ __global__ void __launch_bounds__(32 * S::W, 1) kv16_attend_kernel(const __grid_
                     const float mj = own_j ? m[n][1] : m[n][j], lj = own_j ? l[n][1] : l[n][j];
                     if (begun && ended) {
                         const float inv = lj == 0.0f ? 0.0f : 1.0f / lj;
-                        const int64_t dst = (int64_t) at.seq * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride + (lane >> 2) + 8 * own_h;
+                        const int64_t dst = (int64_t) row * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride + (lane >> 2) + 8 * own_h;
 #pragma unroll
                         for (int h = 0; h < NH; ++h) {
                             if (p.out.type == SJK_F32) store_channels<SJK_F32>(p.out.p, dst + 8 * h, o[n], at_of(j, h), inv);
@@ -782,10 +796,14 @@ __global__ void __launch_bounds__(512) kv16_merge_kernel(const __grid_constant__
     const int warps = blockDim.x >> 5;
     if (blockIdx.x >= entries) {
         const int seq = (blockIdx.x - entries) * warps + (threadIdx.x >> 5);
-        if (blockIdx.y == 0 && seq < p.n_seq && p.len[seq] <= 0)
-            for (int i = threadIdx.x & 31; i < p.out.n_head * D; i += 32)
-                store1(p.out.p, (int64_t) seq * p.out.row_stride + (int64_t) (i / D) * p.out.head_stride + i % D, p.out.type, 0.0f);
-        pdl_wait();
+        if (p.fold > 1) pdl_wait();         // (there the lengths are the kernel's before the attention)
+        if (blockIdx.y == 0 && seq < p.n_seq && p.len[seq] <= 0) {
+            const int row = p.fold > 1 ? seq / p.fold : seq, heads = p.fold > 1 ? p.grp : p.out.n_head;
+            const int64_t dst = (int64_t) row * p.out.row_stride + (int64_t) (seq - row * p.fold) * (p.fold > 1 ? p.grp * p.out.head_stride : 0);
+            for (int i = threadIdx.x & 31; i < heads * D; i += 32)
+                store1(p.out.p, dst + (int64_t) (i / D) * p.out.head_stride + i % D, p.out.type, 0.0f);
+        }
+        if (p.fold <= 1) pdl_wait();
         pdl_release();
         return;
     }
@@ -796,7 +814,8 @@ __global__ void __launch_bounds__(512) kv16_merge_kernel(const __grid_constant__
     const int4 e = p.split[blockIdx.x];
     if (e.x < 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % G;
-    const int kv = e.y / p.tiles, r0 = (e.y - kv * p.tiles) * R, nr = p.grp - r0 < R ? p.grp - r0 : R;
+    const auto [row, kv, r0] = place_of(p, e.x, e.y, R);
+    const int nr = p.grp - r0 < R ? p.grp - r0 : R;
     const int n = e.w - e.z + 1, lo = (int) ((int64_t) n * sub / G), hi = (int) ((int64_t) n * (sub + 1) / G);
     for (int r = blockIdx.y * (warps / G) + warp / G; r < nr; r += gridDim.y * (warps / G)) {
         float top = -INFINITY, sum = 0.0f;
@@ -871,7 +890,7 @@ __global__ void __launch_bounds__(512) kv16_merge_kernel(const __grid_constant__
         }
         if (sub == 0) {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            const int64_t dst = (int64_t) e.x * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride;
+            const int64_t dst = (int64_t) row * p.out.row_stride + (int64_t) (kv * p.grp + r0 + r) * p.out.head_stride;
 #pragma unroll
             for (int v = 0; v < NV; ++v)
                 if (32 * v + lane < D / 4) {
@@ -957,11 +976,12 @@ extern "C" size_t sjk_kv16_attend_scratch_bytes(const sjk_kv16 * c, int n_head) 
     return most;
 }
 
-extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len, const int32_t * rows, int n_seq,
-                               float scale, int window, const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st) {
+// fold > 1: c has one KV head, and the n_seq sequences are `fold` heads of every row of q and out; check: arguments only
+static int attend(const sjk_kv16 * c, int fold, const sjk_rows * q, const int32_t * len, const int32_t * rows, int n_seq, float scale, int window,
+                  const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st, bool check) {
     if (!c || !q || !out || !len || n_seq < 0 || window < 0 || !isfinite(scale)) return SJKVARN_ERR_ARG;
     if (sjk_kv16_check(c)) return SJKVARN_ERR_ARG;
-    if (!q->p || !out->p || !type_ok(q->type) || !type_ok(out->type) || !rows_ok(*q) || !rows_ok(*out) || !list_ok(len) || !list_ok(rows) || q->n_head < 1 || q->n_head != out->n_head || q->n_head % c->n_head_kv)
+    if (!q->p || !out->p || !type_ok(q->type) || !type_ok(out->type) || !rows_ok(*q) || !rows_ok(*out) || !list_ok(len) || !list_ok(rows) || q->n_head < 1 || q->n_head != out->n_head || q->n_head % (c->n_head_kv * fold))
         return SJKVARN_ERR_ARG;
     if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
     const int64_t strides = c->page_stride | c->slot_stride | c->head_stride;
@@ -971,7 +991,7 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     if (!split && (!aligned(q->p, 4) || (q->row_stride & 1) || (q->head_stride & 1))) return SJKVARN_ERR_ARG;
     if (c->slot_stride > 0x7FFFFFFF) return SJK_ERR_UNSUPPORTED;
     Plan pl;
-    const int rc = plan_of(c, q->n_head, split, &pl);
+    const int rc = plan_of(c, q->n_head / fold, split, &pl);
     if (rc) return rc;
     if (n_seq == 0) return 0;
     // a list counts its units in 32 bits, and a worker its run, whatever the lengths
@@ -979,10 +999,11 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     const int HP = c->n_head_kv * pl.tiles;
     if (most > 2e9 || most * HP / pl.work > 2e9) return SJK_ERR_UNSUPPORTED;
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < pl.bytes) return SJKVARN_ERR_BUFFER;
+    if (check) return 0;
     Params p = {};
     p.c = *c; p.q = *q; p.out = *out;
     p.len = len; p.rows = rows; p.n_seq = n_seq;
-    p.grp = q->n_head / c->n_head_kv; p.tiles = pl.tiles;
+    p.grp = q->n_head / (c->n_head_kv * fold); p.tiles = pl.tiles; p.fold = fold;
     p.window = window; p.scale = scale;
     p.slot_stride = (uint32_t) c->slot_stride;
     p.page_shift = -1;
@@ -996,6 +1017,16 @@ extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int
     // a list per head where that leaves under a sixteenth of the workers without one
     p.wph = HP * 16 <= p.n_work ? p.n_work / HP : 0;
     return with_shape(c, split, pl.nt8, [&](auto s) { return run<decltype(s)>(p, pl, st); });
+}
+
+extern "C" int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len, const int32_t * rows, int n_seq,
+                               float scale, int window, const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st) {
+    return attend(c, 1, q, len, rows, n_seq, scale, window, out, scratch, scratch_bytes, st, false);
+}
+
+int sjk_kv16_attend_folded(const sjk_kv16 * c, int fold, const sjk_rows * q, const int32_t * len, int n_seq, float scale, const sjk_rows * out,
+                           void * scratch, size_t scratch_bytes, sjk_stream st, bool check) {
+    return attend(c, fold, q, len, nullptr, n_seq, scale, 0, out, scratch, scratch_bytes, st, check);
 }
 
 int sjk_kv16_status_take(void) {

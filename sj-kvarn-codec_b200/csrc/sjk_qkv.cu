@@ -56,7 +56,7 @@ struct Params {
     int n_rot, layout;
     float amp;
     const uint64_t * step;
-    const int32_t * pos, * rows;
+    const int32_t * pos, * rows, * at;      // at: cache positions, NULL: pos
     sjk_kv16 c;
 };
 
@@ -192,7 +192,11 @@ SJK_DEV void tile_table(const Params & p, int t0, int nt, float4 * tab, int32_t 
     if (tid < nt) {
         const int32_t pos = p.pos ? p.pos[t0 + tid] : 0;
         s_pos[tid] = pos;
-        s_slot[tid] = p.c.k && pos >= 0 ? cache_slot(p, t0 + tid, pos) : -1;
+        s_slot[tid] = -1;
+        if (p.c.k && pos >= 0) {
+            const int32_t at = p.at ? p.at[t0 + tid] : pos;
+            if (at >= 0) s_slot[tid] = cache_slot(p, t0 + tid, at);
+        }
     }
     if (half == 0) return;
     // angles of a word (side by side in the head), as a power of two: a channel each, or in pairs
@@ -462,7 +466,8 @@ __global__ void __launch_bounds__(NT) qkv_scalar_kernel(const __grid_constant__ 
             for (int d = lane; d < D; d += 32) store1(out.p, dst + d, out.type, x[d]);
         }
         if (part && p.c.k) {
-            const int64_t slot = cache_slot(p, tok, pos);
+            const int32_t at = p.at ? p.at[tok] : pos;
+            const int64_t slot = at >= 0 ? cache_slot(p, tok, at) : -1;
             if (slot >= 0) {
                 void * base = part == 1 ? p.c.k : p.c.v;
                 for (int d = lane; d < D; d += 32) store1(base, slot + (int64_t) hh * p.c.head_stride + d, p.c.type, x[d]);
@@ -598,8 +603,10 @@ int sjk_kv16_check(const sjk_kv16 * c) {
     return 0;
 }
 
-extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
-    if (!a || a->n_tok < 0) return SJKVARN_ERR_ARG;
+extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) { return sjk_qkv_at(a, nullptr, st); }
+
+extern "C" int sjk_qkv_at(const sjk_qkv_args * a, const int32_t * at, sjk_stream st) {
+    if (!a || a->n_tok < 0 || !list_ok(at)) return SJKVARN_ERR_ARG;
     if (a->head_dim < 2 || a->head_dim > 512 || (a->head_dim & 1)) return SJKVARN_ERR_HEAD_DIM;
     Params p = {};
     const sjk_rows in[3] = {a->q, a->k, a->v}, out[3] = {a->q_out, a->k_out, a->v_out};
@@ -644,7 +651,7 @@ extern "C" int sjk_qkv(const sjk_qkv_args * a, sjk_stream st) {
     p.w[0] = a->q_norm; p.w[1] = a->k_norm;
     p.w_type = a->norm_type; p.w_bias = a->norm_bias; p.eps = a->eps; p.inv_d = 1.0f / (float) a->head_dim;
     p.n_rot = a->rope.n_rot; p.layout = a->rope.layout; p.amp = a->rope.amp; p.step = a->rope.step;
-    p.pos = a->pos; p.rows = a->rows;
+    p.pos = a->pos; p.rows = a->rows; p.at = at;
     if (cached) p.c = a->cache;
     bool vec = p.D % 16 == 0;
     for (int i = 0; i < 3; ++i) vec = vec && rows_vec(p.in[i]) && rows_vec(p.out[i]);

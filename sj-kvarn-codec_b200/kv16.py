@@ -121,6 +121,39 @@ def rope_steps(n_rot, layout="half", base=10000.0, scaling="none", factor=1.0, n
     return list(step[: n_rot // 2]), a.value
 
 
+class _Scratch:
+    """Scratch memory of calls of one kind on one device: by stream (whose calls follow one another), as large as the
+    largest so far; while torch captures, memory of the capture's pool, since graphs captured on one stream may be
+    replayed on several."""
+
+    def __init__(self, device):
+        self.device, self.by_stream = device, {}
+
+    def get(self, st, size, given=None):
+        """(tensor, address, bytes) for a call on stream st; given: the caller's own."""
+        if given is not None:
+            if given.dtype is not torch.uint8 or not given.is_contiguous() or given.get_device() != self.device:
+                raise ValueError(f"scratch: a contiguous uint8 tensor on cuda:{self.device}")
+            return given, given.data_ptr(), given.numel()
+        captured = _capturing()
+        have = None if captured else self.by_stream.get(st)
+        if have is None or have[2] < size:
+            buf = torch.empty(size, dtype=torch.uint8, device=f"cuda:{self.device}")
+            have = buf, buf.data_ptr(), size
+            if not captured:
+                self.by_stream[st] = have
+        return have
+
+
+def _matrix(t, what, device, shape, dtype=_I32):
+    """Address of a contiguous tensor of this shape and type on device `device` (None passes)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or tuple(t.shape) != shape or t.get_device() != device or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} tensor {list(shape)} on cuda:{device}")
+    return t.data_ptr()
+
+
 class Pages:
     """Owner ledger of the pages behind `tables` (int32 [rows][stride], NO_BLOCK = no page) and `slabs` (CUDA tensors
     [layers][pages][...], contiguous within a page). ids, n_free: an existing stack of free ids (a value per page, of which
@@ -236,9 +269,9 @@ class Cache:
         return cls(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
                    torch.full((n_rows, stride), NO_BLOCK, dtype=torch.int32, device=device))
 
-    def pages(self, ids=None, n_free=None):
-        """A ledger over this cache's pages."""
-        return Pages(self.tables, self.page_tokens, slabs=[self.k, self.v], ids=ids, n_free=n_free)
+    def pages(self, ids=None, n_free=None, slabs=()):
+        """A ledger over this cache's pages. slabs: what else the pages have (the bounds of a Blocks), moved with them."""
+        return Pages(self.tables, self.page_tokens, slabs=[self.k, self.v, *slabs], ids=ids, n_free=n_free)
 
     def scratch_bytes(self, heads):
         """Bytes of scratch that attend needs for queries of so many heads."""
@@ -291,6 +324,134 @@ class Cache:
         return out
 
 
+    def keep(self, lens, path, count, rows=None, new_lens=None):
+        """Accepted drafts to their places, in every layer: K and V of the positions lens[i] + path[i][j], j < count[i], to
+        lens[i] + j. lens, count int32 [n], path int32 [n][width], ascending; rows int32 [n] (None: sequence i is table row
+        i). Returns the lengths with the accepted ones (a new vector unless given; not lens itself)."""
+        n, dev = lens.shape[0], self._dev
+        if path.dim() != 2:
+            raise ValueError("path: int32 [n][width]")
+        new = torch.empty_like(lens) if new_lens is None else new_lens
+        args = (_list(lens, "lens", dev, n), _matrix(path, "path", dev, (n, path.shape[1])), _list(count, "count", dev, n), _list(rows, "rows", dev, n))
+        to = _list(new, "new_lens", dev, n)
+        if n:
+            rc = _launch(dev, self._L.sjk_kv16_keep, self._refs[0], len(self.layers), self.k.stride(0), *args, path.shape[1], n, to, _stream(dev))
+            if rc:
+                raise sjk.SjkError(rc, "kv16_keep")
+        return new
+
+
+class Maps:
+    """The maps of a step in which n_seq sequences bring up to n_tok tokens: first [n_seq + 1], rows, pos, at [n_tok] int32
+    and slots [n_tok] int64 (include/sjk.h, sjk_kv16_step), filled by a call and kept until the next one. For Qkv and
+    Cache.attend_tree: rows=m.rows, pos=m.pos, at=m.at, first=m.first."""
+
+    def __init__(self, cache, n_seq, n_tok):
+        self.cache, self.n_seq, self.n_tok, self._dev = cache, n_seq, n_tok, cache._dev
+        at = cache.tables.device
+        self.first, self.rows, self.pos, self.at = (torch.zeros(n, dtype=_I32, device=at) for n in (n_seq + 1, n_tok, n_tok, n_tok))
+        self.slots = torch.zeros(n_tok, dtype=torch.int64, device=at)
+        some = lambda t: t.data_ptr() or None  # noqa: E731
+        self._out = sjk.Kv16Step(some(self.first), some(self.rows), some(self.pos), some(self.at), some(self.slots))
+        self._ref, self._L = C.byref(self._out), _lib()
+
+    def __call__(self, lens, add, rows=None, masks=None):
+        """lens, add int32 [n_seq]: positions and new tokens of the sequences; rows int32 [n_seq] (None: sequence i is table
+        row i); masks int64 [n_tok]: bit k says that a token sees the k-th of its sequence's (None: positions in a row).
+        Returns itself."""
+        n, dev = self.n_seq, self._dev
+        rc = _launch(dev, self._L.sjk_kv16_maps, self.cache._refs[0], _list(lens, "lens", dev, n), _list(add, "add", dev, n), _list(rows, "rows", dev, n),
+                     _matrix(masks, "masks", dev, (self.n_tok,), torch.int64), n, self.n_tok, self._ref, _stream(dev))
+        if rc:
+            raise sjk.SjkError(rc, "kv16_maps")
+        return self
+
+
+class Blocks:
+    """Attention to chosen pages of a cache: bounds of every page's keys ([layers][pages][2][heads][D] of the cache's type;
+    zeros, unless given), the pages that they choose for a query (select), attention over listed pages (attend). The bounds
+    belong to the pages: cache.pages(slabs=[blocks.bounds]) copies and moves them along."""
+
+    def __init__(self, cache, bounds=None):
+        n_layers, n_pages, _, H, D = cache.k.shape
+        shape = (n_layers, n_pages, 2, H, D)
+        if bounds is None:
+            bounds = torch.zeros(shape, dtype=cache.k.dtype, device=cache.k.device)
+        elif tuple(bounds.shape) != shape or bounds.dtype != cache.k.dtype or bounds.get_device() != cache._dev or not bounds.is_contiguous():
+            raise ValueError(f"bounds: a contiguous tensor {list(shape)} of the cache's type and GPU")
+        self.cache, self.bounds, self._dev, self._L = cache, bounds, cache._dev, _lib()
+        self._at = [b.data_ptr() for b in bounds]
+        self._q, self._o = _Rows(sjk.Rows(), "q", D), _Rows(sjk.Rows(), "out", D)
+        self._qo = C.byref(self._q.c), C.byref(self._o.c)
+        self._lock = threading.Lock()
+        self._select, self._attend = _Scratch(self._dev), _Scratch(self._dev)
+
+    def update(self, first, end, rows=None):
+        """Bounds of the pages with positions in [first[i], end[i]) (int32 [n]), from their positions before end[i], in
+        every layer; rows int32 [n] (None: sequence i is table row i)."""
+        n, dev, c = first.shape[0], self._dev, self.cache
+        args = _list(first, "first", dev, n), _list(end, "end", dev, n), _list(rows, "rows", dev, n)
+        if n == 0:
+            return
+        rc = _launch(dev, self._L.sjk_kv16_bounds, c._refs[0], len(c.layers), c.k.stride(0), self._at[0], self.bounds.stride(0), *args, n, _stream(dev))
+        if rc:
+            raise sjk.SjkError(rc, "kv16_bounds")
+
+    def select(self, layer, q, lens, budget, sink=1, recent=1, rows=None, blocks=None, count=None, scratch=None):
+        """Up to `budget` pages of every sequence and KV head for the query heads q [n][heads][D]: the first `sink`, the
+        newest `recent`, and those with the largest bounds. Returns (blocks int32 [n][KV heads][budget], ascending and then
+        -1; count int32 [n][KV heads])."""
+        n, dev, c = q.shape[0], self._dev, self.cache
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.select(layer, q, lens, budget, sink, recent, rows, blocks, count, scratch)
+        H = c.n_head_kv
+        if budget < 1 or sink < 0 or recent < 0 or sink + recent > budget:
+            raise ValueError("budget: at least 1, and at least sink + recent")
+        if blocks is None:
+            blocks = torch.empty((n, H, budget), dtype=_I32, device=q.device)
+        if count is None:
+            count = torch.empty((n, H), dtype=_I32, device=q.device)
+        to = _matrix(blocks, "blocks", dev, (n, H, budget)), _matrix(count, "count", dev, (n, H))
+        with self._lock:
+            self._q.set(q, n, dev)
+            args = _list(lens, "lens", dev, n), _list(rows, "rows", dev, n)
+            if n == 0:
+                return blocks, count
+            st = _stream(dev)
+            _, address, size = self._select.get(st, self._L.sjk_kv16_select_scratch_bytes(c._refs[layer], n), scratch)
+            rc = self._L.sjk_kv16_select(c._refs[layer], self._at[layer], self._qo[0], *args, n, budget, sink, recent, *to, address, size, st)
+        if rc:
+            raise sjk.SjkError(rc, "kv16_select")
+        return blocks, count
+
+    def attend(self, layer, q, lens, blocks, scale, rows=None, out=None, scratch=None):
+        """Attention of one new token per sequence over the listed pages (select's blocks, or others: int32 [n][KV
+        heads][any], ascending and then -1). Otherwise as Cache.attend. Returns out (q's type unless given)."""
+        n, dev, c = q.shape[0], self._dev, self.cache
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.attend(layer, q, lens, blocks, scale, rows, out, scratch)
+        if out is None:
+            out = torch.empty_like(q)
+        if blocks.dim() != 3:
+            raise ValueError("blocks: int32 [n][KV heads][budget]")
+        budget = blocks.shape[2]
+        lists = _matrix(blocks, "blocks", dev, (n, c.n_head_kv, budget))
+        with self._lock:
+            self._q.set(q, n, dev)
+            self._o.set(out, n, dev)
+            args = _list(lens, "lens", dev, n), _list(rows, "rows", dev, n)
+            if n == 0:
+                return out
+            st = _stream(dev)
+            _, address, size = self._attend.get(st, self._L.sjk_kv16_attend_blocks_scratch_bytes(c._refs[layer], q.shape[1], n, budget), scratch)
+            rc = self._L.sjk_kv16_attend_blocks(c._refs[layer], self._qo[0], *args, lists, n, budget, scale, self._qo[1], address, size, st)
+        if rc:
+            raise sjk.SjkError(rc, "kv16_attend_blocks")
+        return out
+
+
 class Qkv:
     """From a projection's heads to cache rows in one launch: RMS norm of the query and key heads (weights q_norm,
     k_norm; None: none), rotary positions, and the write of K and V into `cache` and / or into row tensors."""
@@ -321,10 +482,11 @@ class Qkv:
         # (the struct's own fields: setting them sets the struct's)
         self._rows = [_Rows(getattr(a, f), f, head_dim) for f in ("q", "k", "v", "q_out", "k_out", "v_out")]
 
-    def __call__(self, q=None, k=None, v=None, pos=None, q_out=None, k_out=None, v_out=None, layer=0, rows=None, to_cache=True):
+    def __call__(self, q=None, k=None, v=None, pos=None, q_out=None, k_out=None, v_out=None, layer=0, rows=None, to_cache=True, at=None):
         """q, k, v: [n][heads][D] (views of one projection's rows are fine); pos int32 [n], a negative one is padding;
         rows int32 [n]: table row of every token (None: token i is row i). K and V go to the cache's layer unless
-        to_cache is false; row outputs go where given (an input's own rows too)."""
+        to_cache is false; row outputs go where given (an input's own rows too). at int32 [n]: the tokens' cache positions
+        where they are others than the rotary ones (drafts on several branches); a negative one: not into the cache."""
         a = self._a
         some = q if q is not None else k if k is not None else v
         n, dev = some.shape[0], some.get_device()
@@ -336,12 +498,16 @@ class Qkv:
             a.n_tok = n
             a.pos = _list(pos, "pos", dev, n)
             a.rows = _list(rows, "rows", dev, n)
+            places = _list(at, "at", dev, n)
             if n == 0:                           # empty tensors have no address
                 return
-            at = layer if self.cache is not None and to_cache else None
-            if at != self._layer:
-                a.cache = self.cache.layers[at] if at is not None else sjk.Kv16()
-                self._layer = at
-            rc = _launch(dev, self._L.sjk_qkv, self._ref, _stream(dev))
+            il = layer if self.cache is not None and to_cache else None
+            if il != self._layer:
+                a.cache = self.cache.layers[il] if il is not None else sjk.Kv16()
+                self._layer = il
+            if at is None:
+                rc = _launch(dev, self._L.sjk_qkv, self._ref, _stream(dev))
+            else:
+                rc = _launch(dev, self._L.sjk_qkv_at, self._ref, places, _stream(dev))
         if rc:
             raise sjk.SjkError(rc, "qkv")

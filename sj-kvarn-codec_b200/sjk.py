@@ -104,6 +104,10 @@ class QkvArgs(C.Structure):
                 ("rope", RopeC), ("pos", vp), ("rows", vp), ("cache", Kv16)]
 
 
+class Kv16Step(C.Structure):
+    _fields_ = [(n, vp) for n in ("first", "row", "pos", "at", "slot")]
+
+
 class Slab(C.Structure):
     _fields_ = [("base", vp), ("page_bytes", C.c_size_t), ("layer_stride", C.c_size_t), ("n_layers", C.c_int)]
 
@@ -235,6 +239,14 @@ SIGNATURES = {
     "sjk_qkv": (C.c_int, [P(QkvArgs), vp]),
     "sjk_kv16_attend_scratch_bytes": (C.c_size_t, [P(Kv16), C.c_int]),
     "sjk_kv16_attend": (C.c_int, [P(Kv16), P(Rows), vp, vp, C.c_int, C.c_float, C.c_int, P(Rows), vp, C.c_size_t, vp]),
+    "sjk_qkv_at": (C.c_int, [P(QkvArgs), vp, vp]),
+    "sjk_kv16_maps": (C.c_int, [P(Kv16), vp, vp, vp, vp, C.c_int, C.c_int, P(Kv16Step), vp]),
+    "sjk_kv16_keep": (C.c_int, [P(Kv16), C.c_int, C.c_int64, vp, vp, vp, vp, C.c_int, C.c_int, vp, vp]),
+    "sjk_kv16_bounds": (C.c_int, [P(Kv16), C.c_int, C.c_int64, vp, C.c_int64, vp, vp, vp, C.c_int, vp]),
+    "sjk_kv16_select_scratch_bytes": (C.c_size_t, [P(Kv16), C.c_int]),
+    "sjk_kv16_select": (C.c_int, [P(Kv16), vp, P(Rows), vp, vp, C.c_int, C.c_int, C.c_int, C.c_int, vp, vp, vp, C.c_size_t, vp]),
+    "sjk_kv16_attend_blocks_scratch_bytes": (C.c_size_t, [P(Kv16), C.c_int, C.c_int, C.c_int]),
+    "sjk_kv16_attend_blocks": (C.c_int, [P(Kv16), P(Rows), vp, vp, vp, C.c_int, C.c_int, C.c_float, P(Rows), vp, C.c_size_t, vp]),
     "sjk_pages_bytes": (C.c_size_t, [u32]),
     "sjk_pages_init": (C.c_int, [P(PagesC), vp]),
     "sjk_pages_shares": (vp, [P(PagesC)]),
