@@ -650,6 +650,22 @@ typedef struct sjk_kv16_step {
 } sjk_kv16_step;
 int sjk_kv16_maps(const sjk_kv16 * c, const int32_t * len, const int32_t * add, const int32_t * rows, const uint64_t * masks,
                   int n_seq, int n_tok, const sjk_kv16_step * out, sjk_stream st);
+/* Attention of the new tokens: token t of q (n_tok rows), the j-th of sequence i, sees the committed positions [0, len[i])
+ * and those drafted ones, at len[i] + k, whose bit k masks[t] has (its own bit as any other; bits behind the sequence's
+ * tokens do not count; masks NULL: itself and the ones before it), of all these the last `window` (0: all). out[t] = sum
+ * of softmax(scale q . k) v over them, zeros where there are none. Tokens of sequence i: [first[i], first[i + 1]) (DEVICE
+ * [n_seq + 1]; NULL: `nodes` each), `nodes` of them at most, nodes <= SJK_TREE_MAX; rows of q in no sequence, or in one with
+ * more, are left as they were (the latter set SJK_DEVICE_PAGE). K and V of the new tokens lie in the cache already (sjk_qkv_at).
+ * Infinities and NaNs reach the tokens that see them alone. Positions on SJKVARN_NO_BLOCK pages are left out. q and out of the
+ * cache's type; q, K and V rows 16-byte aligned; head_dim 64, 96, 128 or 256; up to 148 x 64 rows (nodes x query heads of a
+ * KV head; SJK_ERR_UNSUPPORTED). Sums and statistics are 32-bit, weights sums of two 16-bit terms. scratch:
+ * sjk_kv16_attend_tree_scratch_bytes() bytes, 16-byte aligned, for whatever lengths; not shared by calls that overlap. Two
+ * launches; the same inputs give the same bits. */
+#define SJK_TREE_MAX 64
+size_t sjk_kv16_attend_tree_scratch_bytes(const sjk_kv16 * c);
+int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int n_tok, const int32_t * first, const int32_t * len,
+                         const int32_t * rows, const uint64_t * masks, int n_seq, int nodes, float scale, int window,
+                         const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st);
 /* Accepted drafts to their places: of sequence i the K and V rows of the positions len[i] + path[i][j], j < count[i], go to
  * len[i] + j in all n_layers layers (layer l's rows at c's plus l * layer_stride elements), and new_len[i] (DEVICE, may be
  * NULL, not over len) = len[i] + count[i]. path: DEVICE [n_seq][width], ascending; width <= SJK_KEEP_MAX. Where a path does

@@ -61,6 +61,7 @@ int sjk_kv16_status_take(void);
 int sjk_pages_status_take(void);
 int sjk_step_status_take(void);
 int sjk_blocks_status_take(void);
+int sjk_tree_status_take(void);               // SJK_DEVICE_TIMEOUT too
 // 0 where the fields of a 16-bit cache are possible ones (sjk_qkv.cu)
 int sjk_kv16_check(const sjk_kv16 * c);
 // sjk_kv16_attend over sequences that are one KV head each (sjk_kv16.cu): c has one KV head, n_seq = `fold` heads of

@@ -1,0 +1,847 @@
+// sjk_kv16_tree.cu - attention of several new tokens of every sequence, drafted as a tree or in a row, over a paged 16-bit
+// cache: out_j = sum over V(j) of softmax(scale q_j . k_t) v_t, V(j) = the last `window` of the committed positions [0, len)
+// and the drafted ones len + k whose bit k token j's mask has.
+//
+// All query heads of a KV head's group, of all the tokens of a sequence, are rows of one product: a key read once serves
+// (tokens x heads of a group) rows, up to NMAX = 64 in one pass, more in tiles of rows that CTAs side by side work on at the
+// same time, so that the second one's keys come from L2. Bound: HBM up to some 150 rows a KV head (4 D bytes per position
+// against 6 D flops per row and position here), the tensor cores and the shared memory that feeds them above that.
+//  - S^T = K Q^T with 128 positions as the M rows of tcgen05.mma and the query rows as its N columns (16 to 64), and
+//    O^T += V^T P with 128 channels as M: what a tile costs the softmax goes with the number of query rows, where query rows
+//    as M would make 8 of them as dear as 128. K, V and P lie in shared memory as they come: K rows are K-major for the
+//    first product, the same layout of V is MN-major for the second, and a thread, which has a position of all columns,
+//    writes its weights as whole 16-byte words of an MN-major P. S (two buffers) and O live in TMEM.
+//  - Warps: 8 for the softmax (two halves of the columns), 2 that load K, 2 that load V (rings of their own, so that neither
+//    waits for the other's slots), 1 that issues the products, 1 that loads the queries. Linked by mbarriers only; every
+//    wait is bounded.
+//  - Page tables are read a tile ahead, rows come with 16-byte cp.async into the swizzled layout: any page size, any strides;
+//    positions that are not live are filled with zeros.
+//  - The maximum of a row is looked for when a score is more than SLACK above the one in use (at a pair's start, seldom
+//    afterwards); then O is rescaled in TMEM. Weights reach 2^SLACK, which f16 and 32-bit sums have room for.
+//  - Weights enter as the sum of two 16-bit terms, as in sjk_kv16_attend: 2^-16 (bf16) or 2^-22 (f16) of a weight, and for
+//    f16, whose weights are held 2^10 larger, at most 2^-35 of the row's largest. Sums and statistics are 32-bit.
+//  - Positions that only some of the rows see (drafted ones, a window's edge) may hold infinities or NaNs, and 0 times
+//    those is no zero: such V rows are replaced by zeros and their non-finite values added to the rows that see them.
+// A list of (sequence, KV head) pairs in steps of 128 positions is cut into equal runs, one per CTA, for each tile of rows;
+// lengths are read from device memory. Split pairs leave (m, l, o) in the scratch and a second kernel joins them in order.
+#include "sjk_kv16.cuh"
+#include "sjk_internal.h"
+#include "sjk_tc.cuh"
+
+#include <math.h>
+
+namespace {
+
+using namespace sjk16;
+
+constexpr unsigned FULL = 0xFFFFFFFFu;
+constexpr int NMAX = 64;                    // query rows of a pass
+constexpr int TS = 128;                     // positions of a step
+constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
+constexpr int MIN_RUN = 2;                  // units of a run, at least
+constexpr int N_SOFT = 8, N_LOAD = 4;       // warps; then one that issues products, and one that loads queries
+constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
+constexpr int INFO = 4, TILES = 16;         // rings of what a pair's rows and a tile's positions are
+__device__ unsigned int g_tree_status;
+
+SJK_DEV void flag() { atomicOr(&g_tree_status, (unsigned) SJK_DEVICE_PAGE); }
+
+struct Params {
+    sjk_kv16 c;
+    sjk_rows q, out;
+    const int32_t * first, * len, * rows;
+    const uint64_t * masks;
+    int n_seq, n_tok, nodes, grp;
+    int window, page_shift;
+    int tiles, wl;                          // tiles of rows, and CTAs (runs) of each
+    float scale;
+    float * part;                           // [CTA][2][NMAX][D]
+    float * ml;                             // [CTA][2][NMAX][2]
+    int4 * split;                           // by CTA: sequence (-1: none), KV head, first and last run
+};
+
+// What a sequence is to a tile of rows: its committed length, tokens, positions [lo, hi) that some token sees, rows.
+struct Seq {
+    int len, count, first, row0, nr, step0, steps;
+    uint32_t hi;
+};
+SJK_DEV Seq seq_of(const Params & p, int i, int tile) {
+    Seq s = {0, 0, 0, 0, 0, 0, 0, 0u};
+    int64_t f0, f1;
+    if (p.first) { f0 = p.first[i]; f1 = p.first[i + 1]; }
+    else { f0 = (int64_t) i * p.nodes; f1 = f0 + p.nodes; }
+    if (f0 < 0 || f1 < f0 || f1 > p.n_tok || f1 - f0 > p.nodes) { flag(); return s; }
+    s.count = (int) (f1 - f0);
+    s.first = (int) f0;
+    const int rows = s.count * p.grp, tiles = (rows + NMAX - 1) / NMAX;
+    if (tile >= tiles) return s;
+    s.row0 = (int) ((int64_t) rows * tile / tiles);
+    s.nr = (int) ((int64_t) rows * (tile + 1) / tiles) - s.row0;
+    s.len = max(p.len[i], 0);
+    int64_t hi = (int64_t) s.len + s.count;
+    const int64_t cap = (int64_t) p.c.table_stride * p.c.page_tokens, most = cap < 0x7FFFFFFF ? cap : 0x7FFFFFFF;
+    if (hi > most) { flag(); hi = most; }
+    s.hi = (uint32_t) hi;
+    const int lo = p.window && s.len > p.window ? s.len - p.window : 0;
+    s.step0 = (int) ((uint32_t) min((int64_t) lo, hi - 1) / TS);
+    s.steps = (int) ((s.hi - 1u) / TS) + 1 - s.step0;
+    return s;
+}
+SJK_DEV uint32_t units_of(const Params & p, const Seq & s) { return s.steps > 0 ? (uint32_t) p.c.n_head_kv * (uint32_t) (s.steps + OV) : 0u; }
+
+// A run's place: pair (sequence, KV head), step, units left, unit of the list at which the pair begins.
+struct Cursor {
+    int seq, h, st, rem;
+    uint32_t base;
+    Seq s;
+    // the pair's steps of this run
+    SJK_DEV int take() const { const int left = s.steps - st; return left < rem ? left : rem; }
+    SJK_DEV void next(const Params & p, int tile, int taken) {
+        rem -= taken;
+        st += taken;
+        if (st < s.steps) return;
+        st = 0;
+        rem -= OV;
+        base += (uint32_t) (s.steps + OV);
+        if (rem <= 0) return;
+        if (++h < p.c.n_head_kv) return;
+        h = 0;
+        do { s = seq_of(p, ++seq, tile); } while (s.steps <= 0);
+    }
+};
+
+// What row n of a pair is.
+struct Info {
+    uint64_t mask[NMAX];                    // drafted tokens that it sees
+    int64_t out[NMAX];                      // its place in the output
+    int lo[NMAX];                           // first committed position that it sees
+};
+
+template <int TYPE_, int D_>
+struct Shape {
+    static constexpr int TYPE = TYPE_, D = D_;
+    static constexpr int NB = (D + 63) / 64, HALVES = (D + 127) / 128, CH = D / 8;  // 64-channel blocks, M tiles of O, words of a row
+    static constexpr int TILE = NB * TS * 128, QB = NB * NMAX * 128, PB = TS * 128;  // bytes of a K or V tile, Q, a term of P
+    // slots of K and of V: what 227 KB hold beside Q and P
+    static constexpr int KS = D == 64 ? 4 : D == 256 ? 1 : 3, VS = D == 64 ? 4 : D == 256 ? 1 : 2;
+    static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX;
+    static constexpr float SLACK = TYPE == SJK_F16 ? 5.0f : 8.0f, UP = TYPE == SJK_F16 ? 10.0f : 0.0f;
+};
+
+template <typename S>
+struct Shared {
+    uint8_t k[S::KS * S::TILE], v[S::VS * S::TILE], q[S::QB], pt[2][S::PB];
+    Info info[INFO];
+    uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
+    uint64_t odd[TILES][2];                 // positions whose V row was replaced, of tiles that some rows see only partly
+    float m[NMAX], fac[NMAX], red[N_SOFT][32];
+    uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS];
+    uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
+    Cursor start;
+    uint32_t per, list, tmem;
+};
+
+// ---- products -----------------------------------------------------------------------------------------------------
+// rows of 64 16-bit elements in 128 bytes, 16-byte words swizzled by the row (128-byte swizzle), 8 rows in 1,024 bytes;
+// lbo: from one 64-element block to the next where the elements side by side are M or N
+SJK_DEV uint64_t swizzled(uint32_t addr, uint32_t lbo) {
+    return (uint64_t) ((addr >> 4) & 0x3FFFu) | ((uint64_t) ((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t) (1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// f16 or bf16 operands, 32-bit accumulators, M 128; mn: both operands with M or N side by side in memory
+template <int TYPE>
+SJK_DEV uint32_t idesc(int n, bool mn) {
+    const uint32_t t = TYPE == SJK_BF16 ? 1u : 0u;
+    return (1u << 4) | (t << 7) | (t << 10) | (mn ? 3u << 15 : 0u) | ((uint32_t) (n >> 3) << 17) | (8u << 24);
+}
+SJK_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u));
+}
+SJK_DEV void ld8(uint32_t t, float * v) {
+    uint32_t r[8];
+    tc::ld_x8_u(t, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+SJK_DEV bool any_of(int id, bool x) {       // over the 128 threads of a half
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+                 : "=r"(r) : "r"((uint32_t) x), "r"(id), "r"(128) : "memory");
+    return r != 0;
+}
+// 32 columns of a lane over the warp's lanes: lane c gets column c
+template <bool MAX>
+SJK_DEV float columns32(const float (&v)[32], int lane) {
+    float a[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const bool up = lane & 16;
+        const float send = up ? v[i] : v[i + 16], keep = up ? v[i + 16] : v[i], r = __shfl_xor_sync(FULL, send, 16);
+        a[i] = MAX ? fmaxf(keep, r) : keep + r;
+    }
+#pragma unroll
+    for (int o = 8; o; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < o; ++i) {
+            const bool up = lane & o;
+            const float send = up ? a[i] : a[i + o], keep = up ? a[i + o] : a[i], r = __shfl_xor_sync(FULL, send, o);
+            a[i] = MAX ? fmaxf(keep, r) : keep + r;
+        }
+    return a[0];
+}
+template <int TYPE>
+SJK_DEV bool odd_word(uint32_t w) {         // an infinity or NaN among two
+    constexpr uint32_t E = TYPE == SJK_F16 ? 0x7C00u : 0x7F80u;
+    return (w & E) == E || (w & (E << 16)) == (E << 16);
+}
+
+// Waits that give up once and for all: after one that ran out (the status word says so) a role goes on without waiting, so
+// that everyone meets the same barriers and the CTA ends.
+struct Waiter {
+    bool dead = false;
+    SJK_DEV void operator()(uint64_t * bar, uint32_t parity) {
+        if (!dead && !tc::mbar_wait(bar, parity)) dead = true;
+    }
+    SJK_DEV void warp(uint64_t * bar, uint32_t parity) {    // by a whole warp
+        (*this)(bar, parity);
+        __syncwarp();
+    }
+};
+
+template <typename S>
+__global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
+    constexpr int D = S::D, KS = S::KS, VS = S::VS;
+    extern __shared__ uint8_t raw[];
+    Shared<S> & sm = *reinterpret_cast<Shared<S> *>(raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tile = blockIdx.x % p.tiles, run = blockIdx.x / p.tiles;
+
+    if (tid == 0) {
+        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 2); tc::mbar_init(&sm.k_empty[i], 1); }
+        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 2); tc::mbar_init(&sm.v_empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&sm.s_full[i], 1); tc::mbar_init(&sm.s_empty[i], N_SOFT); }
+        tc::mbar_init(&sm.p_full, N_SOFT);
+        tc::mbar_init(&sm.pv_done, 1);
+        tc::mbar_init(&sm.o_free, N_SOFT);
+        for (int i = 0; i < INFO; ++i) tc::mbar_init(&sm.q_full[i], 1);
+        tc::mbar_init(&sm.q_empty, 1);
+        tc::mbar_fence_init();
+    }
+    if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, 256); tc::tmem_relinquish(); }
+    pdl_wait();
+    pdl_release();
+    // where the run begins: units of all sequences, a block of them per lane
+    if (warp == 0) {
+        const int block = (p.n_seq + 31) / 32;
+        uint32_t mine = 0;
+        for (int i = 0; i < block; ++i)
+            if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile));
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(FULL, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const uint32_t list = __shfl_sync(FULL, incl, 31);
+        uint32_t per = (list + (uint32_t) p.wl - 1u) / (uint32_t) p.wl;
+        if (per < MIN_RUN) per = MIN_RUN;
+        const int64_t o = (int64_t) run * per;
+        Cursor c = {};
+        if (o < list) {
+            const uint32_t off = (uint32_t) o;
+            c.rem = (int) (o + per < list ? per : list - off);
+            const int g = __ffs(__ballot_sync(FULL, incl > off)) - 1;
+            c.base = __shfl_sync(FULL, incl - mine, g);
+            c.seq = g * block;
+            for (;; ++c.seq) {              // (the block's last sequence at the latest: its sum is above off)
+                c.s = seq_of(p, c.seq, tile);
+                const uint32_t u = units_of(p, c.s);
+                if (c.base + u > off) break;
+                c.base += u;
+            }
+            c.h = (int) ((off - c.base) / (uint32_t) (c.s.steps + OV));
+            c.base += (uint32_t) c.h * (uint32_t) (c.s.steps + OV);
+            const int in = (int) (off - c.base);
+            c.st = in > OV ? in - OV : 0;
+            if (in < OV) c.rem -= OV - in;  // no steps where the run has only units before a first step
+        }
+        if (lane == 0) {
+            sm.start = c;
+            sm.per = per;
+            sm.list = list;
+            p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    tc::fence_after_sync();
+    const uint32_t tmem = sm.tmem;
+    Cursor at = sm.start;
+    Waiter wait;
+
+    if (warp < N_SOFT) {
+        // ---- softmax: position 32 (warp % 4) + lane of a tile, columns [half nc, half nc + nc) ----
+        const int half = warp >> 2, quarter = warp & 3, bar = 1 + half, tl = quarter * 32 + lane;
+        const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
+        const float sc = p.scale * 1.4426950408889634f;
+        float l[32];
+        uint32_t jj = 0;                    // tiles so far
+        for (int item = 0; at.rem > 0; ++item) {
+            const Seq s = at.s;
+            const int steps = at.take(), h = at.h, nc = ((s.nr + 15) & ~15) / 2, c0 = half * nc;
+            const bool begun = at.st == 0, ended = at.st + steps == s.steps;
+            const Info & info = sm.info[item % INFO];
+            wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
+            if (tid % 128 < nc) sm.m[c0 + tid % 128] = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) l[c] = 0.0f;
+            tc::nbar_sync(bar, 128);
+            const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
+            auto partly = [&](int step) {   // some rows see a position of the step that others do not
+                const uint32_t t0 = (uint32_t) step * TS;
+                return t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
+            };
+            // non-finite values of V rows that only some rows see, into the sums of those that do
+            auto add_odd = [&](uint32_t tile_no, int step) {
+                uint64_t some[2] = {sm.odd[tile_no % TILES][0], sm.odd[tile_no % TILES][1]};
+                if (!(some[0] | some[1])) return;
+                const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
+                if (row < 0 || row >= (int64_t) p.c.n_rows) return;
+                const uint32_t * table = p.c.tables + row * p.c.table_stride;
+#pragma unroll 1
+                for (int hf = 0; hf < S::HALVES; ++hf) {
+                    const int d = hf * 128 + tl;
+#pragma unroll 1
+                    for (int c = 0; c < nc; c += 8) {
+                        float o[8];
+                        const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + c);
+                        ld8(addr, o);
+                        tc::wait_ld();
+#pragma unroll 1
+                        for (int w = 0; w < 2; ++w)
+#pragma unroll 1
+                            for (uint64_t b = some[w]; b; b &= b - 1) {
+                                const uint32_t t = (uint32_t) step * TS + 64u * w + (uint32_t) __ffsll((long long) b) - 1u, g = t / (uint32_t) p.c.page_tokens;
+                                const uint32_t page = table[g];
+                                if (page >= p.c.n_pages || d >= D) continue;
+                                const float x = load1(p.c.v, (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride +
+                                                      (int64_t) h * p.c.head_stride + d, S::TYPE);
+                                if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const int n = c0 + c + e;
+                                    const bool sees = t >= (uint32_t) s.len ? (info.mask[n] >> (t - (uint32_t) s.len)) & 1ull : t >= (uint32_t) info.lo[n];
+                                    if (sees) o[e] += x;
+                                }
+                            }
+                        uint32_t r[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e]);
+                        __syncwarp();
+                        tc::st_x8(addr, r);
+                    }
+                }
+                tc::wait_st();
+            };
+            for (int i = 0; i < steps; ++i, ++jj) {
+                const int b = jj & 1, step = s.step0 + at.st + i;
+                wait.warp(&sm.s_full[b], (jj >> 1) & 1u);
+                tc::fence_after_sync();
+                float x[32];
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q * 8 < nc) ld8(tmem + lanes + S::COL_S + (uint32_t) (b * NMAX + c0 + q * 8), x + q * 8);
+                tc::wait_ld();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sm.s_empty[b]);
+                const bool on = (sm.live[jj % TILES][quarter] >> lane) & 1u;
+                if (!on) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[c] = -INFINITY;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) x[c] = c < nc ? x[c] * sc : -INFINITY;
+                    if (partly(step)) {
+                        const uint32_t t = (uint32_t) step * TS + (uint32_t) tl;
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (c < nc) {
+                                const bool sees = t >= (uint32_t) s.len ? (info.mask[c0 + c] >> (t - (uint32_t) s.len)) & 1ull : t >= (uint32_t) info.lo[c0 + c];
+                                if (!sees) x[c] = -INFINITY;
+                            }
+                    }
+                }
+                // scores to differences from the row's maximum in use; a new one where some is too far above
+                bool above = false;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (q * 4 < nc) {
+                        const float4 m = *reinterpret_cast<const float4 *>(&sm.m[c0 + q * 4]);
+                        above |= x[4 * q] > m.x + S::SLACK || x[4 * q + 1] > m.y + S::SLACK || x[4 * q + 2] > m.z + S::SLACK || x[4 * q + 3] > m.w + S::SLACK;
+                    }
+                bool waited = false;
+                __syncwarp();
+                if (any_of(bar, above)) {
+                    const float top = columns32<true>(x, lane);
+                    sm.red[warp][lane] = top;
+                    tc::nbar_sync(bar, 128);
+                    if (tid % 128 < nc) {
+                        const int c = tid % 128;
+                        const float old = sm.m[c0 + c];
+                        float m = old;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm.red[half * 4 + w][c]);
+                        sm.fac[c0 + c] = m == old ? 1.0f : tc::num::ex2(old - m);
+                        sm.m[c0 + c] = m;
+                    }
+                    tc::nbar_sync(bar, 128);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (c < nc) l[c] *= sm.fac[c0 + c];
+                    if (i > 0) {            // O has tiles of this pair
+                        wait.warp(&sm.pv_done, (jj - 1) & 1u);
+                        waited = true;
+                        tc::fence_after_sync();
+#pragma unroll 1
+                        for (int hf = 0; hf < S::HALVES; ++hf)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                if (q * 8 < nc) {
+                                    const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + q * 8);
+                                    float o[8];
+                                    ld8(addr, o);
+                                    tc::wait_ld();
+                                    uint32_t r[8];
+#pragma unroll
+                                    for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[c0 + q * 8 + e]);
+                                    tc::st_x8(addr, r);
+                                }
+                        tc::wait_st();
+                    }
+                }
+                if (jj > 0 && !waited) {    // P is free
+                    wait.warp(&sm.pv_done, (jj - 1) & 1u);
+                    tc::fence_after_sync();
+                }
+                if (i > 0 && partly(step - 1)) add_odd(jj - 1, step - 1);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q * 8 < nc) {
+                        uint32_t hi[4], lw[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int c = q * 8 + 2 * e;
+                            const float2 m = *reinterpret_cast<const float2 *>(&sm.m[c0 + c]);
+                            const float a = tc::num::ex2(x[c] - (m.x == -INFINITY ? 0.0f : m.x) + S::UP), y = tc::num::ex2(x[c + 1] - (m.y == -INFINITY ? 0.0f : m.y) + S::UP);
+                            l[c] += a;
+                            l[c + 1] += y;
+                            hi[e] = pack2<S::TYPE>(a, y);
+                            const float2 f = widen2<S::TYPE>(hi[e]);
+                            lw[e] = pack2<S::TYPE>(a - f.x, y - f.y);
+                        }
+                        const uint32_t off = (uint32_t) tl * 128u + ((uint32_t) ((((c0 >> 3) + q) ^ tl) & 7) << 4);
+                        *reinterpret_cast<uint4 *>(&sm.pt[0][off]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(&sm.pt[1][off]) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                    }
+                tc::fence_proxy_async();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sm.p_full);
+            }
+            // the pair's output, or its partial
+            const float sum = columns32<false>(l, lane);
+            sm.red[warp][lane] = sum;
+            wait.warp(&sm.pv_done, (jj - 1) & 1u);
+            tc::fence_after_sync();
+            if (partly(s.step0 + at.st + steps - 1)) add_odd(jj - 1, s.step0 + at.st + steps - 1);
+            tc::nbar_sync(bar, 128);
+            const bool whole = begun && ended;
+            const int64_t slot = ((int64_t) blockIdx.x * 2 + (begun ? 1 : 0)) * NMAX;
+            if (tid % 128 < nc) {
+                const int c = tid % 128;
+                const float all = (sm.red[half * 4][c] + sm.red[half * 4 + 1][c]) + (sm.red[half * 4 + 2][c] + sm.red[half * 4 + 3][c]);
+                sm.fac[c0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
+                if (!whole) *reinterpret_cast<float2 *>(p.ml + (slot + c0 + c) * 2) = make_float2(sm.m[c0 + c], all);
+            }
+            if (tid == 0 && begun && !ended)
+                p.split[blockIdx.x] = make_int4(at.seq, h, run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
+            tc::nbar_sync(bar, 128);
+#pragma unroll 1
+            for (int hf = 0; hf < S::HALVES; ++hf) {
+                const int d = hf * 128 + tl;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (q * 8 < nc) {
+                        float o[8];
+                        ld8(tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + q * 8), o);
+                        tc::wait_ld();
+                        if (d < D) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const int n = c0 + q * 8 + e;
+                                if (n >= s.nr) continue;
+                                if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[n]);
+                                else p.part[(slot + n) * D + d] = o[e];
+                            }
+                        }
+                    }
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.o_free);
+            tc::nbar_sync(bar, 128);        // the factors have been read
+            at.next(p, tile, steps);
+        }
+    } else if (warp < W_MMA) {
+        // ---- K (two warps, 64 positions each) and V (two) ----
+        const bool is_v = warp >= N_SOFT + 2;
+        const int wh = (warp - N_SOFT) & 1, slots = is_v ? VS : KS;
+        uint64_t * full = is_v ? sm.v_full : sm.k_full, * empty = is_v ? sm.v_empty : sm.k_empty;
+        uint8_t * ring = is_v ? sm.v : sm.k;
+        uint32_t jj = 0, told = 0;          // tiles asked for, and announced
+        auto tell = [&](uint32_t upto) {    // copies of the tiles before `upto` have landed
+            tc::fence_proxy_async();
+            __syncwarp();
+            for (; told < upto; ++told)
+                if (lane == 0) tc::mbar_arrive(&full[told % slots]);
+        };
+        while (at.rem > 0) {
+            const Seq s = at.s;
+            const int steps = at.take();
+            const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
+            const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
+            if (!table && lane == 0) flag();
+            const uint16_t * base = static_cast<const uint16_t *>(is_v ? p.c.v : p.c.k) + (int64_t) at.h * p.c.head_stride;
+            const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
+            for (int i = 0; i < steps; ++i, ++jj) {
+                const int step = s.step0 + at.st + i;
+                int64_t off[2];             // rows of the lane's two positions; -1: none
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint32_t t = (uint32_t) step * TS + (uint32_t) (64 * wh + 32 * u + lane);
+                    off[u] = -1;
+                    if (table && t < s.hi && t >= (uint32_t) lo0) {
+                        const uint32_t g = p.page_shift >= 0 ? t >> p.page_shift : t / (uint32_t) p.c.page_tokens, page = table[g];
+                        if (page < p.c.n_pages) off[u] = (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride;
+                        else if (page != SJKVARN_NO_BLOCK) flag();
+                    }
+                }
+                const int slot = (int) (jj % (uint32_t) slots);
+                if (jj >= (uint32_t) slots) {
+                    const uint32_t parity = (jj / (uint32_t) slots - 1u) & 1u;
+                    if (!wait.dead && !tc::mbar_test(&empty[slot], parity)) {
+                        tc::cp_async_wait_group<0>();       // nothing more to ask for now: announce what has been
+                        tell(jj);
+                        wait.warp(&empty[slot], parity);
+                    }
+                    __syncwarp();
+                }
+                uint8_t * dst = ring + slot * S::TILE + 64 * wh * 128;
+                unsigned live[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    live[u] = __ballot_sync(FULL, off[u] >= 0);
+                    if (!is_v && lane == 0) sm.live[jj % TILES][2 * wh + u] = live[u];
+#pragma unroll 4
+                    for (int k = 0; k < S::CH; ++k) {
+                        const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
+                        const int64_t o = __shfl_sync(FULL, off[u], r);
+                        tc::cp_async16(dst + (c >> 3) * (TS * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
+                    }
+                }
+                tc::cp_async_commit();
+                // V rows that only some rows see: drafted ones, and a window's edge
+                if (is_v) {
+                    const uint32_t t0 = (uint32_t) step * TS;
+                    if (t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u)) {
+                        tc::cp_async_wait_group<0>();
+                        __syncwarp();
+                        uint64_t odd = 0ull;
+                        for (int r = 0; r < 64; ++r) {
+                            const uint32_t t = t0 + (uint32_t) (64 * wh + r);
+                            if (!((live[r >> 5] >> (r & 31)) & 1u) || !(t >= (uint32_t) s.len || (p.window && t < (uint32_t) lo0 + 64u))) continue;
+                            bool bad = false;
+                            uint4 * at16 = nullptr;
+                            if (lane < S::CH) {
+                                at16 = reinterpret_cast<uint4 *>(dst + (lane >> 3) * (TS * 128) + r * 128 + (((lane ^ r) & 7) << 4));
+                                const uint4 x = *at16;
+                                bad = odd_word<S::TYPE>(x.x) || odd_word<S::TYPE>(x.y) || odd_word<S::TYPE>(x.z) || odd_word<S::TYPE>(x.w);
+                            }
+                            if (__any_sync(FULL, bad)) {
+                                odd |= 1ull << r;
+                                if (bad) {  // its finite neighbours stay
+                                    uint32_t * w = reinterpret_cast<uint32_t *>(at16);
+#pragma unroll 1
+                                    for (int e = 0; e < 4; ++e) {
+                                        const float2 f = widen2<S::TYPE>(w[e]);
+                                        if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
+                                        if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
+                                    }
+                                }
+                            }
+                        }
+                        if (lane == 0) sm.odd[jj % TILES][wh] = odd;
+                        tell(jj + 1);
+                        continue;
+                    }
+                }
+                if (slots == 1) tc::cp_async_wait_group<0>();
+                else if (slots == 2) tc::cp_async_wait_group<1>();
+                else if (slots == 3) tc::cp_async_wait_group<2>();
+                else tc::cp_async_wait_group<3>();
+                if (jj + 2 > (uint32_t) slots) tell(jj + 2 - (uint32_t) slots);
+            }
+            at.next(p, tile, steps);
+        }
+        tc::cp_async_wait_group<0>();
+        tell(jj);
+    } else if (warp == W_MMA) {
+        // ---- products ----
+        if (lane == 0) {
+            const uint32_t ka = tc::smem_addr(sm.k), va = tc::smem_addr(sm.v), qa = tc::smem_addr(sm.q), pa = tc::smem_addr(sm.pt);
+            uint32_t jj = 0;
+            int pend_n = 0, pend_first = 0, items = 0;       // a tile whose second product is to come
+            auto second = [&](uint32_t j) {                  // O^T += V^T P of tile j
+                if (pend_first && items > 1) wait(&sm.o_free, (uint32_t) (items - 2) & 1u);
+                const uint32_t slot = j % VS;
+                wait(&sm.v_full[slot], (j / VS) & 1u);
+                wait(&sm.p_full, j & 1u);
+                tc::fence_after_sync();
+                if (!wait.dead) {
+                    const uint32_t id = idesc<S::TYPE>(pend_n, true);
+#pragma unroll 1
+                    for (int hf = 0; hf < S::HALVES; ++hf)
+#pragma unroll 1
+                        for (int term = 0; term < 2; ++term)
+#pragma unroll
+                            for (int k = 0; k < TS / 16; ++k)
+                                mma_ss(tmem + S::COL_O + (uint32_t) (hf * NMAX), swizzled(va + slot * S::TILE + hf * 2 * TS * 128 + k * 2048, D == 64 ? 0u : TS * 128u),
+                                       swizzled(pa + term * S::PB + k * 2048, TS * 128u), id, pend_first && term == 0 && k == 0 ? 0u : 1u);
+                    tc::mma_commit(&sm.v_empty[slot]);
+                    tc::mma_commit(&sm.pv_done);
+                }
+            };
+            bool pend = false;
+            for (; at.rem > 0; ) {
+                const int steps = at.take(), n = (at.s.nr + 15) & ~15;
+                const uint32_t id = idesc<S::TYPE>(n, false);
+                if (pend) second(jj - 1);   // the pair's end does not wait for the next one's queries
+                pend = false;
+                wait(&sm.q_full[items % INFO], (uint32_t) (items / INFO) & 1u);
+                for (int i = 0; i < steps; ++i, ++jj) {
+                    const uint32_t slot = jj % KS, b = jj & 1u;
+                    wait(&sm.k_full[slot], (jj / KS) & 1u);
+                    if (jj >= 2) wait(&sm.s_empty[b], ((jj >> 1) - 1u) & 1u);
+                    tc::fence_after_sync();
+                    if (!wait.dead) {
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+                            mma_ss(tmem + S::COL_S + b * NMAX, swizzled(ka + slot * S::TILE + (k >> 2) * TS * 128 + (k & 3) * 32, 16u),
+                                   swizzled(qa + (k >> 2) * NMAX * 128 + (k & 3) * 32, 16u), id, k ? 1u : 0u);
+                        tc::mma_commit(&sm.k_empty[slot]);
+                        if (i + 1 == steps) tc::mma_commit(&sm.q_empty);
+                        tc::mma_commit(&sm.s_full[b]);
+                    }
+                    if (pend) second(jj - 1);
+                    pend = true;
+                    pend_n = n;
+                    pend_first = i == 0;
+                    if (i == 0) ++items;
+                }
+                at.next(p, tile, steps);
+            }
+            if (pend) second(jj - 1);
+        }
+        __syncwarp();
+    } else {
+        // ---- queries, and what the rows see ----
+        for (int item = 0; at.rem > 0; ++item) {
+            const Seq s = at.s;
+            const int steps = at.take(), n = (s.nr + 15) & ~15;
+            if (item > 0) wait.warp(&sm.q_empty, (uint32_t) (item - 1) & 1u);
+            Info & info = sm.info[item % INFO];
+            int64_t from[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = 32 * u + lane;
+                from[u] = -1;
+                if (r >= n) continue;
+                uint64_t mask = 0ull;
+                int lo = 0x7FFFFFFF;
+                if (r < s.nr) {
+                    const int j = (s.row0 + r) / p.grp, g = (s.row0 + r) - j * p.grp, head = at.h * p.grp + g;
+                    mask = p.masks ? p.masks[s.first + j] : (2ull << j) - 1ull;
+                    if (s.count < 64) mask &= (1ull << s.count) - 1ull;
+                    lo = 0;
+                    if (p.window) {         // the last `window` of the committed and the drafted ones
+                        int drop = __popcll(mask) - p.window;
+                        for (; drop > 0; --drop) mask &= mask - 1ull;
+                        const int keep = p.window - __popcll(mask);
+                        lo = s.len > keep ? s.len - keep : 0;
+                    }
+                    from[u] = (int64_t) (s.first + j) * p.q.row_stride + (int64_t) head * p.q.head_stride;
+                    info.out[r] = (int64_t) (s.first + j) * p.out.row_stride + (int64_t) head * p.out.head_stride;
+                }
+                info.mask[r] = mask;
+                info.lo[r] = lo;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (32 * u < n)
+#pragma unroll 4
+                    for (int k = 0; k < S::CH; ++k) {
+                        const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
+                        const int64_t o = __shfl_sync(FULL, from[u], r);
+                        tc::cp_async16(sm.q + (c >> 3) * (NMAX * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4),
+                                       static_cast<const uint16_t *>(p.q.p) + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
+                    }
+            tc::cp_async_wait_all();
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&sm.q_full[item % INFO]);
+            at.next(p, tile, steps);
+        }
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == W_MMA) tc::tmem_dealloc(tmem, 256);
+}
+
+// Joins the runs of a split pair in order. grid: CTAs of the kernel before, rows in groups of 8, a warp each.
+template <int D>
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Params p, int type) {
+    constexpr int NV = (D / 4 + 31) / 32;   // 16-byte words of a lane
+    pdl_wait();
+    pdl_release();
+    const int4 e = p.split[blockIdx.x];
+    if (e.x < 0) return;
+    const int tile = blockIdx.x % p.tiles, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const Seq s = seq_of(p, e.x, tile);
+    if (r >= s.nr) return;
+    auto slot_of = [&](int w) { return (((int64_t) w * p.tiles + tile) * 2 + (w == e.z ? 1 : 0)) * NMAX + r; };
+    float top = -INFINITY, sum = 0.0f;
+    for (int w0 = e.z; w0 <= e.w; w0 += 32) {
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (w0 + lane <= e.w) ml = *reinterpret_cast<const float2 *>(p.ml + slot_of(w0 + lane) * 2);
+        float t = ml.x;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) t = fmaxf(t, __shfl_xor_sync(FULL, t, x));
+        t = fmaxf(t, top);
+        const float use = t == -INFINITY ? 0.0f : t;
+        sum = sum * tc::num::ex2(top - use) + ml.y * tc::num::ex2(ml.x - use);
+        top = t;
+    }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(FULL, sum, x);
+    const float use = top == -INFINITY ? 0.0f : top, inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    float4 o[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) o[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int w = e.z; w <= e.w; ++w) {
+        const int64_t at = slot_of(w);
+        const float f = tc::num::ex2(p.ml[at * 2] - use);
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            if (32 * v + lane < D / 4) {
+                const float4 x = reinterpret_cast<const float4 *>(p.part + at * D)[32 * v + lane];
+                o[v].x = fmaf(x.x, f, o[v].x); o[v].y = fmaf(x.y, f, o[v].y);
+                o[v].z = fmaf(x.z, f, o[v].z); o[v].w = fmaf(x.w, f, o[v].w);
+            }
+    }
+    const int j = (s.row0 + r) / p.grp, head = e.y * p.grp + (s.row0 + r) - j * p.grp;
+    const int64_t dst = (int64_t) (s.first + j) * p.out.row_stride + (int64_t) head * p.out.head_stride;
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+        if (32 * v + lane < D / 4) {
+            const int d = 4 * (32 * v + lane);
+            store1(p.out.p, dst + d, type, o[v].x * inv);
+            store1(p.out.p, dst + d + 1, type, o[v].y * inv);
+            store1(p.out.p, dst + d + 2, type, o[v].z * inv);
+            store1(p.out.p, dst + d + 3, type, o[v].w * inv);
+        }
+}
+
+template <typename S>
+int run(const Params & p, sjk_stream st) {
+    constexpr size_t bytes = sizeof(Shared<S>) + 1024;
+    static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
+    if (smem_limit<tree_kernel<S>>(bytes)) return SJK_ERR_DEVICE;
+    const int ctas = p.tiles * p.wl;
+    const int rc = launch(tree_kernel<S>, dim3((unsigned) ctas), dim3(NT), bytes, st, p);
+    if (rc) return rc;
+    const int rows = p.nodes * p.grp < NMAX ? p.nodes * p.grp : NMAX;
+    return launch(tree_merge_kernel<S::D>, dim3((unsigned) ctas, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE);
+}
+
+template <int TYPE>
+int run_dim(const Params & p, sjk_stream st) {
+    switch (p.c.head_dim) {
+        case 64: return run<Shape<TYPE, 64>>(p, st);
+        case 96: return run<Shape<TYPE, 96>>(p, st);
+        case 128: return run<Shape<TYPE, 128>>(p, st);
+        default: return run<Shape<TYPE, 256>>(p, st);
+    }
+}
+
+constexpr int CTAS = 148;
+
+}  // namespace
+
+extern "C" size_t sjk_kv16_attend_tree_scratch_bytes(const sjk_kv16 * c) {
+    if (!c || (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)) return 0;
+    return (size_t) CTAS * (2 * NMAX * ((size_t) c->head_dim + 2) * sizeof(float) + sizeof(int4));
+}
+
+extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int n_tok, const int32_t * first, const int32_t * len,
+                                    const int32_t * rows, const uint64_t * masks, int n_seq, int nodes, float scale, int window,
+                                    const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st) {
+    if (!c || !q || !out || sjk_kv16_check(c) || n_seq < 0 || n_tok < 0 || nodes < 0 || window < 0 || !isfinite(scale)) return SJKVARN_ERR_ARG;
+    if (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256) return SJK_ERR_UNSUPPORTED;
+    if (nodes > SJK_TREE_MAX) return SJK_ERR_UNSUPPORTED;
+    if (q->type != c->type || out->type != c->type || q->n_head < 1 || q->n_head != out->n_head || q->n_head % c->n_head_kv) return SJKVARN_ERR_ARG;
+    if (!list_ok(first) || !list_ok(len) || !list_ok(rows) || !aligned(masks, 8) || !rows_ok(*out) || (n_seq && !len)) return SJKVARN_ERR_ARG;
+    if (n_tok && (!q->p || !out->p)) return SJKVARN_ERR_ARG;
+    const int64_t strides = c->page_stride | c->slot_stride | c->head_stride | q->row_stride | q->head_stride;
+    if (!aligned(c->k, 16) || !aligned(c->v, 16) || !aligned(q->p, 16) || (strides & 7)) return SJKVARN_ERR_ARG;
+    if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
+    if (!first && (int64_t) n_seq * nodes != (int64_t) n_tok) return SJKVARN_ERR_ARG;
+    const int grp = q->n_head / c->n_head_kv;
+    const int64_t tiles = ((int64_t) nodes * grp + NMAX - 1) / NMAX;
+    if (tiles > CTAS) return SJK_ERR_UNSUPPORTED;
+    // a list counts its units in 32 bits
+    const double steps = fmin((double) c->table_stride * c->page_tokens, 2147483647.0) / TS + OV + 2;
+    if (steps * n_seq * c->n_head_kv > 2e9) return SJK_ERR_UNSUPPORTED;
+    if (n_seq == 0 || n_tok == 0 || nodes == 0) return 0;
+    if (!scratch || !aligned(scratch, 16) || scratch_bytes < sjk_kv16_attend_tree_scratch_bytes(c)) return SJKVARN_ERR_BUFFER;
+    Params p = {};
+    p.c = *c; p.q = *q; p.out = *out;
+    p.first = first; p.len = len; p.rows = rows; p.masks = masks;
+    p.n_seq = n_seq; p.n_tok = n_tok; p.nodes = nodes; p.grp = grp;
+    p.window = window; p.scale = scale;
+    p.page_shift = -1;
+    for (int b = 0; b < 31; ++b)
+        if (c->page_tokens == 1 << b) p.page_shift = b;
+    p.tiles = (int) tiles;
+    p.wl = CTAS / p.tiles;
+    p.part = static_cast<float *>(scratch);
+    p.ml = p.part + (size_t) CTAS * 2 * NMAX * c->head_dim;
+    p.split = reinterpret_cast<int4 *>(p.ml + (size_t) CTAS * 2 * NMAX * 2);
+    return c->type == SJK_F16 ? run_dim<SJK_F16>(p, st) : run_dim<SJK_BF16>(p, st);
+}
+
+SJK_STATUS_READER(tree_wait_status_take)
+
+int sjk_tree_status_take(void) {
+    unsigned v = 0;
+    if (sjk_check(cudaMemcpyFromSymbol(&v, g_tree_status, sizeof v))) return -1;
+    if (v) {
+        const unsigned z = 0;
+        if (sjk_check(cudaMemcpyToSymbol(g_tree_status, &z, sizeof z))) return -1;
+    }
+    const int t = tree_wait_status_take();
+    return t < 0 ? -1 : (int) v | t;
+}

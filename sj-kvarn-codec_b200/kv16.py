@@ -262,6 +262,7 @@ class Cache:
         self._dev, self._L = k.get_device(), _lib()
         self._lock = threading.Lock()
         self._scratch = {}                       # by stream and number of query heads: calls of one stream follow one another
+        self._tree = _Scratch(self._dev)
 
     @classmethod
     def alloc(cls, n_layers, n_pages, page_tokens, n_head_kv, head_dim, dtype, n_rows, stride, device="cuda"):
@@ -323,6 +324,42 @@ class Cache:
             raise sjk.SjkError(rc, "kv16_attend")
         return out
 
+
+    def attend_tree(self, layer, q, lens, masks, scale, first=None, nodes=None, rows=None, window=0, out=None, scratch=None):
+        """Attention of several new tokens of every sequence, whose K and V the cache has: q [n_tok][heads][D] of the cache's
+        type, lens int32 [n] (committed positions: token j of sequence i lies at lens[i] + j), masks int64 [n_tok] (bit k:
+        the token sees its sequence's k-th; None: those up to itself). first int32 [n + 1]: where the sequences' tokens
+        begin (None: n_tok / n each); nodes: at most so many tokens a sequence (None: n_tok / n, or with `first` 64); rows,
+        window, out and scratch (Cache.tree_scratch_bytes) as for attend."""
+        n_tok, n, dev = q.shape[0], lens.shape[0], self._dev
+        if _current_device() != dev:
+            with torch.cuda.device(dev):
+                return self.attend_tree(layer, q, lens, masks, scale, first, nodes, rows, window, out, scratch)
+        if out is None:
+            out = torch.empty_like(q)
+        if first is None:
+            if n_tok != (n_tok // n if n else 0) * n or (nodes is not None and nodes * n != n_tok):
+                raise ValueError("first: needed where the sequences' tokens are not n_tok / n each")
+            nodes = n_tok // n if n else 0
+        elif nodes is None:
+            nodes = 64
+        with self._lock:
+            self._q.set(q, n_tok, dev)
+            self._o.set(out, n_tok, dev)
+            args = (_list(first, "first", dev, n + 1), _list(lens, "lens", dev, n), _list(rows, "rows", dev, n),
+                    _matrix(masks, "masks", dev, (n_tok,), torch.int64))
+            if n == 0 or n_tok == 0:
+                return out
+            st = _stream(dev)
+            _, address, size = self._tree.get(st, self._L.sjk_kv16_attend_tree_scratch_bytes(self._refs[0]), scratch)
+            rc = self._L.sjk_kv16_attend_tree(self._refs[layer], self._qo[0], n_tok, *args, n, nodes, scale, window, self._qo[1], address, size, st)
+        if rc:
+            raise sjk.SjkError(rc, "kv16_attend_tree")
+        return out
+
+    def tree_scratch_bytes(self):
+        """Bytes of scratch that attend_tree needs."""
+        return self._L.sjk_kv16_attend_tree_scratch_bytes(self._refs[0])
 
     def keep(self, lens, path, count, rows=None, new_lens=None):
         """Accepted drafts to their places, in every layer: K and V of the positions lens[i] + path[i][j], j < count[i], to

@@ -241,6 +241,8 @@ SIGNATURES = {
     "sjk_kv16_attend": (C.c_int, [P(Kv16), P(Rows), vp, vp, C.c_int, C.c_float, C.c_int, P(Rows), vp, C.c_size_t, vp]),
     "sjk_qkv_at": (C.c_int, [P(QkvArgs), vp, vp]),
     "sjk_kv16_maps": (C.c_int, [P(Kv16), vp, vp, vp, vp, C.c_int, C.c_int, P(Kv16Step), vp]),
+    "sjk_kv16_attend_tree_scratch_bytes": (C.c_size_t, [P(Kv16)]),
+    "sjk_kv16_attend_tree": (C.c_int, [P(Kv16), P(Rows), C.c_int, vp, vp, vp, vp, C.c_int, C.c_int, C.c_float, C.c_int, P(Rows), vp, C.c_size_t, vp]),
     "sjk_kv16_keep": (C.c_int, [P(Kv16), C.c_int, C.c_int64, vp, vp, vp, vp, C.c_int, C.c_int, vp, vp]),
     "sjk_kv16_bounds": (C.c_int, [P(Kv16), C.c_int, C.c_int64, vp, C.c_int64, vp, vp, vp, C.c_int, vp]),
     "sjk_kv16_select_scratch_bytes": (C.c_size_t, [P(Kv16), C.c_int]),
