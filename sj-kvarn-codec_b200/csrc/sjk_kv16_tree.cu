@@ -28,6 +28,8 @@
 #include "sjk_internal.h"
 #include "sjk_tc.cuh"
 
+#include <cuda.h>
+
 #include <math.h>
 
 namespace {
@@ -58,6 +60,8 @@ struct Params {
     float * part;                           // [CTA][2][NMAX][D]
     float * ml;                             // [CTA][2][NMAX][2]
     int4 * split;                           // by CTA: sequence (-1: none), KV head, first and last run
+    int box;                                // tokens of a box (WHOLE)
+    CUtensorMap maps[2];                    // K, V (WHOLE)
 };
 
 // What a sequence is to a tile of rows: its committed length, tokens, positions [lo, hi) that some token sees, rows.
@@ -120,22 +124,23 @@ struct Info {
 template <int TYPE_, int D_>
 struct Shape {
     static constexpr int TYPE = TYPE_, D = D_;
-    static constexpr int NB = (D + 63) / 64, HALVES = (D + 127) / 128, CH = D / 8;  // 64-channel blocks, M tiles of O, words of a row
-    static constexpr int TILE = NB * TS * 128, QB = NB * NMAX * 128, PB = TS * 128;  // bytes of a K or V tile, Q, a term of P
-    // slots of K and of V: what 227 KB hold beside Q and P
-    static constexpr int KS = D == 64 ? 4 : D == 256 ? 1 : 3, VS = D == 64 ? 4 : D == 256 ? 1 : 2;
+    static constexpr int PARTS = (D + 127) / 128, BLOCKS = D == 64 ? 1 : 2;          // M tiles of O; 64-channel blocks of one
+    static constexpr int CH = D / 8 < 16 ? D / 8 : 16;                               // words of a row in a part
+    static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = TS * 128;  // bytes: part of a K or V tile, of Q; term of P
+    // slots (parts) of K and of V: what 227 KB hold beside Q and P
+    static constexpr int KS = D == 64 ? 5 : D == 256 ? 2 : 3, VS = D == 64 ? 4 : 2;
     static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX;
     static constexpr float SLACK = TYPE == SJK_F16 ? 5.0f : 8.0f, UP = TYPE == SJK_F16 ? 10.0f : 0.0f;
 };
 
 template <typename S>
 struct Shared {
-    uint8_t k[S::KS * S::TILE], v[S::VS * S::TILE], q[S::QB], pt[2][S::PB];
+    uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2][S::PB];
     Info info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
     uint64_t odd[TILES][2];                 // positions whose V row was replaced, of tiles that some rows see only partly
     float m[NMAX], fac[NMAX], red[N_SOFT][32];
-    uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS];
+    uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
     Cursor start;
     uint32_t per, list, tmem;
@@ -158,6 +163,16 @@ SJK_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t ac
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n" ::"r"(d),
         "l"(a), "l"(b), "r"(id), "r"(accumulate), "r"(0u));
+}
+SJK_DEV bool elected() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(r));
+    return r != 0;
+}
+// a box of 64 channels of one head and some tokens of a page
+SJK_DEV void box(uint32_t dst, const CUtensorMap * map, int c, int h, int slot, uint32_t page, uint64_t * bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(map), "r"(c), "r"(h), "r"(slot), "r"(page), "r"(tc::smem_addr(bar)) : "memory");
 }
 SJK_DEV void ld8(uint32_t t, float * v) {
     uint32_t r[8];
@@ -210,7 +225,7 @@ struct Waiter {
     }
 };
 
-template <typename S>
+template <typename S, bool WHOLE>
 __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
     constexpr int D = S::D, KS = S::KS, VS = S::VS;
     extern __shared__ uint8_t raw[];
@@ -219,8 +234,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
     const int tile = blockIdx.x % p.tiles, run = blockIdx.x / p.tiles;
 
     if (tid == 0) {
-        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 2); tc::mbar_init(&sm.k_empty[i], 1); }
-        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 2); tc::mbar_init(&sm.v_empty[i], 1); }
+        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], WHOLE ? 1 : 2); tc::mbar_init(&sm.k_empty[i], 1); }
+        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 2); tc::mbar_init(&sm.v_empty[i], 1); tc::mbar_init(&sm.v_land[i], 1); }
         for (int i = 0; i < 2; ++i) { tc::mbar_init(&sm.s_full[i], 1); tc::mbar_init(&sm.s_empty[i], N_SOFT); }
         tc::mbar_init(&sm.p_full, N_SOFT);
         tc::mbar_init(&sm.pv_done, 1);
@@ -311,7 +326,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 if (row < 0 || row >= (int64_t) p.c.n_rows) return;
                 const uint32_t * table = p.c.tables + row * p.c.table_stride;
 #pragma unroll 1
-                for (int hf = 0; hf < S::HALVES; ++hf) {
+                for (int hf = 0; hf < S::PARTS; ++hf) {
                     const int d = hf * 128 + tl;
 #pragma unroll 1
                     for (int c = 0; c < nc; c += 8) {
@@ -406,7 +421,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         waited = true;
                         tc::fence_after_sync();
 #pragma unroll 1
-                        for (int hf = 0; hf < S::HALVES; ++hf)
+                        for (int hf = 0; hf < S::PARTS; ++hf)
 #pragma unroll
                             for (int q = 0; q < 4; ++q)
                                 if (q * 8 < nc) {
@@ -470,7 +485,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 p.split[blockIdx.x] = make_int4(at.seq, h, run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
             tc::nbar_sync(bar, 128);
 #pragma unroll 1
-            for (int hf = 0; hf < S::HALVES; ++hf) {
+            for (int hf = 0; hf < S::PARTS; ++hf) {
                 const int d = hf * 128 + tl;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
@@ -501,161 +516,224 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         const int wh = (warp - N_SOFT) & 1, slots = is_v ? VS : KS;
         uint64_t * full = is_v ? sm.v_full : sm.k_full, * empty = is_v ? sm.v_empty : sm.k_empty;
         uint8_t * ring = is_v ? sm.v : sm.k;
-        uint32_t jj = 0, told = 0;          // tiles asked for, and announced
-        auto tell = [&](uint32_t upto) {    // copies of the tiles before `upto` have landed
+        uint32_t jj = 0, pp = 0, told = 0;  // tiles; parts asked for, and announced (not WHOLE)
+        uint32_t landed = 0;                // WHOLE: parity of every slot's v_land
+        auto tell = [&](uint32_t upto) {    // copies of the parts before `upto` have landed
             tc::fence_proxy_async();
             __syncwarp();
             for (; told < upto; ++told)
                 if (lane == 0) tc::mbar_arrive(&full[told % slots]);
         };
+        if (WHOLE && !is_v && wh == 1) at.rem = 0;          // one warp asks for all K boxes
         while (at.rem > 0) {
             const Seq s = at.s;
             const int steps = at.take();
             const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
             const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
             if (!table && lane == 0) flag();
-            const uint16_t * base = static_cast<const uint16_t *>(is_v ? p.c.v : p.c.k) + (int64_t) at.h * p.c.head_stride;
             const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
             for (int i = 0; i < steps; ++i, ++jj) {
-                const int step = s.step0 + at.st + i;
-                int64_t off[2];             // rows of the lane's two positions; -1: none
+                const uint32_t t0 = (uint32_t) (s.step0 + at.st + i) * TS;
+                auto page_at = [&](uint32_t t, uint32_t * place) {
+                    const uint32_t g = p.page_shift >= 0 ? t >> p.page_shift : t / (uint32_t) p.c.page_tokens, page = table[g];
+                    *place = t - g * (uint32_t) p.c.page_tokens;
+                    if (page >= p.c.n_pages && page != SJKVARN_NO_BLOCK) flag();
+                    return page;
+                };
+                // the tile's live positions, as every warp needs them: four words, or the two of the warp's own 64
+                unsigned live[4] = {0u, 0u, 0u, 0u};
+                int64_t off[2] = {-1, -1};  // rows of the lane's own two positions; -1: none
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint32_t t = (uint32_t) step * TS + (uint32_t) (64 * wh + 32 * u + lane);
-                    off[u] = -1;
+                for (int u = 0; u < 4; ++u) {
+                    if (!WHOLE && (u >> 1) != wh) continue;
+                    const uint32_t t = t0 + (uint32_t) (32 * u + lane);
+                    bool on = false;
                     if (table && t < s.hi && t >= (uint32_t) lo0) {
-                        const uint32_t g = p.page_shift >= 0 ? t >> p.page_shift : t / (uint32_t) p.c.page_tokens, page = table[g];
-                        if (page < p.c.n_pages) off[u] = (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride;
-                        else if (page != SJKVARN_NO_BLOCK) flag();
+                        uint32_t place;
+                        const uint32_t page = page_at(t, &place);
+                        on = page < p.c.n_pages;
+                        if (!WHOLE && on) off[u & 1] = (int64_t) page * p.c.page_stride + (int64_t) place * p.c.slot_stride;
+                    }
+                    live[u] = __ballot_sync(FULL, on);
+                }
+                if (!is_v && lane == 0)
+                    for (int u = 0; u < 4; ++u)
+                        if (WHOLE || (u >> 1) == wh) sm.live[jj % TILES][u] = live[u];
+                // V rows that only some rows see (drafted ones, a window's edge), and dead ones that came with a box
+                const bool some = t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
+                const bool mend = is_v && (some || (WHOLE && (live[0] & live[1] & live[2] & live[3]) != FULL));
+                uint64_t todo = 0ull;       // of the warp's 64
+                if (mend) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t t = t0 + (uint32_t) (64 * wh + 32 * u + lane);
+                        const bool on = (live[2 * wh + u] >> lane) & 1u;
+                        const bool few = t >= (uint32_t) s.len || (p.window && t < (uint32_t) lo0 + 64u);
+                        todo |= (uint64_t) __ballot_sync(FULL, on ? some && few : WHOLE) << (32 * u);
                     }
                 }
-                const int slot = (int) (jj % (uint32_t) slots);
-                if (jj >= (uint32_t) slots) {
-                    const uint32_t parity = (jj / (uint32_t) slots - 1u) & 1u;
-                    if (!wait.dead && !tc::mbar_test(&empty[slot], parity)) {
-                        tc::cp_async_wait_group<0>();       // nothing more to ask for now: announce what has been
-                        tell(jj);
+                // WHOLE: the lane's box
+                uint32_t place = 0, page = SJKVARN_NO_BLOCK;
+                const uint32_t mine = (uint32_t) (lane / S::BLOCKS) * (uint32_t) p.box;
+                if (WHOLE && mine < TS && t0 + mine < s.hi && t0 + mine + (uint32_t) p.box > (uint32_t) lo0 && table) page = page_at(t0 + mine, &place);
+                const bool asks = WHOLE && wh == 0 && page < p.c.n_pages;
+                const uint32_t tx = WHOLE ? (uint32_t) __popc(__ballot_sync(FULL, asks)) * (uint32_t) p.box * 128u : 0u;
+                uint64_t odd = 0ull;
+#pragma unroll 1
+                for (int part = 0; part < S::PARTS; ++part, ++pp) {
+                    const int slot = (int) (pp % (uint32_t) slots);
+                    if (pp >= (uint32_t) slots) {
+                        const uint32_t parity = (pp / (uint32_t) slots - 1u) & 1u;
+                        if (!WHOLE && !wait.dead && !tc::mbar_test(&empty[slot], parity)) {
+                            tc::cp_async_wait_group<0>();   // nothing more to ask for now: announce what has been
+                            tell(pp);
+                        }
                         wait.warp(&empty[slot], parity);
                     }
-                    __syncwarp();
-                }
-                uint8_t * dst = ring + slot * S::TILE + 64 * wh * 128;
-                unsigned live[2];
+                    uint8_t * dst = ring + slot * S::PART;
+                    if constexpr (WHOLE) {
+                        uint64_t * bar = mend ? &sm.v_land[slot] : &full[slot];
+                        if (wh == 0) {
+                            if (lane == 0) tc::mbar_expect_tx(bar, tx);
+                            __syncwarp();
+                            if (asks)
+                                box(tc::smem_addr(dst) + (uint32_t) (lane % S::BLOCKS) * (TS * 128) + mine * 128u, &p.maps[is_v ? 1 : 0],
+                                    part * 128 + (lane % S::BLOCKS) * 64, at.h, (int) place, page, bar);
+                        } else if (!mend && lane == 0) tc::mbar_arrive(bar);
+                        if (mend) {
+                            wait.warp(bar, (landed >> slot) & 1u);
+                            landed ^= 1u << slot;
+                        }
+                    } else {
+                        const uint16_t * base = static_cast<const uint16_t *>(is_v ? p.c.v : p.c.k) + (int64_t) at.h * p.c.head_stride + part * 128;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    live[u] = __ballot_sync(FULL, off[u] >= 0);
-                    if (!is_v && lane == 0) sm.live[jj % TILES][2 * wh + u] = live[u];
+                        for (int u = 0; u < 2; ++u)
 #pragma unroll 4
-                    for (int k = 0; k < S::CH; ++k) {
-                        const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
-                        const int64_t o = __shfl_sync(FULL, off[u], r);
-                        tc::cp_async16(dst + (c >> 3) * (TS * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
-                    }
-                }
-                tc::cp_async_commit();
-                // V rows that only some rows see: drafted ones, and a window's edge
-                if (is_v) {
-                    const uint32_t t0 = (uint32_t) step * TS;
-                    if (t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u)) {
-                        tc::cp_async_wait_group<0>();
-                        __syncwarp();
-                        uint64_t odd = 0ull;
-                        for (int r = 0; r < 64; ++r) {
-                            const uint32_t t = t0 + (uint32_t) (64 * wh + r);
-                            if (!((live[r >> 5] >> (r & 31)) & 1u) || !(t >= (uint32_t) s.len || (p.window && t < (uint32_t) lo0 + 64u))) continue;
-                            bool bad = false;
-                            uint4 * at16 = nullptr;
-                            if (lane < S::CH) {
-                                at16 = reinterpret_cast<uint4 *>(dst + (lane >> 3) * (TS * 128) + r * 128 + (((lane ^ r) & 7) << 4));
-                                const uint4 x = *at16;
-                                bad = odd_word<S::TYPE>(x.x) || odd_word<S::TYPE>(x.y) || odd_word<S::TYPE>(x.z) || odd_word<S::TYPE>(x.w);
+                            for (int k = 0; k < S::CH; ++k) {
+                                const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
+                                const int64_t o = __shfl_sync(FULL, off[u], r);
+                                tc::cp_async16(dst + (c >> 3) * (TS * 128) + (64 * wh + 32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8,
+                                               o >= 0 ? 16u : 0u);
                             }
-                            if (__any_sync(FULL, bad)) {
-                                odd |= 1ull << r;
-                                if (bad) {  // its finite neighbours stay
-                                    uint32_t * w = reinterpret_cast<uint32_t *>(at16);
+                        tc::cp_async_commit();
+                        if (mend) {
+                            tc::cp_async_wait_group<0>();
+                            __syncwarp();
+                        }
+                    }
+                    if (mend) {
+                        for (uint64_t left = todo; left; left &= left - 1ull) {
+                            const int r = 64 * wh + __ffsll((long long) left) - 1;
+                            const bool on = (live[r >> 5] >> (r & 31)) & 1u;
+                            bool bad = false;
+                            uint4 * at16 = reinterpret_cast<uint4 *>(dst + (lane >> 3) * (TS * 128) + r * 128 + (((lane ^ r) & 7) << 4));
+                            if (lane < S::CH) {
+                                if (!on) *at16 = make_uint4(0u, 0u, 0u, 0u);
+                                else {
+                                    const uint4 x = *at16;
+                                    bad = odd_word<S::TYPE>(x.x) || odd_word<S::TYPE>(x.y) || odd_word<S::TYPE>(x.z) || odd_word<S::TYPE>(x.w);
+                                }
+                            }
+                            if (!__any_sync(FULL, bad)) continue;
+                            odd |= 1ull << (r & 63);
+                            if (bad) {      // its finite neighbours stay
+                                uint32_t * w = reinterpret_cast<uint32_t *>(at16);
 #pragma unroll 1
-                                    for (int e = 0; e < 4; ++e) {
-                                        const float2 f = widen2<S::TYPE>(w[e]);
-                                        if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
-                                        if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
-                                    }
+                                for (int e = 0; e < 4; ++e) {
+                                    const float2 f = widen2<S::TYPE>(w[e]);
+                                    if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
+                                    if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
                                 }
                             }
                         }
                         if (lane == 0) sm.odd[jj % TILES][wh] = odd;
-                        tell(jj + 1);
-                        continue;
+                        if (WHOLE) {
+                            tc::fence_proxy_async();
+                            __syncwarp();
+                            if (lane == 0) tc::mbar_arrive(&full[slot]);
+                        } else tell(pp + 1);
+                    } else if (!WHOLE) {
+                        if (slots == 2) tc::cp_async_wait_group<1>();
+                        else if (slots == 3) tc::cp_async_wait_group<2>();
+                        else tc::cp_async_wait_group<3>();
+                        const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;      // parts still on their way
+                        if (pp + 1 > flight) tell(pp + 1 - flight);
                     }
                 }
-                if (slots == 1) tc::cp_async_wait_group<0>();
-                else if (slots == 2) tc::cp_async_wait_group<1>();
-                else if (slots == 3) tc::cp_async_wait_group<2>();
-                else tc::cp_async_wait_group<3>();
-                if (jj + 2 > (uint32_t) slots) tell(jj + 2 - (uint32_t) slots);
             }
             at.next(p, tile, steps);
         }
-        tc::cp_async_wait_group<0>();
-        tell(jj);
-    } else if (warp == W_MMA) {
-        // ---- products ----
-        if (lane == 0) {
-            const uint32_t ka = tc::smem_addr(sm.k), va = tc::smem_addr(sm.v), qa = tc::smem_addr(sm.q), pa = tc::smem_addr(sm.pt);
-            uint32_t jj = 0;
-            int pend_n = 0, pend_first = 0, items = 0;       // a tile whose second product is to come
-            auto second = [&](uint32_t j) {                  // O^T += V^T P of tile j
-                if (pend_first && items > 1) wait(&sm.o_free, (uint32_t) (items - 2) & 1u);
-                const uint32_t slot = j % VS;
-                wait(&sm.v_full[slot], (j / VS) & 1u);
-                wait(&sm.p_full, j & 1u);
-                tc::fence_after_sync();
-                if (!wait.dead) {
-                    const uint32_t id = idesc<S::TYPE>(pend_n, true);
-#pragma unroll 1
-                    for (int hf = 0; hf < S::HALVES; ++hf)
-#pragma unroll 1
-                        for (int term = 0; term < 2; ++term)
-#pragma unroll
-                            for (int k = 0; k < TS / 16; ++k)
-                                mma_ss(tmem + S::COL_O + (uint32_t) (hf * NMAX), swizzled(va + slot * S::TILE + hf * 2 * TS * 128 + k * 2048, D == 64 ? 0u : TS * 128u),
-                                       swizzled(pa + term * S::PB + k * 2048, TS * 128u), id, pend_first && term == 0 && k == 0 ? 0u : 1u);
-                    tc::mma_commit(&sm.v_empty[slot]);
-                    tc::mma_commit(&sm.pv_done);
-                }
-            };
-            bool pend = false;
-            for (; at.rem > 0; ) {
-                const int steps = at.take(), n = (at.s.nr + 15) & ~15;
-                const uint32_t id = idesc<S::TYPE>(n, false);
-                if (pend) second(jj - 1);   // the pair's end does not wait for the next one's queries
-                pend = false;
-                wait(&sm.q_full[items % INFO], (uint32_t) (items / INFO) & 1u);
-                for (int i = 0; i < steps; ++i, ++jj) {
-                    const uint32_t slot = jj % KS, b = jj & 1u;
-                    wait(&sm.k_full[slot], (jj / KS) & 1u);
-                    if (jj >= 2) wait(&sm.s_empty[b], ((jj >> 1) - 1u) & 1u);
-                    tc::fence_after_sync();
-                    if (!wait.dead) {
-#pragma unroll
-                        for (int k = 0; k < D / 16; ++k)
-                            mma_ss(tmem + S::COL_S + b * NMAX, swizzled(ka + slot * S::TILE + (k >> 2) * TS * 128 + (k & 3) * 32, 16u),
-                                   swizzled(qa + (k >> 2) * NMAX * 128 + (k & 3) * 32, 16u), id, k ? 1u : 0u);
-                        tc::mma_commit(&sm.k_empty[slot]);
-                        if (i + 1 == steps) tc::mma_commit(&sm.q_empty);
-                        tc::mma_commit(&sm.s_full[b]);
-                    }
-                    if (pend) second(jj - 1);
-                    pend = true;
-                    pend_n = n;
-                    pend_first = i == 0;
-                    if (i == 0) ++items;
-                }
-                at.next(p, tile, steps);
-            }
-            if (pend) second(jj - 1);
+        if (!WHOLE) {
+            tc::cp_async_wait_group<0>();
+            tell(pp);
         }
-        __syncwarp();
+    } else if (warp == W_MMA) {
+        // ---- products: the warp stays together and one thread issues, so that descriptors are the same for all lanes ----
+        const bool leader = elected();
+        const uint32_t ka = tc::smem_addr(sm.k), va = tc::smem_addr(sm.v), qa = tc::smem_addr(sm.q), pa = tc::smem_addr(sm.pt);
+        const uint32_t tm = __shfl_sync(FULL, tmem, 0);
+        uint32_t jj = 0, kp = 0, vp = 0;                     // tiles; parts of K and of V
+        int pend_n = 0, items = 0;
+        bool pend = false, pend_first = false;               // a tile whose second product is to come
+        auto second = [&](uint32_t j) {                      // O^T += V^T P of tile j
+            if (pend_first && items > 1) wait.warp(&sm.o_free, (uint32_t) (items - 2) & 1u);
+            wait.warp(&sm.p_full, j & 1u);
+            const uint32_t id = idesc<S::TYPE>(pend_n, true);
+#pragma unroll 1
+            for (int part = 0; part < S::PARTS; ++part, ++vp) {
+                const uint32_t slot = vp % VS;
+                wait.warp(&sm.v_full[slot], (vp / VS) & 1u);
+                tc::fence_after_sync();
+                const uint64_t a = swizzled(va + slot * S::PART, D == 64 ? 0u : TS * 128u), b = swizzled(pa, TS * 128u);
+                const uint32_t d = tm + S::COL_O + (uint32_t) (part * NMAX);
+                if (leader && !wait.dead) {
+#pragma unroll
+                    for (int k = 0; k < 2 * TS / 16; ++k)
+                        mma_ss(d, a + (uint64_t) ((k & 7) * 2048 >> 4), b + (uint64_t) (((k >> 3) * S::PB + (k & 7) * 2048) >> 4), id, pend_first && k == 0 ? 0u : 1u);
+                    tc::mma_commit(&sm.v_empty[slot]);
+                    if (part + 1 == S::PARTS) tc::mma_commit(&sm.pv_done);
+                }
+                __syncwarp();
+            }
+        };
+        while (at.rem > 0) {
+            const int steps = __shfl_sync(FULL, at.take(), 0), n = __shfl_sync(FULL, (at.s.nr + 15) & ~15, 0);
+            const uint32_t id = idesc<S::TYPE>(n, false);
+            if (pend) second(jj - 1);       // the pair's end does not wait for the next one's queries
+            pend = false;
+            wait.warp(&sm.q_full[items % INFO], (uint32_t) (items / INFO) & 1u);
+            for (int i = 0; i < steps; ++i, ++jj) {
+                const uint32_t b = jj & 1u;
+                if (jj >= 2) wait.warp(&sm.s_empty[b], ((jj >> 1) - 1u) & 1u);
+#pragma unroll 1
+                for (int part = 0; part < S::PARTS; ++part, ++kp) {
+                    const uint32_t slot = kp % KS;
+                    wait.warp(&sm.k_full[slot], (kp / KS) & 1u);
+                    tc::fence_after_sync();
+                    const uint64_t ad = swizzled(ka + slot * S::PART, 16u), bd = swizzled(qa + part * S::QP, 16u);
+                    const uint32_t d = tm + S::COL_S + b * NMAX;
+                    if (leader && !wait.dead) {
+#pragma unroll
+                        for (int k = 0; k < (D < 128 ? D : 128) / 16; ++k)
+                            mma_ss(d, ad + (uint64_t) (((k >> 2) * TS * 128 + (k & 3) * 32) >> 4), bd + (uint64_t) (((k >> 2) * NMAX * 128 + (k & 3) * 32) >> 4), id,
+                                   part || k ? 1u : 0u);
+                        tc::mma_commit(&sm.k_empty[slot]);
+                        if (part + 1 == S::PARTS) {
+                            if (i + 1 == steps) tc::mma_commit(&sm.q_empty);
+                            tc::mma_commit(&sm.s_full[b]);
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (pend) second(jj - 1);
+                pend = true;
+                pend_n = n;
+                pend_first = i == 0;
+                if (i == 0) ++items;
+            }
+            at.next(p, tile, steps);
+        }
+        if (pend) second(jj - 1);
     } else {
         // ---- queries, and what the rows see ----
         for (int item = 0; at.rem > 0; ++item) {
@@ -692,8 +770,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             for (int u = 0; u < 2; ++u)
                 if (32 * u < n)
 #pragma unroll 4
-                    for (int k = 0; k < S::CH; ++k) {
-                        const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
+                    for (int k = 0; k < D / 8; ++k) {
+                        const int w = k * 32 + lane, r = w / (D / 8), c = w - r * (D / 8);
                         const int64_t o = __shfl_sync(FULL, from[u], r);
                         tc::cp_async16(sm.q + (c >> 3) * (NMAX * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4),
                                        static_cast<const uint16_t *>(p.q.p) + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
@@ -765,20 +843,53 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
         }
 }
 
-template <typename S>
-int run(const Params & p, sjk_stream st) {
+// Maps of the cache's K and V as boxes of `box` tokens; false where its strides do not allow them.
+bool maps_of(Params * p) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void * f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (!encode) return false;
+    const sjk_kv16 & c = p->c;
+    const cuuint64_t dims[4] = {(cuuint64_t) c.head_dim, (cuuint64_t) c.n_head_kv, (cuuint64_t) c.page_tokens, (cuuint64_t) c.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t) c.head_stride * 2, (cuuint64_t) c.slot_stride * 2, (cuuint64_t) c.page_stride * 2};
+    const cuuint32_t sizes[4] = {64u, 1u, (cuuint32_t) p->box, 1u}, ones[4] = {1u, 1u, 1u, 1u};
+    for (int i = 0; i < 2; ++i)
+        if (encode(&p->maps[i], c.type == SJK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, i ? c.v : c.k, dims, strides, sizes, ones,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
+}
+
+template <typename S, bool WHOLE>
+int tree_launch(const Params & p, sjk_stream st) {
     constexpr size_t bytes = sizeof(Shared<S>) + 1024;
     static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
-    if (smem_limit<tree_kernel<S>>(bytes)) return SJK_ERR_DEVICE;
+    if (smem_limit<tree_kernel<S, WHOLE>>(bytes)) return SJK_ERR_DEVICE;
+    return launch(tree_kernel<S, WHOLE>, dim3((unsigned) (p.tiles * p.wl)), dim3(NT), bytes, st, p);
+}
+
+template <typename S>
+int run(Params & p, sjk_stream st) {
+    // pages of a multiple of 8 tokens come as boxes: as many tokens of a page as end where a tile's rows do
+    p.box = 128;
+    while (p.box > 1 && p.c.page_tokens % p.box) p.box >>= 1;
     const int ctas = p.tiles * p.wl;
-    const int rc = launch(tree_kernel<S>, dim3((unsigned) ctas), dim3(NT), bytes, st, p);
+    const int rc = p.box >= 8 && maps_of(&p) ? tree_launch<S, true>(p, st) : tree_launch<S, false>(p, st);
     if (rc) return rc;
     const int rows = p.nodes * p.grp < NMAX ? p.nodes * p.grp : NMAX;
     return launch(tree_merge_kernel<S::D>, dim3((unsigned) ctas, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE);
 }
 
 template <int TYPE>
-int run_dim(const Params & p, sjk_stream st) {
+int run_dim(Params & p, sjk_stream st) {
     switch (p.c.head_dim) {
         case 64: return run<Shape<TYPE, 64>>(p, st);
         case 96: return run<Shape<TYPE, 96>>(p, st);
