@@ -37,7 +37,6 @@ namespace {
 using namespace sjk16;
 
 constexpr unsigned FULL = 0xFFFFFFFFu;
-constexpr int NMAX = 64;                    // query rows of a pass
 constexpr int TS = 128;                     // positions of a step
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
 constexpr int MIN_RUN = 2;                  // units of a run, at least
@@ -69,7 +68,7 @@ struct Seq {
     int len, count, first, row0, nr, step0, steps;
     uint32_t hi;
 };
-SJK_DEV Seq seq_of(const Params & p, int i, int tile) {
+SJK_DEV Seq seq_of(const Params & p, int i, int tile, int nmax) {
     Seq s = {0, 0, 0, 0, 0, 0, 0, 0u};
     int64_t f0, f1;
     if (p.first) { f0 = p.first[i]; f1 = p.first[i + 1]; }
@@ -77,7 +76,7 @@ SJK_DEV Seq seq_of(const Params & p, int i, int tile) {
     if (f0 < 0 || f1 < f0 || f1 > p.n_tok || f1 - f0 > p.nodes) { flag(); return s; }
     s.count = (int) (f1 - f0);
     s.first = (int) f0;
-    const int rows = s.count * p.grp, tiles = (rows + NMAX - 1) / NMAX;
+    const int rows = s.count * p.grp, tiles = (rows + nmax - 1) / nmax;
     if (tile >= tiles) return s;
     s.row0 = (int) ((int64_t) rows * tile / tiles);
     s.nr = (int) ((int64_t) rows * (tile + 1) / tiles) - s.row0;
@@ -100,7 +99,7 @@ struct Cursor {
     Seq s;
     // the pair's steps of this run
     SJK_DEV int take() const { const int left = s.steps - st; return left < rem ? left : rem; }
-    SJK_DEV void next(const Params & p, int tile, int taken) {
+    SJK_DEV void next(const Params & p, int tile, int nmax, int taken) {
         rem -= taken;
         st += taken;
         if (st < s.steps) return;
@@ -110,36 +109,41 @@ struct Cursor {
         if (rem <= 0) return;
         if (++h < p.c.n_head_kv) return;
         h = 0;
-        do { s = seq_of(p, ++seq, tile); } while (s.steps <= 0);
+        do { s = seq_of(p, ++seq, tile, nmax); } while (s.steps <= 0);
     }
 };
 
+template <int N>
+struct Int { static constexpr int value = N; };
+
 // What row n of a pair is.
+template <int NMAX>
 struct Info {
     uint64_t mask[NMAX];                    // drafted tokens that it sees
     int64_t out[NMAX];                      // its place in the output
     int lo[NMAX];                           // first committed position that it sees
 };
 
-template <int TYPE_, int D_>
+template <int TYPE_, int D_, int NMAX_>
 struct Shape {
-    static constexpr int TYPE = TYPE_, D = D_;
+    static constexpr int TYPE = TYPE_, D = D_, NMAX = NMAX_;        // NMAX: query rows of a pass
+    static constexpr int PASSES = NMAX / 64;                        // of 32 columns of a softmax thread
     static constexpr int PARTS = (D + 127) / 128, BLOCKS = D == 64 ? 1 : 2;          // M tiles of O; 64-channel blocks of one
     static constexpr int CH = D / 8 < 16 ? D / 8 : 16;                               // words of a row in a part
-    static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = TS * 128;  // bytes: part of a K or V tile, of Q; term of P
+    static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = PASSES * TS * 128;  // bytes: part of a K or V tile, of Q; term of P
     // slots (parts) of K and of V: what 227 KB hold beside Q and P
-    static constexpr int KS = D == 64 ? 5 : D == 256 ? 2 : 3, VS = D == 64 ? 4 : 2;
-    static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX;
+    static constexpr int KS = D == 64 ? (NMAX > 64 ? 4 : 5) : D == 256 || NMAX > 64 ? 2 : 3, VS = D == 64 ? (NMAX > 64 ? 3 : 4) : NMAX > 64 ? 1 : 2;
+    static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX, COLS = NMAX > 64 ? 512 : 256;     // of TMEM
     static constexpr float SLACK = TYPE == SJK_F16 ? 5.0f : 8.0f, UP = TYPE == SJK_F16 ? 10.0f : 0.0f;
 };
 
 template <typename S>
 struct Shared {
     uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2][S::PB];
-    Info info[INFO];
+    Info<S::NMAX> info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
     uint64_t odd[TILES][2];                 // positions whose V row was replaced, of tiles that some rows see only partly
-    float m[NMAX], fac[NMAX], red[N_SOFT][32];
+    float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];       // a row's maximum in use; what its scores are shifted by
     uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
     Cursor start;
@@ -186,25 +190,40 @@ SJK_DEV bool any_of(int id, bool x) {       // over the 128 threads of a half
                  : "=r"(r) : "r"((uint32_t) x), "r"(id), "r"(128) : "memory");
     return r != 0;
 }
-// 32 columns of a lane over the warp's lanes: lane c gets column c
-template <bool MAX>
-SJK_DEV float columns32(const float (&v)[32], int lane) {
-    float a[16];
+// 8 K columns of a lane over the warp's lanes: lane c gets column c (with fewer than 32, lanes c + 8 K i as well)
+template <bool MAX, int N>
+SJK_DEV float columns(const float * v, int lane) {
+    float a[N / 2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const bool up = lane & 16;
-        const float send = up ? v[i] : v[i + 16], keep = up ? v[i + 16] : v[i], r = __shfl_xor_sync(FULL, send, 16);
+    for (int i = 0; i < N / 2; ++i) {
+        const bool up = lane & (N / 2);
+        const float send = up ? v[i] : v[i + N / 2], keep = up ? v[i + N / 2] : v[i], r = __shfl_xor_sync(FULL, send, N / 2);
         a[i] = MAX ? fmaxf(keep, r) : keep + r;
     }
 #pragma unroll
-    for (int o = 8; o; o >>= 1)
+    for (int o = N / 4; o; o >>= 1)
 #pragma unroll
         for (int i = 0; i < o; ++i) {
             const bool up = lane & o;
             const float send = up ? a[i] : a[i + o], keep = up ? a[i + o] : a[i], r = __shfl_xor_sync(FULL, send, o);
             a[i] = MAX ? fmaxf(keep, r) : keep + r;
         }
-    return a[0];
+    float x = a[0];
+#pragma unroll
+    for (int o = N; o < 32; o <<= 1) {
+        const float r = __shfl_xor_sync(FULL, x, o);
+        x = MAX ? fmaxf(x, r) : x + r;
+    }
+    return x;
+}
+template <bool MAX, int K>
+SJK_DEV float octets(const float * v, int lane) {
+    if constexpr (K == 3) {
+        float w[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) w[i] = i < 24 ? v[i] : MAX ? -INFINITY : 0.0f;
+        return columns<MAX, 32>(w, lane);
+    } else return columns<MAX, 8 * K>(v, lane);
 }
 template <int TYPE>
 SJK_DEV bool odd_word(uint32_t w) {         // an infinity or NaN among two
@@ -227,7 +246,7 @@ struct Waiter {
 
 template <typename S, bool WHOLE>
 __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
-    constexpr int D = S::D, KS = S::KS, VS = S::VS;
+    constexpr int D = S::D, KS = S::KS, VS = S::VS, NMAX = S::NMAX;
     extern __shared__ uint8_t raw[];
     Shared<S> & sm = *reinterpret_cast<Shared<S> *>(raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -244,7 +263,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         tc::mbar_init(&sm.q_empty, 1);
         tc::mbar_fence_init();
     }
-    if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, 256); tc::tmem_relinquish(); }
+    if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, S::COLS); tc::tmem_relinquish(); }
     pdl_wait();
     pdl_release();
     // where the run begins: units of all sequences, a block of them per lane
@@ -252,7 +271,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         const int block = (p.n_seq + 31) / 32;
         uint32_t mine = 0;
         for (int i = 0; i < block; ++i)
-            if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile));
+            if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile, NMAX));
         uint32_t incl = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -271,7 +290,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             c.base = __shfl_sync(FULL, incl - mine, g);
             c.seq = g * block;
             for (;; ++c.seq) {              // (the block's last sequence at the latest: its sum is above off)
-                c.s = seq_of(p, c.seq, tile);
+                c.s = seq_of(p, c.seq, tile, NMAX);
                 const uint32_t u = units_of(p, c.s);
                 if (c.base + u > off) break;
                 c.base += u;
@@ -297,41 +316,48 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
     Waiter wait;
 
     if (warp < N_SOFT) {
-        // ---- softmax: position 32 (warp % 4) + lane of a tile, columns [half nc, half nc + nc) ----
-        const int half = warp >> 2, quarter = warp & 3, bar = 1 + half, tl = quarter * 32 + lane;
+        // ---- softmax: position 32 (warp % 4) + lane of a tile; two groups of four warps have half of the columns each ----
+        const int group = warp >> 2, quarter = warp & 3, bar = 1 + group, tl = quarter * 32 + lane, tg = tid & 127;
         const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
-        const float sc = p.scale * 1.4426950408889634f;
-        float l[32];
+        // scores are positive multiples of the products (the queries' signs are turned for a negative scale)
+        const float sc = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
+        const float2 sc2 = make_float2(sc, sc);
+        float2 l[NMAX / 4];                 // sums of the thread's columns, in pairs
         uint32_t jj = 0;                    // tiles so far
         for (int item = 0; at.rem > 0; ++item) {
             const Seq s = at.s;
-            const int steps = at.take(), h = at.h, nc = ((s.nr + 15) & ~15) / 2, c0 = half * nc;
+            const int steps = at.take(), h = at.h;
+            const int n8 = (s.nr + 15) / 16, c0 = group * n8 * 8, nc = n8 * 8;      // octets of columns, first and number of columns
             const bool begun = at.st == 0, ended = at.st + steps == s.steps;
-            const Info & info = sm.info[item % INFO];
-            wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
-            if (tid % 128 < nc) sm.m[c0 + tid % 128] = -INFINITY;
+            const Info<NMAX> & info = sm.info[item % INFO];
+            if (tg < nc) {
+                sm.m[c0 + tg] = -INFINITY;
+                sm.up[c0 + tg] = 3e38f;     // (no score so far: any is above)
+            }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) l[c] = 0.0f;
+            for (int c = 0; c < NMAX / 4; ++c) l[c] = make_float2(0.0f, 0.0f);
             tc::nbar_sync(bar, 128);
+            wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
             const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
             auto partly = [&](int step) {   // some rows see a position of the step that others do not
                 const uint32_t t0 = (uint32_t) step * TS;
                 return t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
             };
+            auto sees = [&](uint32_t t, int n) { return t >= (uint32_t) s.len ? (bool) ((info.mask[n] >> (t - (uint32_t) s.len)) & 1ull) : t >= (uint32_t) info.lo[n]; };
             // non-finite values of V rows that only some rows see, into the sums of those that do
             auto add_odd = [&](uint32_t tile_no, int step) {
-                uint64_t some[2] = {sm.odd[tile_no % TILES][0], sm.odd[tile_no % TILES][1]};
+                const uint64_t some[2] = {sm.odd[tile_no % TILES][0], sm.odd[tile_no % TILES][1]};
                 if (!(some[0] | some[1])) return;
                 const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
                 if (row < 0 || row >= (int64_t) p.c.n_rows) return;
                 const uint32_t * table = p.c.tables + row * p.c.table_stride;
 #pragma unroll 1
-                for (int hf = 0; hf < S::PARTS; ++hf) {
-                    const int d = hf * 128 + tl;
+                for (int part = 0; part < S::PARTS; ++part) {
+                    const int d = part * 128 + tl;
 #pragma unroll 1
                     for (int c = 0; c < nc; c += 8) {
                         float o[8];
-                        const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + c);
+                        const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c);
                         ld8(addr, o);
                         tc::wait_ld();
 #pragma unroll 1
@@ -345,11 +371,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                                                       (int64_t) h * p.c.head_stride + d, S::TYPE);
                                 if (fabsf(x) < INFINITY) continue;
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const int n = c0 + c + e;
-                                    const bool sees = t >= (uint32_t) s.len ? (info.mask[n] >> (t - (uint32_t) s.len)) & 1ull : t >= (uint32_t) info.lo[n];
-                                    if (sees) o[e] += x;
-                                }
+                                for (int e = 0; e < 8; ++e)
+                                    if (sees(t, c0 + c + e)) o[e] += x;
                             }
                         uint32_t r[8];
 #pragma unroll
@@ -360,155 +383,187 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 }
                 tc::wait_st();
             };
-            for (int i = 0; i < steps; ++i, ++jj) {
-                const int b = jj & 1, step = s.step0 + at.st + i;
-                wait.warp(&sm.s_full[b], (jj >> 1) & 1u);
-                tc::fence_after_sync();
-                float x[32];
+            // K octets of columns, from cp on, of tile jj: weights into P, sums into lp
+            auto octets_of = [&](auto kk, int cp, float2 * lp, bool fresh, int step, unsigned live, auto && wait_p) {
+                constexpr int K = decltype(kk)::value, N = 8 * K;
+                const uint32_t from = tmem + lanes + S::COL_S + (jj & 1u) * NMAX + (uint32_t) cp;
+                float x[N];
+                const bool all = !partly(step), plain = live == FULL && all;
+                auto load = [&]() {         // products; those of positions that a row does not see: -inf
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q * 8 < nc) ld8(tmem + lanes + S::COL_S + (uint32_t) (b * NMAX + c0 + q * 8), x + q * 8);
-                tc::wait_ld();
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sm.s_empty[b]);
-                const bool on = (sm.live[jj % TILES][quarter] >> lane) & 1u;
-                if (!on) {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) x[c] = -INFINITY;
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) x[c] = c < nc ? x[c] * sc : -INFINITY;
-                    if (partly(step)) {
+                    for (int q = 0; q < K; ++q) ld8(from + 8 * q, x + 8 * q);
+                    tc::wait_ld();
+                    if (!plain) {
                         const uint32_t t = (uint32_t) step * TS + (uint32_t) tl;
+                        uint32_t seen = (live >> lane) & 1u ? FULL : 0u;
+                        if (seen && !all)
+#pragma unroll 1
+                            for (int c = 0; c < N; ++c)
+                                if (!sees(t, cp + c)) seen &= ~(1u << c);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (c < nc) {
-                                const bool sees = t >= (uint32_t) s.len ? (info.mask[c0 + c] >> (t - (uint32_t) s.len)) & 1ull : t >= (uint32_t) info.lo[c0 + c];
-                                if (!sees) x[c] = -INFINITY;
-                            }
+                        for (int c = 0; c < N; ++c)
+                            if (!((seen >> c) & 1u)) x[c] = -INFINITY;
                     }
+                };
+                auto shift = [&]() {        // to exponents of the weights
+#pragma unroll
+                    for (int q = 0; q < N / 4; ++q) {
+                        const float4 u = *reinterpret_cast<const float4 *>(&sm.up[cp + q * 4]);
+                        const float2 a = tc::num::fma2(make_float2(x[4 * q], x[4 * q + 1]), sc2, make_float2(u.x, u.y));
+                        const float2 b = tc::num::fma2(make_float2(x[4 * q + 2], x[4 * q + 3]), sc2, make_float2(u.z, u.w));
+                        x[4 * q] = a.x; x[4 * q + 1] = a.y; x[4 * q + 2] = b.x; x[4 * q + 3] = b.y;
+                    }
+                };
+                load();
+                bool renew = fresh;
+                if (!fresh) {
+                    shift();
+                    float top = x[0];
+#pragma unroll
+                    for (int c = 1; c + 1 < N; c += 2) top = fmaxf(fmaxf(top, x[c]), x[c + 1]);
+                    top = fmaxf(top, x[N - 1]);
+                    renew = any_of(bar, top > S::SLACK + S::UP);
+                    if (renew) load();
                 }
-                // scores to differences from the row's maximum in use; a new one where some is too far above
-                bool above = false;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (q * 4 < nc) {
-                        const float4 m = *reinterpret_cast<const float4 *>(&sm.m[c0 + q * 4]);
-                        above |= x[4 * q] > m.x + S::SLACK || x[4 * q + 1] > m.y + S::SLACK || x[4 * q + 2] > m.z + S::SLACK || x[4 * q + 3] > m.w + S::SLACK;
-                    }
-                bool waited = false;
-                __syncwarp();
-                if (any_of(bar, above)) {
-                    const float top = columns32<true>(x, lane);
+                if (renew) {                // a row's first tile, or a score too far above the maximum in use: a new one
+                    const float top = octets<true, K>(x, lane);
                     sm.red[warp][lane] = top;
                     tc::nbar_sync(bar, 128);
-                    if (tid % 128 < nc) {
-                        const int c = tid % 128;
-                        const float old = sm.m[c0 + c];
-                        float m = old;
+                    if (tg < N) {
+                        const float old = sm.m[cp + tg];
+                        float m = -INFINITY;
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm.red[half * 4 + w][c]);
-                        sm.fac[c0 + c] = m == old ? 1.0f : tc::num::ex2(old - m);
-                        sm.m[c0 + c] = m;
+                        for (int w = 0; w < 4; ++w) m = fmaxf(m, sm.red[group * 4 + w][tg]);
+                        m = fmaxf(m * sc, old);
+                        sm.fac[cp + tg] = m == old ? 1.0f : tc::num::ex2(old - m);
+                        sm.m[cp + tg] = m;
+                        sm.up[cp + tg] = m == -INFINITY ? 3e38f : S::UP - m;
                     }
                     tc::nbar_sync(bar, 128);
+                    shift();
+                    if (!fresh) {
 #pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (c < nc) l[c] *= sm.fac[c0 + c];
-                    if (i > 0) {            // O has tiles of this pair
-                        wait.warp(&sm.pv_done, (jj - 1) & 1u);
-                        waited = true;
-                        tc::fence_after_sync();
+                        for (int c = 0; c < N / 2; ++c) {
+                            lp[c].x *= sm.fac[cp + 2 * c];
+                            lp[c].y *= sm.fac[cp + 2 * c + 1];
+                        }
+                        wait_p();           // O has tiles of this pair
 #pragma unroll 1
-                        for (int hf = 0; hf < S::PARTS; ++hf)
+                        for (int part = 0; part < S::PARTS; ++part)
+#pragma unroll 1
+                            for (int q = 0; q < K; ++q) {
+                                const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + cp + q * 8);
+                                float o[8];
+                                ld8(addr, o);
+                                tc::wait_ld();
+                                uint32_t r[8];
 #pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                if (q * 8 < nc) {
-                                    const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + q * 8);
-                                    float o[8];
-                                    ld8(addr, o);
-                                    tc::wait_ld();
-                                    uint32_t r[8];
-#pragma unroll
-                                    for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[c0 + q * 8 + e]);
-                                    tc::st_x8(addr, r);
-                                }
+                                for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[cp + q * 8 + e]);
+                                tc::st_x8(addr, r);
+                            }
                         tc::wait_st();
                     }
                 }
-                if (jj > 0 && !waited) {    // P is free
+                uint32_t hi[N / 2], lw[N / 2];
+#pragma unroll
+                for (int c = 0; c < N / 2; ++c) {
+                    const float2 a = make_float2(tc::num::ex2(x[2 * c]), tc::num::ex2(x[2 * c + 1]));
+                    lp[c] = tc::num::add2(lp[c], a);
+                    hi[c] = pack2<S::TYPE>(a.x, a.y);
+                    const float2 r = tc::num::fma2(widen2<S::TYPE>(hi[c]), make_float2(-1.0f, -1.0f), a);
+                    lw[c] = pack2<S::TYPE>(r.x, r.y);
+                }
+                wait_p();
+#pragma unroll
+                for (int q = 0; q < K; ++q) {
+                    const uint32_t o8 = (uint32_t) (cp >> 3) + (uint32_t) q, off = (o8 >> 3) * (TS * 128) + (uint32_t) tl * 128u + (((o8 ^ (uint32_t) tl) & 7u) << 4);
+                    *reinterpret_cast<uint4 *>(&sm.pt[0][off]) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+                    *reinterpret_cast<uint4 *>(&sm.pt[1][off]) = make_uint4(lw[4 * q], lw[4 * q + 1], lw[4 * q + 2], lw[4 * q + 3]);
+                }
+            };
+            for (int i = 0; i < steps; ++i, ++jj) {
+                const int step = s.step0 + at.st + i;
+                wait.warp(&sm.s_full[jj & 1u], (jj >> 1) & 1u);
+                tc::fence_after_sync();
+                const unsigned live = sm.live[jj % TILES][quarter];
+                bool free_p = jj == 0;      // the products with the tile before are done
+                auto wait_p = [&]() {
+                    if (free_p) return;
+                    free_p = true;
                     wait.warp(&sm.pv_done, (jj - 1) & 1u);
                     tc::fence_after_sync();
-                }
-                if (i > 0 && partly(step - 1)) add_odd(jj - 1, step - 1);
+                };
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q * 8 < nc) {
-                        uint32_t hi[4], lw[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int c = q * 8 + 2 * e;
-                            const float2 m = *reinterpret_cast<const float2 *>(&sm.m[c0 + c]);
-                            const float a = tc::num::ex2(x[c] - (m.x == -INFINITY ? 0.0f : m.x) + S::UP), y = tc::num::ex2(x[c + 1] - (m.y == -INFINITY ? 0.0f : m.y) + S::UP);
-                            l[c] += a;
-                            l[c + 1] += y;
-                            hi[e] = pack2<S::TYPE>(a, y);
-                            const float2 f = widen2<S::TYPE>(hi[e]);
-                            lw[e] = pack2<S::TYPE>(a - f.x, y - f.y);
-                        }
-                        const uint32_t off = (uint32_t) tl * 128u + ((uint32_t) ((((c0 >> 3) + q) ^ tl) & 7) << 4);
-                        *reinterpret_cast<uint4 *>(&sm.pt[0][off]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(&sm.pt[1][off]) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+                for (int ps = 0; ps < S::PASSES; ++ps) {
+                    float2 * lp = l + 16 * ps;
+                    switch (n8 - 4 * ps) {
+                        case 1: octets_of(Int<1>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
+                        case 2: octets_of(Int<2>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
+                        case 3: octets_of(Int<3>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
+                        default: if (n8 > 4 * ps) octets_of(Int<4>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p);
                     }
+                }
+                wait_p();                   // (no thread falls behind a phase)
+                if (i > 0 && partly(step - 1)) add_odd(jj - 1, step - 1);
                 tc::fence_proxy_async();
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&sm.p_full);
+                if (lane == 0) {
+                    tc::mbar_arrive(&sm.s_empty[jj & 1u]);
+                    tc::mbar_arrive(&sm.p_full);
+                }
             }
             // the pair's output, or its partial
-            const float sum = columns32<false>(l, lane);
-            sm.red[warp][lane] = sum;
             wait.warp(&sm.pv_done, (jj - 1) & 1u);
             tc::fence_after_sync();
             if (partly(s.step0 + at.st + steps - 1)) add_odd(jj - 1, s.step0 + at.st + steps - 1);
-            tc::nbar_sync(bar, 128);
             const bool whole = begun && ended;
             const int64_t slot = ((int64_t) blockIdx.x * 2 + (begun ? 1 : 0)) * NMAX;
-            if (tid % 128 < nc) {
-                const int c = tid % 128;
-                const float all = (sm.red[half * 4][c] + sm.red[half * 4 + 1][c]) + (sm.red[half * 4 + 2][c] + sm.red[half * 4 + 3][c]);
-                sm.fac[c0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
-                if (!whole) *reinterpret_cast<float2 *>(p.ml + (slot + c0 + c) * 2) = make_float2(sm.m[c0 + c], all);
+#pragma unroll
+            for (int ps = 0; ps < S::PASSES; ++ps) {
+                float v[32];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) { v[2 * c] = l[16 * ps + c].x; v[2 * c + 1] = l[16 * ps + c].y; }
+                const float sum = columns<false, 32>(v, lane);
+                if (ps) tc::nbar_sync(bar, 128);
+                sm.red[warp][lane] = sum;
+                tc::nbar_sync(bar, 128);
+                const int c = 32 * ps + tg;
+                if (tg < 32 && c < nc) {
+                    const float (* red)[32] = &sm.red[group * 4];
+                    const float all = (red[0][tg] + red[1][tg]) + (red[2][tg] + red[3][tg]);
+                    sm.fac[c0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
+                    if (!whole) *reinterpret_cast<float2 *>(p.ml + (slot + c0 + c) * 2) = make_float2(sm.m[c0 + c], all);
+                }
             }
             if (tid == 0 && begun && !ended)
                 p.split[blockIdx.x] = make_int4(at.seq, h, run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
             tc::nbar_sync(bar, 128);
+            float * part0 = p.part + slot * D;
 #pragma unroll 1
-            for (int hf = 0; hf < S::PARTS; ++hf) {
-                const int d = hf * 128 + tl;
+            for (int part = 0; part < S::PARTS; ++part) {
+                const int d = part * 128 + tl;
+#pragma unroll 1
+                for (int c = 0; c < nc; c += 8) {
+                    float o[8];
+                    ld8(tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c), o);
+                    tc::wait_ld();
+                    if (d < D) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (q * 8 < nc) {
-                        float o[8];
-                        ld8(tmem + lanes + S::COL_O + (uint32_t) (hf * NMAX + c0 + q * 8), o);
-                        tc::wait_ld();
-                        if (d < D) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) {
-                                const int n = c0 + q * 8 + e;
-                                if (n >= s.nr) continue;
-                                if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[n]);
-                                else p.part[(slot + n) * D + d] = o[e];
-                            }
+                        for (int e = 0; e < 8; ++e) {
+                            const int n = c0 + c + e;
+                            if (n >= s.nr) continue;
+                            if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[n]);
+                            else part0[n * D + d] = o[e];
                         }
                     }
+                }
             }
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&sm.o_free);
             tc::nbar_sync(bar, 128);        // the factors have been read
-            at.next(p, tile, steps);
+            at.next(p, tile, NMAX, steps);
         }
     } else if (warp < W_MMA) {
         // ---- K (two warps, 64 positions each) and V (two) ----
@@ -563,6 +618,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 const bool some = t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
                 const bool mend = is_v && (some || (WHOLE && (live[0] & live[1] & live[2] & live[3]) != FULL));
                 uint64_t todo = 0ull;       // of the warp's 64
+                const uint64_t own = (uint64_t) live[2 * wh + 1] << 32 | live[2 * wh];
                 if (mend) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
@@ -622,27 +678,38 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         }
                     }
                     if (mend) {
-                        for (uint64_t left = todo; left; left &= left - 1ull) {
-                            const int r = 64 * wh + __ffsll((long long) left) - 1;
-                            const bool on = (live[r >> 5] >> (r & 31)) & 1u;
-                            bool bad = false;
-                            uint4 * at16 = reinterpret_cast<uint4 *>(dst + (lane >> 3) * (TS * 128) + r * 128 + (((lane ^ r) & 7) << 4));
-                            if (lane < S::CH) {
-                                if (!on) *at16 = make_uint4(0u, 0u, 0u, 0u);
-                                else {
-                                    const uint4 x = *at16;
-                                    bad = odd_word<S::TYPE>(x.x) || odd_word<S::TYPE>(x.y) || odd_word<S::TYPE>(x.z) || odd_word<S::TYPE>(x.w);
+                        // RI rows at a time, a lane per word; four such loads in flight
+                        constexpr int LR = S::CH == 8 ? 8 : 16, RI = 32 / LR;
+                        const int wd = lane % LR;
+                        for (int r0 = 0; r0 < 64; r0 += 4 * RI) {
+                            if (!((todo >> r0) & ((1ull << (4 * RI)) - 1ull))) continue;
+                            uint4 x[4];
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const int r = r0 + u * RI + lane / LR, rt = 64 * wh + r;
+                                uint4 * at16 = reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4));
+                                x[u] = make_uint4(0u, 0u, 0u, 0u);
+                                if (wd < S::CH && ((todo >> r) & 1ull)) {
+                                    if ((own >> r) & 1ull) x[u] = *at16;
+                                    else *at16 = x[u];
                                 }
                             }
-                            if (!__any_sync(FULL, bad)) continue;
-                            odd |= 1ull << (r & 63);
-                            if (bad) {      // its finite neighbours stay
-                                uint32_t * w = reinterpret_cast<uint32_t *>(at16);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) {
+                                const bool bad = odd_word<S::TYPE>(x[u].x) || odd_word<S::TYPE>(x[u].y) || odd_word<S::TYPE>(x[u].z) || odd_word<S::TYPE>(x[u].w);
+                                const unsigned who = __ballot_sync(FULL, bad);
+                                if (!who) continue;
+                                const int r = r0 + u * RI + lane / LR, rt = 64 * wh + r;
+                                for (int v = 0; v < RI; ++v)
+                                    if ((who >> (v * LR)) & ((1ull << LR) - 1ull)) odd |= 1ull << (r0 + u * RI + v);
+                                if (bad) {  // its finite neighbours stay
+                                    uint32_t * w = reinterpret_cast<uint32_t *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4));
 #pragma unroll 1
-                                for (int e = 0; e < 4; ++e) {
-                                    const float2 f = widen2<S::TYPE>(w[e]);
-                                    if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
-                                    if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
+                                    for (int e = 0; e < 4; ++e) {
+                                        const float2 f = widen2<S::TYPE>(w[e]);
+                                        if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
+                                        if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
+                                    }
                                 }
                             }
                         }
@@ -653,7 +720,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                             if (lane == 0) tc::mbar_arrive(&full[slot]);
                         } else tell(pp + 1);
                     } else if (!WHOLE) {
-                        if (slots == 2) tc::cp_async_wait_group<1>();
+                        if (slots == 1) tc::cp_async_wait_group<0>();
+                        else if (slots == 2) tc::cp_async_wait_group<1>();
                         else if (slots == 3) tc::cp_async_wait_group<2>();
                         else tc::cp_async_wait_group<3>();
                         const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;      // parts still on their way
@@ -661,7 +729,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     }
                 }
             }
-            at.next(p, tile, steps);
+            at.next(p, tile, NMAX, steps);
         }
         if (!WHOLE) {
             tc::cp_async_wait_group<0>();
@@ -731,7 +799,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 pend_first = i == 0;
                 if (i == 0) ++items;
             }
-            at.next(p, tile, steps);
+            at.next(p, tile, NMAX, steps);
         }
         if (pend) second(jj - 1);
     } else {
@@ -740,10 +808,10 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             const Seq s = at.s;
             const int steps = at.take(), n = (s.nr + 15) & ~15;
             if (item > 0) wait.warp(&sm.q_empty, (uint32_t) (item - 1) & 1u);
-            Info & info = sm.info[item % INFO];
-            int64_t from[2];
+            Info<NMAX> & info = sm.info[item % INFO];
+            int64_t from[NMAX / 32];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int u = 0; u < NMAX / 32; ++u) {
                 const int r = 32 * u + lane;
                 from[u] = -1;
                 if (r >= n) continue;
@@ -767,7 +835,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 info.lo[r] = lo;
             }
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < NMAX / 32; ++u)
                 if (32 * u < n)
 #pragma unroll 4
                     for (int k = 0; k < D / 8; ++k) {
@@ -777,29 +845,37 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                                        static_cast<const uint16_t *>(p.q.p) + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
                     }
             tc::cp_async_wait_all();
+            if (p.scale <= 0.0f) {          // scores of the other sign, or none
+                __syncwarp();
+                for (int w = lane; w < S::PARTS * S::QP / 16; w += 32) {
+                    uint4 & x = reinterpret_cast<uint4 *>(sm.q)[w];
+                    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale < 0.0f ? FULL : 0u;
+                    x = make_uint4((x.x ^ flip) & keep, (x.y ^ flip) & keep, (x.z ^ flip) & keep, (x.w ^ flip) & keep);
+                }
+            }
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&sm.q_full[item % INFO]);
-            at.next(p, tile, steps);
+            at.next(p, tile, NMAX, steps);
         }
     }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == W_MMA) tc::tmem_dealloc(tmem, 256);
+    if (warp == W_MMA) tc::tmem_dealloc(tmem, S::COLS);
 }
 
 // Joins the runs of a split pair in order. grid: CTAs of the kernel before, rows in groups of 8, a warp each.
 template <int D>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Params p, int type) {
+__global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__ Params p, int type, int nmax) {
     constexpr int NV = (D / 4 + 31) / 32;   // 16-byte words of a lane
     pdl_wait();
     pdl_release();
     const int4 e = p.split[blockIdx.x];
     if (e.x < 0) return;
     const int tile = blockIdx.x % p.tiles, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const Seq s = seq_of(p, e.x, tile);
+    const Seq s = seq_of(p, e.x, tile, nmax);
     if (r >= s.nr) return;
-    auto slot_of = [&](int w) { return (((int64_t) w * p.tiles + tile) * 2 + (w == e.z ? 1 : 0)) * NMAX + r; };
+    auto slot_of = [&](int w) { return (((int64_t) w * p.tiles + tile) * 2 + (w == e.z ? 1 : 0)) * nmax + r; };
     float top = -INFINITY, sum = 0.0f;
     for (int w0 = e.z; w0 <= e.w; w0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
@@ -884,27 +960,30 @@ int run(Params & p, sjk_stream st) {
     const int ctas = p.tiles * p.wl;
     const int rc = p.box >= 8 && maps_of(&p) ? tree_launch<S, true>(p, st) : tree_launch<S, false>(p, st);
     if (rc) return rc;
-    const int rows = p.nodes * p.grp < NMAX ? p.nodes * p.grp : NMAX;
-    return launch(tree_merge_kernel<S::D>, dim3((unsigned) ctas, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE);
+    const int rows = p.nodes * p.grp < S::NMAX ? p.nodes * p.grp : S::NMAX;
+    return launch(tree_merge_kernel<S::D>, dim3((unsigned) ctas, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE, S::NMAX);
 }
 
 template <int TYPE>
-int run_dim(Params & p, sjk_stream st) {
+int run_dim(Params & p, int nmax, sjk_stream st) {
     switch (p.c.head_dim) {
-        case 64: return run<Shape<TYPE, 64>>(p, st);
-        case 96: return run<Shape<TYPE, 96>>(p, st);
-        case 128: return run<Shape<TYPE, 128>>(p, st);
-        default: return run<Shape<TYPE, 256>>(p, st);
+        case 64: return nmax > 64 ? run<Shape<TYPE, 64, 128>>(p, st) : run<Shape<TYPE, 64, 64>>(p, st);
+        case 96: return nmax > 64 ? run<Shape<TYPE, 96, 128>>(p, st) : run<Shape<TYPE, 96, 64>>(p, st);
+        case 128: return nmax > 64 ? run<Shape<TYPE, 128, 128>>(p, st) : run<Shape<TYPE, 128, 64>>(p, st);
+        default: return run<Shape<TYPE, 256, 64>>(p, st);
     }
 }
 
 constexpr int CTAS = 148;
 
+// Rows of a pass: 128 where a KV head has more than 64 and shared memory holds them beside the tiles.
+int rows_of(const sjk_kv16 * c, int64_t rows) { return rows > 64 && c->head_dim <= 128 ? 128 : 64; }
+
 }  // namespace
 
 extern "C" size_t sjk_kv16_attend_tree_scratch_bytes(const sjk_kv16 * c) {
     if (!c || (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)) return 0;
-    return (size_t) CTAS * (2 * NMAX * ((size_t) c->head_dim + 2) * sizeof(float) + sizeof(int4));
+    return (size_t) CTAS * (2 * (size_t) rows_of(c, 128) * ((size_t) c->head_dim + 2) * sizeof(float) + sizeof(int4));
 }
 
 extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int n_tok, const int32_t * first, const int32_t * len,
@@ -921,7 +1000,8 @@ extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int 
     if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
     if (!first && (int64_t) n_seq * nodes != (int64_t) n_tok) return SJKVARN_ERR_ARG;
     const int grp = q->n_head / c->n_head_kv;
-    const int64_t tiles = ((int64_t) nodes * grp + NMAX - 1) / NMAX;
+    const int nmax = rows_of(c, (int64_t) nodes * grp);
+    const int64_t tiles = ((int64_t) nodes * grp + nmax - 1) / nmax;
     if (tiles > CTAS) return SJK_ERR_UNSUPPORTED;
     // a list counts its units in 32 bits
     const double steps = fmin((double) c->table_stride * c->page_tokens, 2147483647.0) / TS + OV + 2;
@@ -939,9 +1019,9 @@ extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int 
     p.tiles = (int) tiles;
     p.wl = CTAS / p.tiles;
     p.part = static_cast<float *>(scratch);
-    p.ml = p.part + (size_t) CTAS * 2 * NMAX * c->head_dim;
-    p.split = reinterpret_cast<int4 *>(p.ml + (size_t) CTAS * 2 * NMAX * 2);
-    return c->type == SJK_F16 ? run_dim<SJK_F16>(p, st) : run_dim<SJK_BF16>(p, st);
+    p.ml = p.part + (size_t) CTAS * 2 * nmax * c->head_dim;
+    p.split = reinterpret_cast<int4 *>(p.ml + (size_t) CTAS * 2 * nmax * 2);
+    return c->type == SJK_F16 ? run_dim<SJK_F16>(p, nmax, st) : run_dim<SJK_BF16>(p, nmax, st);
 }
 
 SJK_STATUS_READER(tree_wait_status_take)
