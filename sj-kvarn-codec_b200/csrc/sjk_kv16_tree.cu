@@ -11,8 +11,8 @@
 //    as M would make 8 of them as dear as 128. K, V and P lie in shared memory as they come: K rows are K-major for the
 //    first product, the same layout of V is MN-major for the second, and a thread, which has a position of all columns,
 //    writes its weights as whole 16-byte words of an MN-major P. S (two buffers) and O live in TMEM.
-//  - Warps: 8 for the softmax (two halves of the columns), 2 that load K, 2 that load V (rings of their own, so that neither
-//    waits for the other's slots), 1 that issues the products, 1 that loads the queries. Linked by mbarriers only; every
+//  - Warps: 8 for the softmax (two halves of the columns), one each that loads K, loads V (rings of their own, so that neither
+//    waits for the other's slots), issues the products, and loads the queries: 12, which leaves 168 registers a thread. Linked by mbarriers only; every
 //    wait is bounded.
 //  - Page tables are read a tile ahead, rows come with 16-byte cp.async into the swizzled layout: any page size, any strides;
 //    positions that are not live are filled with zeros.
@@ -40,7 +40,7 @@ constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int TS = 128;                     // positions of a step
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
 constexpr int MIN_RUN = 2;                  // units of a run, at least
-constexpr int N_SOFT = 8, N_LOAD = 4;       // warps; then one that issues products, and one that loads queries
+constexpr int N_SOFT = 8, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
 constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
 constexpr int INFO = 4, TILES = 16;         // rings of what a pair's rows and a tile's positions are
 __device__ unsigned int g_tree_status;
@@ -92,6 +92,18 @@ SJK_DEV Seq seq_of(const Params & p, int i, int tile, int nmax) {
 }
 SJK_DEV uint32_t units_of(const Params & p, const Seq & s) { return s.steps > 0 ? (uint32_t) p.c.n_head_kv * (uint32_t) (s.steps + OV) : 0u; }
 
+// First committed position that some token of the pair may see, and whether some of its rows see a position of a tile (from
+// t0 on) that others do not: a drafted one, or one at the window's edge.
+SJK_DEV uint32_t low_of(const Params & p, const Seq & s) { return p.window && s.len > p.window ? (uint32_t) (s.len - p.window) : 0u; }
+SJK_DEV bool few_see(const Params & p, const Seq & s, uint32_t t) { return t >= (uint32_t) s.len || (p.window && t < low_of(p, s) + (uint32_t) s.count); }
+SJK_DEV bool partly(const Params & p, const Seq & s, uint32_t t0) { return t0 + TS > (uint32_t) s.len || (p.window && t0 < low_of(p, s) + (uint32_t) s.count); }
+// Groups of 16 positions of a tile that lie in the pair's span (one at least): the second product takes these alone.
+SJK_DEV int end16(const Seq & s, uint32_t t0) { const uint32_t n = s.hi - t0; return n < TS ? (int) ((n + 15u) >> 4) : TS / 16; }
+SJK_DEV int first16(const Params & p, const Seq & s, uint32_t t0) {
+    const uint32_t lo = low_of(p, s);
+    return lo > t0 ? min((int) ((lo - t0) >> 4), end16(s, t0) - 1) : 0;
+}
+
 // A run's place: pair (sequence, KV head), step, units left, unit of the list at which the pair begins.
 struct Cursor {
     int seq, h, st, rem;
@@ -142,7 +154,7 @@ struct Shared {
     uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2][S::PB];
     Info<S::NMAX> info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
-    uint64_t odd[TILES][2];                 // positions whose V row was replaced, of tiles that some rows see only partly
+    alignas(16) uint32_t odd[TILES][4];                 // positions whose V row was replaced, of tiles that some rows see only partly
     float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];       // a row's maximum in use; what its scores are shifted by
     uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
@@ -225,11 +237,11 @@ SJK_DEV float octets(const float * v, int lane) {
         return columns<MAX, 32>(w, lane);
     } else return columns<MAX, 8 * K>(v, lane);
 }
+// the sign bits of halves that are infinities or NaNs: an exponent of all ones carries into them
 template <int TYPE>
-SJK_DEV bool odd_word(uint32_t w) {         // an infinity or NaN among two
-    constexpr uint32_t E = TYPE == SJK_F16 ? 0x7C00u : 0x7F80u;
-    return (w & E) == E || (w & (E << 16)) == (E << 16);
-}
+SJK_DEV uint32_t odd_bits(uint32_t w) { return ((w & 0x7FFF7FFFu) + (TYPE == SJK_F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u; }
+template <int TYPE>
+SJK_DEV uint32_t odd_bits(const uint4 & x) { return odd_bits<TYPE>(x.x) | odd_bits<TYPE>(x.y) | odd_bits<TYPE>(x.z) | odd_bits<TYPE>(x.w); }
 
 // Waits that give up once and for all: after one that ran out (the status word says so) a role goes on without waiting, so
 // that everyone meets the same barriers and the CTA ends.
@@ -240,7 +252,7 @@ struct Waiter {
     }
     SJK_DEV void warp(uint64_t * bar, uint32_t parity) {    // by a whole warp
         (*this)(bar, parity);
-        __syncwarp();
+        dead = __any_sync(FULL, dead);
     }
 };
 
@@ -253,8 +265,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
     const int tile = blockIdx.x % p.tiles, run = blockIdx.x / p.tiles;
 
     if (tid == 0) {
-        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], WHOLE ? 1 : 2); tc::mbar_init(&sm.k_empty[i], 1); }
-        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 2); tc::mbar_init(&sm.v_empty[i], 1); tc::mbar_init(&sm.v_land[i], 1); }
+        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 1); tc::mbar_init(&sm.k_empty[i], 1); }
+        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 1); tc::mbar_init(&sm.v_empty[i], 1); tc::mbar_init(&sm.v_land[i], 1); }
         for (int i = 0; i < 2; ++i) { tc::mbar_init(&sm.s_full[i], 1); tc::mbar_init(&sm.s_empty[i], N_SOFT); }
         tc::mbar_init(&sm.p_full, N_SOFT);
         tc::mbar_init(&sm.pv_done, 1);
@@ -338,16 +350,11 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             for (int c = 0; c < NMAX / 4; ++c) l[c] = make_float2(0.0f, 0.0f);
             tc::nbar_sync(bar, 128);
             wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
-            const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
-            auto partly = [&](int step) {   // some rows see a position of the step that others do not
-                const uint32_t t0 = (uint32_t) step * TS;
-                return t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
-            };
             auto sees = [&](uint32_t t, int n) { return t >= (uint32_t) s.len ? (bool) ((info.mask[n] >> (t - (uint32_t) s.len)) & 1ull) : t >= (uint32_t) info.lo[n]; };
             // non-finite values of V rows that only some rows see, into the sums of those that do
             auto add_odd = [&](uint32_t tile_no, int step) {
-                const uint64_t some[2] = {sm.odd[tile_no % TILES][0], sm.odd[tile_no % TILES][1]};
-                if (!(some[0] | some[1])) return;
+                const uint4 some = *reinterpret_cast<const uint4 *>(sm.odd[tile_no % TILES]);
+                if (!(some.x | some.y | some.z | some.w)) return;
                 const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
                 if (row < 0 || row >= (int64_t) p.c.n_rows) return;
                 const uint32_t * table = p.c.tables + row * p.c.table_stride;
@@ -361,10 +368,10 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         ld8(addr, o);
                         tc::wait_ld();
 #pragma unroll 1
-                        for (int w = 0; w < 2; ++w)
+                        for (int w = 0; w < 4; ++w)
 #pragma unroll 1
-                            for (uint64_t b = some[w]; b; b &= b - 1) {
-                                const uint32_t t = (uint32_t) step * TS + 64u * w + (uint32_t) __ffsll((long long) b) - 1u, g = t / (uint32_t) p.c.page_tokens;
+                            for (uint32_t b = w == 0 ? some.x : w == 1 ? some.y : w == 2 ? some.z : some.w; b; b &= b - 1u) {
+                                const uint32_t t = (uint32_t) step * TS + 32u * w + (uint32_t) __ffs((int) b) - 1u, g = t / (uint32_t) p.c.page_tokens;
                                 const uint32_t page = table[g];
                                 if (page >= p.c.n_pages || d >= D) continue;
                                 const float x = load1(p.c.v, (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride +
@@ -388,7 +395,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 constexpr int K = decltype(kk)::value, N = 8 * K;
                 const uint32_t from = tmem + lanes + S::COL_S + (jj & 1u) * NMAX + (uint32_t) cp;
                 float x[N];
-                const bool all = !partly(step), plain = live == FULL && all;
+                const bool all = !partly(p, s, (uint32_t) step * TS), plain = live == FULL && all;
                 auto load = [&]() {         // products; those of positions that a row does not see: -inf
 #pragma unroll
                     for (int q = 0; q < K; ++q) ld8(from + 8 * q, x + 8 * q);
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     }
                 }
                 wait_p();                   // (no thread falls behind a phase)
-                if (i > 0 && partly(step - 1)) add_odd(jj - 1, step - 1);
+                if (i > 0 && partly(p, s, (uint32_t) (step - 1) * TS)) add_odd(jj - 1, step - 1);
                 tc::fence_proxy_async();
                 tc::fence_before_sync();
                 __syncwarp();
@@ -516,7 +523,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             // the pair's output, or its partial
             wait.warp(&sm.pv_done, (jj - 1) & 1u);
             tc::fence_after_sync();
-            if (partly(s.step0 + at.st + steps - 1)) add_odd(jj - 1, s.step0 + at.st + steps - 1);
+            if (partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) add_odd(jj - 1, s.step0 + at.st + steps - 1);
             const bool whole = begun && ended;
             const int64_t slot = ((int64_t) blockIdx.x * 2 + (begun ? 1 : 0)) * NMAX;
 #pragma unroll
@@ -566,27 +573,86 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             at.next(p, tile, NMAX, steps);
         }
     } else if (warp < W_MMA) {
-        // ---- K (two warps, 64 positions each) and V (two) ----
-        const bool is_v = warp >= N_SOFT + 2;
-        const int wh = (warp - N_SOFT) & 1, slots = is_v ? VS : KS;
+        // ---- K, and V ----
+        const bool is_v = warp == N_SOFT + 1;
+        const int slots = is_v ? VS : KS;
         uint64_t * full = is_v ? sm.v_full : sm.k_full, * empty = is_v ? sm.v_empty : sm.k_empty;
         uint8_t * ring = is_v ? sm.v : sm.k;
         uint32_t jj = 0, pp = 0, told = 0;  // tiles; parts asked for, and announced (not WHOLE)
-        uint32_t landed = 0;                // WHOLE: parity of every slot's v_land
         auto tell = [&](uint32_t upto) {    // copies of the parts before `upto` have landed
             tc::fence_proxy_async();
             __syncwarp();
             for (; told < upto; ++told)
                 if (lane == 0) tc::mbar_arrive(&full[told % slots]);
         };
-        if (WHOLE && !is_v && wh == 1) at.rem = 0;          // one warp asks for all K boxes
+        // A part of a V tile to be mended: rows (todo) that are dead, or that only some query rows see, of slot `slot`.
+        struct Mend { bool on; int slot, part; uint32_t tile; unsigned todo[4], live[4], odd[4]; } m = {};
+        uint32_t landed = 0;                // WHOLE: parity of every slot's v_land
+        auto mend_rows = [&]() {
+            uint8_t * dst = ring + m.slot * S::PART;
+            if (m.part == 0) m.odd[0] = m.odd[1] = m.odd[2] = m.odd[3] = 0u;
+            // RI rows at a time, a lane per word; four such loads in flight
+            constexpr int LR = S::CH == 8 ? 8 : 16, RI = 32 / LR;
+            const int wd = lane % LR;
+            auto word = [&](int rt) { return reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4)); };
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += 4 * RI) {
+                    const unsigned some = (m.todo[g] >> r0) & (4 * RI == 32 ? FULL : (1u << (4 * RI)) - 1u);
+                    if (!some) continue;
+                    uint4 x[4];
+                    uint32_t bad = 0u;
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = r0 + u * RI + lane / LR;
+                        x[u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (wd < S::CH && ((m.todo[g] >> r) & 1u)) {
+                            if ((m.live[g] >> r) & 1u) x[u] = *word(32 * g + r);
+                            else *word(32 * g + r) = x[u];
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) bad |= odd_bits<S::TYPE>(x[u]);
+                    if (!__any_sync(FULL, bad != 0u)) continue;
+#pragma unroll 1
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = r0 + u * RI + lane / LR;
+                        bool here = false;
+                        if (wd < S::CH && ((m.todo[g] >> r) & (m.live[g] >> r) & 1u)) {
+                            uint32_t * w = reinterpret_cast<uint32_t *>(word(32 * g + r));
+#pragma unroll 1
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t o = odd_bits<S::TYPE>(w[e]);
+                                here |= o != 0u;
+                                if (o & 0x8000u) w[e] &= 0xFFFF0000u;       // (its finite neighbours stay)
+                                if (o >> 31) w[e] &= 0x0000FFFFu;
+                            }
+                        }
+                        const unsigned who = __ballot_sync(FULL, here);
+                        for (int v = 0; v < RI; ++v)
+                            if ((who >> (v * LR)) & ((1u << LR) - 1u)) m.odd[g] |= 1u << (r0 + u * RI + v);
+                    }
+                }
+            if (lane == 0)
+                for (int u = 0; u < 4; ++u) sm.odd[m.tile % TILES][u] = m.odd[u];
+        };
+        auto mend_box = [&]() {             // once it has landed
+            m.on = false;
+            wait.warp(&sm.v_land[m.slot], (landed >> m.slot) & 1u);
+            landed ^= 1u << m.slot;
+            mend_rows();
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(&full[m.slot]);
+        };
         while (at.rem > 0) {
             const Seq s = at.s;
             const int steps = at.take();
             const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
             const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
             if (!table && lane == 0) flag();
-            const int lo0 = p.window && s.len > p.window ? s.len - p.window : 0;
+            const uint32_t lo0 = low_of(p, s);
             for (int i = 0; i < steps; ++i, ++jj) {
                 const uint32_t t0 = (uint32_t) (s.step0 + at.st + i) * TS;
                 auto page_at = [&](uint32_t t, uint32_t * place) {
@@ -595,143 +661,105 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     if (page >= p.c.n_pages && page != SJKVARN_NO_BLOCK) flag();
                     return page;
                 };
-                // the tile's live positions, as every warp needs them: four words, or the two of the warp's own 64
-                unsigned live[4] = {0u, 0u, 0u, 0u};
-                int64_t off[2] = {-1, -1};  // rows of the lane's own two positions; -1: none
+                // the tile's live positions (a lane looks up every 32nd), and their rows
+                unsigned live[4];
+                int64_t off[4];             // -1: none
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    if (!WHOLE && (u >> 1) != wh) continue;
                     const uint32_t t = t0 + (uint32_t) (32 * u + lane);
-                    bool on = false;
-                    if (table && t < s.hi && t >= (uint32_t) lo0) {
+                    off[u] = -1;
+                    if (table && t < s.hi && t >= lo0) {
                         uint32_t place;
                         const uint32_t page = page_at(t, &place);
-                        on = page < p.c.n_pages;
-                        if (!WHOLE && on) off[u & 1] = (int64_t) page * p.c.page_stride + (int64_t) place * p.c.slot_stride;
+                        if (page < p.c.n_pages) off[u] = (int64_t) page * p.c.page_stride + (int64_t) place * p.c.slot_stride;
                     }
-                    live[u] = __ballot_sync(FULL, on);
+                    live[u] = __ballot_sync(FULL, off[u] >= 0);
+                    if (!is_v && lane == 0) sm.live[jj % TILES][u] = live[u];
                 }
-                if (!is_v && lane == 0)
-                    for (int u = 0; u < 4; ++u)
-                        if (WHOLE || (u >> 1) == wh) sm.live[jj % TILES][u] = live[u];
-                // V rows that only some rows see (drafted ones, a window's edge), and dead ones that came with a box
-                const bool some = t0 + TS > (uint32_t) s.len || (p.window && t0 < (uint32_t) lo0 + 64u);
-                const bool mend = is_v && (some || (WHOLE && (live[0] & live[1] & live[2] & live[3]) != FULL));
-                uint64_t todo = 0ull;       // of the warp's 64
-                const uint64_t own = (uint64_t) live[2 * wh + 1] << 32 | live[2 * wh];
-                if (mend) {
+                unsigned todo[4] = {0u, 0u, 0u, 0u};
+                if (is_v) {                 // what the second product takes of V: all of a box, but of copies no dead row
+                    const int a16 = first16(p, s, t0), b16 = end16(s, t0);
+                    const bool some = partly(p, s, t0);
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t t = t0 + (uint32_t) (64 * wh + 32 * u + lane);
-                        const bool on = (live[2 * wh + u] >> lane) & 1u;
-                        const bool few = t >= (uint32_t) s.len || (p.window && t < (uint32_t) lo0 + 64u);
-                        todo |= (uint64_t) __ballot_sync(FULL, on ? some && few : WHOLE) << (32 * u);
+                    for (int u = 0; u < 4; ++u) {
+                        const int g16 = (32 * u + lane) >> 4;
+                        todo[u] = __ballot_sync(FULL, off[u] >= 0 ? some && few_see(p, s, t0 + (uint32_t) (32 * u + lane)) : WHOLE && g16 >= a16 && g16 < b16);
                     }
                 }
+                const bool mend = (todo[0] | todo[1] | todo[2] | todo[3]) != 0u;
+                if (is_v && !mend && lane == 0) *reinterpret_cast<uint4 *>(sm.odd[jj % TILES]) = make_uint4(0u, 0u, 0u, 0u);
                 // WHOLE: the lane's box
                 uint32_t place = 0, page = SJKVARN_NO_BLOCK;
                 const uint32_t mine = (uint32_t) (lane / S::BLOCKS) * (uint32_t) p.box;
-                if (WHOLE && mine < TS && t0 + mine < s.hi && t0 + mine + (uint32_t) p.box > (uint32_t) lo0 && table) page = page_at(t0 + mine, &place);
-                const bool asks = WHOLE && wh == 0 && page < p.c.n_pages;
+                if (WHOLE && mine < TS && t0 + mine < s.hi && t0 + mine + (uint32_t) p.box > lo0 && table) page = page_at(t0 + mine, &place);
+                const bool asks = WHOLE && page < p.c.n_pages;
                 const uint32_t tx = WHOLE ? (uint32_t) __popc(__ballot_sync(FULL, asks)) * (uint32_t) p.box * 128u : 0u;
-                uint64_t odd = 0ull;
 #pragma unroll 1
                 for (int part = 0; part < S::PARTS; ++part, ++pp) {
                     const int slot = (int) (pp % (uint32_t) slots);
                     if (pp >= (uint32_t) slots) {
                         const uint32_t parity = (pp / (uint32_t) slots - 1u) & 1u;
-                        if (!WHOLE && !wait.dead && !tc::mbar_test(&empty[slot], parity)) {
-                            tc::cp_async_wait_group<0>();   // nothing more to ask for now: announce what has been
-                            tell(pp);
+                        if ((!WHOLE || m.on) && !wait.dead && !__all_sync(FULL, tc::mbar_test(&empty[slot], parity))) {
+                            // nothing more to ask for now: hand on what has been
+                            if (WHOLE) mend_box();
+                            else {
+                                tc::cp_async_wait_group<0>();
+                                tell(pp);
+                            }
                         }
+                        if (WHOLE && wait.dead && m.on) mend_box();
                         wait.warp(&empty[slot], parity);
                     }
                     uint8_t * dst = ring + slot * S::PART;
                     if constexpr (WHOLE) {
                         uint64_t * bar = mend ? &sm.v_land[slot] : &full[slot];
-                        if (wh == 0) {
-                            if (lane == 0) tc::mbar_expect_tx(bar, tx);
-                            __syncwarp();
-                            if (asks)
-                                box(tc::smem_addr(dst) + (uint32_t) (lane % S::BLOCKS) * (TS * 128) + mine * 128u, &p.maps[is_v ? 1 : 0],
-                                    part * 128 + (lane % S::BLOCKS) * 64, at.h, (int) place, page, bar);
-                        } else if (!mend && lane == 0) tc::mbar_arrive(bar);
-                        if (mend) {
-                            wait.warp(bar, (landed >> slot) & 1u);
-                            landed ^= 1u << slot;
-                        }
-                    } else {
+                        if (lane == 0) tc::mbar_expect_tx(bar, tx);
+                        __syncwarp();
+                        if (asks)
+                            box(tc::smem_addr(dst) + (uint32_t) (lane % S::BLOCKS) * (TS * 128) + mine * 128u, &p.maps[is_v ? 1 : 0],
+                                part * 128 + (lane % S::BLOCKS) * 64, at.h, (int) place, page, bar);
+                        if (m.on) mend_box();           // the one before, while this one is on its way
+                    }
+                    if (mend) {
+                        m.on = WHOLE;
+                        m.slot = slot;
+                        m.part = part;
+                        m.tile = jj;
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) { m.todo[u] = todo[u]; m.live[u] = live[u]; }
+                    }
+                    if constexpr (!WHOLE) {
                         const uint16_t * base = static_cast<const uint16_t *>(is_v ? p.c.v : p.c.k) + (int64_t) at.h * p.c.head_stride + part * 128;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
+                        for (int u = 0; u < 4; ++u)
 #pragma unroll 4
                             for (int k = 0; k < S::CH; ++k) {
                                 const int w = k * 32 + lane, r = w / S::CH, c = w - r * S::CH;
                                 const int64_t o = __shfl_sync(FULL, off[u], r);
-                                tc::cp_async16(dst + (c >> 3) * (TS * 128) + (64 * wh + 32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8,
-                                               o >= 0 ? 16u : 0u);
+                                tc::cp_async16(dst + (c >> 3) * (TS * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
                             }
                         tc::cp_async_commit();
                         if (mend) {
                             tc::cp_async_wait_group<0>();
                             __syncwarp();
+                            mend_rows();
+                            tell(pp + 1);
+                        } else {
+                            if (slots == 1) tc::cp_async_wait_group<0>();
+                            else if (slots == 2) tc::cp_async_wait_group<1>();
+                            else if (slots == 3) tc::cp_async_wait_group<2>();
+                            else tc::cp_async_wait_group<3>();
+                            const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;  // parts still on their way
+                            if (pp + 1 > flight) tell(pp + 1 - flight);
                         }
-                    }
-                    if (mend) {
-                        // RI rows at a time, a lane per word; four such loads in flight
-                        constexpr int LR = S::CH == 8 ? 8 : 16, RI = 32 / LR;
-                        const int wd = lane % LR;
-                        for (int r0 = 0; r0 < 64; r0 += 4 * RI) {
-                            if (!((todo >> r0) & ((1ull << (4 * RI)) - 1ull))) continue;
-                            uint4 x[4];
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                const int r = r0 + u * RI + lane / LR, rt = 64 * wh + r;
-                                uint4 * at16 = reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4));
-                                x[u] = make_uint4(0u, 0u, 0u, 0u);
-                                if (wd < S::CH && ((todo >> r) & 1ull)) {
-                                    if ((own >> r) & 1ull) x[u] = *at16;
-                                    else *at16 = x[u];
-                                }
-                            }
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) {
-                                const bool bad = odd_word<S::TYPE>(x[u].x) || odd_word<S::TYPE>(x[u].y) || odd_word<S::TYPE>(x[u].z) || odd_word<S::TYPE>(x[u].w);
-                                const unsigned who = __ballot_sync(FULL, bad);
-                                if (!who) continue;
-                                const int r = r0 + u * RI + lane / LR, rt = 64 * wh + r;
-                                for (int v = 0; v < RI; ++v)
-                                    if ((who >> (v * LR)) & ((1ull << LR) - 1ull)) odd |= 1ull << (r0 + u * RI + v);
-                                if (bad) {  // its finite neighbours stay
-                                    uint32_t * w = reinterpret_cast<uint32_t *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4));
-#pragma unroll 1
-                                    for (int e = 0; e < 4; ++e) {
-                                        const float2 f = widen2<S::TYPE>(w[e]);
-                                        if (!(fabsf(f.x) < INFINITY)) w[e] &= 0xFFFF0000u;
-                                        if (!(fabsf(f.y) < INFINITY)) w[e] &= 0x0000FFFFu;
-                                    }
-                                }
-                            }
-                        }
-                        if (lane == 0) sm.odd[jj % TILES][wh] = odd;
-                        if (WHOLE) {
-                            tc::fence_proxy_async();
-                            __syncwarp();
-                            if (lane == 0) tc::mbar_arrive(&full[slot]);
-                        } else tell(pp + 1);
-                    } else if (!WHOLE) {
-                        if (slots == 1) tc::cp_async_wait_group<0>();
-                        else if (slots == 2) tc::cp_async_wait_group<1>();
-                        else if (slots == 3) tc::cp_async_wait_group<2>();
-                        else tc::cp_async_wait_group<3>();
-                        const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;      // parts still on their way
-                        if (pp + 1 > flight) tell(pp + 1 - flight);
                     }
                 }
             }
             at.next(p, tile, NMAX, steps);
         }
-        if (!WHOLE) {
+        if (WHOLE) {
+            if (m.on) mend_box();
+        } else {
             tc::cp_async_wait_group<0>();
             tell(pp);
         }
@@ -741,7 +769,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         const uint32_t ka = tc::smem_addr(sm.k), va = tc::smem_addr(sm.v), qa = tc::smem_addr(sm.q), pa = tc::smem_addr(sm.pt);
         const uint32_t tm = __shfl_sync(FULL, tmem, 0);
         uint32_t jj = 0, kp = 0, vp = 0;                     // tiles; parts of K and of V
-        int pend_n = 0, items = 0;
+        int pend_n = 0, pend_a = 0, pend_b = 0, items = 0;
         bool pend = false, pend_first = false;               // a tile whose second product is to come
         auto second = [&](uint32_t j) {                      // O^T += V^T P of tile j
             if (pend_first && items > 1) wait.warp(&sm.o_free, (uint32_t) (items - 2) & 1u);
@@ -755,9 +783,17 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 const uint64_t a = swizzled(va + slot * S::PART, D == 64 ? 0u : TS * 128u), b = swizzled(pa, TS * 128u);
                 const uint32_t d = tm + S::COL_O + (uint32_t) (part * NMAX);
                 if (leader && !wait.dead) {
+                    if (pend_b - pend_a == TS / 16) {
 #pragma unroll
-                    for (int k = 0; k < 2 * TS / 16; ++k)
-                        mma_ss(d, a + (uint64_t) ((k & 7) * 2048 >> 4), b + (uint64_t) (((k >> 3) * S::PB + (k & 7) * 2048) >> 4), id, pend_first && k == 0 ? 0u : 1u);
+                        for (int k = 0; k < 2 * TS / 16; ++k)
+                            mma_ss(d, a + (uint64_t) ((k & 7) * 2048 >> 4), b + (uint64_t) (((k >> 3) * S::PB + (k & 7) * 2048) >> 4), id, pend_first && k == 0 ? 0u : 1u);
+                    } else {
+#pragma unroll 1
+                        for (int k = pend_a; k < pend_b; ++k) {
+                            mma_ss(d, a + (uint64_t) (k * 2048 >> 4), b + (uint64_t) (k * 2048 >> 4), id, pend_first && k == pend_a ? 0u : 1u);
+                            mma_ss(d, a + (uint64_t) (k * 2048 >> 4), b + (uint64_t) ((S::PB + k * 2048) >> 4), id, 1u);
+                        }
+                    }
                     tc::mma_commit(&sm.v_empty[slot]);
                     if (part + 1 == S::PARTS) tc::mma_commit(&sm.pv_done);
                 }
@@ -796,6 +832,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 if (pend) second(jj - 1);
                 pend = true;
                 pend_n = n;
+                pend_a = first16(p, at.s, (uint32_t) (at.s.step0 + at.st + i) * TS);
+                pend_b = end16(at.s, (uint32_t) (at.s.step0 + at.st + i) * TS);
                 pend_first = i == 0;
                 if (i == 0) ++items;
             }
