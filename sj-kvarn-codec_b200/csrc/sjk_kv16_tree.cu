@@ -40,7 +40,8 @@ constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int TS = 128;                     // positions of a step
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
 constexpr int MIN_RUN = 2;                  // units of a run, at least
-constexpr int N_SOFT = 8, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
+constexpr int GROUPS = 4;                   // of softmax warps, which divide the columns
+constexpr int N_SOFT = 4 * GROUPS, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
 constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
 constexpr int INFO = 4, TILES = 16;         // rings of what a pair's rows and a tile's positions are
 __device__ unsigned int g_tree_status;
@@ -139,10 +140,10 @@ struct Info {
 template <int TYPE_, int D_, int NMAX_>
 struct Shape {
     static constexpr int TYPE = TYPE_, D = D_, NMAX = NMAX_;        // NMAX: query rows of a pass
-    static constexpr int PASSES = NMAX / 64;                        // of 32 columns of a softmax thread
+    static constexpr int MINE = NMAX / GROUPS, PASSES = MINE / 16;        // columns of a softmax thread, 16 at a time
     static constexpr int PARTS = (D + 127) / 128, BLOCKS = D == 64 ? 1 : 2;          // M tiles of O; 64-channel blocks of one
     static constexpr int CH = D / 8 < 16 ? D / 8 : 16;                               // words of a row in a part
-    static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = PASSES * TS * 128;  // bytes: part of a K or V tile, of Q; term of P
+    static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = NMAX / 64 * TS * 128;  // bytes: part of a K or V tile, of Q; term of P
     // slots (parts) of K and of V: what 227 KB hold beside Q and P
     static constexpr int KS = D == 64 ? (NMAX > 64 ? 4 : 5) : D == 256 || NMAX > 64 ? 2 : 3, VS = D == 64 ? (NMAX > 64 ? 3 : 4) : NMAX > 64 ? 1 : 2;
     static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX, COLS = NMAX > 64 ? 512 : 256;     // of TMEM
@@ -334,12 +335,13 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         // scores are positive multiples of the products (the queries' signs are turned for a negative scale)
         const float sc = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
         const float2 sc2 = make_float2(sc, sc);
-        float2 l[NMAX / 4];                 // sums of the thread's columns, in pairs
+        float2 l[S::MINE / 2];              // sums of the thread's columns, in pairs
         uint32_t jj = 0;                    // tiles so far
         for (int item = 0; at.rem > 0; ++item) {
             const Seq s = at.s;
             const int steps = at.take(), h = at.h;
-            const int n8 = (s.nr + 15) / 16, c0 = group * n8 * 8, nc = n8 * 8;      // octets of columns, first and number of columns
+            const int all8 = (s.nr + 15) / 16 * 2, most8 = (all8 + GROUPS - 1) / GROUPS;
+            const int n8 = max(0, min(most8, all8 - group * most8)), c0 = group * most8 * 8, nc = n8 * 8;    // octets of columns, first column, their number
             const bool begun = at.st == 0, ended = at.st + steps == s.steps;
             const Info<NMAX> & info = sm.info[item % INFO];
             if (tg < nc) {
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 sm.up[c0 + tg] = 3e38f;     // (no score so far: any is above)
             }
 #pragma unroll
-            for (int c = 0; c < NMAX / 4; ++c) l[c] = make_float2(0.0f, 0.0f);
+            for (int c = 0; c < S::MINE / 2; ++c) l[c] = make_float2(0.0f, 0.0f);
             tc::nbar_sync(bar, 128);
             wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
             auto sees = [&](uint32_t t, int n) { return t >= (uint32_t) s.len ? (bool) ((info.mask[n] >> (t - (uint32_t) s.len)) & 1ull) : t >= (uint32_t) info.lo[n]; };
@@ -502,13 +504,9 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 };
 #pragma unroll
                 for (int ps = 0; ps < S::PASSES; ++ps) {
-                    float2 * lp = l + 16 * ps;
-                    switch (n8 - 4 * ps) {
-                        case 1: octets_of(Int<1>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
-                        case 2: octets_of(Int<2>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
-                        case 3: octets_of(Int<3>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p); break;
-                        default: if (n8 > 4 * ps) octets_of(Int<4>(), c0 + 32 * ps, lp, i == 0, step, live, wait_p);
-                    }
+                    const int m8 = n8 - 2 * ps;
+                    if (m8 == 1) octets_of(Int<1>(), c0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
+                    else if (m8 > 1) octets_of(Int<2>(), c0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
                 }
                 wait_p();                   // (no thread falls behind a phase)
                 if (i > 0 && partly(p, s, (uint32_t) (step - 1) * TS)) add_odd(jj - 1, step - 1);
@@ -528,15 +526,16 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             const int64_t slot = ((int64_t) blockIdx.x * 2 + (begun ? 1 : 0)) * NMAX;
 #pragma unroll
             for (int ps = 0; ps < S::PASSES; ++ps) {
-                float v[32];
+                constexpr int N = 16;
+                float v[N];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) { v[2 * c] = l[16 * ps + c].x; v[2 * c + 1] = l[16 * ps + c].y; }
-                const float sum = columns<false, 32>(v, lane);
+                for (int c = 0; c < N / 2; ++c) { v[2 * c] = l[8 * ps + c].x; v[2 * c + 1] = l[8 * ps + c].y; }
+                const float sum = columns<false, N>(v, lane);
                 if (ps) tc::nbar_sync(bar, 128);
                 sm.red[warp][lane] = sum;
                 tc::nbar_sync(bar, 128);
-                const int c = 32 * ps + tg;
-                if (tg < 32 && c < nc) {
+                const int c = 16 * ps + tg;
+                if (tg < N && c < nc) {
                     const float (* red)[32] = &sm.red[group * 4];
                     const float all = (red[0][tg] + red[1][tg]) + (red[2][tg] + red[3][tg]);
                     sm.fac[c0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
