@@ -63,23 +63,24 @@ SJK_DEV uint4 pick8(const uint4 & a, const uint4 & b) {
     return make_uint4(pick2<TYPE, MAX>(a.x, b.x), pick2<TYPE, MAX>(a.y, b.y), pick2<TYPE, MAX>(a.z, b.z), pick2<TYPE, MAX>(a.w, b.w));
 }
 
-// grid: sequences, CTAs that take a sequence's pages in turn, layers. A thread has a 16-byte word of a token's key row
-// (all heads side by side) and every TG-th token of the page; groups of threads join in shared memory.
+// A warp takes 32 neighbouring 16-byte words of a page's key rows (all heads side by side; fewer words: several tokens at a
+// time), BATCH rows in flight. grid: sequences, CTAs whose warps take a sequence's (page, words) in turn, layers.
 template <int TYPE>
 __global__ void __launch_bounds__(NT) bounds_kernel(const __grid_constant__ BoundParams p) {
     constexpr int BATCH = 8;
-    __shared__ uint4 s_lo[NT], s_hi[NT];
     pdl_wait();
     pdl_release();
-    const int i = blockIdx.x, P = p.c.page_tokens, per = p.c.head_dim / 8, words = p.c.n_head_kv * per;
+    const int i = blockIdx.x, lane = threadIdx.x & 31, P = p.c.page_tokens, per = p.c.head_dim / 8, words = p.c.n_head_kv * per;
     const uint32_t * table = table_of(p.c, p.rows, i);
     const int first = max(p.first[i], 0), end = fit(p.c, p.end[i]);
     if (!table || first >= end) return;
     const uint16_t * keys = static_cast<const uint16_t *>(p.c.k) + (int64_t) blockIdx.z * p.layer_stride;
     uint4 * out = reinterpret_cast<uint4 *>(p.bounds + (int64_t) blockIdx.z * p.b_layer_stride);
-    const int span = words < NT ? words : NT, TG = NT / span, tg = threadIdx.x / span, w0 = threadIdx.x - tg * span;
-    const int last = (end - 1) / P;
-    for (int g = first / P + (int) blockIdx.y; g <= last; g += (int) gridDim.y) {
+    const int span = words < 32 ? words : 32, rows = 32 / span, at = lane / span, groups = (words + 31) / 32;
+    const int g0 = first / P;
+    const int64_t units = (int64_t) ((end - 1) / P - g0 + 1) * groups;
+    for (int64_t u = (int64_t) blockIdx.y * (NT / 32) + (threadIdx.x >> 5); u < units; u += (int64_t) gridDim.y * (NT / 32)) {
+        const int g = g0 + (int) (u / groups), w = (int) (u % groups) * 32 + lane - at * span, h = w / per;
         const uint32_t page = table[g];
         if (page >= p.c.n_pages) {
             if (page != SJKVARN_NO_BLOCK) flag();
@@ -87,41 +88,35 @@ __global__ void __launch_bounds__(NT) bounds_kernel(const __grid_constant__ Boun
         }
         const int64_t left = (int64_t) end - (int64_t) g * P;
         const int live = (int) (left < P ? left : P);
-        for (int wb = 0; wb < words; wb += span) {
-            const int w = wb + w0, h = w / per;
-            const bool on = tg < TG && w < words;
-            const uint16_t * src = keys + (int64_t) page * p.c.page_stride + (int64_t) h * p.c.head_stride + (w - h * per) * 8;
-            uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-            if (on) {
-                // a thread without a token of its own takes the first one
-                lo = hi = *reinterpret_cast<const uint4 *>(src + (int64_t) (tg < live ? tg : 0) * p.c.slot_stride);
-                for (int t0 = tg + TG; t0 < live; t0 += BATCH * TG) {
-                    uint4 x[BATCH];
+        const bool on = at < rows && w < words;
+        const uint16_t * src = keys + (int64_t) page * p.c.page_stride + (int64_t) h * p.c.head_stride + (w - h * per) * 8;
+        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+        if (on) {
+            // (a lane without a token of its own takes the first one)
+            lo = hi = *reinterpret_cast<const uint4 *>(src + (int64_t) (at < live ? at : 0) * p.c.slot_stride);
+            for (int t0 = at + rows; t0 < live; t0 += BATCH * rows) {
+                uint4 x[BATCH];
 #pragma unroll
-                    for (int b = 0; b < BATCH; ++b) {
-                        const int t = t0 + b * TG;
-                        x[b] = *reinterpret_cast<const uint4 *>(src + (int64_t) (t < live ? t : t0) * p.c.slot_stride);
-                    }
-#pragma unroll
-                    for (int b = 0; b < BATCH; ++b) { lo = pick8<TYPE, false>(lo, x[b]); hi = pick8<TYPE, true>(hi, x[b]); }
+                for (int b = 0; b < BATCH; ++b) {
+                    const int t = t0 + b * rows;
+                    x[b] = *reinterpret_cast<const uint4 *>(src + (int64_t) (t < live ? t : t0) * p.c.slot_stride);
                 }
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b) { lo = pick8<TYPE, false>(lo, x[b]); hi = pick8<TYPE, true>(hi, x[b]); }
             }
-            if (TG > 1) {
-                s_lo[threadIdx.x] = lo;
-                s_hi[threadIdx.x] = hi;
-                __syncthreads();
-                if (tg == 0 && on)
-                    for (int q = 1; q < TG; ++q) {
-                        lo = pick8<TYPE, false>(lo, s_lo[q * span + w0]);
-                        hi = pick8<TYPE, true>(hi, s_hi[q * span + w0]);
-                    }
-                __syncthreads();
-            }
-            if (tg == 0 && on) {
-                uint4 * dst = out + (int64_t) page * 2 * words + w;
-                dst[0] = lo;
-                dst[words] = hi;
-            }
+        }
+        __syncwarp();
+        for (int r = 1; r < rows; ++r) {
+            const int from = (lane + r * span) & 31;        // (what lanes behind the first row's get is not used)
+            uint4 a, b;
+            a.x = __shfl_sync(FULL, lo.x, from); a.y = __shfl_sync(FULL, lo.y, from); a.z = __shfl_sync(FULL, lo.z, from); a.w = __shfl_sync(FULL, lo.w, from);
+            b.x = __shfl_sync(FULL, hi.x, from); b.y = __shfl_sync(FULL, hi.y, from); b.z = __shfl_sync(FULL, hi.z, from); b.w = __shfl_sync(FULL, hi.w, from);
+            if (at == 0) { lo = pick8<TYPE, false>(lo, a); hi = pick8<TYPE, true>(hi, b); }
+        }
+        if (on && at == 0) {
+            uint4 * dst = out + (int64_t) page * 2 * words + w;
+            dst[0] = lo;
+            dst[words] = hi;
         }
     }
 }
@@ -163,30 +158,45 @@ SJK_DEV uint64_t order_of(double x) {
 }
 constexpr uint64_t NEVER = 0ull, ALWAYS = ~0ull;            // no page; first and newest ones
 
-// A warp scores 32 pages of a (sequence, KV head) at a time: a lane has 8 channels of one side (16 where D is 256), and
-// 32 partial sums, which an exchange by halves leaves in the lane of each page. grid: sequences, heads, groups of pages.
+// A warp scores PG pages of a (sequence, KV head) at a time: a lane has 8 channels of one side (16 where D is 256), and a
+// partial sum of every page, which an exchange by halves leaves in the lane of each page. The CTA makes the weights, which
+// all its warps share. grid: sequences, heads, groups of pages. Smaller groups of pages make more warps, whose loads are out
+// at the same time (one sequence of 6,250 pages, 8 heads).
+constexpr int NQ = 128, PG = 16;            // threads; pages of a warp at a time
 template <int TYPE, int D>
-__global__ void __launch_bounds__(NT) score_kernel(const __grid_constant__ SelectParams p) {
+__global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ SelectParams p) {
     constexpr int WORDS = D / 8, NW = D == 256 ? 2 : 1;     // words of a side; words of a lane
     constexpr int HALF = D == 64 ? 2 : 1;                   // pages of one load
+    constexpr int NA = PG / HALF;                           // loads
+    __shared__ double s_w[2][D];                            // sums over the group's heads of the queries below and above zero
     pdl_wait();
     pdl_release();
     const int lane = threadIdx.x & 31, i = blockIdx.x, h = blockIdx.y, P = p.c.page_tokens;
     const int len = fit(p.c, p.len[i]), nb = (int) (((int64_t) len + P - 1) / P);
     const uint32_t * table = table_of(p.c, p.rows, i);
     uint64_t * keys = p.keys + ((int64_t) i * p.c.n_head_kv + h) * p.c.table_stride;
-    const int step = (int) gridDim.z * (NT / 32) * 32, b00 = ((int) blockIdx.z * (NT / 32) + (int) (threadIdx.x >> 5)) * 32;
-    if (b00 >= nb) return;
+    constexpr int CTA = NQ / 32 * PG;                       // pages of a CTA at a time
+    if ((int64_t) blockIdx.z * CTA >= nb) return;
     if (!table || nb <= p.budget) {                         // all pages
-        for (int b0 = b00; b0 < nb; b0 += step)
-            if (b0 + lane < nb) {
-                const uint32_t page = table ? table[b0 + lane] : SJKVARN_NO_BLOCK;
-                if (page >= p.c.n_pages && page != SJKVARN_NO_BLOCK) flag();
-                keys[b0 + lane] = page < p.c.n_pages ? ALWAYS : NEVER;
-            }
+        for (int64_t b = (int64_t) blockIdx.z * NQ + threadIdx.x; b < nb; b += (int64_t) gridDim.z * NQ) {
+            const uint32_t page = table ? table[b] : SJKVARN_NO_BLOCK;
+            if (page >= p.c.n_pages && page != SJKVARN_NO_BLOCK) flag();
+            keys[b] = page < p.c.n_pages ? ALWAYS : NEVER;
+        }
         return;
     }
-    // weights of the lane's channels
+    for (int d = threadIdx.x; d < D; d += NQ) {
+        const int64_t q0 = (int64_t) i * p.q.row_stride + (int64_t) h * p.grp * p.q.head_stride + d;
+        double down = 0.0, up = 0.0;
+        for (int g = 0; g < p.grp; ++g) {
+            const double x = (double) load1(p.q.p, q0 + (int64_t) g * p.q.head_stride, p.q.type);
+            down += x > 0.0 ? 0.0 : x;                      // (a NaN goes to one of them, and from there to every score)
+            up += x > 0.0 ? x : 0.0;
+        }
+        s_w[0][d] = down * weight_by<TYPE>();
+        s_w[1][d] = up * weight_by<TYPE>();
+    }
+    __syncthreads();
     const int sub = HALF == 2 ? lane & 15 : lane;
     const int side = NW == 2 ? 0 : sub / WORDS, c0 = NW == 2 ? lane : sub - side * WORDS;    // (D = 256: a word of both sides)
     const bool on = NW == 2 || sub < 2 * WORDS;
@@ -194,122 +204,120 @@ __global__ void __launch_bounds__(NT) score_kernel(const __grid_constant__ Selec
 #pragma unroll
     for (int n = 0; n < NW; ++n)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) wt[n][e] = 0.0;
-    if (on) {
-        const int64_t q0 = (int64_t) i * p.q.row_stride + (int64_t) h * p.grp * p.q.head_stride + c0 * 8;
-        for (int g = 0; g < p.grp; ++g)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const double x = (double) load1(p.q.p, q0 + (int64_t) g * p.q.head_stride + e, p.q.type);
-                if (NW == 2) { wt[0][e] += x < 0.0 ? x : 0.0; wt[NW - 1][e] += x > 0.0 ? x : 0.0; }
-                else wt[0][e] += side ? (x > 0.0 ? x : 0.0) : (x < 0.0 ? x : 0.0);
-                if (x != x) wt[0][e] = x;
-            }
-#pragma unroll
-        for (int n = 0; n < NW; ++n)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) wt[n][e] *= weight_by<TYPE>();
-    }
+        for (int e = 0; e < 8; ++e) wt[n][e] = on ? s_w[NW == 2 ? n : side][c0 * 8 + e] : 0.0;
     const int64_t row_words = (int64_t) p.c.n_head_kv * WORDS;
     const uint4 * base = reinterpret_cast<const uint4 *>(p.bounds) + (int64_t) h * WORDS + side * row_words + c0;
-    for (int b0 = b00; b0 < nb; b0 += step) {
-        const int b = b0 + lane;
+    for (int64_t b0 = (int64_t) blockIdx.z * CTA + (threadIdx.x >> 5) * PG; b0 < nb; b0 += (int64_t) gridDim.z * CTA) {
+        const int64_t b = b0 + (lane & (PG - 1));
         uint32_t page = SJKVARN_NO_BLOCK;
         if (b < nb) page = table[b];
         const bool have = page < p.c.n_pages;
         if (!have && page != SJKVARN_NO_BLOCK) flag();
         const uint32_t read = have ? page : 0u;
-        double acc[32 / HALF];
+        double acc[NA];
+        uint4 x[NA][NW];
 #pragma unroll
-        for (int u0 = 0; u0 < 32 / HALF; u0 += 8) {
-            uint4 x[8][NW];
+        for (int u = 0; u < NA; ++u) {
+            // (D = 64: the lower lanes have page u, the upper ones the one NA after it)
+            const uint32_t at = __shfl_sync(FULL, read, HALF == 2 ? u + (lane >> 4) * NA : u);
+            const uint4 * src = base + (int64_t) at * 2 * row_words;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                // (D = 64: the lower lanes have page u0 + u, the upper ones the one 16 after it)
-                const uint32_t at = __shfl_sync(FULL, read, HALF == 2 ? u0 + u + (lane & 16) : u0 + u);
-                const uint4 * src = base + (int64_t) at * 2 * row_words;
+            for (int n = 0; n < NW; ++n) x[u][n] = on ? src[n * row_words] : make_uint4(0u, 0u, 0u, 0u);
+        }
 #pragma unroll
-                for (int n = 0; n < NW; ++n) x[u][n] = on ? src[n * row_words] : make_uint4(0u, 0u, 0u, 0u);
-            }
+        for (int u = 0; u < NA; ++u) {
+            double s = 0.0;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                double s = 0.0;
+            for (int n = 0; n < NW; ++n) {
+                const uint32_t w[4] = {x[u][n].x, x[u][n].y, x[u][n].z, x[u][n].w};
+                if (odd2<TYPE>(w[0]) || odd2<TYPE>(w[1]) || odd2<TYPE>(w[2]) || odd2<TYPE>(w[3])) {
 #pragma unroll
-                for (int n = 0; n < NW; ++n) {
-                    const uint32_t w[4] = {x[u][n].x, x[u][n].y, x[u][n].z, x[u][n].w};
-                    if (odd2<TYPE>(w[0]) || odd2<TYPE>(w[1]) || odd2<TYPE>(w[2]) || odd2<TYPE>(w[3])) {
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 f = widen2<TYPE>(w[e]);
+                        s = fma((double) f.x * moved_by<TYPE>(), wt[n][2 * e], s);
+                        s = fma((double) f.y * moved_by<TYPE>(), wt[n][2 * e + 1], s);
+                    }
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 f = widen2<TYPE>(w[e]);
-                            s = fma((double) f.x * moved_by<TYPE>(), wt[n][2 * e], s);
-                            s = fma((double) f.y * moved_by<TYPE>(), wt[n][2 * e + 1], s);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            s = fma(moved<TYPE>(w[e] << 16), wt[n][2 * e], s);
-                            s = fma(moved<TYPE>(w[e]), wt[n][2 * e + 1], s);
-                        }
+                    for (int e = 0; e < 4; ++e) {
+                        s = fma(moved<TYPE>(w[e] << 16), wt[n][2 * e], s);
+                        s = fma(moved<TYPE>(w[e]), wt[n][2 * e + 1], s);
                     }
                 }
-                acc[u0 + u] = s;
             }
+            acc[u] = s;
         }
-        // lane l gets the sum of page l (of its half)
+        // lane l gets the sum of page l % NA (of its half's)
 #pragma unroll
-        for (int o = 16 / HALF; o; o >>= 1)
+        for (int o = NA / 2; o; o >>= 1)
 #pragma unroll
             for (int u = 0; u < o; ++u) {
                 const bool up = lane & o;
                 const double send = up ? acc[u] : acc[u + o], keep = up ? acc[u + o] : acc[u];
                 acc[u] = keep + __shfl_xor_sync(FULL, send, o);
             }
-        if (b < nb) keys[b] = !have ? NEVER : b < p.sink || b >= nb - p.recent ? ALWAYS : order_of(acc[0]);
+#pragma unroll
+        for (int o = NA; o < 32 / HALF; o <<= 1) acc[0] += __shfl_xor_sync(FULL, acc[0], o);
+        // (D = 64: pages 8 to 15 are in the upper half)
+        const double mine = HALF == 2 ? __shfl_sync(FULL, acc[0], (lane & (NA - 1)) + ((lane & (PG - 1)) / NA) * 16) : acc[0];
+        if (lane < PG && b < nb) keys[b] = !have ? NEVER : b < p.sink || b >= nb - p.recent ? ALWAYS : order_of(mine);
     }
 }
 
 // ---- select: the largest `budget` keys of a list ------------------------------------------------------------------
-constexpr int NS = 512;
-// Sum over the CTA; every thread gets it. One barrier: successive calls take the places by turns.
-SJK_DEV uint32_t cta_sum(uint32_t x, uint32_t (*s)[NS / 32], int turn) {
-    x = __reduce_add_sync(FULL, x);
-    if ((threadIdx.x & 31) == 0) s[turn & 1][threadIdx.x >> 5] = x;
+constexpr int NS = 1024, KR = 8;            // threads; keys that a thread holds in registers
+// Sums of three counts over the CTA (each at most 1,023 a warp); every thread gets them. One barrier: successive calls
+// take the places by turns.
+struct Three { uint32_t a, b, c; };
+SJK_DEV Three cta_sums(uint32_t a, uint32_t b, uint32_t c, uint32_t (*s)[3][NS / 32], int turn) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    a = __reduce_add_sync(FULL, a);
+    b = __reduce_add_sync(FULL, b);
+    c = __reduce_add_sync(FULL, c);
+    if (lane == 0) { s[turn & 1][0][warp] = a; s[turn & 1][1][warp] = b; s[turn & 1][2][warp] = c; }
     __syncthreads();
-    uint32_t all = 0;
-#pragma unroll
-    for (int w = 0; w < NS / 32; ++w) all += s[turn & 1][w];
-    return all;
+    return {__reduce_add_sync(FULL, s[turn & 1][0][lane]), __reduce_add_sync(FULL, s[turn & 1][1][lane]), __reduce_add_sync(FULL, s[turn & 1][2][lane])};
 }
 
-// A CTA per (sequence, head): the threshold by bisection over the keys' bits from the first one in which they differ (a
-// count of the keys above a middle each time, until exactly `budget` are left), then the keys above it and the first of
-// those equal to it, in ascending order of their pages. No atomics: the same lists every time.
-__global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ SelectParams p, int room) {
-    extern __shared__ uint64_t s_keys[];
-    __shared__ uint32_t s_sum[2][NS / 32];
+// A CTA per (sequence, head): the threshold by a search that quarters the range of the keys (counts of the keys above three
+// places in it each time, until exactly as many are left as are wanted), then the keys above it and the first of those
+// equal to it, in ascending order of their pages. A thread has a run of KR pages in registers; lists of more than NS KR pages
+// are read anew in every round. No atomics: the same lists every time.
+template <bool NEAR>
+__global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ SelectParams p) {
+    __shared__ uint32_t s_sum[2][3][NS / 32];
     __shared__ uint64_t s_min[NS / 32], s_max[NS / 32];
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = blockIdx.x, h = blockIdx.y, P = p.c.page_tokens;
     const int64_t list = (int64_t) i * p.c.n_head_kv + h;
     const int len = fit(p.c, p.len[i]), nb = (int) (((int64_t) len + P - 1) / P);
-    const uint64_t * far = p.keys + list * p.c.table_stride;
+    const uint64_t * keys = p.keys + list * p.c.table_stride;
     int32_t * out = p.blocks + list * p.budget;
-    const bool near = nb <= room;
-    if (near)
-        for (int b = tid; b < nb; b += NS) s_keys[b] = far[b];
-    __syncthreads();
-    const uint64_t * keys = near ? s_keys : far;
-    // the keys' range, without the pages that are never chosen
+    const int run = NEAR ? KR : (nb + NS - 1) / NS;
+    const int64_t b0 = (int64_t) tid * run;
+    uint64_t mine[KR];
+    if (NEAR)
+#pragma unroll
+        for (int j = 0; j < KR; ++j) mine[j] = b0 + j < nb ? keys[b0 + j] : NEVER;
+    // f(key, page) of the thread's run
+    auto each = [&](auto && f) {
+        if (NEAR) {
+#pragma unroll
+            for (int j = 0; j < KR; ++j) f(mine[j], (int) b0 + j);
+        } else
+            for (int64_t b = b0; b < b0 + run && b < nb; ++b) f(keys[b], (int) b);
+    };
+    // the range of the keys that are neither chosen in any case nor never
     uint64_t lo = ALWAYS, hi = NEVER;
-    uint32_t some = 0;
-    for (int b = tid; b < nb; b += NS) {
-        const uint64_t k = keys[b];
-        if (k == NEVER) continue;
-        ++some;
+    uint32_t some = 0, always = 0;
+    each([&](uint64_t k, int) {
+        some += k != NEVER ? 1u : 0u;
+        always += k == ALWAYS ? 1u : 0u;
+        if (k == NEVER || k == ALWAYS) return;
         lo = k < lo ? k : lo;
         hi = k > hi ? k : hi;
-    }
+    });
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const uint64_t a = __shfl_xor_sync(FULL, lo, o), b = __shfl_xor_sync(FULL, hi, o);
@@ -318,56 +326,57 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
     }
     if (lane == 0) { s_min[warp] = lo; s_max[warp] = hi; }
     int turn = 0;
-    const uint32_t all = cta_sum(some, s_sum, turn++), want = min((uint32_t) p.budget, all);
-    for (int w = 0; w < NS / 32; ++w) {
-        lo = s_min[w] < lo ? s_min[w] : lo;
-        hi = s_max[w] > hi ? s_max[w] : hi;
+    const Three have = cta_sums(some, always, 0u, s_sum, turn++);
+    const uint32_t want = min((uint32_t) p.budget, have.a);
+    lo = s_min[lane];
+    hi = s_max[lane];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const uint64_t a = __shfl_xor_sync(FULL, lo, o), b = __shfl_xor_sync(FULL, hi, o);
+        lo = a < lo ? a : lo;
+        hi = b > hi ? b : hi;
     }
-    // the largest t with at least `want` keys >= t: lo is one such, hi + 1 is none (unless all keys are ALWAYS)
-    uint64_t t = lo;
-    uint32_t at_t = all;                    // keys >= t
-    if (want && all > want) {
-        uint64_t top = hi;                  // t <= top
+    // the largest t with at least `want` keys >= t: all keys from lo on are, and none above hi but those chosen in any case
+    uint64_t t = have.b >= want ? ALWAYS : lo;
+    if (have.b < want && have.a > want) {
+        uint64_t top = hi;
+        uint32_t at_t = have.a;
         while (t < top && at_t != want) {
-            const uint64_t d = top - t, mid = t + (d >> 1) + (d & 1ull);
-            uint32_t n = 0;
-            for (int b = tid; b < nb; b += NS) n += keys[b] >= mid ? 1u : 0u;
-            n = cta_sum(n, s_sum, turn++);
-            if (n >= want) { t = mid; at_t = n; }
-            else top = mid - 1ull;
+            const uint64_t d = top - t, q = d >> 2;
+            const uint64_t m1 = t + q + 1ull, m2 = t + (d >> 1) + 1ull, m3 = t + (d >> 1) + q + 1ull;     // t < m1 <= m2 <= m3 <= top + 1
+            uint32_t n1 = 0, n2 = 0, n3 = 0;
+            each([&](uint64_t k, int) { n1 += k >= m1 ? 1u : 0u; n2 += k >= m2 ? 1u : 0u; n3 += k >= m3 ? 1u : 0u; });
+            const Three n = cta_sums(n1, n2, n3, s_sum, turn++);
+            if (n.c >= want && m3 <= top) { t = m3; at_t = n.c; }
+            else if (n.b >= want && m2 <= top) { t = m2; at_t = n.b; top = m3 - 1ull < top ? m3 - 1ull : top; }
+            else if (n.a >= want && m1 <= top) { t = m1; at_t = n.a; top = m2 - 1ull < top ? m2 - 1ull : top; }
+            else top = m1 - 1ull < top ? m1 - 1ull : top;
         }
     }
-    // keys above t, and the first `ties` of those equal to it: a thread has a run of pages
-    const int run = (nb + NS - 1) / NS, b0 = min(tid * run, nb), b1 = min(b0 + run, nb);
+    // keys above t, and the first `ties` of those equal to it
     uint32_t above = 0, equal = 0;
-    if (want)
-        for (int b = b0; b < b1; ++b) {
-            const uint64_t k = keys[b];
-            above += k > t ? 1u : 0u;
-            equal += k == t ? 1u : 0u;
-        }
-    const uint32_t above_all = cta_sum(above, s_sum, turn++), ties = want - above_all;
-    // exclusive sums over the threads, both in one word each
+    each([&](uint64_t k, int) {
+        above += k > t ? 1u : 0u;
+        equal += k == t && k != NEVER ? 1u : 0u;
+    });
+    const uint32_t ties = want - cta_sums(above, 0u, 0u, s_sum, turn++).a;
     uint32_t xa = above, xe = equal;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint32_t ya = __shfl_up_sync(FULL, xa, o), ye = __shfl_up_sync(FULL, xe, o);
         if (lane >= o) { xa += ya; xe += ye; }
     }
-    __syncthreads();                        // the range's places are free
-    if (lane == 31) { s_min[warp] = xa; s_max[warp] = xe; }
+    if (lane == 31) { s_min[warp] = xa; s_max[warp] = xe; }     // (their readers are a barrier back)
     __syncthreads();
-    xa -= above;
-    xe -= equal;
-    for (int w = 0; w < warp; ++w) { xa += (uint32_t) s_min[w]; xe += (uint32_t) s_max[w]; }
+    const uint32_t wa = (uint32_t) s_min[lane], we = (uint32_t) s_max[lane];
+    xa += __reduce_add_sync(FULL, lane < warp ? wa : 0u) - above;
+    xe += __reduce_add_sync(FULL, lane < warp ? we : 0u) - equal;
     uint32_t at = xa + (xe < ties ? xe : ties);
-    if (want)
-        for (int b = b0; b < b1; ++b) {
-            const uint64_t k = keys[b];
-            bool take = k > t;
-            if (k == t) take = xe++ < ties;
-            if (take) out[at++] = b;
-        }
+    each([&](uint64_t k, int b) {
+        bool take = k > t;
+        if (k == t && k != NEVER) take = xe++ < ties;
+        if (take) out[at++] = b;
+    });
     for (uint32_t e = want + tid; e < (uint32_t) p.budget; e += NS) out[e] = -1;
     if (tid == 0 && p.count) p.count[list] = (int32_t) want;
 }
@@ -412,16 +421,13 @@ __global__ void __launch_bounds__(NT) lists_kernel(const __grid_constant__ ListP
     if (lane == 0) p.lens[list] = count == 0 ? 0 : (int32_t) ((int64_t) (count - 1) * P + (last == nb - 1 ? len - (int64_t) last * P : P));
 }
 
-// keys that lie in shared memory, for tables of up to so many pages
-int room_of(uint32_t stride) { return (int) (stride < 24576u ? stride : 24576u); }
-
 template <int TYPE>
 int score_launch(const SelectParams & p, dim3 grid, sjk_stream st) {
     switch (p.c.head_dim) {
-        case 64: return launch(score_kernel<TYPE, 64>, grid, dim3(NT), 0, st, p);
-        case 96: return launch(score_kernel<TYPE, 96>, grid, dim3(NT), 0, st, p);
-        case 128: return launch(score_kernel<TYPE, 128>, grid, dim3(NT), 0, st, p);
-        default: return launch(score_kernel<TYPE, 256>, grid, dim3(NT), 0, st, p);
+        case 64: return launch(score_kernel<TYPE, 64>, grid, dim3(NQ), 0, st, p);
+        case 96: return launch(score_kernel<TYPE, 96>, grid, dim3(NQ), 0, st, p);
+        case 128: return launch(score_kernel<TYPE, 128>, grid, dim3(NQ), 0, st, p);
+        default: return launch(score_kernel<TYPE, 256>, grid, dim3(NQ), 0, st, p);
     }
 }
 
@@ -470,16 +476,13 @@ extern "C" int sjk_kv16_select(const sjk_kv16 * c, const void * bounds, const sj
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < sjk_kv16_select_scratch_bytes(c, n_seq)) return SJKVARN_ERR_BUFFER;
     const SelectParams p = {*c, static_cast<const uint16_t *>(bounds), *q, len, rows, n_seq, q->n_head / c->n_head_kv, budget, sink, recent,
                             static_cast<uint64_t *>(scratch), blocks, count};
-    const int64_t lists = (int64_t) n_seq * c->n_head_kv, groups = ((int64_t) c->table_stride + NT - 1) / NT;
-    int64_t z = 148 * 8 / lists + 1;
+    const int64_t lists = (int64_t) n_seq * c->n_head_kv, groups = ((int64_t) c->table_stride + NQ / 32 * PG - 1) / (NQ / 32 * PG);
+    int64_t z = 148 * 16 / lists + 1;                       // two waves over all lists
     if (z > groups) z = groups;
-    const dim3 grid((unsigned) n_seq, (unsigned) c->n_head_kv, (unsigned) z);
+    const dim3 grid((unsigned) n_seq, (unsigned) c->n_head_kv, (unsigned) z), one((unsigned) n_seq, (unsigned) c->n_head_kv);
     const int rs = c->type == SJK_F16 ? score_launch<SJK_F16>(p, grid, st) : score_launch<SJK_BF16>(p, grid, st);
     if (rs) return rs;
-    const int room = room_of(c->table_stride);
-    const size_t smem = (size_t) room * sizeof(uint64_t);
-    if (smem > 40 * 1024 && smem_limit<choose_kernel>(24576 * sizeof(uint64_t))) return SJK_ERR_DEVICE;
-    return launch(choose_kernel, dim3((unsigned) n_seq, (unsigned) c->n_head_kv), dim3(NS), smem, st, p, room);
+    return c->table_stride <= (uint32_t) (NS * KR) ? launch(choose_kernel<true>, one, dim3(NS), 0, st, p) : launch(choose_kernel<false>, one, dim3(NS), 0, st, p);
 }
 
 // The attention's part of the scratch behind the lists.

@@ -9,7 +9,8 @@ namespace {
 
 using namespace sjk16;
 
-constexpr int NT = 256;
+constexpr int NT = 256;                     // maps
+constexpr int NK = 128;                     // keep: a token's row of 1,024 16-bit channels is as many 16-byte words
 __device__ unsigned int g_step_status;
 
 SJK_DEV void flag() { atomicOr(&g_step_status, (unsigned) SJK_DEVICE_PAGE); }
@@ -123,7 +124,7 @@ struct KeepParams {
 // rows j .. j + BATCH - 1 is of places j and on, which only writes of the same batch and later ones touch). E: a 16-byte word
 // or an element. The path's checks and page look-ups are one per thread, before the rows move.
 template <typename E>
-__global__ void __launch_bounds__(NT) keep_kernel(const __grid_constant__ KeepParams p) {
+__global__ void __launch_bounds__(NK) keep_kernel(const __grid_constant__ KeepParams p) {
     constexpr int BATCH = 8;
     __shared__ int64_t s_from[SJK_KEEP_MAX], s_to[SJK_KEEP_MAX];
     pdl_wait();
@@ -133,18 +134,17 @@ __global__ void __launch_bounds__(NT) keep_kernel(const __grid_constant__ KeepPa
     const int64_t row = p.rows ? (int64_t) p.rows[i] : (int64_t) i;
     int bad = len < 0 || count < 0 || count > p.width || row < 0 || row >= (int64_t) p.c.n_rows ? 1 : 0;
     if (p.rows)
-        for (int j = tid; j < i && !bad; j += NT) bad = p.rows[j] == (int32_t) row;        // an earlier entry has the row
-    if (!bad && tid < count) {
+        for (int j = tid; j < i && !bad; j += NK) bad = p.rows[j] == (int32_t) row;        // an earlier entry has the row
+    for (int j = tid; j < count && !bad; j += NK) {
         const int32_t * path = p.path + (int64_t) i * p.width;
-        const int32_t from = path[tid];
-        const int64_t a = (int64_t) len + from, b = (int64_t) len + tid;
-        bad = from < tid || (tid > 0 && path[tid - 1] >= from) || a >= (int64_t) p.c.table_stride * P;
-        if (!bad) {
-            const uint32_t ga = (uint32_t) (a / P), gb = (uint32_t) (b / P), pa = page_of(p.c, row, ga), pb = page_of(p.c, row, gb);
-            bad = pa == SJKVARN_NO_BLOCK || pb == SJKVARN_NO_BLOCK;
-            s_from[tid] = (int64_t) pa * p.c.page_stride + (a - (int64_t) ga * P) * p.c.slot_stride;
-            s_to[tid] = (int64_t) pb * p.c.page_stride + (b - (int64_t) gb * P) * p.c.slot_stride;
-        }
+        const int32_t from = path[j];
+        const int64_t a = (int64_t) len + from, b = (int64_t) len + j;
+        bad = from < j || (j > 0 && path[j - 1] >= from) || a >= (int64_t) p.c.table_stride * P;
+        if (bad) break;
+        const uint32_t ga = (uint32_t) (a / P), gb = (uint32_t) (b / P), pa = page_of(p.c, row, ga), pb = page_of(p.c, row, gb);
+        bad = pa == SJKVARN_NO_BLOCK || pb == SJKVARN_NO_BLOCK;
+        s_from[j] = (int64_t) pa * p.c.page_stride + (a - (int64_t) ga * P) * p.c.slot_stride;
+        s_to[j] = (int64_t) pb * p.c.page_stride + (b - (int64_t) gb * P) * p.c.slot_stride;
     }
     bad = __syncthreads_or(bad);
     const bool first = blockIdx.y == 0 && blockIdx.z == 0 && tid == 0;
@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(NT) keep_kernel(const __grid_constant__ KeepPa
     const int per = p.c.head_dim / EL, words = p.c.n_head_kv * per;
     int skip = 0;                           // rows that are in their places
     while (skip < count && s_from[skip] == s_to[skip]) ++skip;
-    for (int w = tid; w < words; w += blockDim.x) {
+    for (int w = tid; w < words; w += NK) {
         const int h = w / per;
         uint16_t * mine = base + (int64_t) h * p.c.head_stride + (w - h * per) * EL;
         for (int j0 = skip; j0 < count; j0 += BATCH) {
@@ -204,7 +204,7 @@ extern "C" int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_str
     const int64_t strides = c->page_stride | c->slot_stride | c->head_stride | (n_layers > 1 ? layer_stride : 0);
     const bool wide = aligned(c->k, 16) && aligned(c->v, 16) && (strides & 7) == 0 && c->head_dim % 8 == 0;
     const dim3 grid((unsigned) n_seq, (unsigned) n_layers, 2);
-    return wide ? launch(keep_kernel<uint4>, grid, dim3(NT), 0, st, p) : launch(keep_kernel<uint16_t>, grid, dim3(NT), 0, st, p);
+    return wide ? launch(keep_kernel<uint4>, grid, dim3(NK), 0, st, p) : launch(keep_kernel<uint16_t>, grid, dim3(NK), 0, st, p);
 }
 
 int sjk_step_status_take(void) {
