@@ -162,7 +162,7 @@ constexpr uint64_t NEVER = 0ull, ALWAYS = ~0ull;            // no page; first an
 // partial sum of every page, which an exchange by halves leaves in the lane of each page. The CTA makes the weights, which
 // all its warps share. grid: sequences, heads, groups of pages. Smaller groups of pages make more warps, whose loads are out
 // at the same time (one sequence of 6,250 pages, 8 heads).
-constexpr int NQ = 128, PG = 16;            // threads; pages of a warp at a time
+constexpr int NQ = 128, PG = 8;             // threads; pages of a warp at a time
 template <int TYPE, int D>
 __global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ SelectParams p) {
     constexpr int WORDS = D / 8, NW = D == 256 ? 2 : 1;     // words of a side; words of a lane
@@ -266,27 +266,33 @@ __global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ Selec
 
 // ---- select: the largest `budget` keys of a list ------------------------------------------------------------------
 constexpr int NS = 1024, KR = 8;            // threads; keys that a thread holds in registers
-// Sums of three counts over the CTA (each at most 1,023 a warp); every thread gets them. One barrier: successive calls
-// take the places by turns.
-struct Three { uint32_t a, b, c; };
-SJK_DEV Three cta_sums(uint32_t a, uint32_t b, uint32_t c, uint32_t (*s)[3][NS / 32], int turn) {
+// Exclusive sum over the CTA's threads, and the whole. s: NS / 32 words, free again behind the caller's next barrier.
+SJK_DEV uint32_t cta_before(uint32_t x, uint32_t * s, uint32_t * all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    a = __reduce_add_sync(FULL, a);
-    b = __reduce_add_sync(FULL, b);
-    c = __reduce_add_sync(FULL, c);
-    if (lane == 0) { s[turn & 1][0][warp] = a; s[turn & 1][1][warp] = b; s[turn & 1][2][warp] = c; }
+    uint32_t incl = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) s[warp] = incl;
     __syncthreads();
-    return {__reduce_add_sync(FULL, s[turn & 1][0][lane]), __reduce_add_sync(FULL, s[turn & 1][1][lane]), __reduce_add_sync(FULL, s[turn & 1][2][lane])};
+    const uint32_t w = s[lane];
+    *all = __reduce_add_sync(FULL, w);
+    return __reduce_add_sync(FULL, lane < warp ? w : 0u) + incl - x;
 }
 
-// A CTA per (sequence, head): the threshold by a search that quarters the range of the keys (counts of the keys above three
-// places in it each time, until exactly as many are left as are wanted), then the keys above it and the first of those
-// equal to it, in ascending order of their pages. A thread has a run of KR pages in registers; lists of more than NS KR pages
-// are read anew in every round. No atomics: the same lists every time.
+// A CTA per (sequence, head): the threshold by counting the keys in BINS equal parts of their range, then those of the part in
+// which it lies in BINS parts of that, until exactly as many are left as are wanted (twice, for keys apart from one
+// another); then the keys above it and the first of those equal to it, in ascending order of their pages. A thread has a run
+// of KR pages in registers; lists of more than NS KR pages are read anew in every round. Counts alone are atomic: the same
+// lists every time.
+constexpr int BINS = 2 * NS;
 template <bool NEAR>
 __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ SelectParams p) {
-    __shared__ uint32_t s_sum[2][3][NS / 32];
-    __shared__ uint64_t s_min[NS / 32], s_max[NS / 32];
+    __shared__ uint32_t s_bin[BINS], s_sum[4][NS / 32];
+    __shared__ uint64_t s_min[NS / 32], s_max[NS / 32], s_from;
+    __shared__ uint32_t s_above, s_in;
     pdl_wait();
     pdl_release();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, i = blockIdx.x, h = blockIdx.y, P = p.c.page_tokens;
@@ -325,9 +331,13 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
         hi = b > hi ? b : hi;
     }
     if (lane == 0) { s_min[warp] = lo; s_max[warp] = hi; }
-    int turn = 0;
-    const Three have = cta_sums(some, always, 0u, s_sum, turn++);
-    const uint32_t want = min((uint32_t) p.budget, have.a);
+    some = __reduce_add_sync(FULL, some);
+    always = __reduce_add_sync(FULL, always);
+    if (lane == 0) { s_sum[0][warp] = some; s_sum[1][warp] = always; }
+    __syncthreads();
+    some = __reduce_add_sync(FULL, s_sum[0][lane]);
+    always = __reduce_add_sync(FULL, s_sum[1][lane]);
+    const uint32_t want = min((uint32_t) p.budget, some);
     lo = s_min[lane];
     hi = s_max[lane];
 #pragma unroll
@@ -336,22 +346,39 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
         lo = a < lo ? a : lo;
         hi = b > hi ? b : hi;
     }
-    // the largest t with at least `want` keys >= t: all keys from lo on are, and none above hi but those chosen in any case
-    uint64_t t = have.b >= want ? ALWAYS : lo;
-    if (have.b < want && have.a > want) {
-        uint64_t top = hi;
-        uint32_t at_t = have.a;
-        while (t < top && at_t != want) {
-            const uint64_t d = top - t, q = d >> 2;
-            const uint64_t m1 = t + q + 1ull, m2 = t + (d >> 1) + 1ull, m3 = t + (d >> 1) + q + 1ull;     // t < m1 <= m2 <= m3 <= top + 1
-            uint32_t n1 = 0, n2 = 0, n3 = 0;
-            each([&](uint64_t k, int) { n1 += k >= m1 ? 1u : 0u; n2 += k >= m2 ? 1u : 0u; n3 += k >= m3 ? 1u : 0u; });
-            const Three n = cta_sums(n1, n2, n3, s_sum, turn++);
-            if (n.c >= want && m3 <= top) { t = m3; at_t = n.c; }
-            else if (n.b >= want && m2 <= top) { t = m2; at_t = n.b; top = m3 - 1ull < top ? m3 - 1ull : top; }
-            else if (n.a >= want && m1 <= top) { t = m1; at_t = n.a; top = m2 - 1ull < top ? m2 - 1ull : top; }
-            else top = m1 - 1ull < top ? m1 - 1ull : top;
+    // the largest t with at least `want` keys >= t. Keys of [from, from + 2^bits) are in question, `over` ones lie above.
+    uint64_t t = always >= want ? ALWAYS : lo;
+    if (always < want && some > want) {
+        uint64_t from = lo;
+        uint32_t over = always;
+        int bits = 64 - __clzll((long long) (hi - lo | 1ull));              // hi - lo < 2^bits
+        for (;;) {
+            const int shift = bits > 11 ? bits - 11 : 0;
+            s_bin[tid] = s_bin[tid + NS] = 0u;
+            __syncthreads();
+            each([&](uint64_t k, int) {
+                if (k == NEVER || k == ALWAYS || k < from) return;
+                const uint64_t d = (k - from) >> shift;
+                if (d < (uint64_t) BINS) atomicAdd(&s_bin[d], 1u);
+            });
+            __syncthreads();
+            // from the highest part down: the first with `want` keys at or above it
+            const uint32_t hi_n = s_bin[BINS - 1 - 2 * tid], lo_n = s_bin[BINS - 2 - 2 * tid];
+            uint32_t all;
+            const uint32_t before = over + cta_before(hi_n + lo_n, s_sum[2], &all);
+            if (before < want && before + hi_n + lo_n >= want) {
+                const bool first = before + hi_n >= want;
+                s_from = from + ((uint64_t) (first ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid) << shift);
+                s_above = first ? before : before + hi_n;
+                s_in = first ? hi_n : lo_n;
+            }
+            __syncthreads();
+            from = s_from;
+            over = s_above;
+            bits = shift;
+            if (shift == 0 || over + s_in == want) break;
         }
+        t = from;                           // keys >= from: `want`, or more that are all equal
     }
     // keys above t, and the first `ties` of those equal to it
     uint32_t above = 0, equal = 0;
@@ -359,18 +386,11 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
         above += k > t ? 1u : 0u;
         equal += k == t && k != NEVER ? 1u : 0u;
     });
-    const uint32_t ties = want - cta_sums(above, 0u, 0u, s_sum, turn++).a;
-    uint32_t xa = above, xe = equal;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t ya = __shfl_up_sync(FULL, xa, o), ye = __shfl_up_sync(FULL, xe, o);
-        if (lane >= o) { xa += ya; xe += ye; }
-    }
-    if (lane == 31) { s_min[warp] = xa; s_max[warp] = xe; }     // (their readers are a barrier back)
     __syncthreads();
-    const uint32_t wa = (uint32_t) s_min[lane], we = (uint32_t) s_max[lane];
-    xa += __reduce_add_sync(FULL, lane < warp ? wa : 0u) - above;
-    xe += __reduce_add_sync(FULL, lane < warp ? we : 0u) - equal;
+    uint32_t above_all, equal_all;
+    const uint32_t xa = cta_before(above, s_sum[0], &above_all);
+    uint32_t xe = cta_before(equal, s_sum[1], &equal_all);
+    const uint32_t ties = want - above_all;
     uint32_t at = xa + (xe < ties ? xe : ties);
     each([&](uint64_t k, int b) {
         bool take = k > t;
