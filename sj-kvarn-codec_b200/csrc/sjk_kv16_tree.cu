@@ -156,7 +156,9 @@ struct Shared {
     Info<S::NMAX> info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
     alignas(16) uint32_t odd[TILES][4];                 // positions whose V row was replaced, of tiles that some rows see only partly
-    float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];       // a row's maximum in use; what its scores are shifted by
+    // of a row (in its group's place, which does not depend on how many rows a pair has): its maximum in use, what its scores are
+    // shifted by, and a factor for its sums
+    float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];
     uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
     Cursor start;
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
 
     if (warp < N_SOFT) {
         // ---- softmax: position 32 (warp % 4) + lane of a tile; two groups of four warps have half of the columns each ----
-        const int group = warp >> 2, quarter = warp & 3, bar = 1 + group, tl = quarter * 32 + lane, tg = tid & 127;
+        const int group = warp >> 2, quarter = warp & 3, bar = 1 + group, tl = quarter * 32 + lane, tg = tid & 127, g0 = group * S::MINE;
         const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
         // scores are positive multiples of the products (the queries' signs are turned for a negative scale)
         const float sc = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
@@ -345,8 +347,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             const bool begun = at.st == 0, ended = at.st + steps == s.steps;
             const Info<NMAX> & info = sm.info[item % INFO];
             if (tg < nc) {
-                sm.m[c0 + tg] = -INFINITY;
-                sm.up[c0 + tg] = 3e38f;     // (no score so far: any is above)
+                sm.m[g0 + tg] = -INFINITY;
+                sm.up[g0 + tg] = 3e38f;     // (no score so far: any is above)
             }
 #pragma unroll
             for (int c = 0; c < S::MINE / 2; ++c) l[c] = make_float2(0.0f, 0.0f);
@@ -392,8 +394,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 }
                 tc::wait_st();
             };
-            // K octets of columns, from cp on, of tile jj: weights into P, sums into lp
-            auto octets_of = [&](auto kk, int cp, float2 * lp, bool fresh, int step, unsigned live, auto && wait_p) {
+            // K octets of columns of tile jj, from cp on (from gp on in the group's places): weights into P, sums into lp
+            auto octets_of = [&](auto kk, int cp, int gp, float2 * lp, bool fresh, int step, unsigned live, auto && wait_p) {
                 constexpr int K = decltype(kk)::value, N = 8 * K;
                 const uint32_t from = tmem + lanes + S::COL_S + (jj & 1u) * NMAX + (uint32_t) cp;
                 float x[N];
@@ -417,7 +419,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 auto shift = [&]() {        // to exponents of the weights
 #pragma unroll
                     for (int q = 0; q < N / 4; ++q) {
-                        const float4 u = *reinterpret_cast<const float4 *>(&sm.up[cp + q * 4]);
+                        const float4 u = *reinterpret_cast<const float4 *>(&sm.up[gp + q * 4]);
                         const float2 a = tc::num::fma2(make_float2(x[4 * q], x[4 * q + 1]), sc2, make_float2(u.x, u.y));
                         const float2 b = tc::num::fma2(make_float2(x[4 * q + 2], x[4 * q + 3]), sc2, make_float2(u.z, u.w));
                         x[4 * q] = a.x; x[4 * q + 1] = a.y; x[4 * q + 2] = b.x; x[4 * q + 3] = b.y;
@@ -439,22 +441,22 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     sm.red[warp][lane] = top;
                     tc::nbar_sync(bar, 128);
                     if (tg < N) {
-                        const float old = sm.m[cp + tg];
+                        const float old = sm.m[gp + tg];
                         float m = -INFINITY;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) m = fmaxf(m, sm.red[group * 4 + w][tg]);
                         m = fmaxf(m * sc, old);
-                        sm.fac[cp + tg] = m == old ? 1.0f : tc::num::ex2(old - m);
-                        sm.m[cp + tg] = m;
-                        sm.up[cp + tg] = m == -INFINITY ? 3e38f : S::UP - m;
+                        sm.fac[gp + tg] = m == old ? 1.0f : tc::num::ex2(old - m);
+                        sm.m[gp + tg] = m;
+                        sm.up[gp + tg] = m == -INFINITY ? 3e38f : S::UP - m;
                     }
                     tc::nbar_sync(bar, 128);
                     shift();
                     if (!fresh) {
 #pragma unroll
                         for (int c = 0; c < N / 2; ++c) {
-                            lp[c].x *= sm.fac[cp + 2 * c];
-                            lp[c].y *= sm.fac[cp + 2 * c + 1];
+                            lp[c].x *= sm.fac[gp + 2 * c];
+                            lp[c].y *= sm.fac[gp + 2 * c + 1];
                         }
                         wait_p();           // O has tiles of this pair
 #pragma unroll 1
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                                 tc::wait_ld();
                                 uint32_t r[8];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[cp + q * 8 + e]);
+                                for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[gp + q * 8 + e]);
                                 tc::st_x8(addr, r);
                             }
                         tc::wait_st();
@@ -505,8 +507,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
 #pragma unroll
                 for (int ps = 0; ps < S::PASSES; ++ps) {
                     const int m8 = n8 - 2 * ps;
-                    if (m8 == 1) octets_of(Int<1>(), c0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
-                    else if (m8 > 1) octets_of(Int<2>(), c0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
+                    if (m8 == 1) octets_of(Int<1>(), c0 + 16 * ps, g0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
+                    else if (m8 > 1) octets_of(Int<2>(), c0 + 16 * ps, g0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
                 }
                 wait_p();                   // (no thread falls behind a phase)
                 if (i > 0 && partly(p, s, (uint32_t) (step - 1) * TS)) add_odd(jj - 1, step - 1);
@@ -538,8 +540,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 if (tg < N && c < nc) {
                     const float (* red)[32] = &sm.red[group * 4];
                     const float all = (red[0][tg] + red[1][tg]) + (red[2][tg] + red[3][tg]);
-                    sm.fac[c0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
-                    if (!whole) *reinterpret_cast<float2 *>(p.ml + (slot + c0 + c) * 2) = make_float2(sm.m[c0 + c], all);
+                    sm.fac[g0 + c] = all == 0.0f ? 0.0f : 1.0f / all;
+                    if (!whole) *reinterpret_cast<float2 *>(p.ml + (slot + c0 + c) * 2) = make_float2(sm.m[g0 + c], all);
                 }
             }
             if (tid == 0 && begun && !ended)
@@ -559,7 +561,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         for (int e = 0; e < 8; ++e) {
                             const int n = c0 + c + e;
                             if (n >= s.nr) continue;
-                            if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[n]);
+                            if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[g0 + c + e]);
                             else part0[n * D + d] = o[e];
                         }
                     }
