@@ -234,8 +234,9 @@ __global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ Selec
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float2 f = widen2<TYPE>(w[e]);
-                        s = fma((double) f.x * moved_by<TYPE>(), wt[n][2 * e], s);
-                        s = fma((double) f.y * moved_by<TYPE>(), wt[n][2 * e + 1], s);
+                        // (an infinity on the side that no head looks at does not count)
+                        if (f.x != f.x || wt[n][2 * e] != 0.0) s = fma((double) f.x * moved_by<TYPE>(), wt[n][2 * e], s);
+                        if (f.y != f.y || wt[n][2 * e + 1] != 0.0) s = fma((double) f.y * moved_by<TYPE>(), wt[n][2 * e + 1], s);
                     }
                 } else {
 #pragma unroll
