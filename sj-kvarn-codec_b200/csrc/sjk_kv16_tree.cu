@@ -39,7 +39,7 @@ using namespace sjk16;
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int TS = 128;                     // positions of a step
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
-constexpr int MIN_RUN = 2;                  // units of a run, at least
+constexpr int MIN_RUN = 1;                  // units of a run, at least
 constexpr int GROUPS = 4;                   // of softmax warps, which divide the columns
 constexpr int N_SOFT = 4 * GROUPS, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
 constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
@@ -407,10 +407,18 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     if (!plain) {
                         const uint32_t t = (uint32_t) step * TS + (uint32_t) tl;
                         uint32_t seen = (live >> lane) & 1u ? FULL : 0u;
-                        if (seen && !all)
-#pragma unroll 1
-                            for (int c = 0; c < N; ++c)
-                                if (!sees(t, cp + c)) seen &= ~(1u << c);
+                        if (seen && !all) {
+                            if (t >= (uint32_t) s.len) {
+                                const uint32_t k = t - (uint32_t) s.len;
+                                seen = 0u;
+#pragma unroll
+                                for (int c = 0; c < N; ++c) seen |= (uint32_t) ((info.mask[cp + c] >> k) & 1ull) << c;
+                            } else if (p.window) {
+                                seen = 0u;
+#pragma unroll
+                                for (int c = 0; c < N; ++c) seen |= (t >= (uint32_t) info.lo[cp + c] ? 1u : 0u) << c;
+                            }
+                        }
 #pragma unroll
                         for (int c = 0; c < N; ++c)
                             if (!((seen >> c) & 1u)) x[c] = -INFINITY;
