@@ -21,7 +21,7 @@
 //  - Weights enter as the sum of two 16-bit terms, as in sjk_kv16_attend: 2^-16 (bf16) or 2^-22 (f16) of a weight, and for
 //    f16, whose weights are held 2^10 larger, at most 2^-35 of the row's largest. Sums and statistics are 32-bit.
 //  - Positions that only some of the rows see (drafted ones, a window's edge) may hold infinities or NaNs, and 0 times
-//    those is no zero: such V rows are replaced by zeros and their non-finite values added to the rows that see them.
+//    those is no zero: where a sum of such a run comes out as no number, its rows are summed anew, position by position.
 // A list of (sequence, KV head) pairs in steps of 128 positions is cut into equal runs, one per CTA, for each tile of rows;
 // lengths are read from device memory. Split pairs leave (m, l, o) in the scratch and a second kernel joins them in order.
 #include "sjk_kv16.cuh"
@@ -96,7 +96,6 @@ SJK_DEV uint32_t units_of(const Params & p, const Seq & s) { return s.steps > 0 
 // First committed position that some token of the pair may see, and whether some of its rows see a position of a tile (from
 // t0 on) that others do not: a drafted one, or one at the window's edge.
 SJK_DEV uint32_t low_of(const Params & p, const Seq & s) { return p.window && s.len > p.window ? (uint32_t) (s.len - p.window) : 0u; }
-SJK_DEV bool few_see(const Params & p, const Seq & s, uint32_t t) { return t >= (uint32_t) s.len || (p.window && t < low_of(p, s) + (uint32_t) s.count); }
 SJK_DEV bool partly(const Params & p, const Seq & s, uint32_t t0) { return t0 + TS > (uint32_t) s.len || (p.window && t0 < low_of(p, s) + (uint32_t) s.count); }
 // Groups of 16 positions of a tile that lie in the pair's span (one at least): the second product takes these alone.
 SJK_DEV int end16(const Seq & s, uint32_t t0) { const uint32_t n = s.hi - t0; return n < TS ? (int) ((n + 15u) >> 4) : TS / 16; }
@@ -155,7 +154,6 @@ struct Shared {
     uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2][S::PB];
     Info<S::NMAX> info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
-    alignas(16) uint32_t odd[TILES][4];                 // positions whose V row was replaced, of tiles that some rows see only partly
     // of a row (in its group's place, which does not depend on how many rows a pair has): its maximum in use, what its scores are
     // shifted by, and a factor for its sums
     float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];
@@ -240,12 +238,6 @@ SJK_DEV float octets(const float * v, int lane) {
         return columns<MAX, 32>(w, lane);
     } else return columns<MAX, 8 * K>(v, lane);
 }
-// the sign bits of halves that are infinities or NaNs: an exponent of all ones carries into them
-template <int TYPE>
-SJK_DEV uint32_t odd_bits(uint32_t w) { return ((w & 0x7FFF7FFFu) + (TYPE == SJK_F16 ? 0x04000400u : 0x00800080u)) & 0x80008000u; }
-template <int TYPE>
-SJK_DEV uint32_t odd_bits(const uint4 & x) { return odd_bits<TYPE>(x.x) | odd_bits<TYPE>(x.y) | odd_bits<TYPE>(x.z) | odd_bits<TYPE>(x.w); }
-
 // Waits that give up once and for all: after one that ran out (the status word says so) a role goes on without waiting, so
 // that everyone meets the same barriers and the CTA ends.
 struct Waiter {
@@ -258,6 +250,47 @@ struct Waiter {
         dead = __any_sync(FULL, dead);
     }
 };
+
+// A row's sum over the positions of a run that it sees, one after the other: for runs in which some V row that not all rows
+// see holds an infinity or NaN (which a product with a weight of 0 does not take out). A warp; the row's maximum in use is m. The
+// sum times inv goes to the output, or (not whole) the sum to `part`.
+struct Run { int seq, h, first, len; uint32_t t0, t1; };
+template <typename S>
+__device__ __noinline__ void slow_row(const Params & p, Run at, int r, uint64_t mask, int lo, float sc, float m, bool whole, float inv, int64_t out, float * part) {
+    constexpr int D = S::D, NC = D / 32;
+    const int lane = threadIdx.x & 31, j = r / p.grp, head = at.h * p.grp + (r - j * p.grp);
+    const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
+    const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
+    float q[NC], o[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        q[c] = load1(p.q.p, (int64_t) (at.first + j) * p.q.row_stride + (int64_t) head * p.q.head_stride + 32 * c + lane, S::TYPE);
+        q[c] = p.scale < 0.0f ? -q[c] : p.scale > 0.0f ? q[c] : 0.0f;
+        o[c] = 0.0f;
+    }
+    for (uint32_t t = at.t0; t < at.t1 && table; ++t) {
+        if (t >= (uint32_t) at.len ? !((mask >> (t - (uint32_t) at.len)) & 1ull) : t < (uint32_t) lo) continue;
+        const uint32_t g = t / (uint32_t) p.c.page_tokens, page = table[g];
+        if (page >= p.c.n_pages) continue;
+        const int64_t at_kv = (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride + (int64_t) at.h * p.c.head_stride + lane;
+        float x = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) x = fmaf(q[c], load1(p.c.k, at_kv + 32 * c, S::TYPE), x);
+#pragma unroll
+        for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(FULL, x, i);
+        const float w = tc::num::ex2(x * sc - (m == -INFINITY ? 0.0f : m) + S::UP);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float v = load1(p.c.v, at_kv + 32 * c, S::TYPE);
+            o[c] = fabsf(v) < INFINITY ? fmaf(w, v, o[c]) : o[c] + v;
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        if (whole) store1(p.out.p, out + 32 * c + lane, S::TYPE, o[c] * inv);
+        else part[32 * c + lane] = o[c];
+    }
+}
 
 template <typename S, bool WHOLE>
 __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
@@ -355,45 +388,6 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             tc::nbar_sync(bar, 128);
             wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
             auto sees = [&](uint32_t t, int n) { return t >= (uint32_t) s.len ? (bool) ((info.mask[n] >> (t - (uint32_t) s.len)) & 1ull) : t >= (uint32_t) info.lo[n]; };
-            // non-finite values of V rows that only some rows see, into the sums of those that do
-            auto add_odd = [&](uint32_t tile_no, int step) {
-                const uint4 some = *reinterpret_cast<const uint4 *>(sm.odd[tile_no % TILES]);
-                if (!(some.x | some.y | some.z | some.w)) return;
-                const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
-                if (row < 0 || row >= (int64_t) p.c.n_rows) return;
-                const uint32_t * table = p.c.tables + row * p.c.table_stride;
-#pragma unroll 1
-                for (int part = 0; part < S::PARTS; ++part) {
-                    const int d = part * 128 + tl;
-#pragma unroll 1
-                    for (int c = 0; c < nc; c += 8) {
-                        float o[8];
-                        const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c);
-                        ld8(addr, o);
-                        tc::wait_ld();
-#pragma unroll 1
-                        for (int w = 0; w < 4; ++w)
-#pragma unroll 1
-                            for (uint32_t b = w == 0 ? some.x : w == 1 ? some.y : w == 2 ? some.z : some.w; b; b &= b - 1u) {
-                                const uint32_t t = (uint32_t) step * TS + 32u * w + (uint32_t) __ffs((int) b) - 1u, g = t / (uint32_t) p.c.page_tokens;
-                                const uint32_t page = table[g];
-                                if (page >= p.c.n_pages || d >= D) continue;
-                                const float x = load1(p.c.v, (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride +
-                                                      (int64_t) h * p.c.head_stride + d, S::TYPE);
-                                if (fabsf(x) < INFINITY) continue;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    if (sees(t, c0 + c + e)) o[e] += x;
-                            }
-                        uint32_t r[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e]);
-                        __syncwarp();
-                        tc::st_x8(addr, r);
-                    }
-                }
-                tc::wait_st();
-            };
             // K octets of columns of tile jj, from cp on (from gp on in the group's places): weights into P, sums into lp
             auto octets_of = [&](auto kk, int cp, int gp, float2 * lp, bool fresh, int step, unsigned live, auto && wait_p) {
                 constexpr int K = decltype(kk)::value, N = 8 * K;
@@ -519,7 +513,6 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     else if (m8 > 1) octets_of(Int<2>(), c0 + 16 * ps, g0 + 16 * ps, l + 8 * ps, i == 0, step, live, wait_p);
                 }
                 wait_p();                   // (no thread falls behind a phase)
-                if (i > 0 && partly(p, s, (uint32_t) (step - 1) * TS)) add_odd(jj - 1, step - 1);
                 tc::fence_proxy_async();
                 tc::fence_before_sync();
                 __syncwarp();
@@ -531,7 +524,6 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             // the pair's output, or its partial
             wait.warp(&sm.pv_done, (jj - 1) & 1u);
             tc::fence_after_sync();
-            if (partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) add_odd(jj - 1, s.step0 + at.st + steps - 1);
             const bool whole = begun && ended;
             const int64_t slot = ((int64_t) blockIdx.x * 2 + (begun ? 1 : 0)) * NMAX;
 #pragma unroll
@@ -556,6 +548,29 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 p.split[blockIdx.x] = make_int4(at.seq, h, run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
             tc::nbar_sync(bar, 128);
             float * part0 = p.part + slot * D;
+            // Where some rows do not see all positions: 0 times what they do not see may have been no zero.
+            bool odd = false;
+            if (partly(p, s, (uint32_t) (s.step0 + at.st) * TS) || partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) {
+#pragma unroll 1
+                for (int part = 0; part < S::PARTS; ++part)
+#pragma unroll 1
+                    for (int c = 0; c < nc; c += 8) {
+                        float o[8];
+                        ld8(tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c), o);
+                        tc::wait_ld();
+                        if (part * 128 + tl < D)
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) odd |= !(fabsf(o[e]) < INFINITY);
+                    }
+                __syncwarp();
+                odd = any_of(bar, odd);
+            }
+            if (odd) {
+                const Run now = {at.seq, h, s.first, s.len, (uint32_t) (s.step0 + at.st) * TS, min(s.hi, (uint32_t) (s.step0 + at.st + steps) * TS)};
+                for (int c = quarter; c < nc && c0 + c < s.nr; c += 4)
+                    slow_row<S>(p, now, s.row0 + c0 + c, info.mask[c0 + c], info.lo[c0 + c], sc, sm.m[g0 + c], whole, sm.fac[g0 + c], info.out[c0 + c],
+                                part0 + (c0 + c) * D);
+            } else
 #pragma unroll 1
             for (int part = 0; part < S::PARTS; ++part) {
                 const int d = part * 128 + tl;
@@ -594,63 +609,22 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             for (; told < upto; ++told)
                 if (lane == 0) tc::mbar_arrive(&full[told % slots]);
         };
-        // A part of a V tile to be mended: rows (todo) that are dead, or that only some query rows see, of slot `slot`.
-        struct Mend { bool on; int slot, part; uint32_t tile; unsigned todo[4], live[4], odd[4]; } m = {};
-        uint32_t landed = 0;                // WHOLE: parity of every slot's v_land
-        auto mend_rows = [&]() {
-            uint8_t * dst = ring + m.slot * S::PART;
-            if (m.part == 0) m.odd[0] = m.odd[1] = m.odd[2] = m.odd[3] = 0u;
-            // RI rows at a time, a lane per word; four such loads in flight
-            constexpr int LR = S::CH == 8 ? 8 : 16, RI = 32 / LR;
-            const int wd = lane % LR;
-            auto word = [&](int rt) { return reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4)); };
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-#pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += 4 * RI) {
-                    const unsigned some = (m.todo[g] >> r0) & (4 * RI == 32 ? FULL : (1u << (4 * RI)) - 1u);
-                    if (!some) continue;
-                    uint4 x[4];
-                    uint32_t bad = 0u;
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = r0 + u * RI + lane / LR;
-                        x[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (wd < S::CH && ((m.todo[g] >> r) & 1u)) {
-                            if ((m.live[g] >> r) & 1u) x[u] = *word(32 * g + r);
-                            else *word(32 * g + r) = x[u];
-                        }
-                    }
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) bad |= odd_bits<S::TYPE>(x[u]);
-                    if (!__any_sync(FULL, bad != 0u)) continue;
-#pragma unroll 1
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = r0 + u * RI + lane / LR;
-                        bool here = false;
-                        if (wd < S::CH && ((m.todo[g] >> r) & (m.live[g] >> r) & 1u)) {
-                            uint32_t * w = reinterpret_cast<uint32_t *>(word(32 * g + r));
-#pragma unroll 1
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t o = odd_bits<S::TYPE>(w[e]);
-                                here |= o != 0u;
-                                if (o & 0x8000u) w[e] &= 0xFFFF0000u;       // (its finite neighbours stay)
-                                if (o >> 31) w[e] &= 0x0000FFFFu;
-                            }
-                        }
-                        const unsigned who = __ballot_sync(FULL, here);
-                        for (int v = 0; v < RI; ++v)
-                            if ((who >> (v * LR)) & ((1u << LR) - 1u)) m.odd[g] |= 1u << (r0 + u * RI + v);
-                    }
-                }
-            if (lane == 0)
-                for (int u = 0; u < 4; ++u) sm.odd[m.tile % TILES][u] = m.odd[u];
-        };
+        // WHOLE: a part of a V tile whose dead rows (that came with a box, or came not) are to be zeros
+        struct Mend { bool on; int slot; unsigned dead[4]; } m = {};
+        uint32_t landed = 0;                // parity of every slot's v_land
         auto mend_box = [&]() {             // once it has landed
             m.on = false;
             wait.warp(&sm.v_land[m.slot], (landed >> m.slot) & 1u);
             landed ^= 1u << m.slot;
-            mend_rows();
+            uint8_t * dst = ring + m.slot * S::PART;
+            constexpr int LR = S::BLOCKS * 8, RI = 32 / LR;         // lanes of a row, rows at a time
+            const int wd = lane % LR;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                for (int r0 = 0; r0 < 32 && m.dead[g] >> r0; r0 += RI) {
+                    const int r = r0 + lane / LR, rt = 32 * g + r;
+                    if ((m.dead[g] >> r) & 1u) *reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+                }
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&full[m.slot]);
@@ -664,44 +638,32 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             const uint32_t lo0 = low_of(p, s);
             for (int i = 0; i < steps; ++i, ++jj) {
                 const uint32_t t0 = (uint32_t) (s.step0 + at.st + i) * TS;
-                auto page_at = [&](uint32_t t, uint32_t * place) {
-                    const uint32_t g = p.page_shift >= 0 ? t >> p.page_shift : t / (uint32_t) p.c.page_tokens, page = table[g];
-                    *place = t - g * (uint32_t) p.c.page_tokens;
-                    if (page >= p.c.n_pages && page != SJKVARN_NO_BLOCK) flag();
-                    return page;
-                };
-                // the tile's live positions (a lane looks up every 32nd), and their rows
-                unsigned live[4];
+                // the tile's live positions (a lane looks up every 32nd) and their rows, and (WHOLE) the lane's box: all look-ups
+                // are out before the first is used
+                uint32_t place[5], page[5];
+                const uint32_t mine = (uint32_t) (lane / S::BLOCKS) * (uint32_t) p.box;
+#pragma unroll
+                for (int u = 0; u < 5; ++u) {
+                    const uint32_t t = u < 4 ? t0 + (uint32_t) (32 * u + lane) : t0 + mine;
+                    const bool on = u < 4 ? t < s.hi && t >= lo0 : WHOLE && mine < TS && t < s.hi && t + (uint32_t) p.box > lo0;
+                    const uint32_t g = p.page_shift >= 0 ? t >> p.page_shift : t / (uint32_t) p.c.page_tokens;
+                    place[u] = t - g * (uint32_t) p.c.page_tokens;
+                    page[u] = on && table ? table[g] : SJKVARN_NO_BLOCK;
+                }
+                unsigned live[4], dead[4];
                 int64_t off[4];             // -1: none
+                const int a16 = first16(p, s, t0), b16 = end16(s, t0);
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const uint32_t t = t0 + (uint32_t) (32 * u + lane);
-                    off[u] = -1;
-                    if (table && t < s.hi && t >= lo0) {
-                        uint32_t place;
-                        const uint32_t page = page_at(t, &place);
-                        if (page < p.c.n_pages) off[u] = (int64_t) page * p.c.page_stride + (int64_t) place * p.c.slot_stride;
-                    }
+                    if (page[u] >= p.c.n_pages && page[u] != SJKVARN_NO_BLOCK) flag();
+                    off[u] = page[u] < p.c.n_pages ? (int64_t) page[u] * p.c.page_stride + (int64_t) place[u] * p.c.slot_stride : -1;
+                    const int g16 = (32 * u + lane) >> 4;
                     live[u] = __ballot_sync(FULL, off[u] >= 0);
+                    dead[u] = __ballot_sync(FULL, WHOLE && is_v && off[u] < 0 && g16 >= a16 && g16 < b16);     // (copies fill theirs with zeros)
                     if (!is_v && lane == 0) sm.live[jj % TILES][u] = live[u];
                 }
-                unsigned todo[4] = {0u, 0u, 0u, 0u};
-                if (is_v) {                 // what the second product takes of V: all of a box, but of copies no dead row
-                    const int a16 = first16(p, s, t0), b16 = end16(s, t0);
-                    const bool some = partly(p, s, t0);
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int g16 = (32 * u + lane) >> 4;
-                        todo[u] = __ballot_sync(FULL, off[u] >= 0 ? some && few_see(p, s, t0 + (uint32_t) (32 * u + lane)) : WHOLE && g16 >= a16 && g16 < b16);
-                    }
-                }
-                const bool mend = (todo[0] | todo[1] | todo[2] | todo[3]) != 0u;
-                if (is_v && !mend && lane == 0) *reinterpret_cast<uint4 *>(sm.odd[jj % TILES]) = make_uint4(0u, 0u, 0u, 0u);
-                // WHOLE: the lane's box
-                uint32_t place = 0, page = SJKVARN_NO_BLOCK;
-                const uint32_t mine = (uint32_t) (lane / S::BLOCKS) * (uint32_t) p.box;
-                if (WHOLE && mine < TS && t0 + mine < s.hi && t0 + mine + (uint32_t) p.box > lo0 && table) page = page_at(t0 + mine, &place);
-                const bool asks = WHOLE && page < p.c.n_pages;
+                const bool mend = (dead[0] | dead[1] | dead[2] | dead[3]) != 0u;
+                const bool asks = WHOLE && page[4] < p.c.n_pages;
                 const uint32_t tx = WHOLE ? (uint32_t) __popc(__ballot_sync(FULL, asks)) * (uint32_t) p.box * 128u : 0u;
 #pragma unroll 1
                 for (int part = 0; part < S::PARTS; ++part, ++pp) {
@@ -726,16 +688,14 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         __syncwarp();
                         if (asks)
                             box(tc::smem_addr(dst) + (uint32_t) (lane % S::BLOCKS) * (TS * 128) + mine * 128u, &p.maps[is_v ? 1 : 0],
-                                part * 128 + (lane % S::BLOCKS) * 64, at.h, (int) place, page, bar);
+                                part * 128 + (lane % S::BLOCKS) * 64, at.h, (int) place[4], page[4], bar);
                         if (m.on) mend_box();           // the one before, while this one is on its way
                     }
                     if (mend) {
-                        m.on = WHOLE;
+                        m.on = true;
                         m.slot = slot;
-                        m.part = part;
-                        m.tile = jj;
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) { m.todo[u] = todo[u]; m.live[u] = live[u]; }
+                        for (int u = 0; u < 4; ++u) m.dead[u] = dead[u];
                     }
                     if constexpr (!WHOLE) {
                         const uint16_t * base = static_cast<const uint16_t *>(is_v ? p.c.v : p.c.k) + (int64_t) at.h * p.c.head_stride + part * 128;
@@ -748,19 +708,12 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                                 tc::cp_async16(dst + (c >> 3) * (TS * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
                             }
                         tc::cp_async_commit();
-                        if (mend) {
-                            tc::cp_async_wait_group<0>();
-                            __syncwarp();
-                            mend_rows();
-                            tell(pp + 1);
-                        } else {
-                            if (slots == 1) tc::cp_async_wait_group<0>();
-                            else if (slots == 2) tc::cp_async_wait_group<1>();
-                            else if (slots == 3) tc::cp_async_wait_group<2>();
-                            else tc::cp_async_wait_group<3>();
-                            const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;  // parts still on their way
-                            if (pp + 1 > flight) tell(pp + 1 - flight);
-                        }
+                        if (slots == 1) tc::cp_async_wait_group<0>();
+                        else if (slots == 2) tc::cp_async_wait_group<1>();
+                        else if (slots == 3) tc::cp_async_wait_group<2>();
+                        else tc::cp_async_wait_group<3>();
+                        const uint32_t flight = slots < 4 ? (uint32_t) slots - 1u : 3u;      // parts still on their way
+                        if (pp + 1 > flight) tell(pp + 1 - flight);
                     }
                 }
             }

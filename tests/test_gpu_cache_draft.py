@@ -193,27 +193,28 @@ def test_infinities_in_masked_places(T, dtype, page, D, window):
     q = T.randn((n, 6, D), device="cuda", generator=g).to(cache.k.dtype)
     out = cache.attend_tree(0, q, _ints(T, [length]), _ints(T, _signed(masks[0]), T.int64), 0.1, window=window)
     sees = [set(_visible(length, masks[0], j, window)) for j in range(n)]
-    # what sees no such place is what it would be without them
+    # what sees no such place is what it would be without them, within the bound of each (the sums may go another way)
     for t, (which, x) in bad.items():
         (cache.v if which == "v" else cache.k)[place(t)][:, D // 3] = 0
     clean = cache.attend_tree(0, q, _ints(T, [length]), _ints(T, _signed(masks[0]), T.int64), 0.1, window=window)
     _check(T, cache, clean, q, [length], [n], masks, 0.1, window)
-    hit = 0
+    hit, mended = 0, out.clone()
     for j in range(n):
         mine = [bad[t] for t in bad if t in sees[j]]
         if not mine:
-            assert T.equal(out[j], clean[j])
             continue
         hit += 1
+        mended[j] = clean[j]
         if any(w == "k" for w, _ in mine):
             assert bool(T.isnan(out[j]).all())
             continue
         assert not bool(T.isfinite(out[j][:, D // 3]).any())
         rest = [d for d in range(D) if d != D // 3]
-        assert T.equal(out[j][:, rest], clean[j][:, rest])
+        mended[j][:, rest] = out[j][:, rest]
         xs = {x for _, x in mine}
         if len(xs) == 1 and not math.isnan(next(iter(xs))):
             assert bool((out[j][:, D // 3] == next(iter(xs))).all())
+    _check(T, cache, mended, q, [length], [n], masks, 0.1, window)
     assert 0 < hit < n and sjk.lib().sjk_device_status() == 0
 
 
