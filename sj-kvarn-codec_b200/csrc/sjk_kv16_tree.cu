@@ -38,6 +38,7 @@ using namespace sjk16;
 
 constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int TS = 128;                     // positions of a step
+constexpr int CTAS = 148;                   // one per SM
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
 constexpr int MIN_RUN = 1;                  // units of a run, at least
 constexpr int GROUPS = 4;                   // of softmax warps, which divide the columns
@@ -55,11 +56,10 @@ struct Params {
     const uint64_t * masks;
     int n_seq, n_tok, nodes, grp;
     int window, page_shift;
-    int tiles, wl;                          // tiles of rows, and CTAs (runs) of each
     float scale;
     float * part;                           // [CTA][2][NMAX][D]
     float * ml;                             // [CTA][2][NMAX][2]
-    int4 * split;                           // by CTA: sequence (-1: none), KV head, first and last run
+    int4 * split;                           // by CTA: sequence (-1: none), KV head, first and last run; behind them: tiles
     int box;                                // tokens of a box (WHOLE)
     CUtensorMap maps[2];                    // K, V (WHOLE)
 };
@@ -69,14 +69,19 @@ struct Seq {
     int len, count, first, row0, nr, step0, steps;
     uint32_t hi;
 };
+// its first token and their number (0: none, or more than there may be)
+SJK_DEV int2 tokens_of(const Params & p, int i) {
+    if (!p.first) return make_int2(i * p.nodes, p.nodes);
+    const int64_t f0 = p.first[i], f1 = p.first[i + 1];
+    if (f0 < 0 || f1 < f0 || f1 > p.n_tok || f1 - f0 > p.nodes) { flag(); return make_int2(0, 0); }
+    return make_int2((int) f0, (int) (f1 - f0));
+}
+SJK_DEV int tiles_of(const Params & p, int i, int nmax) { return (tokens_of(p, i).y * p.grp + nmax - 1) / nmax; }
 SJK_DEV Seq seq_of(const Params & p, int i, int tile, int nmax) {
     Seq s = {0, 0, 0, 0, 0, 0, 0, 0u};
-    int64_t f0, f1;
-    if (p.first) { f0 = p.first[i]; f1 = p.first[i + 1]; }
-    else { f0 = (int64_t) i * p.nodes; f1 = f0 + p.nodes; }
-    if (f0 < 0 || f1 < f0 || f1 > p.n_tok || f1 - f0 > p.nodes) { flag(); return s; }
-    s.count = (int) (f1 - f0);
-    s.first = (int) f0;
+    const int2 tok = tokens_of(p, i);
+    s.first = tok.x;
+    s.count = tok.y;
     const int rows = s.count * p.grp, tiles = (rows + nmax - 1) / nmax;
     if (tile >= tiles) return s;
     s.row0 = (int) ((int64_t) rows * tile / tiles);
@@ -160,7 +165,8 @@ struct Shared {
     uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
     Cursor start;
-    uint32_t per, list, tmem;
+    uint32_t per, tmem;
+    int tile, run;
 };
 
 // ---- products -----------------------------------------------------------------------------------------------------
@@ -298,7 +304,6 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
     extern __shared__ uint8_t raw[];
     Shared<S> & sm = *reinterpret_cast<Shared<S> *>(raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int tile = blockIdx.x % p.tiles, run = blockIdx.x / p.tiles;
 
     if (tid == 0) {
         for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 1); tc::mbar_init(&sm.k_empty[i], 1); }
@@ -314,10 +319,16 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
     if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, S::COLS); tc::tmem_relinquish(); }
     pdl_wait();
     pdl_release();
-    // where the run begins: units of all sequences, a block of them per lane
+    // As many lists as the sequence with the most rows has tiles, side by side in the grid, and where the CTA's run begins in
+    // its own: units of all sequences, a block of them per lane.
     if (warp == 0) {
         const int block = (p.n_seq + 31) / 32;
+        int tiles = 1;
         uint32_t mine = 0;
+        for (int i = 0; i < block; ++i)
+            if (lane * block + i < p.n_seq) tiles = max(tiles, tiles_of(p, lane * block + i, NMAX));
+        tiles = (int) __reduce_max_sync(FULL, (unsigned) tiles);
+        const int tile = blockIdx.x % tiles, run = blockIdx.x / tiles, wl = gridDim.x / tiles;
         for (int i = 0; i < block; ++i)
             if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile, NMAX));
         uint32_t incl = mine;
@@ -327,11 +338,11 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             if (lane >= o) incl += y;
         }
         const uint32_t list = __shfl_sync(FULL, incl, 31);
-        uint32_t per = (list + (uint32_t) p.wl - 1u) / (uint32_t) p.wl;
+        uint32_t per = (list + (uint32_t) wl - 1u) / (uint32_t) wl;
         if (per < MIN_RUN) per = MIN_RUN;
         const int64_t o = (int64_t) run * per;
         Cursor c = {};
-        if (o < list) {
+        if (o < list && run < wl) {
             const uint32_t off = (uint32_t) o;
             c.rem = (int) (o + per < list ? per : list - off);
             const int g = __ffs(__ballot_sync(FULL, incl > off)) - 1;
@@ -352,8 +363,10 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         if (lane == 0) {
             sm.start = c;
             sm.per = per;
-            sm.list = list;
+            sm.tile = tile;
+            sm.run = run;
             p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            if (blockIdx.x == 0) p.split[gridDim.x] = make_int4(tiles, 0, 0, 0);
         }
     }
     tc::fence_before_sync();
@@ -545,7 +558,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 }
             }
             if (tid == 0 && begun && !ended)
-                p.split[blockIdx.x] = make_int4(at.seq, h, run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
+                p.split[blockIdx.x] = make_int4(at.seq, h, sm.run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
             tc::nbar_sync(bar, 128);
             float * part0 = p.part + slot * D;
             // Where some rows do not see all positions: 0 times what they do not see may have been no zero.
@@ -594,7 +607,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&sm.o_free);
             tc::nbar_sync(bar, 128);        // the factors have been read
-            at.next(p, tile, NMAX, steps);
+            at.next(p, sm.tile, NMAX, steps);
         }
     } else if (warp < W_MMA) {
         // ---- K, and V ----
@@ -717,7 +730,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     }
                 }
             }
-            at.next(p, tile, NMAX, steps);
+            at.next(p, sm.tile, NMAX, steps);
         }
         if (WHOLE) {
             if (m.on) mend_box();
@@ -799,7 +812,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 pend_first = i == 0;
                 if (i == 0) ++items;
             }
-            at.next(p, tile, NMAX, steps);
+            at.next(p, sm.tile, NMAX, steps);
         }
         if (pend) second(jj - 1);
     } else {
@@ -856,7 +869,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&sm.q_full[item % INFO]);
-            at.next(p, tile, NMAX, steps);
+            at.next(p, sm.tile, NMAX, steps);
         }
     }
     tc::fence_before_sync();
@@ -872,10 +885,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
     pdl_release();
     const int4 e = p.split[blockIdx.x];
     if (e.x < 0) return;
-    const int tile = blockIdx.x % p.tiles, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int tiles = p.split[gridDim.x].x, tile = blockIdx.x % tiles, lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
     const Seq s = seq_of(p, e.x, tile, nmax);
     if (r >= s.nr) return;
-    auto slot_of = [&](int w) { return (((int64_t) w * p.tiles + tile) * 2 + (w == e.z ? 1 : 0)) * nmax + r; };
+    auto slot_of = [&](int w) { return (((int64_t) w * tiles + tile) * 2 + (w == e.z ? 1 : 0)) * nmax + r; };
     float top = -INFINITY, sum = 0.0f;
     for (int w0 = e.z; w0 <= e.w; w0 += 32) {
         float2 ml = make_float2(-INFINITY, 0.0f);
@@ -949,7 +962,7 @@ int tree_launch(const Params & p, sjk_stream st) {
     constexpr size_t bytes = sizeof(Shared<S>) + 1024;
     static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
     if (smem_limit<tree_kernel<S, WHOLE>>(bytes)) return SJK_ERR_DEVICE;
-    return launch(tree_kernel<S, WHOLE>, dim3((unsigned) (p.tiles * p.wl)), dim3(NT), bytes, st, p);
+    return launch(tree_kernel<S, WHOLE>, dim3(CTAS), dim3(NT), bytes, st, p);
 }
 
 template <typename S>
@@ -957,11 +970,10 @@ int run(Params & p, sjk_stream st) {
     // pages of a multiple of 8 tokens come as boxes: as many tokens of a page as end where a tile's rows do
     p.box = 128;
     while (p.box > 1 && p.c.page_tokens % p.box) p.box >>= 1;
-    const int ctas = p.tiles * p.wl;
     const int rc = p.box >= 8 && maps_of(&p) ? tree_launch<S, true>(p, st) : tree_launch<S, false>(p, st);
     if (rc) return rc;
     const int rows = p.nodes * p.grp < S::NMAX ? p.nodes * p.grp : S::NMAX;
-    return launch(tree_merge_kernel<S::D>, dim3((unsigned) ctas, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE, S::NMAX);
+    return launch(tree_merge_kernel<S::D>, dim3(CTAS, (unsigned) ((rows + 7) / 8)), dim3(256), 0, st, p, S::TYPE, S::NMAX);
 }
 
 template <int TYPE>
@@ -974,8 +986,6 @@ int run_dim(Params & p, int nmax, sjk_stream st) {
     }
 }
 
-constexpr int CTAS = 148;
-
 // Rows of a pass: 128 where a KV head has more than 64 and shared memory holds them beside the tiles.
 int rows_of(const sjk_kv16 * c, int64_t rows) { return rows > 64 && c->head_dim <= 128 ? 128 : 64; }
 
@@ -983,7 +993,7 @@ int rows_of(const sjk_kv16 * c, int64_t rows) { return rows > 64 && c->head_dim 
 
 extern "C" size_t sjk_kv16_attend_tree_scratch_bytes(const sjk_kv16 * c) {
     if (!c || (c->head_dim != 64 && c->head_dim != 96 && c->head_dim != 128 && c->head_dim != 256)) return 0;
-    return (size_t) CTAS * (2 * (size_t) rows_of(c, 128) * ((size_t) c->head_dim + 2) * sizeof(float) + sizeof(int4));
+    return (size_t) CTAS * (2 * (size_t) rows_of(c, 128) * ((size_t) c->head_dim + 2) * sizeof(float) + sizeof(int4)) + sizeof(int4);
 }
 
 extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int n_tok, const int32_t * first, const int32_t * len,
@@ -1016,8 +1026,6 @@ extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int 
     p.page_shift = -1;
     for (int b = 0; b < 31; ++b)
         if (c->page_tokens == 1 << b) p.page_shift = b;
-    p.tiles = (int) tiles;
-    p.wl = CTAS / p.tiles;
     p.part = static_cast<float *>(scratch);
     p.ml = p.part + (size_t) CTAS * 2 * nmax * c->head_dim;
     p.split = reinterpret_cast<int4 *>(p.ml + (size_t) CTAS * 2 * nmax * 2);
