@@ -266,8 +266,9 @@ __global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ Selec
 }
 
 // ---- select: the largest `budget` keys of a list ------------------------------------------------------------------
-constexpr int NS = 1024, KR = 8;            // threads; keys that a thread holds in registers
-// Exclusive sum over the CTA's threads, and the whole. s: NS / 32 words, free again behind the caller's next barrier.
+constexpr int KR = 8;                       // keys that a thread holds in registers
+// Exclusive sum over the CTA's NS threads, and the whole. s: NS / 32 words, free again behind the caller's next barrier.
+template <int NS>
 SJK_DEV uint32_t cta_before(uint32_t x, uint32_t * s, uint32_t * all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t incl = x;
@@ -278,7 +279,7 @@ SJK_DEV uint32_t cta_before(uint32_t x, uint32_t * s, uint32_t * all) {
     }
     if (lane == 31) s[warp] = incl;
     __syncthreads();
-    const uint32_t w = s[lane];
+    const uint32_t w = lane < NS / 32 ? s[lane] : 0u;
     *all = __reduce_add_sync(FULL, w);
     return __reduce_add_sync(FULL, lane < warp ? w : 0u) + incl - x;
 }
@@ -287,10 +288,12 @@ SJK_DEV uint32_t cta_before(uint32_t x, uint32_t * s, uint32_t * all) {
 // which it lies in BINS parts of that, until exactly as many are left as are wanted (twice, for keys apart from one
 // another); then the keys above it and the first of those equal to it, in ascending order of their pages. A thread has a run
 // of KR pages in registers; lists of more than NS KR pages are read anew in every round. Counts alone are atomic: the same
-// lists every time.
-constexpr int BINS = 2 * NS;
-template <bool NEAR>
+// lists every time. NS threads: 256 for lists of up to 2,048 pages, whose barriers cost less (128 lists of up to 512: the
+// choice with its scores 24.7 us against 26.4 with 1,024).
+template <int NS, bool NEAR>
 __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int BINS = 2 * NS, LOG = NS == 1024 ? 11 : 9;
+    static_assert(BINS == 1 << LOG, "two bins a thread");
     __shared__ uint32_t s_bin[BINS], s_sum[4][NS / 32];
     __shared__ uint64_t s_min[NS / 32], s_max[NS / 32], s_from;
     __shared__ uint32_t s_above, s_in;
@@ -336,11 +339,12 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
     always = __reduce_add_sync(FULL, always);
     if (lane == 0) { s_sum[0][warp] = some; s_sum[1][warp] = always; }
     __syncthreads();
-    some = __reduce_add_sync(FULL, s_sum[0][lane]);
-    always = __reduce_add_sync(FULL, s_sum[1][lane]);
+    const bool on = lane < NS / 32;
+    some = __reduce_add_sync(FULL, on ? s_sum[0][lane] : 0u);
+    always = __reduce_add_sync(FULL, on ? s_sum[1][lane] : 0u);
     const uint32_t want = min((uint32_t) p.budget, some);
-    lo = s_min[lane];
-    hi = s_max[lane];
+    lo = on ? s_min[lane] : ALWAYS;
+    hi = on ? s_max[lane] : NEVER;
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         const uint64_t a = __shfl_xor_sync(FULL, lo, o), b = __shfl_xor_sync(FULL, hi, o);
@@ -354,7 +358,7 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
         uint32_t over = always;
         int bits = 64 - __clzll((long long) (hi - lo | 1ull));              // hi - lo < 2^bits
         for (;;) {
-            const int shift = bits > 11 ? bits - 11 : 0;
+            const int shift = bits > LOG ? bits - LOG : 0;
             s_bin[tid] = s_bin[tid + NS] = 0u;
             __syncthreads();
             each([&](uint64_t k, int) {
@@ -366,7 +370,7 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
             // from the highest part down: the first with `want` keys at or above it
             const uint32_t hi_n = s_bin[BINS - 1 - 2 * tid], lo_n = s_bin[BINS - 2 - 2 * tid];
             uint32_t all;
-            const uint32_t before = over + cta_before(hi_n + lo_n, s_sum[2], &all);
+            const uint32_t before = over + cta_before<NS>(hi_n + lo_n, s_sum[2], &all);
             if (before < want && before + hi_n + lo_n >= want) {
                 const bool first = before + hi_n >= want;
                 s_from = from + ((uint64_t) (first ? BINS - 1 - 2 * tid : BINS - 2 - 2 * tid) << shift);
@@ -389,8 +393,8 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
     });
     __syncthreads();
     uint32_t above_all, equal_all;
-    const uint32_t xa = cta_before(above, s_sum[0], &above_all);
-    uint32_t xe = cta_before(equal, s_sum[1], &equal_all);
+    const uint32_t xa = cta_before<NS>(above, s_sum[0], &above_all);
+    uint32_t xe = cta_before<NS>(equal, s_sum[1], &equal_all);
     const uint32_t ties = want - above_all;
     uint32_t at = xa + (xe < ties ? xe : ties);
     each([&](uint64_t k, int b) {
@@ -503,7 +507,9 @@ extern "C" int sjk_kv16_select(const sjk_kv16 * c, const void * bounds, const sj
     const dim3 grid((unsigned) n_seq, (unsigned) c->n_head_kv, (unsigned) z), one((unsigned) n_seq, (unsigned) c->n_head_kv);
     const int rs = c->type == SJK_F16 ? score_launch<SJK_F16>(p, grid, st) : score_launch<SJK_BF16>(p, grid, st);
     if (rs) return rs;
-    return c->table_stride <= (uint32_t) (NS * KR) ? launch(choose_kernel<true>, one, dim3(NS), 0, st, p) : launch(choose_kernel<false>, one, dim3(NS), 0, st, p);
+    if (c->table_stride <= 256u * KR) return launch(choose_kernel<256, true>, one, dim3(256), 0, st, p);
+    if (c->table_stride <= 1024u * KR) return launch(choose_kernel<1024, true>, one, dim3(1024), 0, st, p);
+    return launch(choose_kernel<1024, false>, one, dim3(1024), 0, st, p);
 }
 
 // The attention's part of the scratch behind the lists.
