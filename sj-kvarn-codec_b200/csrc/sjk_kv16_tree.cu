@@ -150,13 +150,17 @@ struct Shape {
     static constexpr int PART = BLOCKS * TS * 128, QP = BLOCKS * NMAX * 128, PB = NMAX / 64 * TS * 128;  // bytes: part of a K or V tile, of Q; term of P
     // slots (parts) of K and of V: what 227 KB hold beside Q and P
     static constexpr int KS = D == 64 ? (NMAX > 64 ? 4 : 5) : D == 256 || NMAX > 64 ? 2 : 3, VS = D == 64 ? (NMAX > 64 ? 3 : 4) : NMAX > 64 ? 1 : 2;
-    static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX, COLS = NMAX > 64 ? 512 : 256;     // of TMEM
+    // A weight's two terms as columns side by side (V is read once for both, 64 rows of 256 channels: 881 us sustained -> 846 for
+    // 32 sequences of 8K-64K), or one product after the other into the same sums (fewer columns of O: 128 rows of 128 channels,
+    // 100,000 tokens 242 against 260, 64 pieces of prompts 103 against 106).
+    static constexpr bool SIDE = PARTS > 1;
+    static constexpr uint32_t COL_S = 0, COL_O = 2 * NMAX, PART_O = SIDE ? 2 * NMAX : NMAX, COLS = COL_O + PARTS * PART_O > 256 ? 512 : 256;     // of TMEM
     static constexpr float SLACK = TYPE == SJK_F16 ? 5.0f : 8.0f, UP = TYPE == SJK_F16 ? 10.0f : 0.0f;
 };
 
 template <typename S>
 struct Shared {
-    uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2][S::PB];
+    uint8_t k[S::KS * S::PART], v[S::VS * S::PART], q[S::PARTS * S::QP], pt[2 * S::PB];
     Info<S::NMAX> info[INFO];
     uint32_t live[TILES][4];                // positions of a tile that have a row in the cache
     // of a row (in its group's place, which does not depend on how many rows a pair has): its maximum in use, what its scores are
@@ -388,7 +392,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         for (int item = 0; at.rem > 0; ++item) {
             const Seq s = at.s;
             const int steps = at.take(), h = at.h;
-            const int all8 = (s.nr + 15) / 16 * 2, most8 = (all8 + GROUPS - 1) / GROUPS;
+            const int n = (s.nr + 15) & ~15, all8 = n / 8, most8 = (all8 + GROUPS - 1) / GROUPS;     // columns of the products
             const int n8 = max(0, min(most8, all8 - group * most8)), c0 = group * most8 * 8, nc = n8 * 8;    // octets of columns, first column, their number
             const bool begun = at.st == 0, ended = at.st + steps == s.steps;
             const Info<NMAX> & info = sm.info[item % INFO];
@@ -478,14 +482,20 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                         for (int part = 0; part < S::PARTS; ++part)
 #pragma unroll 1
                             for (int q = 0; q < K; ++q) {
-                                const uint32_t addr = tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + cp + q * 8);
-                                float o[8];
+                                const uint32_t addr = tmem + lanes + S::COL_O + part * S::PART_O + (uint32_t) (cp + q * 8);
+                                float o[8], y[8];
                                 ld8(addr, o);
+                                if (S::SIDE) ld8(addr + (uint32_t) n, y);
                                 tc::wait_ld();
-                                uint32_t r[8];
+                                uint32_t r[8], z[8];
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) r[e] = __float_as_uint(o[e] * sm.fac[gp + q * 8 + e]);
+                                for (int e = 0; e < 8; ++e) {
+                                    const float f = sm.fac[gp + q * 8 + e];
+                                    r[e] = __float_as_uint(o[e] * f);
+                                    if (S::SIDE) z[e] = __float_as_uint(y[e] * f);
+                                }
                                 tc::st_x8(addr, r);
+                                if (S::SIDE) tc::st_x8(addr + (uint32_t) n, z);
                             }
                         tc::wait_st();
                     }
@@ -502,9 +512,11 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 wait_p();
 #pragma unroll
                 for (int q = 0; q < K; ++q) {
-                    const uint32_t o8 = (uint32_t) (cp >> 3) + (uint32_t) q, off = (o8 >> 3) * (TS * 128) + (uint32_t) tl * 128u + (((o8 ^ (uint32_t) tl) & 7u) << 4);
-                    *reinterpret_cast<uint4 *>(&sm.pt[0][off]) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
-                    *reinterpret_cast<uint4 *>(&sm.pt[1][off]) = make_uint4(lw[4 * q], lw[4 * q + 1], lw[4 * q + 2], lw[4 * q + 3]);
+                    const uint32_t h8 = (uint32_t) (cp >> 3) + (uint32_t) q;
+                    auto place = [&](uint32_t o8) { return (o8 >> 3) * (TS * 128) + (uint32_t) tl * 128u + (((o8 ^ (uint32_t) tl) & 7u) << 4); };
+                    const uint32_t ph = place(h8), pl = S::SIDE ? place(h8 + (uint32_t) (n >> 3)) : ph + S::PB;
+                    *reinterpret_cast<uint4 *>(&sm.pt[ph]) = make_uint4(hi[4 * q], hi[4 * q + 1], hi[4 * q + 2], hi[4 * q + 3]);
+                    *reinterpret_cast<uint4 *>(&sm.pt[pl]) = make_uint4(lw[4 * q], lw[4 * q + 1], lw[4 * q + 2], lw[4 * q + 3]);
                 }
             };
             for (int i = 0; i < steps; ++i, ++jj) {
@@ -568,12 +580,14 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 for (int part = 0; part < S::PARTS; ++part)
 #pragma unroll 1
                     for (int c = 0; c < nc; c += 8) {
-                        float o[8];
-                        ld8(tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c), o);
+                        float o[8], y[8];
+                        const uint32_t addr = tmem + lanes + S::COL_O + part * S::PART_O + (uint32_t) (c0 + c);
+                        ld8(addr, o);
+                        if (S::SIDE) ld8(addr + (uint32_t) n, y);
                         tc::wait_ld();
                         if (part * 128 + tl < D)
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) odd |= !(fabsf(o[e]) < INFINITY);
+                            for (int e = 0; e < 8; ++e) odd |= !(fabsf(S::SIDE ? o[e] + y[e] : o[e]) < INFINITY);
                     }
                 __syncwarp();
                 odd = any_of(bar, odd);
@@ -589,16 +603,19 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 const int d = part * 128 + tl;
 #pragma unroll 1
                 for (int c = 0; c < nc; c += 8) {
-                    float o[8];
-                    ld8(tmem + lanes + S::COL_O + (uint32_t) (part * NMAX + c0 + c), o);
+                    float o[8], y[8];
+                    const uint32_t addr = tmem + lanes + S::COL_O + part * S::PART_O + (uint32_t) (c0 + c);
+                    ld8(addr, o);
+                    if (S::SIDE) ld8(addr + (uint32_t) n, y);
                     tc::wait_ld();
                     if (d < D) {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
-                            const int n = c0 + c + e;
-                            if (n >= s.nr) continue;
-                            if (whole) store1(p.out.p, info.out[n] + d, S::TYPE, o[e] * sm.fac[g0 + c + e]);
-                            else part0[n * D + d] = o[e];
+                            const int r = c0 + c + e;
+                            if (r >= s.nr) continue;
+                            const float sum = S::SIDE ? o[e] + y[e] : o[e];
+                            if (whole) store1(p.out.p, info.out[r] + d, S::TYPE, sum * sm.fac[g0 + c + e]);
+                            else part0[r * D + d] = sum;
                         }
                     }
                 }
@@ -749,24 +766,25 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         auto second = [&](uint32_t j) {                      // O^T += V^T P of tile j
             if (pend_first && items > 1) wait.warp(&sm.o_free, (uint32_t) (items - 2) & 1u);
             wait.warp(&sm.p_full, j & 1u);
-            const uint32_t id = idesc<S::TYPE>(pend_n, true);
+            const uint32_t id = idesc<S::TYPE>(S::SIDE ? 2 * pend_n : pend_n, true);
 #pragma unroll 1
             for (int part = 0; part < S::PARTS; ++part, ++vp) {
                 const uint32_t slot = vp % VS;
                 wait.warp(&sm.v_full[slot], (vp / VS) & 1u);
                 tc::fence_after_sync();
                 const uint64_t a = swizzled(va + slot * S::PART, D == 64 ? 0u : TS * 128u), b = swizzled(pa, TS * 128u);
-                const uint32_t d = tm + S::COL_O + (uint32_t) (part * NMAX);
+                const uint32_t d = tm + S::COL_O + part * S::PART_O;
                 if (leader && !wait.dead) {
+                    constexpr int TERMS = S::SIDE ? 1 : 2;
                     if (pend_b - pend_a == TS / 16) {
 #pragma unroll
-                        for (int k = 0; k < 2 * TS / 16; ++k)
+                        for (int k = 0; k < TERMS * TS / 16; ++k)
                             mma_ss(d, a + (uint64_t) ((k & 7) * 2048 >> 4), b + (uint64_t) (((k >> 3) * S::PB + (k & 7) * 2048) >> 4), id, pend_first && k == 0 ? 0u : 1u);
                     } else {
 #pragma unroll 1
                         for (int k = pend_a; k < pend_b; ++k) {
                             mma_ss(d, a + (uint64_t) (k * 2048 >> 4), b + (uint64_t) (k * 2048 >> 4), id, pend_first && k == pend_a ? 0u : 1u);
-                            mma_ss(d, a + (uint64_t) (k * 2048 >> 4), b + (uint64_t) ((S::PB + k * 2048) >> 4), id, 1u);
+                            if (!S::SIDE) mma_ss(d, a + (uint64_t) (k * 2048 >> 4), b + (uint64_t) ((S::PB + k * 2048) >> 4), id, 1u);
                         }
                     }
                     tc::mma_commit(&sm.v_empty[slot]);
