@@ -532,7 +532,9 @@ int    sjk_truncate_batch(const sjk_trunc_req * reqs, int n, void * dev_pool, sj
  * Beside sealed layers a model may keep some at 16 bits (heads of 64 or 96 channels, first and last layers, a
  * draft model). These calls are their cache, what writes it, what reads it, and who owns its pages: sjk_qkv (norm
  * of every query and key head, rotary positions, cache write, in one pass), sjk_kv16_attend (attention of one new
- * token per sequence over the pages) and sjk_pages_* (fork, extend with copy on write, free, compact). sjk_qkv also
+ * token per sequence over the pages) and sjk_pages_* (fork, extend with copy on write, free, compact). Steps with several
+ * new tokens of every sequence (drafted trees, pieces of prompts) have sjk_kv16_maps, sjk_qkv_at, sjk_kv16_attend_tree and
+ * sjk_kv16_keep; attention to a part of a long context sjk_kv16_bounds, sjk_kv16_select and sjk_kv16_attend_blocks. sjk_qkv also
  * makes the rows that sjk_store and sjk_attend_model take, and the page calls work on the record pool's slab and
  * block tables as well. Lengths, positions, tables and row lists are DEVICE memory, read when the kernels run, so a
  * captured step replays. Like the other calls these launch on the current device: make the one current that the
@@ -619,8 +621,8 @@ int sjk_qkv_at(const sjk_qkv_args * a, const int32_t * at, sjk_stream st);
  * the query heads q[i] (type any); query head h reads KV head h / (n_head / n_head_kv). out[i] = sum over its last
  * min(len, window) positions (window 0: all) of softmax(scale q . k) v; a sequence without a live position (len <= 0,
  * or all its pages SJKVARN_NO_BLOCK) gets zeros. Positions on a SJKVARN_NO_BLOCK page are left out (pages that a
- * window has passed may be given back). A draft's several positions are so many entries with one row, each of which reads
- * the row's K and V anew (a prompt's own attention belongs in a kernel for many positions; there is none here). Any page
+ * window has passed may be given back). Several new positions of a sequence are so many entries with one row, each of which
+ * reads the row's K and V anew; sjk_kv16_attend_tree reads them once for all. Any page
  * size, any number of query heads per KV head; head_dim 64, 96, 128 or 256 (SJK_ERR_UNSUPPORTED), K and V rows 16-byte
  * aligned (SJKVARN_ERR_ARG); q of the cache's type 4-byte aligned. Sums and softmax statistics are 32-bit; weights, and
  * queries that are not of the cache's type, enter the products as sums of two or three 16-bit terms: 2^-16 (bf16 rows) or

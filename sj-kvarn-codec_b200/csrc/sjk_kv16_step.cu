@@ -1,7 +1,10 @@
 // sjk_kv16_step.cu - what a step that brings several tokens of every sequence needs beside its attention: the maps from
 // the sequences' lengths to tokens (sjk_kv16_maps), and the move of accepted drafts to their places (sjk_kv16_keep).
 //
-// Bound: a launch's latency, and for large calls the bytes: 20 written per token, a row once in and once out.
+// Bound: a launch's latency, and for large calls the bytes: 20 written per token, a row once in and once out. Measured (us a
+// pass from Python, on the GPU by CUDA graphs): maps of one chat's 8 drafts 5.4 and 2.3, of 512 requests with 15,500 tokens 5.0 and
+// 3.1; paths of up to 5 tokens in 16 layers 6.8 and 2.9; 64 paths of up to 9 in 32 layers of 4 x 256 f16 channels 16.1 and 16.1
+// (75 MB: 4.7 TB/s; 20 with 256 threads a CTA, of which half had no word).
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 

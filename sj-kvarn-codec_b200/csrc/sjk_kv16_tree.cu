@@ -3,19 +3,26 @@
 // and the drafted ones len + k whose bit k token j's mask has.
 //
 // All query heads of a KV head's group, of all the tokens of a sequence, are rows of one product: a key read once serves
-// (tokens x heads of a group) rows, up to NMAX = 64 in one pass, more in tiles of rows that CTAs side by side work on at the
-// same time, so that the second one's keys come from L2. Bound: HBM up to some 150 rows a KV head (4 D bytes per position
-// against 6 D flops per row and position here), the tensor cores and the shared memory that feeds them above that.
-//  - S^T = K Q^T with 128 positions as the M rows of tcgen05.mma and the query rows as its N columns (16 to 64), and
+// (tokens x heads of a group) rows, up to NMAX = 64 or 128 in one pass, more in tiles of rows that CTAs side by side work on at
+// the same time, so that the second one's keys come from L2 (100,000 tokens, 256 rows: 411 MB of DRAM reads for 410 MB of live
+// rows). Bound: HBM up to 64 rows a KV head, above that what the softmax warps issue (0.47 a cycle), and for short sequences the
+// chain of a tile (rows, products, maximum, weights, products), of some 4,000 cycles. Measured (us a pass from Python, of a
+// program that keeps the GPU busy, which then runs at 1.2 GHz under its power cap in the second case): one chat of 611 tokens with 8
+// drafts 14.2; 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels, 16 drafts x 4 heads 803 (6,260 GB/s of live rows: 95 % of
+// a plain copy's rate); 100,000 tokens, 8 heads of 128 f16 channels, 64 drafts x 4 heads 248 (424 TFLOP/s); 64 pieces of up to 33
+// tokens over windows of 512, 24 heads of 64 channels 101.
+//  - S^T = K Q^T with 128 positions as the M rows of tcgen05.mma and the query rows as its N columns (16 to 128), and
 //    O^T += V^T P with 128 channels as M: what a tile costs the softmax goes with the number of query rows, where query rows
 //    as M would make 8 of them as dear as 128. K, V and P lie in shared memory as they come: K rows are K-major for the
 //    first product, the same layout of V is MN-major for the second, and a thread, which has a position of all columns,
 //    writes its weights as whole 16-byte words of an MN-major P. S (two buffers) and O live in TMEM.
-//  - Warps: 8 for the softmax (two halves of the columns), one each that loads K, loads V (rings of their own, so that neither
-//    waits for the other's slots), issues the products, and loads the queries: 12, which leaves 168 registers a thread. Linked by mbarriers only; every
-//    wait is bounded.
-//  - Page tables are read a tile ahead, rows come with 16-byte cp.async into the swizzled layout: any page size, any strides;
-//    positions that are not live are filled with zeros.
+//  - Warps: 16 for the softmax (a quarter of the columns each four, 16 columns at a time: 260 us at 100,000 tokens, where 8 with 32
+//    columns took 269 and 16 with 32 spilled registers, 299), one each that loads K, loads V (rings of their own, so that neither
+//    waits for the other's slots), issues the products (a whole warp, so that descriptors are uniform: 32 sequences 1,355 -> 930
+//    with it and the boxes), and loads the queries. Linked by mbarriers only; every wait is bounded.
+//  - Pages of a multiple of 8 tokens come as TMA boxes of up to 128 tokens of a page and 64 channels, into the swizzled layout;
+//    others row by row with 16-byte cp.async. Rows of a box that are not live are zeroed on their way, and the second product
+//    takes groups of 16 positions with a live one alone.
 //  - The maximum of a row is looked for when a score is more than SLACK above the one in use (at a pair's start, seldom
 //    afterwards); then O is rescaled in TMEM. Weights reach 2^SLACK, which f16 and 32-bit sums have room for.
 //  - Weights enter as the sum of two 16-bit terms, as in sjk_kv16_attend: 2^-16 (bf16) or 2^-22 (f16) of a weight, and for

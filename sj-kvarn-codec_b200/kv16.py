@@ -11,6 +11,19 @@ that reads it (Cache), and who owns the pages (Pages: fork, extend with copy on 
     step(q, k, v, lens, q_out=q2, rows=rows, layer=il)  # position lens[i] of table row rows[i]
     out = cache.attend(il, q2, lens + 1, scale, rows=rows)
 
+Several new tokens of every sequence (a drafted tree, a piece of a prompt): Maps says whose each token is and where it goes,
+Qkv(at=) writes it there, Cache.attend_tree attends, Cache.keep moves the accepted path to its place. A part of a long
+context: Blocks keeps bounds of every page's keys, chooses pages for a query by them, and attends to these.
+
+    m = maps(lens, add, masks=masks)
+    step(q, k, v, m.pos, q_out=q2, rows=m.rows, at=m.at, layer=il)
+    out = cache.attend_tree(il, q2, lens, masks, scale, first=m.first, nodes=8)
+    lens = cache.keep(lens, path, count)
+    ...
+    lists, count = blocks.select(il, q2, lens + 1, 128)
+    out = blocks.attend(il, q2, lens + 1, lists, scale)
+    blocks.update(lens, lens + 1)                     # all layers, once a step
+
 Calls run on the tensors' device, on torch's current stream there, and do not synchronise; tensors of another device raise
 ValueError. Threads may share an object (a call of one waits for that of another until it is launched); what they launch on
 several streams is theirs to order. Lengths, positions and row lists are int32 CUDA tensors, read when the kernels run;
