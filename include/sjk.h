@@ -683,7 +683,7 @@ int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_stride, const 
  * among a page's tokens. sjk_kv16_bounds makes them anew, from the page's first position on, for the pages that hold
  * positions in [first[i], end[i]) of sequence i (DEVICE), from their positions before end[i], in n_layers layers (keys
  * layer_stride, bounds bounds_stride elements apart). A channel with a NaN has NaN as its bounds. Pages without a token
- * keep theirs. One launch.
+ * keep theirs; of sequences that share a page and name other ends on it, one's bounds stay. One launch.
  *
  * sjk_kv16_select chooses for every sequence and KV head up to `budget` pages of its table row, as their numbers there:
  * the first `sink` and the newest `recent` ones, and of the others those with the largest

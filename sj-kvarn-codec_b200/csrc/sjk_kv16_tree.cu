@@ -86,14 +86,18 @@ SJK_DEV int2 tokens_of(const Params & p, int i) {
 SJK_DEV int tiles_of(const Params & p, int i, int nmax) { return (tokens_of(p, i).y * p.grp + nmax - 1) / nmax; }
 SJK_DEV Seq seq_of(const Params & p, int i, int tile, int nmax) {
     Seq s = {0, 0, 0, 0, 0, 0, 0, 0u};
+    const int len = p.len[i];
     const int2 tok = tokens_of(p, i);
     s.first = tok.x;
     s.count = tok.y;
     const int rows = s.count * p.grp, tiles = (rows + nmax - 1) / nmax;
     if (tile >= tiles) return s;
-    s.row0 = (int) ((int64_t) rows * tile / tiles);
-    s.nr = (int) ((int64_t) rows * (tile + 1) / tiles) - s.row0;
-    s.len = max(p.len[i], 0);
+    s.nr = rows;
+    if (tiles > 1) {                        // (rows are at most CTAS NMAX: the products fit)
+        s.row0 = (int) ((unsigned) rows * (unsigned) tile / (unsigned) tiles);
+        s.nr = (int) ((unsigned) rows * (unsigned) (tile + 1) / (unsigned) tiles) - s.row0;
+    }
+    s.len = max(len, 0);
     int64_t hi = (int64_t) s.len + s.count;
     const int64_t cap = (int64_t) p.c.table_stride * p.c.page_tokens, most = cap < 0x7FFFFFFF ? cap : 0x7FFFFFFF;
     if (hi > most) { flag(); hi = most; }
@@ -580,31 +584,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 p.split[blockIdx.x] = make_int4(at.seq, h, sm.run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
             tc::nbar_sync(bar, 128);
             float * part0 = p.part + slot * D;
-            // Where some rows do not see all positions: 0 times what they do not see may have been no zero.
             bool odd = false;
-            if (partly(p, s, (uint32_t) (s.step0 + at.st) * TS) || partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) {
-#pragma unroll 1
-                for (int part = 0; part < S::PARTS; ++part)
-#pragma unroll 1
-                    for (int c = 0; c < nc; c += 8) {
-                        float o[8], y[8];
-                        const uint32_t addr = tmem + lanes + S::COL_O + part * S::PART_O + (uint32_t) (c0 + c);
-                        ld8(addr, o);
-                        if (S::SIDE) ld8(addr + (uint32_t) n, y);
-                        tc::wait_ld();
-                        if (part * 128 + tl < D)
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) odd |= !(fabsf(S::SIDE ? o[e] + y[e] : o[e]) < INFINITY);
-                    }
-                __syncwarp();
-                odd = any_of(bar, odd);
-            }
-            if (odd) {
-                const Run now = {at.seq, h, s.first, s.len, (uint32_t) (s.step0 + at.st) * TS, min(s.hi, (uint32_t) (s.step0 + at.st + steps) * TS)};
-                for (int c = quarter; c < nc && c0 + c < s.nr; c += 4)
-                    slow_row<S>(p, now, s.row0 + c0 + c, info.mask[c0 + c], info.lo[c0 + c], sc, sm.m[g0 + c], whole, sm.fac[g0 + c], info.out[c0 + c],
-                                part0 + (c0 + c) * D);
-            } else
 #pragma unroll 1
             for (int part = 0; part < S::PARTS; ++part) {
                 const int d = part * 128 + tl;
@@ -619,13 +599,22 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const int r = c0 + c + e;
-                            if (r >= s.nr) continue;
                             const float sum = S::SIDE ? o[e] + y[e] : o[e];
+                            odd |= !(fabsf(sum) < INFINITY);
+                            if (r >= s.nr) continue;
                             if (whole) store1(p.out.p, info.out[r] + d, S::TYPE, sum * sm.fac[g0 + c + e]);
                             else part0[r * D + d] = sum;
                         }
                     }
                 }
+            }
+            // Where some rows do not see all positions, 0 times what they do not see may have been no zero.
+            __syncwarp();
+            if ((partly(p, s, (uint32_t) (s.step0 + at.st) * TS) || partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) && any_of(bar, odd)) {
+                const Run now = {at.seq, h, s.first, s.len, (uint32_t) (s.step0 + at.st) * TS, min(s.hi, (uint32_t) (s.step0 + at.st + steps) * TS)};
+                for (int c = quarter; c < nc && c0 + c < s.nr; c += 4)
+                    slow_row<S>(p, now, s.row0 + c0 + c, info.mask[c0 + c], info.lo[c0 + c], sc, sm.m[g0 + c], whole, sm.fac[g0 + c], info.out[c0 + c],
+                                part0 + (c0 + c) * D);
             }
             tc::fence_before_sync();
             __syncwarp();
