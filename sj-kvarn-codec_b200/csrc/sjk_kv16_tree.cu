@@ -8,8 +8,8 @@
 // rows). Bound: HBM up to 64 rows a KV head, above that what the softmax warps issue (0.47 a cycle), and for short sequences the
 // chain of a tile (rows, products, maximum, weights, products), of some 4,000 cycles. Measured (us a pass from Python, of a
 // program that keeps the GPU busy, which then runs at 1.2 GHz under its power cap in the second case): one chat of 611 tokens with 8
-// drafts 14.2; 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels, 16 drafts x 4 heads 803 (6,260 GB/s of live rows: 95 % of
-// a plain copy's rate); 100,000 tokens, 8 heads of 128 f16 channels, 64 drafts x 4 heads 248 (424 TFLOP/s); 64 pieces of up to 33
+// drafts 13.6; 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels, 16 drafts x 4 heads 803-858 (89 to 95 % of a plain copy's
+// rate, box by box; 760 in bursts, at the full clock); 100,000 tokens, 8 heads of 128 f16 channels, 64 drafts x 4 heads 248 (424 TFLOP/s); 64 pieces of up to 33
 // tokens over windows of 512, 24 heads of 64 channels 101.
 //  - S^T = K Q^T with 128 positions as the M rows of tcgen05.mma and the query rows as its N columns (16 to 128), and
 //    O^T += V^T P with 128 channels as M: what a tile costs the softmax goes with the number of query rows, where query rows
