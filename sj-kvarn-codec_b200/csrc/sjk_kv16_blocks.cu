@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(NQ) score_kernel(const __grid_constant__ Selec
             }
 #pragma unroll
         for (int o = NA; o < 32 / HALF; o <<= 1) acc[0] += __shfl_xor_sync(FULL, acc[0], o);
-        // (D = 64: pages 8 to 15 are in the upper half)
+        // (D = 64: pages 4 to 7 are in the upper half)
         const double mine = HALF == 2 ? __shfl_sync(FULL, acc[0], (lane & (NA - 1)) + ((lane & (PG - 1)) / NA) * 16) : acc[0];
         if (lane < PG && b < nb) keys[b] = !have ? NEVER : b < p.sink || b >= nb - p.recent ? ALWAYS : order_of(mine);
     }
@@ -364,12 +364,13 @@ __global__ void __launch_bounds__(NS) choose_kernel(const __grid_constant__ Sele
         int bits = 64 - __clzll((long long) (hi - lo | 1ull));              // hi - lo < 2^bits
         for (;;) {
             const int shift = bits > LOG ? bits - LOG : 0;
+            const uint64_t parts = 1ull << (bits - shift);                  // BINS, or fewer in a last round: keys behind them are in `over`
             s_bin[tid] = s_bin[tid + NS] = 0u;
             __syncthreads();
             each([&](uint64_t k, int) {
                 if (k == NEVER || k == ALWAYS || k < from) return;
                 const uint64_t d = (k - from) >> shift;
-                if (d < (uint64_t) BINS) atomicAdd(&s_bin[d], 1u);
+                if (d < parts) atomicAdd(&s_bin[d], 1u);
             });
             __syncthreads();
             // from the highest part down: the first with `want` keys at or above it
