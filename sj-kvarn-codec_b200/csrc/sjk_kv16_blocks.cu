@@ -441,9 +441,9 @@ __global__ void __launch_bounds__(NT) lists_kernel(const __grid_constant__ ListP
         int before = __shfl_up_sync(FULL, b, 1);
         if (lane == 0) before = last;
         const bool ok = b >= 0 && b < nb && b > before;
-        if (!ok && e < p.budget && b != -1) flag();
         const unsigned good = __ballot_sync(FULL, ok);
         const int n = good == FULL ? 32 : __ffs(~good) - 1;      // up to the first that is none
+        if (lane == n && e < p.budget && b != -1) flag();        // (what lies behind it is not looked at)
         if (lane < n) pages[e] = table[b];
         count += n;
         if (n) last = __shfl_sync(FULL, b, n - 1);

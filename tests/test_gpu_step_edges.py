@@ -1,0 +1,57 @@
+"""Edges of the calls for several new tokens and for chosen pages: what lies behind a list's end, sequences of one
+position."""
+import pytest
+
+import kv16
+import sjk
+from test_gpu_blocks import _cache, _check, _ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def T():
+    import build
+    build.build()
+    import torch
+    assert torch.cuda.is_available()
+    return torch
+
+
+def test_nothing_counts_behind_a_list(T):
+    """Entries behind a list's -1 are not looked at: whatever they are, the result is that of the list and nothing is reported."""
+    lens = [200, 90]
+    cache, g = _cache(T, lens, 16, 2, 64, T.bfloat16)
+    blocks = kv16.Blocks(cache)
+    q = T.randn((2, 4, 64), device="cuda", generator=g).bfloat16()
+    tail = [5, 4, 2 ** 31 - 1, -2 ** 31, -9, 3, 3, 100] * 6
+    for head in ([], [3], [0, 5], list(range(6))):
+        mine = [[(head + [-1] + tail)[:40]] * 2] * 2
+        out = blocks.attend(0, q, _ints(T, lens), _ints(T, mine), 0.1)
+        _check(T, cache, out, q, lens, [[head] * 2] * 2, 0.1)
+        assert sjk.lib().sjk_device_status() == 0
+    # what ends a list without a -1 is reported, as before, wherever in the list it is
+    for at in (1, 31, 32, 33, 39):
+        for wrong in (0, -2, 13):
+            cache, g = _cache(T, [40 * 16], 16, 1, 64, T.bfloat16)
+            mine = list(range(40))
+            mine[at] = wrong if wrong != 13 else 10 ** 6
+            q1 = T.randn((1, 2, 64), device="cuda", generator=g).bfloat16()
+            out = kv16.Blocks(cache).attend(0, q1, _ints(T, [640]), _ints(T, [[mine]]), 0.1)
+            _check(T, cache, out, q1, [640], [[mine[:at]]], 0.1)
+            assert sjk.lib().sjk_device_status() == sjk.DEVICE_PAGE
+
+
+def test_lists_over_short_sequences(T):
+    """Lists over sequences of one position and of none."""
+    lens = [1, 0, 17, 1]
+    cache, g = _cache(T, [max(x, 1) for x in lens], 16, 2, 64, T.bfloat16)
+    q = T.randn((4, 6, 64), device="cuda", generator=g).bfloat16()
+    lists = [[[0, -1, -1]] * 2, [[-1, -1, -1]] * 2, [[1, -1, -1], [0, 1, -1]], [[-1, -1, -1], [0, -1, -1]]]
+    out = kv16.Blocks(cache).attend(0, q, _ints(T, lens), _ints(T, lists), 0.1)
+    _check(T, cache, out, q, lens, lists, 0.1)
+    assert bool((out[0] != 0).any()) and bool((out[3, 3:] != 0).any()) and sjk.lib().sjk_device_status() == 0
+    # (a list over a sequence without positions: its pages lie behind it)
+    out = kv16.Blocks(cache).attend(0, q, _ints(T, [-3, 0, 1, 1]), _ints(T, [[[0, -1, -1]] * 2] * 4), 0.1)
+    _check(T, cache, out, q, [0, 0, 1, 1], [[[]] * 2, [[]] * 2, [[0]] * 2, [[0]] * 2], 0.1)
+    assert sjk.lib().sjk_device_status() == sjk.DEVICE_PAGE
