@@ -142,7 +142,7 @@ __global__ void __launch_bounds__(NK) keep_kernel(const __grid_constant__ KeepPa
         const int32_t * path = p.path + (int64_t) i * p.width;
         const int32_t from = path[j];
         const int64_t a = (int64_t) len + from, b = (int64_t) len + j;
-        bad = from < j || (j > 0 && path[j - 1] >= from) || a >= (int64_t) p.c.table_stride * P;
+        bad = from < j || (j > 0 && path[j - 1] >= from) || a >= (int64_t) p.c.table_stride * P || a > 0x7FFFFFFE;   // (lengths are 32 bits)
         if (bad) break;
         const uint32_t ga = (uint32_t) (a / P), gb = (uint32_t) (b / P), pa = page_of(p.c, row, ga), pb = page_of(p.c, row, gb);
         bad = pa == SJKVARN_NO_BLOCK || pb == SJKVARN_NO_BLOCK;

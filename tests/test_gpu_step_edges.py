@@ -1,5 +1,5 @@
 """Edges of the calls for several new tokens and for chosen pages: what lies behind a list's end, sequences of one
-position."""
+position, and positions past the last one that 32 bits number."""
 import pytest
 
 import kv16
@@ -55,3 +55,24 @@ def test_lists_over_short_sequences(T):
     out = kv16.Blocks(cache).attend(0, q, _ints(T, [-3, 0, 1, 1]), _ints(T, [[[0, -1, -1]] * 2] * 4), 0.1)
     _check(T, cache, out, q, [0, 0, 1, 1], [[[]] * 2, [[]] * 2, [[0]] * 2, [[0]] * 2], 0.1)
     assert sjk.lib().sjk_device_status() == sjk.DEVICE_PAGE
+
+
+def test_kept_positions_end_at_2_31(T):
+    """Paths that reach past position 2^31 - 2 are left out, as the maps leave such tokens out, however long the table row is."""
+    page, D = 2 ** 20, 64
+    cache = kv16.Cache.alloc(1, 2, page, 1, D, T.bfloat16, 1, 2050)
+    g = T.Generator(device="cuda")
+    g.manual_seed(1)
+    cache.k.normal_(generator=g)
+    cache.v.normal_(generator=g)
+    cache.tables.fill_(-1)
+    cache.tables[0, 2047:2049] = _ints(T, [1, 0])
+    length, k, v = 2 ** 31 - 6, cache.k.clone(), cache.v.clone()
+    for path in ([0, 2, 6], [1, 3, 5], [7]):
+        new = cache.keep(_ints(T, [length]), _ints(T, [path]), _ints(T, [len(path)]))
+        assert new.tolist() == [length] and sjk.lib().sjk_device_status() == sjk.DEVICE_PAGE
+        assert T.equal(cache.k, k) and T.equal(cache.v, v)
+    new = cache.keep(_ints(T, [length]), _ints(T, [[1, 4]]), _ints(T, [2]))
+    assert new.tolist() == [length + 2] and sjk.lib().sjk_device_status() == 0
+    place = page - 6
+    assert T.equal(cache.k[0, 1, place: place + 2], k[0, 1, [place + 1, place + 4]]) and T.equal(cache.v[0, 1, place: place + 2], v[0, 1, [place + 1, place + 4]])
