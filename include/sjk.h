@@ -670,7 +670,7 @@ int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int n_tok, cons
                          const sjk_rows * out, void * scratch, size_t scratch_bytes, sjk_stream st);
 /* Accepted drafts to their places: of sequence i the K and V rows of the positions len[i] + path[i][j], j < count[i], go to
  * len[i] + j in all n_layers layers (layer l's rows at c's plus l * layer_stride elements), and new_len[i] (DEVICE, may be
- * NULL, not over len) = len[i] + count[i]. path: DEVICE [n_seq][width], ascending; width <= SJK_KEEP_MAX. Where a path does
+ * NULL, not over an input) = len[i] + count[i]. path: DEVICE [n_seq][width], ascending; width <= SJK_KEEP_MAX. Where a path does
  * not ascend, a position has no page or lies past 2^31 - 2, or an earlier entry has the same table row, nothing of the sequence
  * moves, new_len is len, and SJK_DEVICE_PAGE is set. The pages written to are the sequence's own (sjk_pages_extend has split them). One
  * launch. */

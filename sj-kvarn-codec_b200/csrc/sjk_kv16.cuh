@@ -18,6 +18,11 @@ static inline bool aligned(const void * p, size_t n) { return (reinterpret_cast<
 // rows whose address is a multiple of an element's size; a list of int32 (NULL passes)
 static inline bool rows_ok(const sjk_rows & r) { return aligned(r.p, type_bytes(r.type)); }
 static inline bool list_ok(const void * p) { return aligned(p, 4); }
+// no byte of `na` from a is one of `nb` from b (NULL passes): what one CTA writes while others still read
+static inline bool apart(const void * a, size_t na, const void * b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return !a || !b || !na || !nb || (x < y ? y - x >= na : x - y >= nb);
+}
 
 // two 16-bit values of a word, widened; two floats rounded to nearest even and packed
 template <int TYPE>

@@ -198,9 +198,9 @@ extern "C" int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_str
     if (!c || sjk_kv16_check(c) || n_layers < 1 || n_layers > 65535 || layer_stride < 0 || width < 1 || width > SJK_KEEP_MAX || n_seq < 0) return SJKVARN_ERR_ARG;
     if ((n_seq && (!len || !path || !count)) || !list_ok(len) || !list_ok(path) || !list_ok(count) || !list_ok(rows) || !list_ok(new_len)) return SJKVARN_ERR_ARG;
     if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
-    // every CTA of a sequence reads its length, one writes the new one
-    if (new_len && n_seq && reinterpret_cast<uintptr_t>(new_len) < reinterpret_cast<uintptr_t>(len + n_seq) &&
-        reinterpret_cast<uintptr_t>(len) < reinterpret_cast<uintptr_t>(new_len + n_seq))
+    // every CTA of a sequence reads its length, path, count and row (and the rows before it), one writes the new length
+    const size_t list = (size_t) n_seq * sizeof(int32_t);
+    if (!apart(new_len, list, len, list) || !apart(new_len, list, path, list * width) || !apart(new_len, list, count, list) || !apart(new_len, list, rows, list))
         return SJKVARN_ERR_ARG;
     if (n_seq == 0) return 0;
     const KeepParams p = {*c, layer_stride, len, path, count, rows, n_seq, width, new_len};

@@ -377,7 +377,7 @@ class Cache:
     def keep(self, lens, path, count, rows=None, new_lens=None):
         """Accepted drafts to their places, in every layer: K and V of the positions lens[i] + path[i][j], j < count[i], to
         lens[i] + j. lens, count int32 [n], path int32 [n][width], ascending; rows int32 [n] (None: sequence i is table row
-        i). Returns the lengths with the accepted ones (a new vector unless given; not lens itself)."""
+        i). Returns the lengths with the accepted ones (a new vector unless given; not an input's own)."""
         n, dev = lens.shape[0], self._dev
         if path.dim() != 2:
             raise ValueError("path: int32 [n][width]")

@@ -76,3 +76,17 @@ def test_kept_positions_end_at_2_31(T):
     assert new.tolist() == [length + 2] and sjk.lib().sjk_device_status() == 0
     place = page - 6
     assert T.equal(cache.k[0, 1, place: place + 2], k[0, 1, [place + 1, place + 4]]) and T.equal(cache.v[0, 1, place: place + 2], v[0, 1, [place + 1, place + 4]])
+
+
+def test_new_lengths_beside_the_inputs(T):
+    """Lengths, paths, counts, rows and new lengths side by side in one buffer."""
+    cache, g = _cache(T, [60, 60, 60], 16, 1, 64, T.bfloat16)
+    k, v = cache.k.clone(), cache.v.clone()
+    buf = _ints(T, [50, 51, 52] + [1, 3, 0, 2, 4, 5] + [2, 1, 2] + [7, 7, 7] + [2, 1, 0])
+    lens, path, count, new, rows = buf[:3], buf[3:9].view(3, 2), buf[9:12], buf[12:15], buf[15:]
+    assert cache.keep(lens, path, count, rows=rows, new_lens=new) is new
+    assert buf.tolist() == [50, 51, 52, 1, 3, 0, 2, 4, 5, 2, 1, 2, 52, 52, 54, 2, 1, 0] and sjk.lib().sjk_device_status() == 0
+    for row, length, p in ((2, 50, [1, 3]), (1, 51, [0]), (0, 52, [4, 5])):
+        for j, t in enumerate(p):
+            a, b = ((int(cache.tables[row, x // 16]), x % 16) for x in (length + t, length + j))
+            assert T.equal(cache.k[0, b[0], b[1]], k[0, a[0], a[1]]) and T.equal(cache.v[0, b[0], b[1]], v[0, a[0], a[1]])
