@@ -644,7 +644,7 @@ int sjk_kv16_attend(const sjk_kv16 * c, const sjk_rows * q, const int32_t * len,
  *             sequence's) len[i] plus the number of others that it sees; padding -1
  *   slot[t]   page * page_tokens + place on the page, -1 without a page
  * Tokens beyond n_tok, negative lengths and counts, rows and pages outside their arrays are left out (SJK_DEVICE_PAGE).
- * row, pos and at are what sjk_qkv_at takes. One launch. */
+ * Outputs do not lie over inputs. row, pos and at are what sjk_qkv_at takes. One launch. */
 #define SJK_MAPS_MAX 8192
 typedef struct sjk_kv16_step {
     int32_t * first, * row, * pos, * at;

@@ -188,6 +188,13 @@ extern "C" int sjk_kv16_maps(const sjk_kv16 * c, const int32_t * len, const int3
         !list_ok(out->row) || !list_ok(out->pos) || !list_ok(out->at) || !aligned(out->slot, 8))
         return SJKVARN_ERR_ARG;
     if (!rows && (int64_t) n_seq > (int64_t) c->n_rows) return SJKVARN_ERR_ARG;
+    // every CTA reads all counts, and its tokens' lengths, rows and masks, while others write
+    const size_t seqs = (size_t) n_seq * sizeof(int32_t), toks = (size_t) n_tok * sizeof(int32_t);
+    const struct { const void * p; size_t n; } in[4] = {{len, seqs}, {add, seqs}, {rows, seqs}, {masks, 2 * toks}},
+        to[5] = {{out->first, seqs + sizeof(int32_t)}, {out->row, toks}, {out->pos, toks}, {out->at, toks}, {out->slot, 2 * toks}};
+    for (const auto & x : in)
+        for (const auto & y : to)
+            if (!apart(x.p, x.n, y.p, y.n)) return SJKVARN_ERR_ARG;
     MapParams p = {*c, len, add, rows, masks, n_seq, n_tok, *out};
     const int64_t ctas = ((int64_t) n_tok + NT - 1) / NT;
     return launch(maps_kernel, dim3((unsigned) (ctas < 1 ? 1 : ctas < 148 * 4 ? ctas : 148 * 4)), dim3(NT), (size_t) (n_seq + 1) * sizeof(int32_t), st, p);

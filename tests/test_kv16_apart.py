@@ -25,3 +25,26 @@ def _keep(L, new, n=2, width=4, rows=ROWS):
 def test_keep_refuses_new_lengths_over_its_inputs(L, new):
     assert _keep(L, new) == -100
     assert _keep(L, new, n=0) == 0
+
+
+def _maps(L, n=2, n_tok=8, masks=P + 0x5000, rows=ROWS, c=None, **out):
+    step = sjk.Kv16Step(*(P + 0x10000 + i * 0x1000 for i in range(5)))
+    for k, v in out.items():
+        setattr(step, k, v)
+    return L.sjk_kv16_maps(C.byref(c or _cache()), LEN, COUNT, rows, masks, n, n_tok, C.byref(step), None)
+
+
+@pytest.mark.parametrize("what", ["first", "row", "pos", "at", "slot"])
+@pytest.mark.parametrize("over", [LEN, COUNT, ROWS, P + 0x5000])
+def test_maps_refuse_outputs_over_inputs(L, what, over):
+    """(The inputs are 8 bytes, the masks 64; outputs 12, 32 or 64.)"""
+    size = {"first": 12, "slot": 64}.get(what, 32)
+    last = over + (64 if over == P + 0x5000 else 8)
+    for at in (over, last - 8, over - size + 8):
+        assert _maps(L, **{what: at}) == -100
+
+
+@pytest.mark.parametrize("bad", [dict(n=-1), dict(n=8193), dict(n_tok=-1), dict(rows=ROWS + 2), dict(masks=P + 0x5004), dict(first=NEW + 1), dict(row=NEW + 2),
+                                 dict(pos=NEW + 3), dict(at=NEW + 2), dict(slot=NEW + 4), dict(n=5, rows=None), dict(c=_cache(tables=None)), dict(c=_cache(page_tokens=0))])
+def test_maps_refusals_of_lists_apart(L, bad):
+    assert _maps(L, **bad) == -100
