@@ -690,8 +690,8 @@ int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_stride, const 
  *   sum over the group's query heads of sum_d max(q_d lo_d, q_d hi_d)
  * (in 64 bits; ties to the lower number; a sum that is no number counts as the largest), all where there are no more than
  * `budget`. blocks[i][h] (DEVICE [n_seq][n_head_kv][budget]): ascending, then -1; count (DEVICE [n_seq][n_head_kv], may be
- * NULL): how many. Pages that are SJKVARN_NO_BLOCK are never chosen. The newest page's bounds may be older than its last
- * tokens where `recent` covers it. Two launches.
+ * NULL): how many; neither lies over len. Pages that are SJKVARN_NO_BLOCK are never chosen. The newest page's bounds may be
+ * older than its last tokens where `recent` covers it. Two launches.
  *
  * sjk_kv16_attend_blocks is sjk_kv16_attend over the positions on the listed pages alone: blocks as above, from any
  * source; a list ends at its first entry that is -1, does not ascend or lies behind the sequence (the last two set

@@ -505,6 +505,9 @@ extern "C" int sjk_kv16_select(const sjk_kv16 * c, const void * bounds, const sj
     if (c->n_head_kv > 65535) return SJK_ERR_UNSUPPORTED;
     if (n_seq == 0) return 0;
     if (!scratch || !aligned(scratch, 16) || scratch_bytes < sjk_kv16_select_scratch_bytes(c, n_seq)) return SJKVARN_ERR_BUFFER;
+    // the lists of a sequence's other heads are still chosen by its length when one head's are written
+    const size_t lens = (size_t) n_seq * sizeof(int32_t), all = lens * c->n_head_kv;
+    if (!apart(len, lens, blocks, all * budget) || !apart(len, lens, count, all)) return SJKVARN_ERR_ARG;
     const SelectParams p = {*c, static_cast<const uint16_t *>(bounds), *q, len, rows, n_seq, q->n_head / c->n_head_kv, budget, sink, recent,
                             static_cast<uint64_t *>(scratch), blocks, count};
     const int64_t lists = (int64_t) n_seq * c->n_head_kv, groups = ((int64_t) c->table_stride + NQ / 32 * PG - 1) / (NQ / 32 * PG);

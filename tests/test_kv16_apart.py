@@ -4,7 +4,7 @@ import ctypes as C
 import pytest
 
 import sjk
-from test_kv16 import P, _cache
+from test_kv16 import P, _cache, _rows
 
 
 @pytest.fixture(scope="module")
@@ -48,3 +48,10 @@ def test_maps_refuse_outputs_over_inputs(L, what, over):
                                  dict(pos=NEW + 3), dict(at=NEW + 2), dict(slot=NEW + 4), dict(n=5, rows=None), dict(c=_cache(tables=None)), dict(c=_cache(page_tokens=0))])
 def test_maps_refusals_of_lists_apart(L, bad):
     assert _maps(L, **bad) == -100
+
+
+@pytest.mark.parametrize("over", [dict(blocks=LEN), dict(blocks=LEN + 4), dict(blocks=LEN - 60), dict(count=LEN), dict(count=LEN + 4), dict(count=LEN - 12)])
+def test_select_refuses_lists_over_lengths(L, over):
+    """(Lengths 8 bytes, lists 2 x 2 x 4 numbers, counts 2 x 2.)"""
+    a = dict(dict(blocks=PATH, count=COUNT), **over)
+    assert L.sjk_kv16_select(C.byref(_cache()), P + 0x8000, C.byref(_rows(4)), LEN, ROWS, 2, 4, 1, 1, a["blocks"], a["count"], P + 0x20000, 1 << 30, None) == -100
