@@ -658,9 +658,11 @@ int sjk_kv16_maps(const sjk_kv16 * c, const int32_t * len, const int32_t * add, 
  * of softmax(scale q . k) v over them, zeros where there are none. Tokens of sequence i: [first[i], first[i + 1]) (DEVICE
  * [n_seq + 1]; NULL: `nodes` each), `nodes` of them at most, nodes <= SJK_TREE_MAX; rows of q in no sequence, or in one with
  * more, are left as they were (the latter set SJK_DEVICE_PAGE). K and V of the new tokens lie in the cache already (sjk_qkv_at).
- * Infinities and NaNs reach the tokens that see them alone. Positions on SJKVARN_NO_BLOCK pages are left out. q and out of the
- * cache's type; q, K and V rows 16-byte aligned; head_dim 64, 96, 128 or 256; up to 148 x 64 rows, or 148 x 128 for
- * head_dim <= 128 (nodes x query heads of a KV head; SJK_ERR_UNSUPPORTED). Sums and statistics are 32-bit, weights sums of two 16-bit terms. scratch:
+ * Infinities and NaNs reach the tokens that see them alone; an output element is the sum of those that its token sees in V (an
+ * infinity, or NaN), whatever the call's other sequences. out may be q's own rows. Positions on SJKVARN_NO_BLOCK pages are left
+ * out. q and out of the cache's type; q, K and V rows 16-byte aligned; head_dim 64, 96, 128 or 256; up to 148 x 64 rows, or
+ * 148 x 128 for head_dim <= 128 (nodes x query heads of a KV head; SJK_ERR_UNSUPPORTED). Sums and statistics are 32-bit, weights
+ * sums of two 16-bit terms. scratch:
  * sjk_kv16_attend_tree_scratch_bytes() bytes, 16-byte aligned, for whatever lengths; not shared by calls that overlap. Two
  * launches; the same inputs give the same bits. */
 #define SJK_TREE_MAX 64

@@ -27,8 +27,13 @@
 //    afterwards); then O is rescaled in TMEM. Weights reach 2^SLACK, which f16 and 32-bit sums have room for.
 //  - Weights enter as the sum of two 16-bit terms, as in sjk_kv16_attend: 2^-16 (bf16) or 2^-22 (f16) of a weight, and for
 //    f16, whose weights are held 2^10 larger, at most 2^-35 of the row's largest. Sums and statistics are 32-bit.
-//  - Positions that only some of the rows see (drafted ones, a window's edge) may hold infinities or NaNs, and 0 times
-//    those is no zero: where a sum of such a run comes out as no number, its rows are summed anew, position by position.
+//  - V may hold infinities or NaNs in positions that only some of the rows see (drafted ones, a window's edge), and 0 times those is no
+//    zero, nor is it one in a weight's second term. Pairs of which a sum comes out as no number are gone through once more behind
+//    all others, with V's infinities and NaNs as zeros (noted on the way, per channel or, where rows see different positions, per
+//    position) and then put into the sums of the rows that see them. So a bad value costs its CTA's pairs a second time in the same
+//    pipeline, however long they are, and no role waits longer than for a tile (rows summed anew where they occur, a position
+//    at a time, would hold the others up beyond what they wait). Looking for them in every V tile instead slows all calls. A NaN in
+//    every sequence (us, a call without and with): 1 x 611 13.5 and 32, 1 x 100,000 217 and 971, 32 x 36,000 746 and 4,450.
 // A list of (sequence, KV head) pairs in steps of 128 positions is cut into equal runs, one per CTA, for each tile of rows;
 // lengths are read from device memory. Split pairs leave (m, l, o) in the scratch and a second kernel joins them in order.
 #include "sjk_kv16.cuh"
@@ -52,6 +57,8 @@ constexpr int GROUPS = 4;                   // of softmax warps, which divide th
 constexpr int N_SOFT = 4 * GROUPS, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
 constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
 constexpr int INFO = 4, TILES = 16;         // rings of what a pair's rows and a tile's positions are
+constexpr int SEG = 1024;                   // pairs that are gone through before those of them that come again
+constexpr int EDGES = 4;                    // tiles of a pair of which rows see different positions: up to 64 positions from two places on
 __device__ unsigned int g_tree_status;
 
 SJK_DEV void flag() { atomicOr(&g_tree_status, (unsigned) SJK_DEVICE_PAGE); }
@@ -64,6 +71,7 @@ struct Params {
     int n_seq, n_tok, nodes, grp;
     int window, page_shift;
     float scale;
+    bool over;                              // outputs may lie over the queries
     float * part;                           // [CTA][2][NMAX][D]
     float * ml;                             // [CTA][2][NMAX][2]
     int4 * split;                           // by CTA: sequence (-1: none), KV head, first and last run; behind them: tiles
@@ -179,9 +187,16 @@ struct Shared {
     float m[S::NMAX], up[S::NMAX], fac[S::NMAX], red[N_SOFT][32];
     uint64_t k_full[S::KS], k_empty[S::KS], v_full[S::VS], v_empty[S::VS], v_land[S::VS];
     uint64_t s_full[2], s_empty[2], q_full[INFO], p_full, pv_done, o_free, q_empty;
-    Cursor start;
+    Cursor start, next;                     // of this segment, and of the one behind it
+    uint32_t tiles, pairs, landed;          // gone through so far: where the roles are in their rings
     uint32_t per, tmem;
     int tile, run;
+    // pairs of the segment that come again (a bit per group of softmax warps), and of the one that is gone through again: the sum of V's
+    // infinities and NaNs in places that all rows see, and the places of the others
+    uint32_t again[SEG * GROUPS / 32], any_again;
+    float bad[S::PARTS * 128];
+    uint32_t edge[EDGES][4], edge_t0[EDGES];
+    int edges;
 };
 
 // ---- products -----------------------------------------------------------------------------------------------------
@@ -272,125 +287,112 @@ struct Waiter {
     }
 };
 
-// A row's sum over the positions of a run that it sees, one after the other: for runs in which some V row that not all rows
-// see holds an infinity or NaN (which a product with a weight of 0 does not take out). A warp; the row's maximum in use is m. The
-// sum times inv goes to the output, or (not whole) the sum to `part`.
-struct Run { int seq, h, first, len; uint32_t t0, t1; };
+// A part of a V tile of a pair that is gone through again, by a warp: infinities and NaNs become zeros and are noted, per channel or (`edge`
+// not negative: the tile's place among those of which rows see different positions) per position; rows that are not live: zeros.
 template <typename S>
-__device__ __noinline__ void slow_row(const Params & p, Run at, int r, uint64_t mask, int lo, float sc, float m, bool whole, float inv, int64_t out, float * part) {
-    constexpr int D = S::D, NC = D / 32;
-    const int lane = threadIdx.x & 31, j = r / p.grp, head = at.h * p.grp + (r - j * p.grp);
-    const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
-    const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
-    float q[NC], o[NC];
+__device__ __noinline__ void clean_tile(Shared<S> & sm, uint8_t * tile, unsigned live0, unsigned live1, unsigned live2, unsigned live3, int part, int edge) {
+    constexpr int LR = S::BLOCKS * 8, RI = 32 / LR;         // lanes of a row, rows at a time
+    constexpr uint32_t E = S::TYPE == SJK_F16 ? 0x7C00u : 0x7F80u;
+    const int lane = threadIdx.x & 31, wd = lane % LR, d = part * 128 + wd * 8;
+    for (int r0 = lane / LR; r0 < TS; r0 += 4 * RI) {
+        auto place = [&](int b) { const int rt = r0 + b * RI; return reinterpret_cast<uint4 *>(tile + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4)); };
+        uint4 x[4];                         // (their loads are out together)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        q[c] = load1(p.q.p, (int64_t) (at.first + j) * p.q.row_stride + (int64_t) head * p.q.head_stride + 32 * c + lane, S::TYPE);
-        q[c] = p.scale < 0.0f ? -q[c] : p.scale > 0.0f ? q[c] : 0.0f;
-        o[c] = 0.0f;
-    }
-    for (uint32_t t = at.t0; t < at.t1 && table; ++t) {
-        if (t >= (uint32_t) at.len ? !((mask >> (t - (uint32_t) at.len)) & 1ull) : t < (uint32_t) lo) continue;
-        const uint32_t g = t / (uint32_t) p.c.page_tokens, page = table[g];
-        if (page >= p.c.n_pages) continue;
-        const int64_t at_kv = (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride + (int64_t) at.h * p.c.head_stride + lane;
-        float x = 0.0f;
+        for (int b = 0; b < 4; ++b) x[b] = *place(b);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) x = fmaf(q[c], load1(p.c.k, at_kv + 32 * c, S::TYPE), x);
+        for (int b = 0; b < 4; ++b) {
+            const int rt = r0 + b * RI;
+            const unsigned live = rt < 32 ? live0 : rt < 64 ? live1 : rt < 96 ? live2 : live3;
+            if (!((live >> (rt & 31)) & 1u)) { *place(b) = make_uint4(0u, 0u, 0u, 0u); continue; }
+            if (d >= S::D) continue;
+            uint32_t w[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
+            bool found = false;
 #pragma unroll
-        for (int i = 16; i; i >>= 1) x += __shfl_xor_sync(FULL, x, i);
-        const float w = tc::num::ex2(x * sc - (m == -INFINITY ? 0.0f : m) + S::UP);
+            for (int e = 0; e < 4; ++e) found |= (w[e] & E) == E || (w[e] & (E << 16)) == E << 16;
+            if (!found) continue;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const float v = load1(p.c.v, at_kv + 32 * c, S::TYPE);
-            o[c] = fabsf(v) < INFINITY ? fmaf(w, v, o[c]) : o[c] + v;
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t sh = (e & 1) * 16;
+                if (((w[e / 2] >> sh) & E) != E) continue;
+                const float2 f = widen2<S::TYPE>(w[e / 2]);
+                if (edge < 0) atomicAdd(&sm.bad[d + e], e & 1 ? f.y : f.x);  // (infinities and NaNs alone: any order gives the same)
+                w[e / 2] &= ~(0xFFFFu << sh);
+            }
+            if (edge >= 0) atomicOr(&sm.edge[edge][rt >> 5], 1u << (rt & 31));
+            *place(b) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     }
+    __syncwarp();
+}
+
+// What V's infinities and NaNs make of a row of a pair that was gone through again: where it sees some, their sum in place of the finite one. A
+// warp; to the output, or (not whole) to `part`.
+template <typename S>
+__device__ __noinline__ void mark_row(const Params & p, const Shared<S> & sm, int seq, int h, int len, uint64_t mask, int lo, bool whole, int64_t out, float * part) {
+    constexpr int NC = S::D / 32;
+    const int lane = threadIdx.x & 31;
+    const int64_t row = p.rows ? (int64_t) p.rows[seq] : (int64_t) seq;
+    const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
+    float x[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x[c] = sm.bad[32 * c + lane];
+    for (int k = 0; k < sm.edges * 4 && table; ++k)
+        for (uint32_t bits = sm.edge[k >> 2][k & 3]; bits; bits &= bits - 1u) {
+            const uint32_t t = sm.edge_t0[k >> 2] + (uint32_t) (32 * (k & 3) + __ffs((int) bits) - 1);
+            if (t >= (uint32_t) len ? !((mask >> (t - (uint32_t) len)) & 1ull) : t < (uint32_t) lo) continue;
+            const uint32_t g = t / (uint32_t) p.c.page_tokens, page = table[g];
+            if (page >= p.c.n_pages) continue;
+            const int64_t at = (int64_t) page * p.c.page_stride + (int64_t) (t - g * (uint32_t) p.c.page_tokens) * p.c.slot_stride + (int64_t) h * p.c.head_stride + lane;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float v = load1(p.c.v, at + 32 * c, S::TYPE);
+                if (!(fabsf(v) < INFINITY)) x[c] += v;
+            }
+        }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        if (whole) store1(p.out.p, out + 32 * c + lane, S::TYPE, o[c] * inv);
-        else part[32 * c + lane] = o[c];
+        if (fabsf(x[c]) < INFINITY) continue;
+        if (whole) store1(p.out.p, out + 32 * c + lane, S::TYPE, x[c]);
+        else part[32 * c + lane] = x[c];
     }
 }
 
-template <typename S, bool WHOLE>
-__global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
-    constexpr int D = S::D, KS = S::KS, VS = S::VS, NMAX = S::NMAX;
-    extern __shared__ uint8_t raw[];
-    Shared<S> & sm = *reinterpret_cast<Shared<S> *>(raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u));
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-    if (tid == 0) {
-        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 1); tc::mbar_init(&sm.k_empty[i], 1); }
-        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 1); tc::mbar_init(&sm.v_empty[i], 1); tc::mbar_init(&sm.v_land[i], 1); }
-        for (int i = 0; i < 2; ++i) { tc::mbar_init(&sm.s_full[i], 1); tc::mbar_init(&sm.s_empty[i], N_SOFT); }
-        tc::mbar_init(&sm.p_full, N_SOFT);
-        tc::mbar_init(&sm.pv_done, 1);
-        tc::mbar_init(&sm.o_free, N_SOFT);
-        for (int i = 0; i < INFO; ++i) tc::mbar_init(&sm.q_full[i], 1);
-        tc::mbar_init(&sm.q_empty, 1);
-        tc::mbar_fence_init();
-    }
-    if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, S::COLS); tc::tmem_relinquish(); }
-    pdl_wait();
-    pdl_release();
-    // As many lists as the sequence with the most rows has tiles, side by side in the grid, and where the CTA's run begins in
-    // its own: units of all sequences, a block of them per lane.
-    if (warp == 0) {
-        const int block = (p.n_seq + 31) / 32;
-        int tiles = 1;
-        uint32_t mine = 0;
-        for (int i = 0; i < block; ++i)
-            if (lane * block + i < p.n_seq) tiles = max(tiles, tiles_of(p, lane * block + i, NMAX));
-        tiles = (int) __reduce_max_sync(FULL, (unsigned) tiles);
-        const int tile = blockIdx.x % tiles, run = blockIdx.x / tiles, wl = gridDim.x / tiles;
-        for (int i = 0; i < block; ++i)
-            if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile, NMAX));
-        uint32_t incl = mine;
+// Whether one of a thread's sums (nc columns from addr on, n columns apart where a weight's terms lie side by side) is no number. A function, since
+// few calls come here and its registers cost the others 1 to 3 % in line.
+template <typename S>
+__device__ __noinline__ bool odd_sums(uint32_t addr, int n, int nc, int tl) {
+    bool odd = false;
+    for (int part = 0; part < S::PARTS; ++part)
+        for (int c = 0; c < nc; c += 8) {
+            float o[8], y[8];
+            ld8(addr + part * S::PART_O + (uint32_t) c, o);
+            if (S::SIDE) ld8(addr + part * S::PART_O + (uint32_t) (c + n), y);
+            tc::wait_ld();
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(FULL, incl, o);
-            if (lane >= o) incl += y;
+            for (int e = 0; e < 8; ++e) odd |= c + e < nc && part * 128 + tl < S::D && !(fabsf(S::SIDE ? o[e] + y[e] : o[e]) < INFINITY);
         }
-        const uint32_t list = __shfl_sync(FULL, incl, 31);
-        uint32_t per = (list + (uint32_t) wl - 1u) / (uint32_t) wl;
-        if (per < MIN_RUN) per = MIN_RUN;
-        const int64_t o = (int64_t) run * per;
-        Cursor c = {};
-        if (o < list && run < wl) {
-            const uint32_t off = (uint32_t) o;
-            c.rem = (int) (o + per < list ? per : list - off);
-            const int g = __ffs(__ballot_sync(FULL, incl > off)) - 1;
-            c.base = __shfl_sync(FULL, incl - mine, g);
-            c.seq = g * block;
-            for (;; ++c.seq) {              // (the block's last sequence at the latest: its sum is above off)
-                c.s = seq_of(p, c.seq, tile, NMAX);
-                const uint32_t u = units_of(p, c.s);
-                if (c.base + u > off) break;
-                c.base += u;
-            }
-            c.h = (int) ((off - c.base) / (uint32_t) (c.s.steps + OV));
-            c.base += (uint32_t) c.h * (uint32_t) (c.s.steps + OV);
-            const int in = (int) (off - c.base);
-            c.st = in > OV ? in - OV : 0;
-            if (in < OV) c.rem -= OV - in;  // no steps where the run has only units before a first step
-        }
-        if (lane == 0) {
-            sm.start = c;
-            sm.per = per;
-            sm.tile = tile;
-            sm.run = run;
-            p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
-            if (blockIdx.x == 0) p.split[gridDim.x] = make_int4(tiles, 0, 0, 0);
-        }
-    }
-    tc::fence_before_sync();
-    __syncthreads();
-    tc::fence_after_sync();
+    return odd;
+}
+
+// Every role's way through the pairs of a segment: all of them, or (again) those of which a sum came out as no number. FIRST: the first
+// segment's pairs for the first time, which is all that most calls have.
+template <typename S, bool WHOLE, bool FIRST>
+SJK_DEV void pass(const Params & p, Shared<S> & sm, bool anew) {
+    constexpr int D = S::D, KS = S::KS, VS = S::VS, NMAX = S::NMAX;
+    const bool again = !FIRST && anew;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t tmem = sm.tmem;
     Cursor at = sm.start;
     Waiter wait;
-
+    int place = -1;                         // of the pair in the segment
+    // whether there is one more
+    auto more = [&]() {
+        for (++place; at.rem > 0 && place < SEG; ++place) {
+            if (!again || ((sm.again[place * GROUPS / 32] >> (place * GROUPS % 32)) & ((1u << GROUPS) - 1u))) return true;
+            at.next(p, sm.tile, NMAX, at.take());
+        }
+        return false;
+    };
     if (warp < N_SOFT) {
         // ---- softmax: position 32 (warp % 4) + lane of a tile; two groups of four warps have half of the columns each ----
         const int group = warp >> 2, quarter = warp & 3, bar = 1 + group, tl = quarter * 32 + lane, tg = tid & 127, g0 = group * S::MINE;
@@ -399,8 +401,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         const float sc = p.scale == 0.0f ? 1.0f : fabsf(p.scale) * 1.4426950408889634f;
         const float2 sc2 = make_float2(sc, sc);
         float2 l[S::MINE / 2];              // sums of the thread's columns, in pairs
-        uint32_t jj = 0;                    // tiles so far
-        for (int item = 0; at.rem > 0; ++item) {
+        uint32_t jj = FIRST ? 0u : sm.tiles;                 // tiles so far
+        for (int item = FIRST ? 0 : (int) sm.pairs; more(); ++item) {
             const Seq s = at.s;
             const int steps = at.take(), h = at.h;
             const int n = (s.nr + 15) & ~15, all8 = n / 8, most8 = (all8 + GROUPS - 1) / GROUPS;     // columns of the products
@@ -582,12 +584,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             }
             if (tid == 0 && begun && !ended)
                 p.split[blockIdx.x] = make_int4(at.seq, h, sm.run, (int) ((at.base + (uint32_t) (s.steps + OV) - 1u) / sm.per));
-            tc::nbar_sync(bar, 128);
-            float * part0 = p.part + slot * D;
-            bool odd = false;
-#pragma unroll 1
-            for (int part = 0; part < S::PARTS; ++part) {
-                const int d = part * 128 + tl;
+            // f(column, sum of the thread's channel of this part) over the group's rows
+            auto sums = [&](int part, auto && f) {
 #pragma unroll 1
                 for (int c = 0; c < nc; c += 8) {
                     float o[8], y[8];
@@ -595,26 +593,41 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     ld8(addr, o);
                     if (S::SIDE) ld8(addr + (uint32_t) n, y);
                     tc::wait_ld();
-                    if (d < D) {
+                    if (part * 128 + tl < D)
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int r = c0 + c + e;
-                            const float sum = S::SIDE ? o[e] + y[e] : o[e];
-                            odd |= !(fabsf(sum) < INFINITY);
-                            if (r >= s.nr) continue;
-                            if (whole) store1(p.out.p, info.out[r] + d, S::TYPE, sum * sm.fac[g0 + c + e]);
-                            else part0[r * D + d] = sum;
-                        }
-                    }
+                        for (int e = 0; e < 8; ++e)
+                            if (c0 + c + e < s.nr) f(c + e, S::SIDE ? o[e] + y[e] : o[e]);
+                }
+            };
+            // Rows of a group with a sum that is no number are stored the second time (there: no others); the first time as well, unless
+            // outputs lie over the queries, which the second one reads.
+            tc::nbar_sync(bar, 128);
+            const uint32_t bit = 1u << (place * GROUPS % 32 + group);
+            uint32_t & word = sm.again[place * GROUPS / 32];
+            const bool mine = again ? (word & bit) != 0u : !p.over || !any_of(bar, odd_sums<S>(tmem + lanes + S::COL_O + (uint32_t) c0, n, min(nc, s.nr - c0), tl));
+            float * part0 = p.part + slot * D;
+            bool odd = !mine;
+            if (mine) {
+#pragma unroll 1
+                for (int part = 0; part < S::PARTS; ++part) {
+                    const int d = part * 128 + tl;
+                    sums(part, [&](int c, float x) {
+                        odd |= !(fabsf(x) < INFINITY);
+                        if (whole) store1(p.out.p, info.out[c0 + c] + d, S::TYPE, x * sm.fac[g0 + c]);
+                        else part0[(c0 + c) * D + d] = x;
+                    });
                 }
             }
-            // Where some rows do not see all positions, 0 times what they do not see may have been no zero.
             __syncwarp();
-            if ((partly(p, s, (uint32_t) (s.step0 + at.st) * TS) || partly(p, s, (uint32_t) (s.step0 + at.st + steps - 1) * TS)) && any_of(bar, odd)) {
-                const Run now = {at.seq, h, s.first, s.len, (uint32_t) (s.step0 + at.st) * TS, min(s.hi, (uint32_t) (s.step0 + at.st + steps) * TS)};
+            if (!again) {
+                if (any_of(bar, odd) && tg == 0) {
+                    atomicOr(&word, bit);
+                    sm.any_again = 1u;
+                }
+            } else if (mine) {
+                tc::nbar_sync(bar, 128);
                 for (int c = quarter; c < nc && c0 + c < s.nr; c += 4)
-                    slow_row<S>(p, now, s.row0 + c0 + c, info.mask[c0 + c], info.lo[c0 + c], sc, sm.m[g0 + c], whole, sm.fac[g0 + c], info.out[c0 + c],
-                                part0 + (c0 + c) * D);
+                    mark_row<S>(p, sm, at.seq, h, s.len, info.mask[c0 + c], info.lo[c0 + c], whole, info.out[c0 + c], part0 + (c0 + c) * D);
             }
             tc::fence_before_sync();
             __syncwarp();
@@ -628,7 +641,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
         const int slots = is_v ? VS : KS;
         uint64_t * full = is_v ? sm.v_full : sm.k_full, * empty = is_v ? sm.v_empty : sm.k_empty;
         uint8_t * ring = is_v ? sm.v : sm.k;
-        uint32_t jj = 0, pp = 0, told = 0;  // tiles; parts asked for, and announced (not WHOLE)
+        uint32_t jj = FIRST ? 0u : sm.tiles, pp = jj * S::PARTS, told = pp;     // tiles; parts asked for, and announced (not WHOLE)
         auto tell = [&](uint32_t upto) {    // copies of the parts before `upto` have landed
             tc::fence_proxy_async();
             __syncwarp();
@@ -636,8 +649,9 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 if (lane == 0) tc::mbar_arrive(&full[told % slots]);
         };
         // WHOLE: a part of a V tile whose dead rows (that came with a box, or came not) are to be zeros
-        struct Mend { bool on; int slot; unsigned dead[4]; } m = {};
-        uint32_t landed = 0;                // parity of every slot's v_land
+        struct Mend { bool on; int slot, part, edge; unsigned dead[4]; } m = {};
+        uint32_t landed = FIRST ? 0u : sm.landed;            // parity of every slot's v_land
+        int item = FIRST ? 0 : (int) sm.pairs, edges = 0;
         auto mend_box = [&]() {             // once it has landed
             m.on = false;
             wait.warp(&sm.v_land[m.slot], (landed >> m.slot) & 1u);
@@ -645,9 +659,10 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             uint8_t * dst = ring + m.slot * S::PART;
             constexpr int LR = S::BLOCKS * 8, RI = 32 / LR;         // lanes of a row, rows at a time
             const int wd = lane % LR;
+            if (again) clean_tile<S>(sm, dst, ~m.dead[0], ~m.dead[1], ~m.dead[2], ~m.dead[3], m.part, m.edge);
 #pragma unroll
             for (int g = 0; g < 4; ++g)
-                for (int r0 = 0; r0 < 32 && m.dead[g] >> r0; r0 += RI) {
+                for (int r0 = 0; !again && r0 < 32 && m.dead[g] >> r0; r0 += RI) {
                     const int r = r0 + lane / LR, rt = 32 * g + r;
                     if ((m.dead[g] >> r) & 1u) *reinterpret_cast<uint4 *>(dst + (wd >> 3) * (TS * 128) + rt * 128 + (((wd ^ rt) & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
                 }
@@ -655,9 +670,27 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&full[m.slot]);
         };
-        while (at.rem > 0) {
+        auto flush = [&] {
+            if (WHOLE) {
+                if (m.on) mend_box();
+            } else {
+                tc::cp_async_wait_group<0>();
+                tell(pp);
+            }
+        };
+        for (; more(); ++item) {
             const Seq s = at.s;
             const int steps = at.take();
+            const bool clean = again && is_v;
+            if (clean) {                    // the notes of the pair before have been read
+                flush();
+                if (item > 0) wait.warp(&sm.o_free, (uint32_t) (item - 1) & 1u);
+                for (int d = lane; d < S::PARTS * 128; d += 32) sm.bad[d] = 0.0f;
+                if (lane < EDGES * 4) sm.edge[lane >> 2][lane & 3] = 0u;
+                edges = 0;
+                if (lane == 0) sm.edges = 0;
+                __syncwarp();
+            }
             const int64_t row = p.rows ? (int64_t) p.rows[at.seq] : (int64_t) at.seq;
             const uint32_t * table = row >= 0 && row < (int64_t) p.c.n_rows ? p.c.tables + row * p.c.table_stride : nullptr;
             if (!table && lane == 0) flag();
@@ -688,7 +721,16 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     dead[u] = __ballot_sync(FULL, WHOLE && is_v && off[u] < 0 && g16 >= a16 && g16 < b16);     // (copies fill theirs with zeros)
                     if (!is_v && lane == 0) sm.live[jj % TILES][u] = live[u];
                 }
-                const bool mend = (dead[0] | dead[1] | dead[2] | dead[3]) != 0u;
+                int edge = -1;
+                if (clean) {
+                    if (partly(p, s, t0)) {
+                        edge = edges++;
+                        if (lane == 0) { sm.edge_t0[edge] = t0; sm.edges = edges; }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) dead[u] = ~live[u];
+                }
+                const bool mend = WHOLE && (clean || (dead[0] | dead[1] | dead[2] | dead[3]) != 0u);
                 const bool asks = WHOLE && page[4] < p.c.n_pages;
                 const uint32_t tx = WHOLE ? (uint32_t) __popc(__ballot_sync(FULL, asks)) * (uint32_t) p.box * 128u : 0u;
 #pragma unroll 1
@@ -720,6 +762,8 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                     if (mend) {
                         m.on = true;
                         m.slot = slot;
+                        m.part = part;
+                        m.edge = edge;
 #pragma unroll
                         for (int u = 0; u < 4; ++u) m.dead[u] = dead[u];
                     }
@@ -734,6 +778,13 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                                 tc::cp_async16(dst + (c >> 3) * (TS * 128) + (32 * u + r) * 128 + (((c ^ r) & 7) << 4), base + (o >= 0 ? o : 0) + c * 8, o >= 0 ? 16u : 0u);
                             }
                         tc::cp_async_commit();
+                        if (clean) {
+                            tc::cp_async_wait_group<0>();
+                            __syncwarp();
+                            clean_tile<S>(sm, dst, live[0], live[1], live[2], live[3], part, edge);
+                            tell(pp + 1);
+                            continue;
+                        }
                         if (slots == 1) tc::cp_async_wait_group<0>();
                         else if (slots == 2) tc::cp_async_wait_group<1>();
                         else if (slots == 3) tc::cp_async_wait_group<2>();
@@ -745,19 +796,15 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             }
             at.next(p, sm.tile, NMAX, steps);
         }
-        if (WHOLE) {
-            if (m.on) mend_box();
-        } else {
-            tc::cp_async_wait_group<0>();
-            tell(pp);
-        }
+        flush();
+        if (is_v && lane == 0) sm.landed = landed;
     } else if (warp == W_MMA) {
         // ---- products: the warp stays together and one thread issues, so that descriptors are the same for all lanes ----
         const bool leader = elected();
         const uint32_t ka = tc::smem_addr(sm.k), va = tc::smem_addr(sm.v), qa = tc::smem_addr(sm.q), pa = tc::smem_addr(sm.pt);
         const uint32_t tm = __shfl_sync(FULL, tmem, 0);
-        uint32_t jj = 0, kp = 0, vp = 0;                     // tiles; parts of K and of V
-        int pend_n = 0, pend_a = 0, pend_b = 0, items = 0;
+        uint32_t jj = FIRST ? 0u : sm.tiles, kp = jj * S::PARTS, vp = kp;       // tiles; parts of K and of V
+        int pend_n = 0, pend_a = 0, pend_b = 0, items = FIRST ? 0 : (int) sm.pairs;
         bool pend = false, pend_first = false;               // a tile whose second product is to come
         auto second = [&](uint32_t j) {                      // O^T += V^T P of tile j
             if (pend_first && items > 1) wait.warp(&sm.o_free, (uint32_t) (items - 2) & 1u);
@@ -789,7 +836,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
                 __syncwarp();
             }
         };
-        while (at.rem > 0) {
+        while (more()) {
             const int steps = __shfl_sync(FULL, at.take(), 0), n = __shfl_sync(FULL, (at.s.nr + 15) & ~15, 0);
             const uint32_t id = idesc<S::TYPE>(n, false);
             if (pend) second(jj - 1);       // the pair's end does not wait for the next one's queries
@@ -829,9 +876,14 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             at.next(p, sm.tile, NMAX, steps);
         }
         if (pend) second(jj - 1);
+        if (lane == 0) {
+            sm.tiles = jj;
+            sm.pairs = (uint32_t) items;
+            if (!again) sm.next = at;
+        }
     } else {
         // ---- queries, and what the rows see ----
-        for (int item = 0; at.rem > 0; ++item) {
+        for (int item = FIRST ? 0 : (int) sm.pairs; more(); ++item) {
             const Seq s = at.s;
             const int steps = at.take(), n = (s.nr + 15) & ~15;
             if (item > 0) wait.warp(&sm.q_empty, (uint32_t) (item - 1) & 1u);
@@ -886,9 +938,107 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             at.next(p, sm.tile, NMAX, steps);
         }
     }
+}
+// What follows a segment's first turn: its pairs that come again, and the segments behind it. A function of its own and not inlined: as a second
+// turn of the same code it cost the first one 3 to 20 % (registers).
+template <typename S, bool WHOLE>
+__device__ __noinline__ void rest(const Params & p, Shared<S> & sm) {
+    const int tid = threadIdx.x;
+    for (bool again = sm.any_again;; again = !again && sm.any_again) {
+        if (!again) {
+            if (sm.next.rem <= 0) return;
+            __syncthreads();                // all have looked at what is made new here
+            if (tid == 0) { sm.start = sm.next; sm.any_again = 0u; }
+            if (tid < SEG * GROUPS / 32) sm.again[tid] = 0u;
+            __syncthreads();
+        }
+        pass<S, WHOLE, false>(p, sm, again);
+        __syncthreads();
+    }
+}
+
+template <typename S, bool WHOLE>
+__global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Params p) {
+    constexpr int KS = S::KS, VS = S::VS, NMAX = S::NMAX;
+    extern __shared__ uint8_t raw[];
+    Shared<S> & sm = *reinterpret_cast<Shared<S> *>(raw + ((1024u - (tc::smem_addr(raw) & 1023u)) & 1023u));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < KS; ++i) { tc::mbar_init(&sm.k_full[i], 1); tc::mbar_init(&sm.k_empty[i], 1); }
+        for (int i = 0; i < VS; ++i) { tc::mbar_init(&sm.v_full[i], 1); tc::mbar_init(&sm.v_empty[i], 1); tc::mbar_init(&sm.v_land[i], 1); }
+        for (int i = 0; i < 2; ++i) { tc::mbar_init(&sm.s_full[i], 1); tc::mbar_init(&sm.s_empty[i], N_SOFT); }
+        tc::mbar_init(&sm.p_full, N_SOFT);
+        tc::mbar_init(&sm.pv_done, 1);
+        tc::mbar_init(&sm.o_free, N_SOFT);
+        for (int i = 0; i < INFO; ++i) tc::mbar_init(&sm.q_full[i], 1);
+        tc::mbar_init(&sm.q_empty, 1);
+        tc::mbar_fence_init();
+        sm.any_again = 0u;
+    }
+    if (tid < SEG * GROUPS / 32) sm.again[tid] = 0u;
+    if (warp == W_MMA) { tc::tmem_alloc(&sm.tmem, S::COLS); tc::tmem_relinquish(); }
+    pdl_wait();
+    pdl_release();
+    // As many lists as the sequence with the most rows has tiles, side by side in the grid, and where the CTA's run begins in
+    // its own: units of all sequences, a block of them per lane.
+    if (warp == 0) {
+        const int block = (p.n_seq + 31) / 32;
+        int tiles = 1;
+        uint32_t mine = 0;
+        for (int i = 0; i < block; ++i)
+            if (lane * block + i < p.n_seq) tiles = max(tiles, tiles_of(p, lane * block + i, NMAX));
+        tiles = (int) __reduce_max_sync(FULL, (unsigned) tiles);
+        const int tile = blockIdx.x % tiles, run = blockIdx.x / tiles, wl = gridDim.x / tiles;
+        for (int i = 0; i < block; ++i)
+            if (lane * block + i < p.n_seq) mine += units_of(p, seq_of(p, lane * block + i, tile, NMAX));
+        uint32_t incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(FULL, incl, o);
+            if (lane >= o) incl += y;
+        }
+        const uint32_t list = __shfl_sync(FULL, incl, 31);
+        uint32_t per = (list + (uint32_t) wl - 1u) / (uint32_t) wl;
+        if (per < MIN_RUN) per = MIN_RUN;
+        const int64_t o = (int64_t) run * per;
+        Cursor c = {};
+        if (o < list && run < wl) {
+            const uint32_t off = (uint32_t) o;
+            c.rem = (int) (o + per < list ? per : list - off);
+            const int g = __ffs(__ballot_sync(FULL, incl > off)) - 1;
+            c.base = __shfl_sync(FULL, incl - mine, g);
+            c.seq = g * block;
+            for (;; ++c.seq) {              // (the block's last sequence at the latest: its sum is above off)
+                c.s = seq_of(p, c.seq, tile, NMAX);
+                const uint32_t u = units_of(p, c.s);
+                if (c.base + u > off) break;
+                c.base += u;
+            }
+            c.h = (int) ((off - c.base) / (uint32_t) (c.s.steps + OV));
+            c.base += (uint32_t) c.h * (uint32_t) (c.s.steps + OV);
+            const int in = (int) (off - c.base);
+            c.st = in > OV ? in - OV : 0;
+            if (in < OV) c.rem -= OV - in;  // no steps where the run has only units before a first step
+        }
+        if (lane == 0) {
+            sm.start = c;
+            sm.per = per;
+            sm.tile = tile;
+            sm.run = run;
+            p.split[blockIdx.x] = make_int4(-1, 0, 0, 0);
+            if (blockIdx.x == 0) p.split[gridDim.x] = make_int4(tiles, 0, 0, 0);
+        }
+    }
     tc::fence_before_sync();
     __syncthreads();
-    if (warp == W_MMA) tc::tmem_dealloc(tmem, S::COLS);
+    tc::fence_after_sync();
+    pass<S, WHOLE, true>(p, sm, false);
+    __syncthreads();
+    if (sm.any_again || sm.next.rem > 0) rest<S, WHOLE>(p, sm);
+    tc::fence_before_sync();
+    __syncthreads();
+    if (warp == W_MMA) tc::tmem_dealloc(sm.tmem, S::COLS);
 }
 
 // Joins the runs of a split pair in order. grid: CTAs of the kernel before, rows in groups of 8, a warp each.
@@ -929,8 +1079,10 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const __grid_constant__
         for (int v = 0; v < NV; ++v)
             if (32 * v + lane < D / 4) {
                 const float4 x = reinterpret_cast<const float4 *>(p.part + at * D)[32 * v + lane];
-                o[v].x = fmaf(x.x, f, o[v].x); o[v].y = fmaf(x.y, f, o[v].y);
-                o[v].z = fmaf(x.z, f, o[v].z); o[v].w = fmaf(x.w, f, o[v].w);
+                // (an infinity stays one, however small the run's share)
+                auto add = [&](float a, float y) { return fabsf(a) < INFINITY ? fmaf(a, f, y) : a + y; };
+                o[v].x = add(x.x, o[v].x); o[v].y = add(x.y, o[v].y);
+                o[v].z = add(x.z, o[v].z); o[v].w = add(x.w, o[v].w);
             }
     }
     const int j = (s.row0 + r) / p.grp, head = e.y * p.grp + (s.row0 + r) - j * p.grp;
@@ -1037,6 +1189,8 @@ extern "C" int sjk_kv16_attend_tree(const sjk_kv16 * c, const sjk_rows * q, int 
     p.first = first; p.len = len; p.rows = rows; p.masks = masks;
     p.n_seq = n_seq; p.n_tok = n_tok; p.nodes = nodes; p.grp = grp;
     p.window = window; p.scale = scale;
+    auto span = [&](const sjk_rows & r) { return ((size_t) (n_tok - 1) * r.row_stride + (size_t) (r.n_head - 1) * r.head_stride + c->head_dim) * 2; };
+    p.over = (q->row_stride | q->head_stride | out->row_stride | out->head_stride) < 0 || !apart(q->p, span(*q), out->p, span(*out));
     p.page_shift = -1;
     for (int b = 0; b < 31; ++b)
         if (c->page_tokens == 1 << b) p.page_shift = b;
