@@ -52,7 +52,6 @@ constexpr unsigned FULL = 0xFFFFFFFFu;
 constexpr int TS = 128;                     // positions of a step
 constexpr int CTAS = 148;                   // one per SM
 constexpr int OV = 1;                       // what a pair costs beside its steps, in steps
-constexpr int MIN_RUN = 1;                  // units of a run, at least
 constexpr int GROUPS = 4;                   // of softmax warps, which divide the columns
 constexpr int N_SOFT = 4 * GROUPS, N_LOAD = 2;       // warps; then one that issues products, and one that loads queries
 constexpr int W_MMA = N_SOFT + N_LOAD, W_Q = W_MMA + 1, NT = 32 * (W_Q + 1);
@@ -233,13 +232,13 @@ SJK_DEV void ld8(uint32_t t, float * v) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
-SJK_DEV bool any_of(int id, bool x) {       // over the 128 threads of a half
+SJK_DEV bool any_of(int id, bool x) {       // over the 128 threads of a group
     uint32_t r;
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
                  : "=r"(r) : "r"((uint32_t) x), "r"(id), "r"(128) : "memory");
     return r != 0;
 }
-// 8 K columns of a lane over the warp's lanes: lane c gets column c (with fewer than 32, lanes c + 8 K i as well)
+// N columns of a lane over the warp's lanes: lane c gets column c (with fewer than 32, lanes c + N i as well)
 template <bool MAX, int N>
 SJK_DEV float columns(const float * v, int lane) {
     float a[N / 2];
@@ -264,15 +263,6 @@ SJK_DEV float columns(const float * v, int lane) {
         x = MAX ? fmaxf(x, r) : x + r;
     }
     return x;
-}
-template <bool MAX, int K>
-SJK_DEV float octets(const float * v, int lane) {
-    if constexpr (K == 3) {
-        float w[32];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) w[i] = i < 24 ? v[i] : MAX ? -INFINITY : 0.0f;
-        return columns<MAX, 32>(w, lane);
-    } else return columns<MAX, 8 * K>(v, lane);
 }
 // Waits that give up once and for all: after one that ran out (the status word says so) a role goes on without waiting, so
 // that everyone meets the same barriers and the CTA ends.
@@ -394,7 +384,7 @@ SJK_DEV void pass(const Params & p, Shared<S> & sm, bool anew) {
         return false;
     };
     if (warp < N_SOFT) {
-        // ---- softmax: position 32 (warp % 4) + lane of a tile; two groups of four warps have half of the columns each ----
+        // ---- softmax: position 32 (warp % 4) + lane of a tile; four groups of four warps have a quarter of the columns each ----
         const int group = warp >> 2, quarter = warp & 3, bar = 1 + group, tl = quarter * 32 + lane, tg = tid & 127, g0 = group * S::MINE;
         const uint32_t lanes = (uint32_t) (quarter * 32) << 16;
         // scores are positive multiples of the products (the queries' signs are turned for a negative scale)
@@ -417,7 +407,6 @@ SJK_DEV void pass(const Params & p, Shared<S> & sm, bool anew) {
             for (int c = 0; c < S::MINE / 2; ++c) l[c] = make_float2(0.0f, 0.0f);
             tc::nbar_sync(bar, 128);
             wait.warp(&sm.q_full[item % INFO], (uint32_t) (item / INFO) & 1u);
-            auto sees = [&](uint32_t t, int n) { return t >= (uint32_t) s.len ? (bool) ((info.mask[n] >> (t - (uint32_t) s.len)) & 1ull) : t >= (uint32_t) info.lo[n]; };
             // K octets of columns of tile jj, from cp on (from gp on in the group's places): weights into P, sums into lp
             auto octets_of = [&](auto kk, int cp, int gp, float2 * lp, bool fresh, int step, unsigned live, auto && wait_p) {
                 constexpr int K = decltype(kk)::value, N = 8 * K;
@@ -469,7 +458,7 @@ SJK_DEV void pass(const Params & p, Shared<S> & sm, bool anew) {
                     if (renew) load();
                 }
                 if (renew) {                // a row's first tile, or a score too far above the maximum in use: a new one
-                    const float top = octets<true, K>(x, lane);
+                    const float top = columns<true, N>(x, lane);
                     sm.red[warp][lane] = top;
                     tc::nbar_sync(bar, 128);
                     if (tg < N) {
@@ -999,8 +988,7 @@ __global__ void __launch_bounds__(NT, 1) tree_kernel(const __grid_constant__ Par
             if (lane >= o) incl += y;
         }
         const uint32_t list = __shfl_sync(FULL, incl, 31);
-        uint32_t per = (list + (uint32_t) wl - 1u) / (uint32_t) wl;
-        if (per < MIN_RUN) per = MIN_RUN;
+        const uint32_t per = (list + (uint32_t) wl - 1u) / (uint32_t) wl;        // (at least a unit, where there is one)
         const int64_t o = (int64_t) run * per;
         Cursor c = {};
         if (o < list && run < wl) {
