@@ -657,7 +657,7 @@ int sjk_kv16_maps(const sjk_kv16 * c, const int32_t * len, const int32_t * add, 
  * tokens do not count; masks NULL: itself and the ones before it), of all these the last `window` (0: all). out[t] = sum
  * of softmax(scale q . k) v over them, zeros where there are none. Tokens of sequence i: [first[i], first[i + 1]) (DEVICE
  * [n_seq + 1]; NULL: `nodes` each), `nodes` of them at most, nodes <= SJK_TREE_MAX; rows of q in no sequence, or in one with
- * more, are left as they were (the latter set SJK_DEVICE_PAGE). K and V of the new tokens lie in the cache already (sjk_qkv_at).
+ * more, are left as they were (the latter set SJK_DEVICE_PAGE); a negative length counts as 0. K and V of the new tokens lie in the cache already (sjk_qkv_at).
  * Infinities and NaNs reach the tokens that see them alone; an output element is the sum of those that its token sees in V (an
  * infinity, or NaN), whatever the call's other sequences. out may be q's own rows. Positions on SJKVARN_NO_BLOCK pages are left
  * out. q and out of the cache's type; q, K and V rows 16-byte aligned; head_dim 64, 96, 128 or 256; up to 148 x 64 rows, or
@@ -685,12 +685,14 @@ int sjk_kv16_keep(const sjk_kv16 * c, int n_layers, int64_t layer_stride, const 
  * among a page's tokens. sjk_kv16_bounds makes them anew, from the page's first position on, for the pages that hold
  * positions in [first[i], end[i]) of sequence i (DEVICE), from their positions before end[i], in n_layers layers (keys
  * layer_stride, bounds bounds_stride elements apart). A channel with a NaN has NaN as its bounds. Pages without a token
- * keep theirs; of sequences that share a page and name other ends on it, one's bounds stay. One launch.
+ * keep theirs; of sequences that share a page and name other ends on it, one's bounds stay, channel by channel (which one's
+ * is open). One launch.
  *
  * sjk_kv16_select chooses for every sequence and KV head up to `budget` pages of its table row, as their numbers there:
  * the first `sink` and the newest `recent` ones, and of the others those with the largest
  *   sum over the group's query heads of sum_d max(q_d lo_d, q_d hi_d)
- * (in 64 bits; ties to the lower number; a sum that is no number counts as the largest), all where there are no more than
+ * (in 64 bits; ties to the lower number; a sum that is no number counts as the largest; for a negative scale of the attention
+ * give -q, since the keys with the smallest products matter there), all where there are no more than
  * `budget`. blocks[i][h] (DEVICE [n_seq][n_head_kv][budget]): ascending, then -1; count (DEVICE [n_seq][n_head_kv], may be
  * NULL): how many; neither lies over len. Pages that are SJKVARN_NO_BLOCK are never chosen. The newest page's bounds may be
  * older than its last tokens where `recent` covers it. Two launches.

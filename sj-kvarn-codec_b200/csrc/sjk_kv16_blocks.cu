@@ -13,7 +13,8 @@
 // launches of a choice with its attention, each a chain of dependent loads. Measured (us on the GPU by CUDA graphs): bounds of a
 // decode step of 64 sequences in 4 layers 4.7, of a prompt of 32,700 tokens in 2 layers 29 (138 MB: 4.8 TB/s; 31 with a CTA per page
 // and its warps joined in shared memory); the choice among 6,250 pages for each of 8 heads 19, among up to 512 for 128 lists 24, the
-// attention over the chosen 2,048 positions 13 and 59 (268 MB of rows: 4.6 TB/s).
+// attention over the chosen 2,048 positions 13 and 59 (268 MB of rows: 4.6 TB/s). Long lists: 22 among 8,192 pages (in registers), 24
+// among 8,200 (read anew in every round), 148 among 62,500 (a million tokens: 256 MB of bounds, 39 us at a copy's rate).
 #include "sjk_kv16.cuh"
 #include "sjk_internal.h"
 

@@ -13,7 +13,9 @@ namespace {
 using namespace sjk16;
 
 constexpr int NT = 256;                     // maps
-constexpr int NK = 128;                     // keep: a token's row of 1,024 16-bit channels is as many 16-byte words
+// keep: a thread a 16-byte word of a row, and more of wider rows in turn. 1,024 channels are 128 words (20 us with 256 threads, 16.1 with 128);
+// of narrower rows' CTAs some threads have none, which such calls, of a few us, do not show
+constexpr int NK = 128;
 __device__ unsigned int g_step_status;
 
 SJK_DEV void flag() { atomicOr(&g_step_status, (unsigned) SJK_DEVICE_PAGE); }

@@ -5,12 +5,14 @@
 // All query heads of a KV head's group, of all the tokens of a sequence, are rows of one product: a key read once serves
 // (tokens x heads of a group) rows, up to NMAX = 64 or 128 in one pass, more in tiles of rows that CTAs side by side work on at
 // the same time, so that the second one's keys come from L2 (100,000 tokens, 256 rows: 411 MB of DRAM reads for 410 MB of live
-// rows). Bound: HBM up to 64 rows a KV head, above that what the softmax warps issue (0.47 a cycle), and for short sequences the
-// chain of a tile (rows, products, maximum, weights, products), of some 4,000 cycles. Measured (us a pass from Python, of a
-// program that keeps the GPU busy, which then runs at 1.2 GHz under its power cap in the second case): one chat of 611 tokens with 8
-// drafts 13.6; 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels, 16 drafts x 4 heads 803-858 (89 to 95 % of a plain copy's
-// rate, box by box; 760 in bursts, at the full clock); 100,000 tokens, 8 heads of 128 f16 channels, 64 drafts x 4 heads 248 (424 TFLOP/s); 64 pieces of up to 33
-// tokens over windows of 512, 24 heads of 64 channels 101.
+// rows). Bound: HBM up to 64 rows a KV head; above that waits between the steps of a tile's chain (rows, products, maximum, weights,
+// products: some 4,000 to 5,000 cycles, in which the warps issue 0.47 instructions a cycle), and for short sequences that chain
+// alone; for hundreds of them the walk over the sequences, a warp's in every CTA and then each role's. Measured (us a pass from
+// Python, of a program that keeps the GPU busy, which in the second case then runs at 1.2 GHz under its power cap, box by box):
+// one chat of 611 tokens with 8 drafts 12.9; 32 sequences of 8K-64K, 4 KV heads of 256 bf16 channels, 16 drafts x 4 heads 870-910 (84 to
+// 88 % of a plain copy's rate); 100,000 tokens, 8 heads of 128 f16 channels, 64 drafts x 4 heads 244-251 (420-430 TFLOP/s); 64 pieces of
+// up to 33 tokens over windows of 512, 24 heads of 64 channels 103. 1,024 sequences of 100 tokens with 4 drafts, 2 KV heads of 128
+// channels, on the GPU: 90, and 106 with `first`; 4,096 of 20: 329 and 382.
 //  - S^T = K Q^T with 128 positions as the M rows of tcgen05.mma and the query rows as its N columns (16 to 128), and
 //    O^T += V^T P with 128 channels as M: what a tile costs the softmax goes with the number of query rows, where query rows
 //    as M would make 8 of them as dear as 128. K, V and P lie in shared memory as they come: K rows are K-major for the

@@ -343,7 +343,8 @@ class Cache:
         type, lens int32 [n] (committed positions: token j of sequence i lies at lens[i] + j), masks int64 [n_tok] (bit k:
         the token sees its sequence's k-th; None: those up to itself). first int32 [n + 1]: where the sequences' tokens
         begin (None: n_tok / n each); nodes: at most so many tokens a sequence (None: n_tok / n, or with `first` 64); rows,
-        window, out and scratch (Cache.tree_scratch_bytes) as for attend."""
+        window, out and scratch (Cache.tree_scratch_bytes) as for attend. Rows of q that no sequence has are left as they are in `out`: give
+        one that is filled where a padded batch is read whole. out may be q."""
         n_tok, n, dev = q.shape[0], lens.shape[0], self._dev
         if _current_device() != dev:
             with torch.cuda.device(dev):
@@ -392,9 +393,10 @@ class Cache:
 
 
 class Maps:
-    """The maps of a step in which n_seq sequences bring up to n_tok tokens: first [n_seq + 1], rows, pos, at [n_tok] int32
-    and slots [n_tok] int64 (include/sjk.h, sjk_kv16_step), filled by a call and kept until the next one. For Qkv and
-    Cache.attend_tree: rows=m.rows, pos=m.pos, at=m.at, first=m.first."""
+    """The maps of a step in which n_seq sequences (always as many: a smaller batch fills up with ones that add 0) bring up to
+    n_tok tokens: first [n_seq + 1], rows, pos, at [n_tok] int32 and slots [n_tok] int64 (include/sjk.h, sjk_kv16_step), filled
+    by a call and kept until the next one; not an input of it as well. For Qkv and Cache.attend_tree: rows=m.rows, pos=m.pos,
+    at=m.at, first=m.first."""
 
     def __init__(self, cache, n_seq, n_tok):
         self.cache, self.n_seq, self.n_tok, self._dev = cache, n_seq, n_tok, cache._dev
@@ -449,7 +451,7 @@ class Blocks:
 
     def select(self, layer, q, lens, budget, sink=1, recent=1, rows=None, blocks=None, count=None, scratch=None):
         """Up to `budget` pages of every sequence and KV head for the query heads q [n][heads][D]: the first `sink`, the
-        newest `recent`, and those with the largest bounds. Returns (blocks int32 [n][KV heads][budget], ascending and then
+        newest `recent`, and those with the largest bounds of q . k (for a negative scale: give -q). Returns (blocks int32 [n][KV heads][budget], ascending and then
         -1; count int32 [n][KV heads])."""
         n, dev, c = q.shape[0], self._dev, self.cache
         if _current_device() != dev:
