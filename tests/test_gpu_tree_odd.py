@@ -175,3 +175,44 @@ def test_more_pairs_than_are_gone_through_at_once(T, page):
         e = 2.0 ** -18 * (1 + float((T.einsum("njhd,nthd->njht", x.abs(), k.abs()) * 0.2).max()))
         bound = 2.0 ** -8 * want.abs() * (1 + 2.0 ** -7) + (2.0 ** -16 + 2 * e + 2.0 ** -26 * 1700) * mag + 1e-37
         assert bool(((out[b].double() - want).abs() <= bound)[~odd[b]].all())
+
+
+@pytest.mark.parametrize("page", [16, 5])
+def test_replays_with_and_without(T, page):
+    """A captured call replays over values that come and go, on two streams at once; a page is missing, and slots of nobody are NaN."""
+    lens, counts, H, D = [700, 30, 20000], [5, 9, 16], 2, 128
+    cache, g = _cache(T, [a + b for a, b in zip(lens, counts)], page, H, D, T.float16, seed=page)
+    cache.tables[2, 3] = -1
+    masks = [_tree(random.Random(i), n) for i, n in enumerate(counts)]
+    flat, first, dl = _ints(T, [m for x in masks for m in _signed(x)], T.int64), _ints(T, _first(counts)), _ints(T, lens)
+    qs = [T.randn((sum(counts), 3 * H, D), device="cuda", generator=g).half() for _ in range(2)]
+    call = lambda q: cache.attend_tree(0, q, dl, flat, 0.1, first=first)  # noqa: E731
+    clean = [call(q) for q in qs]
+    graphs, outs = [], []
+    for q in qs:
+        gr = T.cuda.CUDAGraph()
+        with T.cuda.graph(gr):
+            outs.append(call(q))
+        graphs.append(gr)
+    streams = [T.cuda.Stream() for _ in range(2)]
+    place = (0, int(cache.tables[2, 20003 // page]), 20003 % page)
+    was = cache.v[place][1, 7].clone()
+    for x in (None, INF, None, NAN, -INF, None):
+        cache.v[place][1, 7] = was if x is None else x
+        T.cuda.synchronize()
+        for gr, s in zip(graphs, streams):
+            with T.cuda.stream(s):
+                gr.replay()
+                gr.replay()
+        T.cuda.synchronize()
+        for o, c in zip(outs, clean):
+            if x is None:
+                assert T.equal(o, c)
+                continue
+            hit = T.zeros(o.shape, dtype=T.bool, device="cuda")
+            for j in range(counts[2]):
+                hit[14 + j, 3:, 7] = bool(masks[2][j] >> 3 & 1)
+            assert T.equal(o[hit].nan_to_num(7.0), T.full_like(o[hit], x).nan_to_num(7.0)) and bool(T.isfinite(o[~hit]).all())
+            # what does not see it is as without it: a sum of the same terms, of which one is now left out where its weight was 0
+            assert T.equal(o[~hit], c[~hit])
+    assert sjk.lib().sjk_device_status() == 0
